@@ -279,6 +279,80 @@ int pto_b200_flash_attn_fwd_f16_ex(const uint16_t *q, const uint16_t *k, const u
 int pto_b200_flash_attn_fwd_f16_host(const uint16_t *q, const uint16_t *k, const uint16_t *v, void *o,
                                      int batch_heads, int sq, int sk, int d, int causal, float scale, int out_f16);
 
+/* ---- serving: paged key / value cache, attention over a shared prefix, 4-bit weights ---------------- */
+
+/* (These have no counterpart in the reference.)
+ *
+ * A cache holds K and V in pages of page_size positions: k / v are (num_pages, kv_heads, page_size, row) with a row of
+ * head_dim elements as 16-bit values, MX fp8 (float8_e4m3fn) or MX fp4 (float4_e2m1, two a byte, the lower index in the
+ * low nibble), and for the MX formats k_scale / v_scale (num_pages, kv_heads, page_size, head_dim / 32) float8_e8m0
+ * bytes, one per 32 consecutive elements: the formats of the MX GEMMs above.  head_dim is 64 or 128, page_size a power
+ * of two from 16 to 1024; everything is dense and 16-byte aligned.
+ *
+ * Page tables and lengths are read on the device, so one captured graph serves changing contents.  An index found out of
+ * range there (a slot or page beyond the cache, a length below 0 or beyond its bound) touches no memory: it is skipped (a
+ * length is cut to its range) and the first one is put in the status record: {PTO_B200_ERR_BAD_ARGUMENT, block, where,
+ * value} with where 10 = slot, 11 = page, 12 = length. */
+#define PTO_B200_KV_F16 0
+#define PTO_B200_KV_BF16 1
+#define PTO_B200_KV_MXFP8 2
+#define PTO_B200_KV_MXFP4 3
+typedef struct pto_b200_kv_cache {
+    void *k;
+    void *v;
+    uint8_t *k_scale; /* NULL for the 16-bit formats */
+    uint8_t *v_scale;
+    int64_t num_pages;
+    int32_t format; /* PTO_B200_KV_* */
+    int32_t kv_heads;
+    int32_t page_size;
+    int32_t head_dim;
+} pto_b200_kv_cache;
+
+/* Writes rows k[i], v[i] (kv_heads x head_dim; dtype PTO_B200_DTYPE_F16 or _BF16, for a 16-bit cache its own type) to
+ * position slots[i] = page * page_size + offset for i < tokens.  A negative slot is skipped; the other slots of a call
+ * have to be distinct.  strides: elements between K's tokens, K's heads, V's tokens, V's heads, multiples of 8.
+ * Per 32 elements the scale is the smallest power of two at which none of them saturates (2^119 at most for fp8, 2^125
+ * for fp4: larger values saturate) and the elements are rounded to nearest even; a block that holds a NaN or an infinity
+ * reads back as NaN. */
+int pto_b200_kv_cache_write(const pto_b200_kv_cache *cache, const void *k, const void *v, int dtype, const int32_t *slots,
+                            int64_t tokens, const int64_t strides[4], void *stream);
+/* Reads sequences back: k_out, v_out (batch, kv_heads, max_len, head_dim) of `dtype` receive position t < seq_lens[b]
+ * of sequence b from page page_table[b * table_stride + t / page_size], and zeros from seq_lens[b] on.  The table has
+ * table_cols columns; positions beyond them, and in pages out of range, read as zeros. */
+int pto_b200_kv_cache_read(const pto_b200_kv_cache *cache, const int32_t *page_table, int64_t table_stride, int table_cols,
+                           const int32_t *seq_lens, int batch, int max_len, void *k_out, void *v_out, int dtype,
+                           void *stream);
+/* Attention of `tokens` query tokens for each of `batch` sequences that share a prefix.  q (batch, tokens, heads, head_dim)
+ * of `dtype` (for a 16-bit cache its own type; q_strides: elements between sequences, tokens and heads, multiples of 8);
+ * heads a multiple of kv_heads, query head h reads kv head h / (heads / kv_heads).  Keys of query token j of sequence b: the
+ * prefix's prefix_len positions in pages prefix_pages[0 ..], then the sequence's own positions
+ * 0 .. seq_lens[b] - (tokens - 1 - j) - 1 through its row of page_table (table_cols columns): the query tokens are
+ * the last `tokens` of the sequence.  max_seq_len bounds seq_lens (at most table_cols * page_size).
+ *   o = softmax(scale q K^T) V, (batch, tokens, heads, head_dim) of `dtype`, zeros where there is no key;
+ *   lse (optional, (batch, tokens, heads) fp32) = log(sum(exp(scale q K^T))), -infinity where there is no key.
+ * Logits, statistics and sums are fp32; the probabilities are rounded to `dtype` for the second product.  With float16
+ * queries cached values beyond float16's range count as infinities.  A NaN in a position that one of a sequence's query
+ * tokens sees can reach the others'; positions at and after seq_lens[b] may hold anything.
+ * `workspace`: device memory of at least pto_b200_prefix_attn_workspace_bytes(...) bytes, 16-byte aligned, not shared by
+ * calls that may run at the same time. */
+int64_t pto_b200_prefix_attn_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int prefix_len,
+                                             int max_seq_len);
+int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtype, const int64_t q_strides[3],
+                         const int32_t *prefix_pages, int prefix_len, const int32_t *page_table, int64_t table_stride,
+                         int table_cols, const int32_t *seq_lens, int max_seq_len, int batch, int tokens, int heads,
+                         float scale, void *o, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+/* y[m x n] = x[m x k] W[n x k]^T with 4-bit weights, two a byte with the lower k index in the low nibble, m <= 64.
+ * dtype: the 16-bit type of x (rows x_stride elements apart, a multiple of 8), of int4 scales and zeros, and of y unless
+ * out_f32.  format PTO_B200_W4_MXFP4: float4_e2m1 codes with float8_e8m0 bytes scale (n x k / 32), the operand b of
+ * pto_b200_mxgemm_fp4 (group must be 32, zero NULL); PTO_B200_W4_INT4: W = scale * (code - zero), scale and zero
+ * (n x k / group), group 32, 64 or 128, zero = 8 when NULL.  k a multiple of group; sums in fp32.  For more rows use the
+ * GEMMs. */
+#define PTO_B200_W4_MXFP4 0
+#define PTO_B200_W4_INT4 1
+int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const void *scale, const void *zero, void *y, int m,
+                       int n, int k, int group, int format, int dtype, int out_f32, void *stream);
+
 /* ---- drop-in shims with the reference's FFI signatures ------------------------------------------ */
 
 /* demos/torch_jit/gemm/gemm_kernel.cpp:259-262 `call_kernel(blockDim, stream, out, src0, src1)`: the 6144^3

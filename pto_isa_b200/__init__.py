@@ -13,4 +13,6 @@ from .ops import (  # noqa: F401
     TROWEXPAND, TROWEXPANDADD, TROWEXPANDMAX, TROWEXPANDMIN, TROWEXPANDEXPDIF, TROWMIN, TCOLSUM, TCOLMAX, TCOLMIN,
     TFILLPAD, TTRANS, TTRI, TRESHAPE, TSEL, TCMPS, TCMP, TADD, TSUB, TMUL, TDIV, TMAX, TMIN, TMULS, TADDS, gemm, gemm_i8, gemm_out16, gemm_bf16, gemm_host, gemm_host_batched, mx_gemm, mx_gemm_fp4, flash_attn_fwd, flash_attn_fwd_host, device_status,
     device_status_record, set_profile_buffer, probe_random_reads,
+    KV_F16, KV_BF16, KV_MXFP8, KV_MXFP4, KVCache, kv_cache_empty, kv_cache_write, kv_cache_read, prefix_attn,
+    prefix_attn_workspace_bytes, w4_matvec,
 )

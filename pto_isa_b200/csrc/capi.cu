@@ -115,6 +115,61 @@ int finish_host_call(int rc, cudaStream_t s)
     return fetch_device_status(s);
 }
 
+inline bool misaligned16(const void *p)
+{
+    return (reinterpret_cast<uintptr_t>(p) & 15u) != 0;
+}
+
+// checks a cache's description and turns it into the kernels' view of it
+int kv_view(const pto_b200_kv_cache *c, int dtype, const char *what, KvCacheView *out)
+{
+    if (c == nullptr || c->num_pages < 0 || c->kv_heads <= 0 || (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr))) {
+        set_error_text("%s: null cache or bad extents", what);
+        return kErrBadArgument;
+    }
+    if (c->format < PTO_B200_KV_F16 || c->format > PTO_B200_KV_MXFP4) {
+        set_error_text("%s: unknown cache format %d", what, c->format);
+        return kErrBadArgument;
+    }
+    if (dtype != PTO_B200_DTYPE_F16 && dtype != PTO_B200_DTYPE_BF16) {
+        set_error_text("%s: dtype is PTO_B200_DTYPE_F16 or PTO_B200_DTYPE_BF16", what);
+        return kErrBadArgument;
+    }
+    const bool mx = c->format >= PTO_B200_KV_MXFP8;
+    if (mx && c->num_pages > 0 && (c->k_scale == nullptr || c->v_scale == nullptr)) {
+        set_error_text("%s: an MX cache needs its scales", what);
+        return kErrBadArgument;
+    }
+    int shift = 4;
+    while (shift < 10 && (1 << shift) != c->page_size) {
+        ++shift;
+    }
+    if ((1 << shift) != c->page_size || (c->head_dim != 64 && c->head_dim != 128)) {
+        set_error_text("%s: page_size is a power of two from 16 to 1024, head_dim 64 or 128", what);
+        return kErrUnsupportedShape;
+    }
+    if (misaligned16(c->k) || misaligned16(c->v) || (mx && (misaligned16(c->k_scale) || misaligned16(c->v_scale)))) {
+        set_error_text("%s: the cache must be 16-byte aligned", what);
+        return kErrUnsupportedShape;
+    }
+    if (c->num_pages > (static_cast<int64_t>(0x7fffffff) >> shift)) {
+        set_error_text("%s: the cache has more positions than 32-bit slots can name", what);
+        return kErrTooLarge;
+    }
+    *out = KvCacheView{c->k, c->v, c->k_scale, c->v_scale, c->num_pages, c->format, c->kv_heads, shift, c->head_dim};
+    return kOk;
+}
+
+// a 16-bit cache is read and written without conversion where this is asked
+int kv_same_type(const KvCacheView &c, int dtype, const char *what)
+{
+    if ((c.fmt == PTO_B200_KV_F16 && dtype != PTO_B200_DTYPE_F16) || (c.fmt == PTO_B200_KV_BF16 && dtype != PTO_B200_DTYPE_BF16)) {
+        set_error_text("%s: a 16-bit cache takes its own type", what);
+        return kErrBadArgument;
+    }
+    return kOk;
+}
+
 } // namespace
 
 #pragma GCC visibility push(default)
@@ -637,6 +692,141 @@ int pto_b200_flash_attn_fwd_f16_host(const uint16_t *q, const uint16_t *k, const
         rc = check_cuda(cudaMemcpyAsync(o, dout, o_bytes, cudaMemcpyDeviceToHost, s), "D2H O");
     }
     return finish_host_call(rc, s);
+}
+
+// ------------------------------------------------------------------ serving
+
+int pto_b200_kv_cache_write(const pto_b200_kv_cache *cache, const void *k, const void *v, int dtype, const int32_t *slots,
+                            int64_t tokens, const int64_t strides[4], void *stream)
+{
+    KvCacheView view;
+    int rc = kv_view(cache, dtype, "kv_cache_write", &view);
+    if (rc == kOk) {
+        rc = kv_same_type(view, dtype, "kv_cache_write");
+    }
+    if (rc != kOk) {
+        return rc;
+    }
+    if (tokens < 0 || (tokens > 0 && (k == nullptr || v == nullptr || slots == nullptr || strides == nullptr))) {
+        return bad("kv_cache_write: null pointer or negative length");
+    }
+    if (tokens == 0) {
+        return kOk;
+    }
+    if (misaligned16(k) || misaligned16(v) || ((strides[0] | strides[1] | strides[2] | strides[3]) & 7) != 0) {
+        set_error_text("kv_cache_write: rows of k and v must be 16-byte aligned");
+        return kErrUnsupportedShape;
+    }
+    return launch_kv_write(view, static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v),
+                           dtype == PTO_B200_DTYPE_BF16, slots, tokens, strides, as_stream(stream));
+}
+
+int pto_b200_kv_cache_read(const pto_b200_kv_cache *cache, const int32_t *page_table, int64_t table_stride, int table_cols,
+                           const int32_t *seq_lens, int batch, int max_len, void *k_out, void *v_out, int dtype,
+                           void *stream)
+{
+    KvCacheView view;
+    const int rc = kv_view(cache, dtype, "kv_cache_read", &view);
+    if (rc != kOk) {
+        return rc;
+    }
+    if (batch < 0 || max_len < 0 || table_cols < 0 || table_stride < 0) {
+        return bad("kv_cache_read: negative extent");
+    }
+    if (batch == 0 || max_len == 0) {
+        return kOk;
+    }
+    if (seq_lens == nullptr || (table_cols > 0 && page_table == nullptr) || k_out == nullptr || v_out == nullptr) {
+        return bad("kv_cache_read: null pointer");
+    }
+    if (misaligned16(k_out) || misaligned16(v_out)) {
+        set_error_text("kv_cache_read: the outputs must be 16-byte aligned");
+        return kErrUnsupportedShape;
+    }
+    return launch_kv_read(view, page_table, table_stride, table_cols, seq_lens, batch, max_len, static_cast<uint16_t *>(k_out),
+                          static_cast<uint16_t *>(v_out), dtype == PTO_B200_DTYPE_BF16, as_stream(stream));
+}
+
+int64_t pto_b200_prefix_attn_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int head_dim, int prefix_len,
+                                             int max_seq_len)
+{
+    if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 ||
+        prefix_len < 0 || max_seq_len < 0 || static_cast<int64_t>(batch) * tokens * (heads / kv_heads) > (1 << 26)) {
+        return 0;
+    }
+    return prefix_attn_workspace_bytes(batch, tokens, heads, kv_heads, head_dim, prefix_len, max_seq_len);
+}
+
+int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtype, const int64_t q_strides[3],
+                         const int32_t *prefix_pages, int prefix_len, const int32_t *page_table, int64_t table_stride,
+                         int table_cols, const int32_t *seq_lens, int max_seq_len, int batch, int tokens, int heads,
+                         float scale, void *o, float *lse, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    KvCacheView view;
+    int rc = kv_view(cache, dtype, "prefix_attn", &view);
+    if (rc == kOk) {
+        rc = kv_same_type(view, dtype, "prefix_attn");
+    }
+    if (rc != kOk) {
+        return rc;
+    }
+    if (batch < 0 || tokens <= 0 || heads <= 0 || prefix_len < 0 || table_cols < 0 || table_stride < 0 || max_seq_len < 0 ||
+        heads % view.kv_heads != 0) {
+        return bad("prefix_attn: bad extents (heads must be a multiple of kv_heads, tokens at least 1)");
+    }
+    if (batch == 0) {
+        return kOk;
+    }
+    if (q == nullptr || o == nullptr || q_strides == nullptr || (prefix_len > 0 && prefix_pages == nullptr) ||
+        seq_lens == nullptr || (max_seq_len > 0 && page_table == nullptr)) {
+        return bad("prefix_attn: null pointer");
+    }
+    if (max_seq_len > (static_cast<int64_t>(table_cols) << view.page_shift)) {
+        return bad("prefix_attn: max_seq_len is more than the page table covers");
+    }
+    if (static_cast<int64_t>(batch) * tokens * (heads / view.kv_heads) > (1 << 26) || prefix_len > (1 << 30) || max_seq_len > (1 << 30)) {
+        set_error_text("prefix_attn: more than 2^26 query rows per kv head, or 2^30 keys");
+        return kErrTooLarge;
+    }
+    if (misaligned16(q) || misaligned16(o) || misaligned16(workspace) || ((q_strides[0] | q_strides[1] | q_strides[2]) & 7) != 0) {
+        set_error_text("prefix_attn: q's rows, o and the workspace must be 16-byte aligned");
+        return kErrUnsupportedShape;
+    }
+    return launch_prefix_attn(view, static_cast<const uint16_t *>(q), dtype == PTO_B200_DTYPE_BF16, q_strides, prefix_pages,
+                              prefix_len, page_table, table_stride, table_cols, seq_lens, max_seq_len, batch, tokens, heads,
+                              scale, static_cast<uint16_t *>(o), lse, workspace, workspace_bytes, as_stream(stream));
+}
+
+int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const void *scale, const void *zero, void *y, int m,
+                       int n, int k, int group, int format, int dtype, int out_f32, void *stream)
+{
+    if (m < 0 || n < 0 || k < 0 || (format != PTO_B200_W4_MXFP4 && format != PTO_B200_W4_INT4) ||
+        (dtype != PTO_B200_DTYPE_F16 && dtype != PTO_B200_DTYPE_BF16)) {
+        return bad("w4_matvec: negative extent, unknown format or dtype");
+    }
+    if (m == 0 || n == 0) {
+        return kOk;
+    }
+    if (x == nullptr || w == nullptr || scale == nullptr || y == nullptr) {
+        return bad("w4_matvec: null pointer");
+    }
+    if (m > 64) {
+        set_error_text("w4_matvec: at most 64 rows of x (more rows: the GEMMs)");
+        return kErrUnsupportedShape;
+    }
+    if (format == PTO_B200_W4_MXFP4 ? (group != 32 || zero != nullptr) : (group != 32 && group != 64 && group != 128)) {
+        return bad("w4_matvec: MX fp4 weights have groups of 32 and no zeros, int4 weights groups of 32, 64 or 128");
+    }
+    if (k == 0 || k % group != 0) {
+        set_error_text("w4_matvec: k must be a positive multiple of the group (%d)", group);
+        return kErrUnsupportedShape;
+    }
+    if (misaligned16(x) || misaligned16(w) || (x_stride & 7) != 0) {
+        set_error_text("w4_matvec: rows of x and w must be 16-byte aligned");
+        return kErrUnsupportedShape;
+    }
+    return launch_w4_matvec(static_cast<const uint16_t *>(x), x_stride, w, scale, static_cast<const uint16_t *>(zero), y, m, n, k,
+                            group, dtype == PTO_B200_DTYPE_BF16, format == PTO_B200_W4_MXFP4, out_f32 != 0, as_stream(stream));
 }
 
 // ------------------------------------------------------------------ reference-shaped shims

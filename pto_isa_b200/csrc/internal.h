@@ -113,4 +113,27 @@ size_t gemm_static_scratch_bytes();
 int launch_flash_attn_fwd(const uint16_t *q, const uint16_t *k, const uint16_t *v, void *o, int bh, int sq, int sk,
                           int d, int causal, float scale, int out_f16, cudaStream_t stream, int defer_rescale = -1);
 
+// a paged key / value cache: rows of d elements in (num_pages, kv_heads, 1 << page_shift), fmt one of PTO_B200_KV_*
+struct KvCacheView {
+    void *k, *v;
+    uint8_t *k_scale, *v_scale; // e8m0 bytes per 32 elements; null for 16-bit caches
+    int64_t num_pages;
+    int fmt, kv_heads, page_shift, d;
+};
+// quantises rows (tokens, kv_heads, d) into the cache; strides: k token, k head, v token, v head (elements)
+int launch_kv_write(const KvCacheView &cache, const uint16_t *k, const uint16_t *v, bool bf16, const int32_t *slots,
+                    int64_t tokens, const int64_t strides[4], cudaStream_t stream);
+// reads sequences back as (batch, kv_heads, max_len, d) 16-bit tensors, zeros from their lengths on
+int launch_kv_read(const KvCacheView &cache, const int32_t *table, int64_t table_stride, int table_cols,
+                   const int32_t *lens, int batch, int max_len, uint16_t *k, uint16_t *v, bool bf16, cudaStream_t stream);
+// attention of `tokens` query rows per sequence over a shared prefix and the sequences' own keys
+int64_t prefix_attn_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int d, int prefix_len, int own_max);
+int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, const int64_t q_strides[3],
+                       const int32_t *prefix_pages, int prefix_len, const int32_t *table, int64_t table_stride,
+                       int table_cols, const int32_t *lens, int own_max, int batch, int tokens, int heads, float scale,
+                       uint16_t *o, float *lse, void *workspace, int64_t workspace_bytes, cudaStream_t stream);
+// y[m, n] = sum_k x[m, k] W[n, k] with 4-bit weights; arguments validated by the caller
+int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, const void *scale, const uint16_t *zero, void *y,
+                     int m, int n, int k, int group, bool bf16, bool mx, bool out_f32, cudaStream_t stream);
+
 } // namespace pto_b200

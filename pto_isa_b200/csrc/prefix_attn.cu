@@ -1,0 +1,789 @@
+// Attention of few query tokens per sequence over a paged cache, for a batch whose sequences share a prefix.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m)  over the prefix's keys and the sequence's own keys.
+//
+// The prefix's keys are read once for the whole batch: for each kv head the rows are all (sequence, query token, head of
+// the group), so a key feeds batch * tokens * group rows of a product.  A sequence's own keys feed tokens * group rows.
+// Both parts are cut along the keys into pieces that run side by side; each piece leaves (sum p v, sum p, m) in fp32
+// for its rows and a second kernel joins them:  o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+//
+// piece kernel (16 rows a block): four warps, each walking every fourth group of 16 keys of the piece with a cp.async
+// ring of its own, so no warp waits for another until the piece ends.  A lane's operands come from 16-byte reads:
+//   S = Q K^T   the order of the head dimension inside a block of 32 is free as long as Q and K agree: lane t of a quad
+//               takes elements 8t .. 8t+7 of the block, two k steps of four.  Codes are multiplied unscaled (exact in
+//               16 bits) and the block's power of two is applied to the fp32 sums: S += 2^e (q_blk . code_blk).
+//   O += P V    a product's eight columns are head-dimension elements W g + i (g the lane's group, W = d / 8), so a
+//               lane reads W consecutive elements of its four keys and the operands need no transposition; V's scale
+//               depends on the key, so it is applied to the code pair (exact in 16 bits within the type's range).
+// Softmax statistics and all sums are fp32; P is rounded to the 16-bit type of q for the second product.
+#include "ptx.cuh"
+#include "internal.h"
+#include "mx_format.cuh"
+
+#include <type_traits>
+
+namespace pto_b200 {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStep = 16; // keys a warp takes at a time
+constexpr int kRows = 16; // query rows of a block
+constexpr int kSms = 148; // planning constant: what the cut along the keys aims at
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16 bytes global -> shared; what lies past the first `bytes` is not read and arrives as zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a)
+{
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a)
+{
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+struct AttnArgs {
+    const uint8_t *k, *v, *ks, *vs;
+    const uint16_t *q;
+    int64_t q_batch, q_token, q_head; // strides in elements
+    const int32_t *prefix_pages;
+    const int32_t *table;
+    const int32_t *lens;
+    int64_t table_stride;
+    int64_t num_pages;
+    float *part_o;   // [slot][16][d]
+    float2 *part_ml; // [slot][16]: m (log2 units), l
+    uint16_t *o;
+    float *lse;
+    float scale_log2;
+    int table_cols, page_shift;
+    int batch, tokens, heads, kv_heads, group;
+    int prefix_len, own_max;
+    int prefix_tiles, prefix_splits, prefix_chunk;
+    int own_tiles, own_splits, own_min;
+};
+
+__host__ __device__ inline int ceil_div(int a, int b)
+{
+    return (a + b - 1) / b;
+}
+
+// keys of one piece of a sequence with `len` own keys: a multiple of 64, so that the four warps share it evenly
+__device__ __forceinline__ int own_chunk(int len, int splits, int least)
+{
+    const int c = ((len + splits - 1) / splits + 63) & ~63;
+    return c < least ? least : c;
+}
+
+// a sequence's number of own keys: never negative, never more than the table (or the caller's bound) covers
+__device__ __forceinline__ int own_len(const AttnArgs &a, int b)
+{
+    const int n = a.lens[b];
+    return n < 0 ? 0 : (n > a.own_max ? a.own_max : n);
+}
+
+// ---- shared-memory image of 16 rows of RB bytes: 16-byte chunks, exclusive-or swizzled within 128-byte lines so that
+// the lanes of one access phase meet distinct banks.  K is read a key per quad (rows g), V a key per lane of a quad
+// (rows 2t, 2t + 1).
+template <int RB, int kFmt>
+__device__ __forceinline__ uint32_t swz_k(int row, int byte)
+{
+    const int chunk = (row * RB + byte) >> 4;
+    const int x = RB == 256 ? (row & 1) * 4
+                  : RB == 128 ? (kFmt == kKvMxFp8 ? (2 * row) & 6 : (row & 1) * 4)
+                  : RB == 64 ? (kFmt == kKvMxFp4 ? (row >> 1) & 3 : 2 * ((row >> 1) & 1))
+                             : (row >> 2) & 1;
+    return static_cast<uint32_t>(((chunk ^ x) << 4) | (byte & 15));
+}
+template <int RB>
+__device__ __forceinline__ uint32_t swz_v(int row, int byte)
+{
+    const int chunk = (row * RB + byte) >> 4;
+    const int t = (row >> 1) & 3;
+    const int x = RB == 256 ? (t & 1) | ((t & 2) << 1) : RB == 128 ? row & 6 : RB == 64 ? 2 * t : 2 * ((row >> 2) & 1);
+    return static_cast<uint32_t>(((chunk ^ x) << 4) | (byte & 15));
+}
+
+template <int kD, int kFmt>
+struct Stage {
+    static constexpr int kRowBytes = kv_row_bytes(kFmt, kD);
+    static constexpr int kRowsBytes = kStep * kRowBytes;
+    static constexpr int kScaleBytes = kFmt >= kKvMxFp8 ? kStep * kD / 32 : 0; // per K or V
+    static constexpr int kBytes = 2 * kRowsBytes + 2 * kScaleBytes;
+    static constexpr int kCount = kFmt <= kKvBf16 ? (kD == 128 ? 2 : 4) : (kFmt == kKvMxFp8 ? 4 : 6);
+    static constexpr int kMergeBytes = kWarps * kRows * kD * 4 + kWarps * kRows * 8;
+    static constexpr int kRing = kWarps * kCount * kBytes;
+    static constexpr int kSmem = kRing > kMergeBytes ? kRing : kMergeBytes;
+};
+
+// pair of codes (bytes / nibbles already placed) -> 16-bit pair, times nothing: the codes' own values
+// fp8: `two` = bytes {lo, hi} in bits 0..15
+template <bool kBf16>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t word, int sel)
+{
+    if constexpr (!kBf16) {
+        return e4m3x2_to_f16x2(sel ? word >> 16 : word & 0xffffu);
+    } else {
+        // each byte at the top of a half: sign in place, exponent and mantissa 4 bits down; as bfloat16 that is the
+        // code times 2^-120 (e4m3's bias 7 against 127), subnormals included
+        uint32_t r = __byte_perm(word, 0, sel ? 0x3424 : 0x1404);
+        r = (r & 0x80008000u) | ((r >> 4) & 0x07f007f0u);
+        return mul_16x2<true>(r, 0x7b807b80u); // 2^120
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t e2m1_pair(uint32_t byte)
+{
+    const uint32_t h = e2m1x2_to_f16x2(byte);
+    if constexpr (!kBf16) {
+        return h;
+    } else {
+        const uint32_t r = (h & 0x80008000u) | ((h >> 3) & 0x0fff0fffu); // times 2^-112
+        return mul_16x2<true>(r, 0x77807780u);                           // 2^112
+    }
+}
+
+// 2^(byte - 127) of two scale bytes as a 16-bit pair.  bfloat16: exact but for byte 0 (0 instead of 2^-127) and 255
+// (infinity; a block with that byte holds zeros, and 0 * infinity is the NaN it stands for).  float16: rounded to
+// float16's range, as the values themselves are.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t b0, uint32_t b1)
+{
+    if constexpr (kBf16) {
+        return (b0 << 7) | (b1 << 23);
+    } else {
+        return pack_16x2<false>(__uint_as_float(b0 << 23), __uint_as_float(b1 << 23));
+    }
+}
+
+template <bool kBf16, int kD, int kFmt>
+__global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __grid_constant__ AttnArgs a, DeviceStatus *status)
+{
+    using St = Stage<kD, kFmt>;
+    constexpr int RB = St::kRowBytes;
+    constexpr int kBlk = kD / 32;
+    constexpr int kTiles = kD / 8; // column tiles of O
+    extern __shared__ __align__(128) uint8_t smem[];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+
+    // ---- which piece
+    const int prefix_items = a.prefix_splits * a.kv_heads * a.prefix_tiles;
+    const int row_span = a.tokens * a.group; // rows of one sequence and kv head
+    int64_t item = blockIdx.x;
+    int h, tile, b = 0, k_begin, k_end, rows;
+    const bool own = item >= prefix_items;
+    const int32_t *pages;
+    int64_t slot = item;
+    if (!own) {
+        tile = static_cast<int>(item % a.prefix_tiles);
+        h = static_cast<int>(item / a.prefix_tiles) % a.kv_heads;
+        const int split = static_cast<int>(item / a.prefix_tiles) / a.kv_heads;
+        k_begin = split * a.prefix_chunk;
+        k_end = min(k_begin + a.prefix_chunk, a.prefix_len);
+        rows = a.batch * row_span;
+        pages = a.prefix_pages;
+    } else {
+        item -= prefix_items;
+        tile = static_cast<int>(item % a.own_tiles);
+        item /= a.own_tiles;
+        h = static_cast<int>(item % a.kv_heads);
+        item /= a.kv_heads;
+        b = static_cast<int>(item % a.batch);
+        const int split = static_cast<int>(item / a.batch);
+        const int len = own_len(a, b);
+        if (split == 0 && tile == 0 && h == 0 && threadIdx.x == 0 && len != a.lens[b] && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+            status->block = blockIdx.x;
+            status->where = 12;
+            status->detail = a.lens[b];
+        }
+        const int chunk = own_chunk(len, a.own_splits, a.own_min);
+        k_begin = split * chunk;
+        k_end = min(k_begin + chunk, len);
+        rows = row_span;
+        pages = a.table + b * a.table_stride;
+        if (k_begin >= k_end) {
+            return; // past this sequence's last piece: the joining kernel does not look here
+        }
+    }
+
+    // ---- this lane's two rows: g and g + 8 of the tile
+    int limit[2];
+    const uint16_t *q_row[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = tile * kRows + g + 8 * i;
+        const bool live = r < rows;
+        const int rr = live ? r : 0;
+        const int bb = own ? b : rr / row_span;
+        const int in = own ? rr : rr % row_span;
+        const int tok = in / a.group;
+        q_row[i] = live ? a.q + bb * a.q_batch + tok * a.q_token + static_cast<int64_t>(h * a.group + in % a.group) * a.q_head : nullptr;
+        // own keys: token `tok` of `tokens` sees all but the last tokens - 1 - tok
+        limit[i] = !live ? 0 : (own ? min(k_end, own_len(a, b) - (a.tokens - 1 - tok)) : k_end);
+    }
+    // Q operands: block kb, words {step 0: low pair, high pair, step 1: low pair, high pair}
+    uint32_t qf[kBlk][2][4];
+#pragma unroll
+    for (int kb = 0; kb < kBlk; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (q_row[i] != nullptr) {
+                v = *reinterpret_cast<const uint4 *>(q_row[i] + 32 * kb + 8 * t);
+            }
+            qf[kb][i][0] = v.x;
+            qf[kb][i][1] = v.y;
+            qf[kb][i][2] = v.z;
+            qf[kb][i][3] = v.w;
+        }
+    }
+
+    // ---- this warp's steps and ring
+    const int steps = ceil_div(k_end - k_begin, kStep);
+    const uint32_t ring = smem_u32(smem) + warp * St::kCount * St::kBytes;
+    uint32_t bad_pages = 0; // bit s: the step in ring stage s lies in a page that does not exist
+    auto load = [&](int step, int stage) {
+        if (step < steps) {
+            const int key = k_begin + step * kStep;
+            const int64_t page = pages[key >> a.page_shift];
+            const bool ok = page >= 0 && page < a.num_pages;
+            bad_pages = (bad_pages & ~(1u << stage)) | (ok ? 0u : 1u << stage);
+            if (!ok) {
+                if (lane == 0 && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+                    status->block = blockIdx.x;
+                    status->where = 11;
+                    status->detail = static_cast<int>(page);
+                }
+            }
+            const int64_t row = (((ok ? page : 0) * a.kv_heads + h) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+            const int live = ok ? min(kStep, k_end - key) : 0; // rows past the end arrive as zeros
+            const uint32_t base = ring + stage * St::kBytes;
+            constexpr int kChunks = St::kRowsBytes / 16;
+#pragma unroll
+            for (int c0 = 0; c0 < kChunks; c0 += 32) {
+                const int c = c0 + lane;
+                if (kChunks >= 32 || c < kChunks) {
+                    const int r = (c * 16) / RB, byte = (c * 16) % RB;
+                    const int64_t off = row * RB + c * 16;
+                    cp_async16(base + swz_k<RB, kFmt>(r, byte), a.k + off, r < live ? 16 : 0);
+                    cp_async16(base + St::kRowsBytes + swz_v<RB>(r, byte), a.v + off, r < live ? 16 : 0);
+                }
+            }
+            if constexpr (St::kScaleBytes > 0) {
+                // the scales of 16 rows that start at a multiple of 16 are one run of kScaleBytes, 16-byte aligned
+                constexpr int kSc = St::kScaleBytes / 16;
+                if (lane < 2 * kSc) {
+                    const int c = lane % kSc;
+                    const uint8_t *src = (lane < kSc ? a.ks : a.vs) + row * (kD / 32) + c * 16;
+                    // scales past the end arrive as 0, not as whatever the cache holds there: 0 * 2^128 would be NaN
+                    cp_async16(base + 2 * St::kRowsBytes + lane * 16, src, max(0, min(16, live * (kD / 32) - c * 16)));
+                }
+            }
+        }
+        cp_async_commit();
+    };
+
+    float o[kTiles][4];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[i][j] = 0.0f;
+        }
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+#pragma unroll
+    for (int s = 0; s < St::kCount - 1; ++s) {
+        load(warp + s * kWarps, s);
+    }
+    int stage = 0;
+    for (int step = warp; step < steps; step += kWarps) {
+        {
+            const int ahead = stage == 0 ? St::kCount - 1 : stage - 1;
+            load(step + (St::kCount - 1) * kWarps, ahead);
+        }
+        cp_async_wait<St::kCount - 1>();
+        __syncwarp();
+        const uint32_t base = ring + stage * St::kBytes;
+        const int key0 = k_begin + step * kStep;
+        const bool bad = (bad_pages >> stage) & 1u;
+
+        // ---- S = Q K^T
+        float s[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[n][j] = 0.0f;
+            }
+            uint32_t sc[2] = {0, 0}; // scale bytes of the lane's two columns (keys 8n + 2t, + 1)
+            if constexpr (kFmt >= kKvMxFp8) {
+                const uint32_t at = base + 2 * St::kRowsBytes + (8 * n + 2 * t) * kBlk;
+                if constexpr (kBlk == 4) {
+                    const uint2 v = lds64(at);
+                    sc[0] = v.x;
+                    sc[1] = v.y;
+                } else {
+                    const uint32_t v = lds32(at);
+                    sc[0] = v & 0xffffu;
+                    sc[1] = v >> 16;
+                }
+            }
+#pragma unroll
+            for (int kb = 0; kb < kBlk; ++kb) {
+                uint32_t w[4];
+                if constexpr (kFmt <= kKvBf16) {
+                    const uint4 v = lds128(base + swz_k<RB, kFmt>(8 * n + g, 64 * kb + 16 * t));
+                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                    mma_16816<kBf16>(s[n], qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
+                    mma_16816<kBf16>(s[n], qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
+                } else {
+                    if constexpr (kFmt == kKvMxFp8) {
+                        const uint2 v = lds64(base + swz_k<RB, kFmt>(8 * n + g, 32 * kb + 8 * t));
+                        w[0] = e4m3_pair<kBf16>(v.x, 0);
+                        w[1] = e4m3_pair<kBf16>(v.x, 1);
+                        w[2] = e4m3_pair<kBf16>(v.y, 0);
+                        w[3] = e4m3_pair<kBf16>(v.y, 1);
+                    } else {
+                        const uint32_t v = lds32(base + swz_k<RB, kFmt>(8 * n + g, 16 * kb + 4 * t));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = e2m1_pair<kBf16>((v >> (8 * i)) & 0xffu);
+                        }
+                    }
+                    float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_16816<kBf16>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
+                    mma_16816<kBf16>(p, qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
+                    const float f0 = __uint_as_float(((sc[0] >> (8 * kb)) & 0xffu) << 23);
+                    const float f1 = __uint_as_float(((sc[1] >> (8 * kb)) & 0xffu) << 23);
+                    s[n][0] = fmaf(p[0], f0, s[n][0]);
+                    s[n][1] = fmaf(p[1], f1, s[n][1]);
+                    s[n][2] = fmaf(p[2], f0, s[n][2]);
+                    s[n][3] = fmaf(p[3], f1, s[n][3]);
+                }
+            }
+        }
+
+        // ---- running maximum and sum, log2 units
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = key0 + 8 * n + 2 * t + (j & 1);
+                const bool seen = key < limit[j >> 1] && !bad;
+                s[n][j] = seen ? s[n][j] * a.scale_log2 : -INFINITY;
+                mx[j >> 1] = fmaxf(mx[j >> 1], s[n][j]);
+            }
+        }
+        float ref[2], alpha[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            const float m_new = fmaxf(m[i], mx[i]);
+            ref[i] = m_new == -INFINITY ? 0.0f : m_new; // a row that has seen no key yet
+            alpha[i] = ex2(m[i] - ref[i]);
+            m[i] = m_new;
+            l[i] *= alpha[i];
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                o[i][0] *= alpha[0];
+                o[i][1] *= alpha[0];
+                o[i][2] *= alpha[1];
+                o[i][3] *= alpha[1];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[n][j] = ex2(s[n][j] - ref[j >> 1]);
+                l[j >> 1] += s[n][j];
+            }
+        }
+        const uint32_t p0 = pack_16x2<kBf16>(s[0][0], s[0][1]), p1 = pack_16x2<kBf16>(s[0][2], s[0][3]);
+        const uint32_t p2 = pack_16x2<kBf16>(s[1][0], s[1][1]), p3 = pack_16x2<kBf16>(s[1][2], s[1][3]);
+
+        // ---- O += P V: keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step, elements W g .. W g + W - 1
+        const uint32_t vbase = base + St::kRowsBytes;
+        uint32_t scale01 = 0, scale23 = 0;
+        if constexpr (kFmt >= kKvMxFp8) {
+            const uint32_t sbase = base + 2 * St::kRowsBytes + St::kScaleBytes;
+            const int blk = (g * (kD / 8)) / 32;
+            scale01 = scale_pair<kBf16>(lds8(sbase + (2 * t) * kBlk + blk), lds8(sbase + (2 * t + 1) * kBlk + blk));
+            scale23 = scale_pair<kBf16>(lds8(sbase + (2 * t + 8) * kBlk + blk), lds8(sbase + (2 * t + 9) * kBlk + blk));
+        }
+        if constexpr (kFmt <= kKvBf16) {
+#pragma unroll
+            for (int half = 0; half < kTiles / 8; ++half) { // eight elements (16 bytes) of each key at a time
+                const int byte = g * (kD / 4) + half * 16;
+                const uint4 x0 = lds128(vbase + swz_v<RB>(2 * t, byte)), x1 = lds128(vbase + swz_v<RB>(2 * t + 1, byte));
+                const uint4 x2 = lds128(vbase + swz_v<RB>(2 * t + 8, byte)), x3 = lds128(vbase + swz_v<RB>(2 * t + 9, byte));
+                const uint32_t y0[4] = {x0.x, x0.y, x0.z, x0.w}, y1[4] = {x1.x, x1.y, x1.z, x1.w};
+                const uint32_t y2[4] = {x2.x, x2.y, x2.z, x2.w}, y3[4] = {x3.x, x3.y, x3.z, x3.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    mma_16816<kBf16>(o[half * 8 + 2 * i], p0, p1, p2, p3, __byte_perm(y0[i], y1[i], 0x5410),
+                                     __byte_perm(y2[i], y3[i], 0x5410));
+                    mma_16816<kBf16>(o[half * 8 + 2 * i + 1], p0, p1, p2, p3, __byte_perm(y0[i], y1[i], 0x7632),
+                                     __byte_perm(y2[i], y3[i], 0x7632));
+                }
+            }
+        } else {
+            constexpr int kWords = kFmt == kKvMxFp8 ? kD / 32 : kD / 64; // 32-bit words of a lane's elements, per key
+            uint32_t x[4][kWords];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t at = vbase + swz_v<RB>(2 * t + (i & 1) + (i >> 1) * 8, g * kWords * 4);
+                if constexpr (kWords == 4) {
+                    const uint4 v = lds128(at);
+                    x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+                } else if constexpr (kWords == 2) {
+                    const uint2 v = lds64(at);
+                    x[i][0] = v.x, x[i][1] = v.y;
+                } else {
+                    x[i][0] = lds32(at);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+                if constexpr (kFmt == kKvMxFp8) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) { // bytes 2c and 2c + 1 of the word: {key 0, key 1} side by side
+                        const uint32_t lo = __byte_perm(x[0][w], x[1][w], c ? 0x7362 : 0x5140);
+                        const uint32_t hi = __byte_perm(x[2][w], x[3][w], c ? 0x7362 : 0x5140);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t b0 = mul_16x2<kBf16>(e4m3_pair<kBf16>(lo, e), scale01);
+                            const uint32_t b1 = mul_16x2<kBf16>(e4m3_pair<kBf16>(hi, e), scale23);
+                            mma_16816<kBf16>(o[4 * w + 2 * c + e], p0, p1, p2, p3, b0, b1);
+                        }
+                    }
+                } else {
+                    // even nibbles of both keys in one byte, then odd ones
+                    const uint32_t even_lo = (x[0][w] & 0x0f0f0f0fu) | ((x[1][w] << 4) & 0xf0f0f0f0u);
+                    const uint32_t odd_lo = ((x[0][w] >> 4) & 0x0f0f0f0fu) | (x[1][w] & 0xf0f0f0f0u);
+                    const uint32_t even_hi = (x[2][w] & 0x0f0f0f0fu) | ((x[3][w] << 4) & 0xf0f0f0f0u);
+                    const uint32_t odd_hi = ((x[2][w] >> 4) & 0x0f0f0f0fu) | (x[3][w] & 0xf0f0f0f0u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mma_16816<kBf16>(o[8 * w + 2 * i], p0, p1, p2, p3,
+                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((even_lo >> (8 * i)) & 0xffu), scale01),
+                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((even_hi >> (8 * i)) & 0xffu), scale23));
+                        mma_16816<kBf16>(o[8 * w + 2 * i + 1], p0, p1, p2, p3,
+                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((odd_lo >> (8 * i)) & 0xffu), scale01),
+                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((odd_hi >> (8 * i)) & 0xffu), scale23));
+                    }
+                }
+            }
+        }
+        __syncwarp(); // every lane has read the stage before it is loaded again
+        stage = stage + 1 == St::kCount ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+
+    // ---- the four warps' sums joined through shared memory
+    float *mo = reinterpret_cast<float *>(smem);                                       // [warp][row][d]
+    float2 *ml = reinterpret_cast<float2 *>(smem + kWarps * kRows * kD * sizeof(float)); // [warp][row]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (t == 0) {
+            ml[warp * kRows + g + 8 * i] = make_float2(m[i], l[i]);
+        }
+        // columns 2t and 2t + 1 of every tile: elements W (2t + c) .. + W - 1
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float4 *dst = reinterpret_cast<float4 *>(mo + (warp * kRows + g + 8 * i) * kD + kTiles * (2 * t + c));
+#pragma unroll
+            for (int n = 0; n < kTiles / 4; ++n) {
+                dst[n] = make_float4(o[4 * n][2 * i + c], o[4 * n + 1][2 * i + c], o[4 * n + 2][2 * i + c], o[4 * n + 3][2 * i + c]);
+            }
+        }
+    }
+    __syncthreads();
+    {
+        constexpr int kCols = kRows * kD / kThreads; // elements of one row a thread joins
+        const int r = threadIdx.x / (kThreads / kRows), c0 = (threadIdx.x % (kThreads / kRows)) * kCols;
+        float top = -INFINITY, w[kWarps], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            top = fmaxf(top, ml[i * kRows + r].x);
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const float2 v = ml[i * kRows + r];
+            w[i] = ex2(v.x - ref);
+            sum += v.y * w[i];
+        }
+        float4 *dst = reinterpret_cast<float4 *>(a.part_o + (slot * kRows + r) * kD + c0);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                const float4 v = *reinterpret_cast<const float4 *>(mo + (i * kRows + r) * kD + c0 + c);
+                acc.x = fmaf(v.x, w[i], acc.x);
+                acc.y = fmaf(v.y, w[i], acc.y);
+                acc.z = fmaf(v.z, w[i], acc.z);
+                acc.w = fmaf(v.w, w[i], acc.w);
+            }
+            dst[c / 4] = acc;
+        }
+        if (c0 == 0) {
+            a.part_ml[slot * kRows + r] = make_float2(top, sum);
+        }
+    }
+}
+
+// one warp per output row: joins the row's pieces in a fixed order
+template <bool kBf16, int kD>
+__global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_constant__ AttnArgs a)
+{
+    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (idx >= static_cast<int64_t>(a.batch) * a.tokens * a.heads) {
+        return;
+    }
+    const int head = static_cast<int>(idx % a.heads);
+    const int tok = static_cast<int>(idx / a.heads % a.tokens);
+    const int b = static_cast<int>(idx / a.heads / a.tokens);
+    const int h = head / a.group, in = tok * a.group + head % a.group;
+    const int prow = b * a.tokens * a.group + in;
+    const int len = own_len(a, b);
+    const int own_pieces = len > 0 ? ceil_div(len, own_chunk(len, a.own_splits, a.own_min)) : 0;
+    const int64_t prefix_items = static_cast<int64_t>(a.prefix_splits) * a.kv_heads * a.prefix_tiles;
+    const int pieces = a.prefix_splits + own_pieces;
+    auto row_of = [&](int i) -> int64_t { // where piece i keeps this row
+        if (i < a.prefix_splits) {
+            return ((static_cast<int64_t>(i) * a.kv_heads + h) * a.prefix_tiles + prow / kRows) * kRows + prow % kRows;
+        }
+        const int64_t s = i - a.prefix_splits;
+        return (prefix_items + ((s * a.batch + b) * a.kv_heads + h) * a.own_tiles + in / kRows) * kRows + in % kRows;
+    };
+    float top = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) {
+        top = fmaxf(top, a.part_ml[row_of(i)].x);
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    constexpr int kPer = kD / 32;
+    float acc[kPer], sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+        acc[c] = 0.0f;
+    }
+    for (int i = 0; i < pieces; ++i) {
+        const int64_t row = row_of(i);
+        const float2 v = a.part_ml[row];
+        const float w = ex2(v.x - ref);
+        sum = fmaf(v.y, w, sum);
+        const float *src = a.part_o + row * kD + lane * kPer;
+        if constexpr (kPer == 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(src);
+            acc[0] = fmaf(x.x, w, acc[0]);
+            acc[1] = fmaf(x.y, w, acc[1]);
+            acc[2] = fmaf(x.z, w, acc[2]);
+            acc[3] = fmaf(x.w, w, acc[3]);
+        } else {
+            const float2 x = *reinterpret_cast<const float2 *>(src);
+            acc[0] = fmaf(x.x, w, acc[0]);
+            acc[1] = fmaf(x.y, w, acc[1]);
+        }
+    }
+    const bool none = top == -INFINITY && sum == 0.0f; // no key at all: zeros
+    const float inv = none ? 0.0f : 1.0f / sum;
+    uint16_t *dst = a.o + idx * kD + lane * kPer;
+    if constexpr (kPer == 4) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_16x2<kBf16>(acc[0] * inv, acc[1] * inv), pack_16x2<kBf16>(acc[2] * inv, acc[3] * inv));
+    } else {
+        *reinterpret_cast<uint32_t *>(dst) = pack_16x2<kBf16>(acc[0] * inv, acc[1] * inv);
+    }
+    if (a.lse != nullptr && lane == 0) {
+        a.lse[idx] = none ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
+    }
+}
+
+// How the keys are cut.  About three blocks of 16 rows fit an SM; a piece is at least 64 keys (16 for each warp).
+struct Plan {
+    int prefix_tiles, prefix_splits, prefix_chunk;
+    int own_tiles, own_splits, own_min;
+    int64_t slots;
+};
+
+Plan make_plan(int batch, int tokens, int heads, int kv_heads, int prefix_len, int own_max)
+{
+    Plan p = {0, 0, 0, 0, 0, 0, 0};
+    const int row_span = tokens * (heads / kv_heads);
+    const int target = 3 * kSms;
+    if (prefix_len > 0) {
+        p.prefix_tiles = ceil_div(batch * row_span, kRows);
+        const int64_t units = static_cast<int64_t>(p.prefix_tiles) * kv_heads;
+        int64_t splits = (target + units - 1) / units;
+        const int most = ceil_div(prefix_len, 64);
+        splits = splits > most ? most : splits;
+        p.prefix_chunk = (ceil_div(prefix_len, static_cast<int>(splits)) + 63) & ~63;
+        p.prefix_splits = ceil_div(prefix_len, p.prefix_chunk);
+    }
+    p.own_tiles = ceil_div(row_span, kRows);
+    p.own_min = 64;
+    if (own_max > 0) {
+        const int64_t units = static_cast<int64_t>(p.own_tiles) * kv_heads * batch;
+        int64_t splits = (target + units - 1) / units;
+        if (units >= target) { // the batch alone fills the GPU: pieces only for the sake of uneven lengths
+            splits = ceil_div(own_max, 1024);
+            p.own_min = 512;
+        }
+        const int most = ceil_div(own_max, 64);
+        p.own_splits = static_cast<int>(splits > most ? most : splits);
+    }
+    p.slots = (static_cast<int64_t>(p.prefix_splits) * p.prefix_tiles +
+               static_cast<int64_t>(p.own_splits) * p.own_tiles * batch) * kv_heads;
+    return p;
+}
+
+template <bool kBf16, int kD, int kFmt>
+int launch_pieces(const AttnArgs &a, int64_t blocks, DeviceStatus *status, cudaStream_t stream)
+{
+    constexpr int kSmem = Stage<kD, kFmt>::kSmem;
+    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&prefix_attn_piece_kernel<kBf16, kD, kFmt>), kSmem);
+    if (rc != kOk) {
+        return rc;
+    }
+    prefix_attn_piece_kernel<kBf16, kD, kFmt><<<static_cast<unsigned>(blocks), kThreads, kSmem, stream>>>(a, status);
+    return check_launch();
+}
+
+template <bool kBf16, int kD>
+int launch_typed(int fmt, const AttnArgs &a, int64_t blocks, DeviceStatus *status, cudaStream_t stream)
+{
+    if (blocks > 0) {
+        const int rc = fmt == kKvMxFp8   ? launch_pieces<kBf16, kD, kKvMxFp8>(a, blocks, status, stream)
+                       : fmt == kKvMxFp4 ? launch_pieces<kBf16, kD, kKvMxFp4>(a, blocks, status, stream)
+                                         : launch_pieces<kBf16, kD, kBf16 ? kKvBf16 : kKvF16>(a, blocks, status, stream);
+        if (rc != kOk) {
+            return rc;
+        }
+    }
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
+    prefix_attn_join_kernel<kBf16, kD><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(a);
+    return check_launch();
+}
+
+} // namespace
+
+int64_t prefix_attn_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int d, int prefix_len, int own_max)
+{
+    return make_plan(batch, tokens, heads, kv_heads, prefix_len, own_max).slots * kRows * (d * 4 + 8);
+}
+
+int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, const int64_t q_strides[3],
+                       const int32_t *prefix_pages, int prefix_len, const int32_t *table, int64_t table_stride,
+                       int table_cols, const int32_t *lens, int own_max, int batch, int tokens, int heads, float scale,
+                       uint16_t *o, float *lse, void *workspace, int64_t workspace_bytes, cudaStream_t stream)
+{
+    const Plan p = make_plan(batch, tokens, heads, cache.kv_heads, prefix_len, own_max);
+    if (workspace_bytes < p.slots * kRows * (cache.d * 4 + 8) || (p.slots > 0 && workspace == nullptr)) {
+        set_error_text("prefix_attn: the workspace is smaller than pto_b200_prefix_attn_workspace_bytes says");
+        return kErrBadArgument;
+    }
+    if (p.slots > 0x7fffffffLL) {
+        set_error_text("prefix_attn: too many rows and pieces for one call");
+        return kErrTooLarge;
+    }
+    DeviceStatus *status = device_status_ptr();
+    if (status == nullptr) {
+        return kErrCuda;
+    }
+    AttnArgs a;
+    a.k = static_cast<const uint8_t *>(cache.k);
+    a.v = static_cast<const uint8_t *>(cache.v);
+    a.ks = cache.k_scale;
+    a.vs = cache.v_scale;
+    a.q = q;
+    a.q_batch = q_strides[0];
+    a.q_token = q_strides[1];
+    a.q_head = q_strides[2];
+    a.prefix_pages = prefix_pages;
+    a.table = table;
+    a.lens = lens;
+    a.table_stride = table_stride;
+    a.num_pages = cache.num_pages;
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + p.slots * kRows * cache.d);
+    a.o = o;
+    a.lse = lse;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.table_cols = table_cols;
+    a.page_shift = cache.page_shift;
+    a.batch = batch;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.kv_heads = cache.kv_heads;
+    a.group = heads / cache.kv_heads;
+    a.prefix_len = prefix_len;
+    a.own_max = own_max;
+    a.prefix_tiles = p.prefix_tiles;
+    a.prefix_splits = p.prefix_splits;
+    a.prefix_chunk = p.prefix_chunk;
+    a.own_tiles = p.own_tiles;
+    a.own_splits = p.own_splits;
+    a.own_min = p.own_min;
+    if (cache.d == 128) {
+        return bf16 ? launch_typed<true, 128>(cache.fmt, a, p.slots, status, stream)
+                    : launch_typed<false, 128>(cache.fmt, a, p.slots, status, stream);
+    }
+    return bf16 ? launch_typed<true, 64>(cache.fmt, a, p.slots, status, stream)
+                : launch_typed<false, 64>(cache.fmt, a, p.slots, status, stream);
+}
+
+} // namespace pto_b200

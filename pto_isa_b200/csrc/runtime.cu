@@ -159,8 +159,9 @@ int fetch_device_status(cudaStream_t stream, int *record)
         record[3] = h.detail;
     }
     if (h.code != 0) {
-        set_error_text("device-side wait gave up: code %d, block %d, where %d, detail %d", h.code, h.block, h.where,
-                       h.detail);
+        set_error_text(h.code == kErrBadArgument ? "a kernel skipped an index out of range: code %d, block %d, where %d, detail %d"
+                                                 : "device-side wait gave up: code %d, block %d, where %d, detail %d",
+                       h.code, h.block, h.where, h.detail);
         cudaMemsetAsync(p, 0, 4 * sizeof(int), stream); // the four status words; the profile settings stay
     }
     return h.code;

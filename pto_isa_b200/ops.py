@@ -7,9 +7,11 @@ TROWEXPAND :1049 and TROWEXPANDSUB/MUL/DIV/ADD/MAX/MIN/EXPDIF :1057-1108, TROWMI
 and :238, TMULS :1188, TADDS :1161; `gemm` stands for
 LaunchGEMME2E (kernels/manual/a2a3/gemm_performance/gemm_performance_kernel.cpp:243) and `flash_attn_fwd` for
 LaunchTFA (kernels/manual/common/flash_atten/fa_performance_kernel.cpp:970).  A whole tensor plays the role of
-the tile: destination first is replaced by a returned (or `out=`) tensor.  Everything runs on the current
+the tile: destination first is replaced by a returned (or `out=`) tensor.  The serving operators at the end
+(kv_cache_*, prefix_attn, w4_matvec) have no counterpart in the reference.  Everything runs on the current
 CUDA stream of the tensors' device; nothing is computed by torch.
 """
+import collections
 import ctypes
 
 import torch
@@ -632,6 +634,258 @@ def flash_attn_fwd_host(q, k, v, o, causal=False, scale=None):
                                                 int(bool(causal)), scale, 1 if o.dtype == torch.float16 else 0)
     check(rc, "flash_attn_fwd_host")
     return o
+
+
+# ---- serving: paged key / value cache, attention over a shared prefix, 4-bit weights
+
+KV_F16, KV_BF16, KV_MXFP8, KV_MXFP4 = 0, 1, 2, 3
+_DTYPE16 = {torch.float16: 2, torch.bfloat16: 4}  # PTO_B200_DTYPE_F16 / _BF16
+_KV_DTYPE = {KV_F16: torch.float16, KV_BF16: torch.bfloat16}
+
+
+class KVCache(collections.namedtuple("KVCache", "k v k_scale v_scale fmt")):
+    """A paged key / value cache.  k, v: (num_pages, kv_heads, page_size, head_dim) float16 / bfloat16 (KV_F16, KV_BF16),
+    or uint8 codes: float8_e4m3fn bytes (KV_MXFP8), or float4_e2m1 two a byte, the lower index in the low nibble, head_dim / 2
+    wide (KV_MXFP4); k_scale, v_scale: (num_pages, kv_heads, page_size, head_dim / 32) float8_e8m0 bytes, None for the
+    16-bit formats.  page_size is a power of two from 16 to 1024, head_dim 64 or 128.  The functions that take a cache
+    take any 5-tuple of this order; the tensors may be of torch's 8-bit float types as well."""
+    __slots__ = ()
+
+
+class _CacheStruct(ctypes.Structure):  # pto_b200_kv_cache
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("format", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+def kv_cache_empty(num_pages, kv_heads, page_size, head_dim, fmt=KV_MXFP8, device="cuda"):
+    """A KVCache of uninitialised memory: what was not written through kv_cache_write is not to be read."""
+    if fmt not in (KV_F16, KV_BF16, KV_MXFP8, KV_MXFP4):
+        raise PtoB200Error(f"kv_cache_empty: unknown cache format {fmt}")
+    if head_dim not in (64, 128) or page_size not in (16, 32, 64, 128, 256, 512, 1024) or kv_heads < 1 or num_pages < 0:
+        raise PtoB200Error("kv_cache_empty: head_dim is 64 or 128, page_size a power of two from 16 to 1024")
+    shape = (num_pages, kv_heads, page_size)
+    if fmt in _KV_DTYPE:
+        return KVCache(*(torch.empty(*shape, head_dim, dtype=_KV_DTYPE[fmt], device=device) for _ in range(2)), None, None, fmt)
+    width = head_dim if fmt == KV_MXFP8 else head_dim // 2
+    return KVCache(*(torch.empty(*shape, width, dtype=torch.uint8, device=device) for _ in range(2)),
+                   *(torch.empty(*shape, head_dim // 32, dtype=torch.uint8, device=device) for _ in range(2)), fmt)
+
+
+def _cache_struct(cache, what):
+    """The cache's C description after its checks, and (num_pages, kv_heads, page_size, head_dim)."""
+    k, v, k_scale, v_scale, fmt = cache
+    if fmt not in (KV_F16, KV_BF16, KV_MXFP8, KV_MXFP4):
+        raise PtoB200Error(f"{what}: unknown cache format {fmt}")
+    mx = fmt >= KV_MXFP8
+    if mx:
+        if k_scale is None or v_scale is None:
+            raise PtoB200Error(f"{what}: an MX cache needs its scales")
+        _need_cuda(k, v, k_scale, v_scale)
+        _same_device(what, k, v, k_scale, v_scale)
+    else:
+        if k_scale is not None or v_scale is not None:
+            raise PtoB200Error(f"{what}: a 16-bit cache has no scales")
+        _need_cuda(k, v)
+        _same_device(what, k, v)
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or k.dtype != v.dtype:
+        raise PtoB200Error(f"{what}: k and v of the cache are (num_pages, kv_heads, page_size, row) of one type")
+    pages, heads, page_size, row = shape
+    if (k.dtype.itemsize != 1) if mx else (k.dtype != _KV_DTYPE[fmt]):
+        raise PtoB200Error(f"{what}: the cache's tensors do not have the type of its format")
+    d = row * 2 if fmt == KV_MXFP4 else row
+    if d not in (64, 128) or page_size not in (16, 32, 64, 128, 256, 512, 1024):
+        raise PtoB200Error(f"{what}: head_dim is 64 or 128 and page_size a power of two from 16 to 1024, got {d} and {page_size}")
+    if mx:
+        want = (pages, heads, page_size, d // 32)
+        if k_scale.shape != want or v_scale.shape != want or k_scale.dtype.itemsize != 1 or v_scale.dtype.itemsize != 1:
+            raise PtoB200Error(f"{what}: the cache's scales are {want} bytes")
+    return _CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if mx else None, v_scale.data_ptr() if mx else None,
+                        pages, fmt, heads, page_size, d), pages, heads, page_size, d
+
+
+def _index_vector(t, n, what, name):
+    _need_cuda(t)
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise PtoB200Error(f"{what}: {name} is an int32 vector" + ("" if n is None else f" of {n}"))
+
+
+def _page_table(t, batch, what):
+    if not t.is_cuda and batch:
+        _need_cuda(t)
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != batch or (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+        raise PtoB200Error(f"{what}: the page table is (batch, pages) int32 with contiguous rows")
+
+
+def _rows16(t, dims, what, name):
+    """A 16-bit tensor whose last dimension is contiguous and whose rows start on 16 bytes."""
+    if not t.is_cuda:
+        _need_cuda(t)
+    if t.dtype not in _DTYPE16:
+        raise PtoB200Error(f"{what}: {name} is float16 or bfloat16")
+    if t.dim() != dims:
+        raise PtoB200Error(f"{what}: {name} has {dims} dimensions")
+    if (t.shape[-1] > 1 and t.stride(-1) != 1) or t.data_ptr() & 15 or any(s & 7 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        raise PtoB200Error(f"{what}: {name}'s last dimension must be contiguous and its rows 16-byte aligned")
+
+
+def _strides(t):
+    """Strides of the leading dimensions; those of extent 1 are never taken and may be anything."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+
+
+def kv_cache_write(cache, k, v, slots):
+    """Writes rows k, v (tokens, kv_heads, head_dim), float16 or bfloat16 (a 16-bit cache: its own type), to the positions
+    slots (tokens,) int32, slot = page * page_size + offset; a negative slot is skipped, the others have to be distinct.
+    k and v may be slices of a fused projection's output (any strides with contiguous, 16-byte aligned rows).
+    MX formats: per 32 elements the smallest power of two at which none saturates (2^119 at most for fp8, 2^125 for fp4),
+    elements rounded to nearest even; a block that holds a NaN or an infinity reads back as NaN.  A slot beyond the cache is
+    skipped and reported by device_status().  Returns the cache."""
+    c, _, heads, _, d = _cache_struct(cache, "kv_cache_write")
+    _rows16(k, 3, "kv_cache_write", "k")
+    _rows16(v, 3, "kv_cache_write", "v")
+    if k.shape != v.shape or k.shape[1] != heads or k.shape[2] != d or k.dtype != v.dtype:
+        raise PtoB200Error(f"kv_cache_write: k and v are (tokens, {heads}, {d}) of one type")
+    if c.format in _KV_DTYPE and k.dtype != _KV_DTYPE[c.format]:
+        raise PtoB200Error("kv_cache_write: a 16-bit cache takes rows of its own type")
+    _index_vector(slots, k.shape[0], "kv_cache_write", "slots")
+    _same_device("kv_cache_write", cache[0], k, v, slots)
+    strides = (ctypes.c_int64 * 4)(*_strides(k), *_strides(v))
+    with torch.cuda.device(k.device):
+        rc = lib().pto_b200_kv_cache_write(ctypes.byref(c), k.data_ptr(), v.data_ptr(), _DTYPE16[k.dtype], slots.data_ptr(),
+                                           k.shape[0], strides, _stream(k))
+    check(rc, "kv_cache_write")
+    return cache
+
+
+def kv_cache_read(cache, page_table, seq_lens, max_len, dtype=torch.float16, out=None):
+    """Reads sequences back: (k, v), each (batch, kv_heads, max_len, head_dim) of `dtype`, the layout flash_attn_fwd takes.
+    Position t of sequence b comes from page page_table[b, t // page_size] ((batch, pages) int32) for t < seq_lens[b] ((batch,)
+    int32) and is zero from there on.  Values are rounded to `dtype` once (overflow to infinity); `out`: a pair of tensors."""
+    c, _, heads, _, d = _cache_struct(cache, "kv_cache_read")
+    if dtype not in _DTYPE16:
+        raise PtoB200Error("kv_cache_read: dtype is float16 or bfloat16")
+    batch, max_len = seq_lens.shape[0] if seq_lens.dim() == 1 else -1, int(max_len)
+    _index_vector(seq_lens, None, "kv_cache_read", "seq_lens")
+    _page_table(page_table, batch, "kv_cache_read")
+    _same_device("kv_cache_read", cache[0], page_table, seq_lens)
+    if max_len < 0:
+        raise PtoB200Error("kv_cache_read: max_len is negative")
+    dev = cache[0].device
+    outs = [_out(o, (batch, heads, max_len, d), dtype, dev, "kv_cache_read") for o in ((None, None) if out is None else out)]
+    with torch.cuda.device(dev):
+        rc = lib().pto_b200_kv_cache_read(ctypes.byref(c), page_table.data_ptr(), page_table.stride(0) if batch > 1 else 0,
+                                          page_table.shape[1], seq_lens.data_ptr(), batch, max_len, outs[0].data_ptr(),
+                                          outs[1].data_ptr(), _DTYPE16[dtype], _stream(cache[0]))
+    check(rc, "kv_cache_read")
+    return tuple(outs)
+
+
+def prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale=None, max_seq_len=None, out=None,
+                return_lse=False, workspace=None):
+    """Attention of a batch whose sequences share a prefix, over a paged cache; the prefix's keys are read once for all.
+
+    q: (batch, tokens, heads, head_dim), or (batch, heads, head_dim) for one token each, float16 or bfloat16 (a 16-bit
+    cache: its own type); heads a multiple of the cache's kv_heads.  prefix_pages: int32 vector, the pages of the prefix's
+    prefix_len positions (a host int, may be 0).  page_table (batch, pages) and seq_lens (batch,) int32: the positions of each
+    sequence after the prefix, its `tokens` query tokens the last of them: query token j sees the prefix and the first
+    seq_lens[b] - (tokens - 1 - j) own positions.  max_seq_len: a bound of seq_lens (default: what the table covers); a
+    tight one makes better pieces.
+    Returns O like q, zeros for a row without any key; with return_lse also the natural logarithm of the sum of
+    exponentials, float32 of q's shape without head_dim, -inf for such a row.  `workspace`: a CUDA byte tensor of at least
+    prefix_attn_workspace_bytes(...), 16-byte aligned; without it one is taken from torch's allocator per call."""
+    c, _, kv_heads, page_size, d = _cache_struct(cache, "prefix_attn")
+    single = q.dim() == 3
+    q4 = q.unsqueeze(1) if single else q
+    _rows16(q4, 4, "prefix_attn", "q")
+    batch, tokens, heads = q4.shape[:3]
+    if q4.shape[3] != d or heads < 1 or heads % kv_heads or tokens < 1:
+        raise PtoB200Error(f"prefix_attn: q is (batch, tokens, heads, {d}) with heads a multiple of {kv_heads}")
+    if c.format in _KV_DTYPE and q.dtype != _KV_DTYPE[c.format]:
+        raise PtoB200Error("prefix_attn: a 16-bit cache takes queries of its own type")
+    prefix_len = int(prefix_len)
+    _index_vector(prefix_pages, None, "prefix_attn", "prefix_pages")
+    if prefix_len < 0 or prefix_len > prefix_pages.shape[0] * page_size:
+        raise PtoB200Error("prefix_attn: prefix_len must lie within prefix_pages")
+    _index_vector(seq_lens, batch, "prefix_attn", "seq_lens")
+    _page_table(page_table, batch, "prefix_attn")
+    covered = page_table.shape[1] * page_size
+    max_seq_len = covered if max_seq_len is None else int(max_seq_len)
+    if max_seq_len < 0 or max_seq_len > covered:
+        raise PtoB200Error("prefix_attn: max_seq_len must lie within the page table")
+    _same_device("prefix_attn", q, cache[0], prefix_pages, page_table, seq_lens)
+    dev = q.device
+    o = _out(out, q.shape, q.dtype, dev, "prefix_attn")
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
+    if batch:
+        need = lib().pto_b200_prefix_attn_workspace_bytes(batch, tokens, heads, kv_heads, d, prefix_len, max_seq_len)
+        if workspace is None:  # from the allocator on every call: two captured graphs, or two streams, never share one
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        else:
+            _need_cuda(workspace)
+            _same_device("prefix_attn", q, workspace)
+            if workspace.numel() * workspace.element_size() < need:
+                raise PtoB200Error(f"prefix_attn: the workspace needs {need} bytes")
+        strides = (ctypes.c_int64 * 3)(*_strides(q4))
+        with torch.cuda.device(dev):
+            rc = lib().pto_b200_prefix_attn(ctypes.byref(c), q.data_ptr(), _DTYPE16[q.dtype], strides, prefix_pages.data_ptr(),
+                                            prefix_len, page_table.data_ptr(), page_table.stride(0) if batch > 1 else 0,
+                                            page_table.shape[1], seq_lens.data_ptr(), max_seq_len, batch, tokens, heads,
+                                            (1.0 / d ** 0.5) if scale is None else float(scale), o.data_ptr(),
+                                            lse.data_ptr() if return_lse else None, workspace.data_ptr(),
+                                            workspace.numel() * workspace.element_size(), _stream(q))
+        check(rc, "prefix_attn")
+    return (o, lse) if return_lse else o
+
+
+def prefix_attn_workspace_bytes(batch, tokens, heads, kv_heads, head_dim, prefix_len, max_seq_len):
+    """Bytes of workspace that prefix_attn needs for these extents."""
+    return lib().pto_b200_prefix_attn_workspace_bytes(batch, tokens, heads, kv_heads, head_dim, prefix_len, max_seq_len)
+
+
+def w4_matvec(x, w, scale, zero=None, out_dtype=None, out=None):
+    """y (m, n) = x (m, k) @ W (n, k)^T for a few rows (m <= 64) of float16 or bfloat16 x and 4-bit weights w (n, k / 2) uint8,
+    two codes a byte, the lower k in the low nibble.  scale (n, k / group):
+      one byte each, group 32: MX fp4, W = e2m1(code) * 2^(scale - 127), mx_gemm_fp4's operand b;
+      of x's type, group 32, 64 or 128: int4, W = scale * (code - zero), zero like scale, 8 when None.
+    A 1-D x is one row and gives a 1-D y.  y is of x's type, or float32 with out_dtype=torch.float32."""
+    vector = x.dim() == 1
+    x2 = x.unsqueeze(0) if vector else x
+    _rows16(x2, 2, "w4_matvec", "x")
+    _need_cuda(w, scale)
+    m, k = x2.shape
+    if w.dim() != 2 or w.dtype.itemsize != 1 or w.shape[1] * 2 != k:
+        raise PtoB200Error(f"w4_matvec: w is (n, {k // 2}) bytes")
+    n = w.shape[0]
+    if m > 64:
+        raise PtoB200Error("w4_matvec: at most 64 rows of x (more rows: the GEMMs)")
+    if scale.dim() != 2 or scale.shape[0] != n or scale.shape[1] < 1 or k % scale.shape[1]:
+        raise PtoB200Error(f"w4_matvec: scale is ({n}, {k} / group)")
+    group = k // scale.shape[1]
+    mx = scale.dtype.itemsize == 1
+    if mx:
+        if group != 32 or zero is not None:
+            raise PtoB200Error("w4_matvec: MX fp4 weights have one scale byte per 32 k and no zeros")
+    else:
+        if scale.dtype != x.dtype or group not in (32, 64, 128):
+            raise PtoB200Error("w4_matvec: int4 weights have scales of x's type, one per 32, 64 or 128 k")
+        if zero is not None:
+            _need_cuda(zero)
+            if zero.shape != scale.shape or zero.dtype != scale.dtype:
+                raise PtoB200Error("w4_matvec: zero is like scale")
+            _same_device("w4_matvec", x, zero)
+    _same_device("w4_matvec", x, w, scale)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype != x.dtype and out_dtype != torch.float32:
+        raise PtoB200Error("w4_matvec: the output is of x's type or float32")
+    y = _out(out, (n,) if vector else (m, n), out_dtype, x.device, "w4_matvec")
+    with torch.cuda.device(x.device):
+        rc = lib().pto_b200_w4_matvec(x.data_ptr(), x2.stride(0) if m > 1 else 0, w.data_ptr(), scale.data_ptr(),
+                                      None if zero is None else zero.data_ptr(), y.data_ptr(), m, n, k, group, 0 if mx else 1,
+                                      _DTYPE16[x.dtype], 1 if out_dtype == torch.float32 else 0, _stream(x))
+    check(rc, "w4_matvec")
+    return y
 
 
 def device_status(device=None):
