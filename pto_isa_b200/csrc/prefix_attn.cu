@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                             w[i] = e2m1_pair<kBf16>((v >> (8 * i)) & 0xffu);
                         }
                     }
-                    float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_16816<kBf16>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
+                    float p[4];
+                    mma_16816_first<kBf16>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
                     mma_16816<kBf16>(p, qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
                     const float f0 = __uint_as_float(((sc[0] >> (8 * kb)) & 0xffu) << 23);
                     const float f1 = __uint_as_float(((sc[1] >> (8 * kb)) & 0xffu) << 23);

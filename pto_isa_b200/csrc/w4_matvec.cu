@@ -2,14 +2,25 @@
 //
 //   MX fp4   W = e2m1(code) 2^(byte - 127), one scale byte per 32 k: the weights of the MX fp4 GEMM, byte for byte
 //   int4     W = s (code - z), code 0 .. 15, one 16-bit s (and z; 8 without) per group of 32, 64 or 128 k
-// two codes a byte, the lower k in the low nibble.  The sum of a group is taken on the codes (exact in 16 bits, fp32
-// accumulation on the tensor core) and scaled once:  y += s_group * (sum over the group of (code - z) x).
+// two codes a byte, the lower k in the low nibble.  The sum of 32 k is taken on the codes, exactly representable in
+// float16, by the tensor core with fp32 accumulation, and scaled afterwards:
+//   y += 2^E s (sum (code) x' - z sum x'),   x = 2^E x'
+// x' is x in float16.  float16 rows go in as they are (E = 0).  bfloat16 rows have float16's precision and more range,
+// so each run of 256 gets the power of two that brings its largest element into [2^14, 2^15): every element down to
+// 2^-31 of the largest keeps all its bits, below that the error is at most 2^-40 of the largest, far under the
+// rounding of the fp32 sum.  Weights go through float16 because one conversion instruction turns two e2m1 codes into a
+// float16 pair, and an int4 code is the float16 subnormal code * 2^-24 after one mask; to bfloat16 both take three to
+// four half-rate integer operations a pair.
 //
-// Bound by HBM: n k / 2 bytes of weights are read once, everything else is small.  A block owns 16 * kRt rows of W and its
-// eight warps share the k axis, each with a cp.async ring of its own (256 k = 128 bytes of every row a stage), so that no
-// warp waits for another before the sums are joined.  Weights are the 16-row operand of mma.m16n8k16, the rows of x its
-// eight columns.  The order of k inside a group of 32 is free as long as both operands agree: lane t of a quad takes
-// k = 8t .. 8t + 7 (one 32-bit word of codes), paired (i, i + 4), so that one shift and one mask give a pair.
+// Bound by HBM: n k / 2 bytes of weights are read once, everything else is small.  Weights are the 16-row operand of
+// mma.m16n8k16, the rows of x its eight columns; the order of k inside 32 is free as long as both operands agree: lane t
+// of a quad takes k = 8t .. 8t + 7 (one word of codes).  The rows of W are dealt out evenly, to the row, over as many
+// blocks as are resident; two kernels:
+//   resident  all of x fits beside the ring of two blocks an SM (m k up to about 21 000): x is prepared once a block; the
+//             eight warps share the k axis, each with a cp.async ring of its own that runs on across the block's row
+//             tiles, so that no warp waits for another but once a tile, where the shares of k are joined.
+//   streamed  x comes in pieces of 256 k, prepared by the whole block an iteration ahead; kWr of the warps lie along the
+//             rows of W (x is read from L2 once for all of them), 8 / kWr share the k axis.
 #include "ptx.cuh"
 #include "internal.h"
 #include "mx_format.cuh"
@@ -20,240 +31,726 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStepK = 256;               // k a warp takes at a time
-constexpr int kStepBytes = kStepK / 2;    // bytes of a row of W in a stage
-constexpr int kPitch = kStepBytes + 16;   // 8 rows x 4 words of a quad's reads meet 32 distinct banks
-constexpr int kStages = 3;
+constexpr int kStepK = 256;              // k of one warp's step
+constexpr int kStepBytes = kStepK / 2;   // bytes of a row of W in a step
+constexpr int kPitch = kStepBytes + 16;  // 8 rows x 4 words of a quad's reads meet 32 distinct banks
+constexpr int kNarrowPitch = kStepBytes;  // odd rows with their 64-byte halves exchanged: two rows x 4 lanes of a 16-byte read
+constexpr int kXPitch = kStepK * 2 + 64; // two rows x 4 lanes of a 16-byte read phase likewise
+constexpr int kStages = 3;               // of the streamed kernel's ring
+constexpr int kResidentStages = 3;       // of a warp's ring in the resident kernel
+constexpr int kResidentSmem = 112 * 1024; // two blocks an SM
+constexpr int kNarrowSmem = 75 * 1024;    // three
+constexpr int kSms = 148;
 
 struct W4Args {
     const uint16_t *x;
     const uint8_t *w;
-    const void *scale;
-    const uint16_t *zero;
+    const uint8_t *scale;
+    const uint8_t *zero;
     void *y;
     int64_t x_stride;
-    int m, n, k, group_shift, out_f32;
+    int m, n, k, group_shift, out_f32, out_bf16;
+    int rows_each, rows_more; // rows of W a block owns; the first rows_more blocks one more
+    int scale_async; // the scales of a step are 4, 8 or 16 aligned bytes a row: they ride in the ring
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes)
+// bytes global -> shared, 4, 8 or 16, zeros where not live
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int size, bool live)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    const int n = live ? size : 0;
+    if (size == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    } else if (size == 8) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    } else {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    }
 }
 
-// the four pairs (code i, code i + 4) of a word of eight codes, as 16-bit values
-template <bool kBf16, bool kMx>
-__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&p)[4])
+// eight e2m1 codes -> four float16 pairs (codes 2i, 2i + 1)
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&p)[4])
 {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
+        : "r"(w));
+}
+
+// eight int4 codes as float16 subnormals: codes (0, 4) and (2, 6) times 2^-24, codes (1, 5) and (3, 7) times 2^-20
+__device__ __forceinline__ void int4x8_to_f16(uint32_t w, uint32_t (&p)[4])
+{
+    p[0] = w & 0x000f000fu;
+    p[1] = (w >> 8) & 0x000f000fu;
+    p[2] = w & 0x00f000f0u;
+    p[3] = (w >> 8) & 0x00f000f0u;
+}
+
+// Where a prepared run of 256 k of x lies: x_rows rows of kXPitch bytes, then per row 8 sums of x' (int4) and the factor
+// 2^E (bfloat16), 36 bytes.  x_rows is m, and one row of zeros for the columns past it unless m fills the tiles.
+constexpr int kXRow = kXPitch + 36;
+
+// One warp prepares row `row`, k run `run` of x: eight elements a lane.
+template <bool kBf16, bool kMx>
+__device__ __forceinline__ void prepare_run(uint4 in, uint8_t *at, int x_rows, int row, int lane)
+{
+    uint32_t v[4] = {in.x, in.y, in.z, in.w};
+    float *side = reinterpret_cast<float *>(at + x_rows * kXPitch) + row * 9;
+    if constexpr (kBf16) {
+        float2 f[4];
+        float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {
+            f[i] = unpack_16x2<true>(v[i]);
+            top = fmaxf(top, fmaxf(fabsf(f[i].x), fabsf(f[i].y)));
+        }
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))); // not negative: ordered as integers
+        // E = exponent of top - 14, kept where 2^E and 2^-E are normal numbers: -112 .. 113
+        const int field = min(max(static_cast<int>(__float_as_uint(top) >> 23), 29), 254);
+        const float inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = pack_16x2<false>(f[i].x * inv, f[i].y * inv);
+        }
+        if (lane == 0) {
+            side[8] = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
+        }
+    }
+    if constexpr (!kMx) { // sums of x' over runs of 32, for the zero points
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack_16x2<false>(v[i]);
+            sum += f.x + f.y;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if ((lane & 3) == 0) {
+            side[lane >> 2] = sum;
+        }
+        // codes (i, i + 4) share a mask: k order (0, 4) (2, 6) (1, 5) (3, 7)
+        const uint32_t y0 = v[0], y1 = v[1], y2 = v[2], y3 = v[3];
+        v[0] = __byte_perm(y0, y2, 0x5410);
+        v[1] = __byte_perm(y1, y3, 0x5410);
+        v[2] = __byte_perm(y0, y2, 0x7632);
+        v[3] = __byte_perm(y1, y3, 0x7632);
+    }
+    *reinterpret_cast<uint4 *>(at + row * kXPitch + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// where a lane finds its row of x in a prepared run, and the sums and factor of its columns of the result
+template <int kMt>
+struct LaneX {
+    int row[kMt], col[kMt][2];
+    __device__ __forceinline__ LaneX(int x_rows, int g, int t)
+    {
+#pragma unroll
+        for (int c = 0; c < kMt; ++c) {
+            row[c] = min(8 * c + g, x_rows - 1) * kXPitch + 16 * t;
+            col[c][0] = x_rows * kXPitch + min(8 * c + 2 * t, x_rows - 1) * 36;
+            col[c][1] = x_rows * kXPitch + min(8 * c + 2 * t + 1, x_rows - 1) * 36;
+        }
+    }
+};
+
+// 16 rows of W times the prepared run at `xs`: acc += .  `ws`: the lane's first word of the run's codes (row g, word t),
+// `ss`, `zs`: the run's scales and zeros of row g (rows 16 bytes apart); blks: runs of 32 that exist.
+template <bool kBf16, bool kMx, int kMt>
+__device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t *ws, const uint8_t *ss, const uint8_t *zs,
+                                            const uint8_t *xs, const LaneX<kMt> &lx, int group_shift, bool zero, int blks)
+{
+    float f[kMt][2]; // 2^E of the lane's columns
+#pragma unroll
+    for (int c = 0; c < kMt; ++c) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            f[c][j] = kBf16 ? *reinterpret_cast<const float *>(xs + lx.col[c][j] + 32) : 1.0f;
+        }
+    }
+    uint2 sv[2];
+    if constexpr (kMx) {
+        sv[0] = *reinterpret_cast<const uint2 *>(ss);
+        sv[1] = *reinterpret_cast<const uint2 *>(ss + 128);
+    }
+    auto block = [&](int blk) {
+        const uint32_t w0 = ws[blk * 4], w1 = ws[blk * 4 + 8 * kPitch / 4];
+        float s[2], z[2] = {8.0f, 8.0f};
+        uint32_t lo[4], hi[4];
         if constexpr (kMx) {
-            // sign to the top of each half, exponent and mantissa below it; the value is the code's times 2^-14 (float16:
-            // exact even where subnormal, undone at the end) or 2^-126 (bfloat16: undone here, fp32 sums would underflow)
-            const uint32_t top = i == 3 ? w : w << (4 * (3 - i));
-            if constexpr (kBf16) {
-                p[i] = mul_16x2<true>((top & 0x80008000u) | ((top >> 6) & 0x01c001c0u), 0x7e807e80u);
-            } else {
-                p[i] = (top & 0x80008000u) | ((top >> 3) & 0x0e000e00u);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t v = (blk & 4) ? sv[i].y : sv[i].x;
+                s[i] = __uint_as_float(((v >> (8 * (blk & 3))) & 0xffu) << 23);
+                s[i] = fmaf(s[i], 0.0f, s[i]); // 255: infinity times 0 plus itself is NaN; 0 stands for 0, not 2^-127
             }
-        } else if constexpr (kBf16) {
-            // 0x4300 | code = 128 + code; minus 136 = code - 8, exact
-            const uint32_t v = ((i == 0 ? w : w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-            asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v), "r"(0x43084308u));
+            e2m1x8_to_f16(w0, lo);
+            e2m1x8_to_f16(w1, hi);
         } else {
-            // 0x6400 | code = 1024 + code; minus 1032 = code - 8, exact
-            const uint32_t v = ((i == 0 ? w : w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-            asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v), "r"(0x64086408u));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = i * 128 + (blk >> (group_shift - 5)) * 2;
+                s[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(ss + at)).x ;
+                if (zero) {
+                    z[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(zs + at)).x;
+                }
+            }
+            int4x8_to_f16(w0, lo);
+            int4x8_to_f16(w1, hi);
+        }
+#pragma unroll
+        for (int c = 0; c < kMt; ++c) {
+            const uint4 xf = *reinterpret_cast<const uint4 *>(xs + lx.row[c] + blk * 64);
+            float d[4];
+            mma_16816_first<false>(d, lo[0], hi[0], lo[1], hi[1], xf.x, xf.y);
+            if constexpr (kMx) {
+                mma_16816<false>(d, lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+            } else {
+                float e[4];
+                mma_16816_first<false>(e, lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+                const float u[2] = {*reinterpret_cast<const float *>(xs + lx.col[c][0] + blk * 4),
+                                    *reinterpret_cast<const float *>(xs + lx.col[c][1] + blk * 4)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    d[i] = fmaf(d[i], 16777216.0f, fmaf(e[i], 1048576.0f, -z[i >> 1] * u[i & 1]));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // 2^E before the scale: no product leaves fp32's range that x and W keep in it
+                acc[c][i] = fmaf(kBf16 ? d[i] * f[c][i & 1] : d[i], s[i >> 1], acc[c][i]);
+            }
+        }
+    };
+    if (blks >= kStepK / 32) {
+#pragma unroll
+        for (int blk = 0; blk < kStepK / 32; ++blk) {
+            block(blk);
+        }
+    } else {
+#pragma unroll 1
+        for (int blk = 0; blk < blks; ++blk) {
+            block(blk);
         }
     }
 }
 
-// kRt: tiles of 16 rows of W a block owns; kMt: tiles of 8 rows of x
-template <bool kBf16, bool kMx, bool kZero, int kRt, int kMt>
-__global__ void __launch_bounds__(kThreads) w4_matvec_kernel(const __grid_constant__ W4Args a)
+// The same for one or two rows of x.  Of the product's eight columns, columns 0 .. 3 take the four groups of 32 of half a
+// run for the first row of x, columns 4 .. 7 for the second: lane t of a quad feeds group t (16 consecutive bytes of codes,
+// one shared-memory read), and the x operand of column c is zero but in the k places of lane c mod 4.  So a column sums one
+// group over eight products, and scales are applied once per 128 k where the wide form does so per 32: 17 instead of about
+// 50 instructions per 32 k and 16 rows of W (8192 x 8192, one row: 17.1 us in the wide form).
+// ws: row g, 16 bytes 16 t; odd: 64 in odd rows, whose halves are exchanged; acc: rows g and g + 8, the lane's two groups; xs: x of group t, or zeros; side: sums and 2^E of
+// x row t / 2
+template <bool kBf16, bool kMx>
+__device__ __forceinline__ void run_product_narrow(float (&acc)[2], const uint8_t *ws, const uint8_t *ss, const uint8_t *zs,
+                                                   const uint8_t *xs, const float *side, int group_shift, bool zero, int t, int odd)
+{
+    const float f = kBf16 ? side[8] : 1.0f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const uint4 a4 = *reinterpret_cast<const uint4 *>(ws + ((half * 64) ^ odd)), b4 = *reinterpret_cast<const uint4 *>(ws + ((half * 64) ^ odd) + 8 * kNarrowPitch);
+        const uint32_t wa[4] = {a4.x, a4.y, a4.z, a4.w}, wb[4] = {b4.x, b4.y, b4.z, b4.w};
+        float d[4], e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t lo[4], hi[4];
+            if constexpr (kMx) {
+                e2m1x8_to_f16(wa[j], lo);
+                e2m1x8_to_f16(wb[j], hi);
+            } else {
+                int4x8_to_f16(wa[j], lo);
+                int4x8_to_f16(wb[j], hi);
+            }
+            const uint4 xf = *reinterpret_cast<const uint4 *>(xs + half * 256 + j * 16);
+            if (j == 0) {
+                mma_16816_first<false>(d, lo[0], hi[0], lo[1], hi[1], xf.x, xf.y);
+                mma_16816_first<false>(e, lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+            } else {
+                mma_16816<false>(d, lo[0], hi[0], lo[1], hi[1], xf.x, xf.y);
+                mma_16816<false>(e, lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+            }
+        }
+        // the lane's columns: groups 2 (t mod 2) and + 1 of this half
+        const int blk = half * 4 + (t & 1) * 2;
+        float s[2][2], z[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (kMx) {
+                const uint32_t v = *reinterpret_cast<const uint16_t *>(ss + i * 128 + blk);
+                s[i][0] = __uint_as_float((v & 0xffu) << 23);
+                s[i][1] = __uint_as_float((v >> 8) << 23);
+                s[i][0] = fmaf(s[i][0], 0.0f, s[i][0]); // 255: infinity times 0 plus itself is NaN; 0 stands for 0, not 2^-127
+                s[i][1] = fmaf(s[i][1], 0.0f, s[i][1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int at = i * 128 + ((blk + j) >> (group_shift - 5)) * 2;
+                    s[i][j] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(ss + at)).x;
+                    z[i][j] = zero ? unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(zs + at)).x : 8.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v;
+            if constexpr (kMx) {
+                v = d[i] + e[i];
+            } else {
+                v = fmaf(d[i], 16777216.0f, fmaf(e[i], 1048576.0f, -z[i >> 1][i & 1] * side[blk + (i & 1)]));
+            }
+            acc[i >> 1] = fmaf(kBf16 ? v * f : v, s[i >> 1][i & 1], acc[i >> 1]);
+        }
+    }
+}
+
+// row of zeros (with its sums and factor) of one run
+__device__ __forceinline__ void clear_last_row(uint8_t *at, int x_rows, int thread, int threads)
+{
+    for (int i = thread; i < kXPitch / 16 + 9; i += threads) {
+        if (i < kXPitch / 16) {
+            *reinterpret_cast<uint4 *>(at + (x_rows - 1) * kXPitch + i * 16) = make_uint4(0, 0, 0, 0);
+        } else {
+            reinterpret_cast<float *>(at + x_rows * kXPitch)[(x_rows - 1) * 9 + i - kXPitch / 16] = 0.0f;
+        }
+    }
+}
+
+// the scales (or zeros) of one row in one step, to a 16-byte slot
+__device__ __forceinline__ void load_scales(uint32_t dst, const uint8_t *row, int64_t first, int64_t row_bytes, int bytes, bool live, bool async)
+{
+    if (async) { // k a multiple of 256: a step's scales are whole and aligned
+        live = live && first < row_bytes;
+        cp_async(dst, live ? row + first : row, bytes, live);
+    } else { // any k: byte by byte
+        for (int i = 0; i < bytes; ++i) {
+            const uint32_t v = live && first + i < row_bytes ? row[first + i] : 0u;
+            asm volatile("st.shared.u8 [%0], %1;" ::"r"(dst + i), "r"(v) : "memory");
+        }
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void store_y(const W4Args &a, int64_t at, float v)
+{
+    if (a.out_f32) {
+        static_cast<float *>(a.y)[at] = v;
+    } else {
+        static_cast<uint16_t *>(a.y)[at] = static_cast<uint16_t>(pack_16x2<kBf16>(v, 0.0f));
+    }
+}
+
+// ------------------------------------------------------------------ resident x
+
+// kMt: column tiles, 0 = the narrow form for one or two rows of x
+template <bool kMx, int kMt>
+__host__ __device__ constexpr int resident_stage_bytes()
+{
+    return 16 * (kMt == 0 ? kNarrowPitch : kPitch) + (kMx ? 1 : 2) * 256;
+}
+
+template <int kMt>
+__host__ __device__ constexpr int resident_columns() // rows of x that a warp's sums have room for
+{
+    return kMt == 0 ? 2 : 8 * kMt;
+}
+
+// rows of a prepared run: m and one of zeros where columns are left over (in the narrow form always, and once for all runs)
+template <int kMt>
+__host__ __device__ int resident_x_rows(int m)
+{
+    return kMt == 0 ? m : (m < 8 * kMt ? m + 1 : m);
+}
+
+// shared memory: the warps' rings, two buffers of shares of k [8][16][columns + 1], x (all runs), the narrow form's zeros
+template <bool kMx, int kMt>
+int resident_smem(int m, int k)
+{
+    return kWarps * kResidentStages * resident_stage_bytes<kMx, kMt>() + 2 * kWarps * 16 * (resident_columns<kMt>() + 1) * 4 +
+           (k + kStepK - 1) / kStepK * ((resident_x_rows<kMt>(m) * kXRow + 15) & ~15) + (kMt == 0 ? 512 : 0);
+}
+
+template <bool kBf16, bool kMx, int kMt>
+__global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel(const __grid_constant__ W4Args a)
 {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int kStageBytes = 16 * kRt * kPitch;
+    constexpr int kStage = resident_stage_bytes<kMx, kMt>();
+    constexpr int kRowPitch = kMt == 0 ? kNarrowPitch : kPitch;
+    constexpr int kCols = resident_columns<kMt>() + 1;
+    constexpr int kShare = 16 * kCols; // floats of a warp's share of a tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16 * kRt;
+    uint8_t *ring = smem + warp * kResidentStages * kStage;
+    float *shares = reinterpret_cast<float *>(smem + kWarps * kResidentStages * kStage);
+    uint8_t *xs = smem + kWarps * kResidentStages * kStage + 2 * kWarps * kShare * 4;
+    const int x_rows = resident_x_rows<kMt>(a.m);
+    const int x_run = (x_rows * kXRow + 15) & ~15;
+    const int block = static_cast<int>(blockIdx.x);
+    const int row_begin = block * a.rows_each + min(block, a.rows_more), row_end = row_begin + a.rows_each + (block < a.rows_more ? 1 : 0);
+    const int tiles = (row_end - row_begin + 15) / 16;
     const int64_t row_bytes = a.k / 2;
-    const int groups = a.k >> a.group_shift;
-    const int steps = (a.k + kStepK - 1) / kStepK;
-    const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
+    const int64_t row_scale = static_cast<int64_t>(a.k >> a.group_shift) * (kMx ? 1 : 2);
+    const int scale_bytes = kMx ? 8 : 512 >> a.group_shift;
+    const int runs = (a.k + kStepK - 1) / kStepK;
+    const int mine = (runs - warp + kWarps - 1) / kWarps; // this warp's runs of a tile: warp, warp + 8, ..
 
-    auto load = [&](int step, int stage) {
-        if (step < steps) {
-            const uint32_t base = ring + stage * kStageBytes;
+    // what is loaded next: run `ahead_run` of tile `ahead_tile`, at `src` for this lane (row lane / 8, 16 bytes lane % 8)
+    int ahead_tile = mine > 0 ? 0 : tiles, ahead_run = warp;
+    const int64_t four_rows = 4 * row_bytes;
+    const uint8_t *src = a.w + (row_begin + (lane >> 3)) * row_bytes + warp * kStepBytes + (lane & 7) * 16;
+    const bool zeros = lane >= 16, has_scale = !zeros || (!kMx && a.zero != nullptr);
+    const uint8_t *scale_src = (zeros ? a.zero : a.scale) + (row_begin + (lane & 15)) * row_scale + warp * scale_bytes;
+    const uint32_t dst = smem_u32(ring) + (lane >> 3) * kRowPitch + (((lane & 7) * 16) ^ (kMt == 0 ? (lane & 8) * 8 : 0)), scale_dst = smem_u32(ring) + 16 * kRowPitch + lane * 16;
+    auto load_next = [&](int stage) {
+        if (ahead_tile < tiles) {
+            const int rows = row_end - row_begin - ahead_tile * 16; // of this tile
+            const uint32_t to = stage * kStage;
+            if (rows >= 16 && (ahead_run + 1) * kStepK <= a.k) {
 #pragma unroll
-            for (int i = 0; i < 4 * kRt; ++i) { // 128 chunks of 16 bytes per 16 rows
-                const int c = i * 32 + lane;
-                const int r = c >> 3, at = (c & 7) * 16;
-                const int64_t col = static_cast<int64_t>(step) * kStepBytes + at;
-                const bool live = n0 + r < a.n && col < row_bytes; // k is a multiple of 32: chunks are whole
-                cp_async16(base + r * kPitch + at, a.w + (live ? (n0 + r) * row_bytes + col : 0), live ? 16 : 0);
+                for (int i = 0; i < 4; ++i) {
+                    cp_async(dst + to + i * 4 * kRowPitch, src + i * four_rows, 16, true);
+                }
+            } else { // the end of the rows or of k (a multiple of 32: chunks are whole)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool live = i * 4 + (lane >> 3) < rows && ahead_run * kStepBytes + (lane & 7) * 16 < row_bytes;
+                    cp_async(dst + to + i * 4 * kRowPitch, live ? src + i * four_rows : a.w, 16, live);
+                }
+            }
+            if (has_scale) {
+                if (a.scale_async) { // k a multiple of 256: a step's scales are whole and aligned
+                    const bool live = (lane & 15) < rows;
+                    cp_async(scale_dst + to, live ? scale_src : a.scale, scale_bytes, live);
+                } else { // any k: byte by byte
+                    for (int i = 0; i < scale_bytes; ++i) {
+                        const uint32_t v = (lane & 15) < rows && ahead_run * scale_bytes + i < row_scale ? scale_src[i] : 0u;
+                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(scale_dst + to + i), "r"(v) : "memory");
+                    }
+                }
+            }
+            ahead_run += kWarps;
+            src += kWarps * kStepBytes;
+            scale_src += kWarps * scale_bytes;
+            if (ahead_run >= runs) {
+                ahead_run = warp;
+                ++ahead_tile;
+                src += 16 * row_bytes - static_cast<int64_t>(mine) * kWarps * kStepBytes;
+                scale_src += 16 * row_scale - static_cast<int64_t>(mine) * kWarps * scale_bytes;
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-
-    float acc[kRt][kMt][4];
+    const LaneX<kMt == 0 ? 1 : kMt> lx(x_rows, g, t);
+    // narrow form: the lane feeds column g if that is group t of a row of x that exists
+    uint8_t *nothing = xs + runs * x_run;
+    const bool feeds = (g & 3) == t && (g >> 2) < a.m;
+    const int x_at = (g >> 2) * kXPitch + t * 64, side_at = x_rows * kXPitch + min(t >> 1, a.m - 1) * 36;
 #pragma unroll
-    for (int r = 0; r < kRt; ++r) {
-#pragma unroll
-        for (int c = 0; c < kMt; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                acc[r][c][i] = 0.0f;
-            }
+    for (int s = 0; s < kResidentStages - 1; ++s) {
+        load_next(s);
+    }
+    // x: a warp prepares one row of one run at a time
+    for (int i = warp; i < runs * a.m; i += kWarps) {
+        const int run = i / a.m, row = i - run * a.m;
+        const int64_t k0 = static_cast<int64_t>(run) * kStepK + lane * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k0 < a.k) {
+            v = __ldg(reinterpret_cast<const uint4 *>(a.x + row * a.x_stride + k0));
+        }
+        prepare_run<kBf16, kMx>(v, xs + run * x_run, x_rows, row, lane);
+    }
+    if constexpr (kMt == 0) {
+        if (threadIdx.x < 32) {
+            reinterpret_cast<uint4 *>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+        }
+    } else if (x_rows > a.m) {
+        for (int run = warp; run < runs; run += kWarps) {
+            clear_last_row(xs + run * x_run, x_rows, lane, 32);
         }
     }
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        load(warp + s * kWarps, s);
-    }
+    __syncthreads();
+
     int stage = 0;
-    for (int step = warp; step < steps; step += kWarps) {
-        load(step + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-        __syncwarp();
-        const uint32_t base = ring + stage * kStageBytes;
-#pragma unroll 2
-        for (int blk = 0; blk < kStepK / 32; ++blk) {
-            const int k0 = step * kStepK + blk * 32;
-            if (k0 >= a.k) {
-                break;
+    for (int tile = 0; tile < tiles; ++tile) {
+        constexpr int kAcc = kMt == 0 ? 1 : kMt;
+        float acc[kAcc][4];
+#pragma unroll
+        for (int c = 0; c < kAcc; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[c][i] = 0.0f;
             }
-            // x: eight k of row 8c + g as pairs (i, i + 4)
-            uint32_t xf[kMt][4];
+        }
+        float narrow[2] = {0.0f, 0.0f};
+        for (int j = 0; j < mine; ++j) {
+            load_next(stage == 0 ? kResidentStages - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kResidentStages - 1) : "memory");
+            __syncwarp();
+            const uint8_t *base = ring + stage * kStage;
+            const int run = warp + j * kWarps;
+            const uint8_t *ss = base + 16 * kRowPitch + g * 16, *x = xs + run * x_run;
+            if constexpr (kMt == 0) { // codes, scales and x past the end of k are zeros: no run is short
+                run_product_narrow<kBf16, kMx>(narrow, base + g * kRowPitch + 16 * t, ss, ss + 256, feeds ? x + x_at : nothing,
+                                               reinterpret_cast<const float *>(x + side_at), a.group_shift, a.zero != nullptr, t, (g & 1) * 64);
+            } else {
+                run_product<kBf16, kMx, kMt>(acc, reinterpret_cast<const uint32_t *>(base + g * kRowPitch) + t, ss, ss + 256, x, lx,
+                                             a.group_shift, a.zero != nullptr, (a.k - run * kStepK) / 32);
+            }
+            __syncwarp(); // every lane has read the stage before it is loaded again
+            stage = stage + 1 == kResidentStages ? 0 : stage + 1;
+        }
+        // the warps' shares of k joined in a fixed order; the buffers alternate, so one barrier a tile is enough
+        float *share = shares + (tile & 1) * kWarps * kShare;
+        if constexpr (kMt == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                narrow[i] += __shfl_xor_sync(0xffffffffu, narrow[i], 1); // groups 0, 1 and 2, 3
+                if ((t & 1) == 0) {
+                    share[warp * kShare + (g + 8 * i) * kCols + (t >> 1)] = narrow[i];
+                }
+            }
+        } else {
 #pragma unroll
             for (int c = 0; c < kMt; ++c) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (8 * c + g < a.m) {
-                    v = *reinterpret_cast<const uint4 *>(a.x + (8 * c + g) * a.x_stride + k0 + 8 * t);
-                }
-                xf[c][0] = __byte_perm(v.x, v.z, 0x5410);
-                xf[c][1] = __byte_perm(v.x, v.z, 0x7632);
-                xf[c][2] = __byte_perm(v.y, v.w, 0x5410);
-                xf[c][3] = __byte_perm(v.y, v.w, 0x7632);
-            }
-            // zero points other than 8: (code - z) x = (code - 8) x + (8 - z) x, the sum of x by a product with ones
-            float xsum[kMt][2];
-            if constexpr (kZero) {
-                constexpr uint32_t kOnes = kBf16 ? 0x3f803f80u : 0x3c003c00u;
 #pragma unroll
-                for (int c = 0; c < kMt; ++c) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_16816<kBf16>(d, kOnes, kOnes, kOnes, kOnes, xf[c][0], xf[c][1]);
-                    mma_16816<kBf16>(d, kOnes, kOnes, kOnes, kOnes, xf[c][2], xf[c][3]);
-                    xsum[c][0] = d[0];
-                    xsum[c][1] = d[1];
-                }
-            }
-            const int grp = k0 >> a.group_shift;
-#pragma unroll
-            for (int r = 0; r < kRt; ++r) {
-                uint32_t lo[4], hi[4];
-                uint32_t w0, w1;
-                const uint32_t at = base + (16 * r + g) * kPitch + blk * 16 + 4 * t;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(at) : "memory");
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"(at + 8 * kPitch) : "memory");
-                codes_to_pairs<kBf16, kMx>(w0, lo);
-                codes_to_pairs<kBf16, kMx>(w1, hi);
-                float s[2], z[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int row = min(n0 + 16 * r + g + 8 * i, a.n - 1);
-                    const int64_t at_s = static_cast<int64_t>(row) * groups + grp;
-                    if constexpr (kMx) {
-                        s[i] = e8m0_value(static_cast<const uint8_t *>(a.scale)[at_s]);
-                    } else {
-                        s[i] = unpack_16x2<kBf16>(static_cast<const uint16_t *>(a.scale)[at_s]).x;
-                    }
-                    if constexpr (kZero) {
-                        z[i] = 8.0f - unpack_16x2<kBf16>(a.zero[at_s]).x;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < kMt; ++c) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_16816<kBf16>(d, lo[0], hi[0], lo[1], hi[1], xf[c][0], xf[c][1]);
-                    mma_16816<kBf16>(d, lo[2], hi[2], lo[3], hi[3], xf[c][2], xf[c][3]);
-                    if constexpr (kZero) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            d[i] = fmaf(z[i >> 1], xsum[c][i & 1], d[i]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        acc[r][c][i] = fmaf(d[i], s[i >> 1], acc[r][c][i]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    share[warp * kShare + (g + 8 * (i >> 1)) * kCols + 8 * c + 2 * t + (i & 1)] = acc[c][i];
                 }
             }
         }
-        __syncwarp();
-        stage = stage + 1 == kStages ? 0 : stage + 1;
+        __syncthreads();
+        const int n0 = row_begin + tile * 16;
+        for (int i = threadIdx.x; i < a.m * 16; i += kThreads) {
+            const int col = i >> 4, row = i & 15;
+            if (n0 + row < row_end) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    v += share[w * kShare + row * kCols + col];
+                }
+                store_y<kBf16>(a, static_cast<int64_t>(col) * a.n + n0 + row, v);
+            }
+        }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
+}
 
-    // the warps' shares of k joined in a fixed order: [warp][column of x][row of W]
-    float *sums = reinterpret_cast<float *>(smem);
-    constexpr int kN = 16 * kRt, kM = 8 * kMt;
+// ------------------------------------------------------------------ streamed x
+
+// shared memory of a stage: W [kWk][16 kWr rows][kPitch], scales and zeros [kWk][16 kWr rows][16]; x apart, two buffers of
+// kWk prepared runs; the shares of k are joined in the ring's place
+template <bool kMx, int kWr, int kMt>
+struct Layout {
+    static constexpr int kWk = kWarps / kWr;
+    static constexpr int kRows = 16 * kWr;
+    static constexpr int kW = kWk * kRows * kPitch;
+    static constexpr int kScale = kWk * kRows * 16;
+    static constexpr int kStage = kW + (kMx ? 1 : 2) * kScale;
+    static constexpr int kSums = kWk * 8 * kMt * kRows * 4;
+    static constexpr int kRing = kStages * kStage > kSums ? kStages * kStage : kSums;
+    static __host__ __device__ int x_rows(int m) { return m < 8 * kMt ? m + 1 : m; }
+    static __host__ __device__ int x_run(int m) { return (x_rows(m) * kXRow + 15) & ~15; }
+    static int smem_bytes(int m) { return kRing + 2 * kWk * x_run(m); }
+};
+
+template <bool kBf16, bool kMx, int kWr, int kMt>
+__global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel(const __grid_constant__ W4Args a)
+{
+    using L = Layout<kMx, kWr, kMt>;
+    constexpr int kWk = L::kWk;
+    constexpr int kPasses = kMt * kWk; // rows times runs of an iteration, by the eight warps
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int wr = warp % kWr, wk = warp / kWr;
+    const int block = static_cast<int>(blockIdx.x);
+    const int row_begin = block * a.rows_each + min(block, a.rows_more), row_end = row_begin + a.rows_each + (block < a.rows_more ? 1 : 0);
+    const int64_t row_bytes = a.k / 2;
+    const int64_t row_scale = static_cast<int64_t>(a.k >> a.group_shift) * (kMx ? 1 : 2);
+    const int iters = (a.k + kStepK * kWk - 1) / (kStepK * kWk);
+    const int x_rows = L::x_rows(a.m), x_run = L::x_run(a.m);
+    const int scale_bytes = kMx ? 8 : 512 >> a.group_shift; // of a row in a step
+    uint8_t *xbuf = smem + L::kRing;
+    const LaneX<kMt> lx(x_rows, g, t);
+    if (x_rows > a.m) {
+        for (int i = warp; i < 2 * kWk; i += kWarps) {
+            clear_last_row(xbuf + i * x_run, x_rows, lane, 32);
+        }
+    }
+
+    for (int n0 = row_begin; n0 < row_end; n0 += L::kRows) {
+        auto load_w = [&](int it) {
+            if (it < iters) {
+                const uint32_t base = smem_u32(smem) + (it % kStages) * L::kStage;
 #pragma unroll
-    for (int r = 0; r < kRt; ++r) {
+                for (int i = 0; i < L::kRows * kWk * 8 / kThreads; ++i) {
+                    const int c = i * kThreads + threadIdx.x; // 16-byte chunk: eight a row and step
+                    const int row = (c >> 3) % L::kRows, step = (c >> 3) / L::kRows;
+                    const int64_t col = (static_cast<int64_t>(it) * kWk + step) * kStepBytes + (c & 7) * 16;
+                    const bool live = n0 + row < row_end && col < row_bytes; // k is a multiple of 32: chunks are whole
+                    cp_async(base + (step * L::kRows + row) * kPitch + (c & 7) * 16, a.w + (live ? (n0 + row) * row_bytes + col : 0), 16, live);
+                }
+                // 16 kWr rows x kWk steps = 128 runs of scales, then as many of zeros
+                const int r = threadIdx.x & 127, row = r % L::kRows, step = r / L::kRows;
+                const bool zeros = threadIdx.x >= 128, live = n0 + row < row_end;
+                if (!zeros || (!kMx && a.zero != nullptr)) {
+                    load_scales(base + L::kW + (zeros ? L::kScale : 0) + (step * L::kRows + row) * 16,
+                                (zeros ? a.zero : a.scale) + (live ? (n0 + row) * row_scale : 0),
+                                (static_cast<int64_t>(it) * kWk + step) * scale_bytes, row_scale, scale_bytes, live, a.scale_async);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // x: loaded an iteration ahead, a warp one row of one run at a time
+        uint4 xr[kPasses];
+        const int units = a.m * kWk;
+        auto load_x = [&](int it) {
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+                const int unit = p * kWarps + warp;
+                xr[p] = make_uint4(0, 0, 0, 0);
+                if (it < iters && unit < units) {
+                    const int64_t k0 = (static_cast<int64_t>(it) * kWk + unit % kWk) * kStepK + lane * 8;
+                    if (k0 < a.k) {
+                        xr[p] = __ldg(reinterpret_cast<const uint4 *>(a.x + (unit / kWk) * a.x_stride + k0));
+                    }
+                }
+            }
+        };
+        auto store_x = [&](int it) {
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+                const int unit = p * kWarps + warp;
+                if (unit < units) {
+                    prepare_run<kBf16, kMx>(xr[p], xbuf + ((it & 1) * kWk + unit % kWk) * x_run, x_rows, unit / kWk, lane);
+                }
+            }
+        };
+
+        float acc[kMt][4];
 #pragma unroll
         for (int c = 0; c < kMt; ++c) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sums[(warp * kM + 8 * c + 2 * t + (i & 1)) * kN + 16 * r + g + 8 * (i >> 1)] = acc[r][c][i];
+                acc[c][i] = 0.0f;
             }
         }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kM * kN; i += kThreads) {
-        const int col = i / kN, row = i % kN;
-        if (col < a.m && n0 + row < a.n) {
-            float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                v += sums[(w * kM + col) * kN + row];
+        for (int s = 0; s < kStages - 1; ++s) {
+            load_w(s);
+        }
+        load_x(0);
+        store_x(0);
+        for (int it = 0; it < iters; ++it) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncthreads(); // stage `it` of W and x is there, and everybody is done with the stage the next loads overwrite
+            load_w(it + kStages - 1);
+            load_x(it + 1);
+            const uint8_t *base = smem + (it % kStages) * L::kStage;
+            const int row = wk * L::kRows + wr * 16 + g;
+            const int left = (a.k - (it * kWk + wk) * kStepK) / 32;
+            if (left > 0 && n0 + wr * 16 < row_end) {
+                run_product<kBf16, kMx, kMt>(acc, reinterpret_cast<const uint32_t *>(base + row * kPitch) + t, base + L::kW + row * 16,
+                                             base + L::kW + L::kScale + row * 16, xbuf + ((it & 1) * kWk + wk) * x_run, lx,
+                                             a.group_shift, a.zero != nullptr, left);
             }
-            if constexpr (kMx && !kBf16) {
-                v *= 16384.0f; // the codes went in as 2^-14 times their values
-            }
-            const int64_t to = static_cast<int64_t>(col) * a.n + n0 + row;
-            if (a.out_f32) {
-                static_cast<float *>(a.y)[to] = v;
-            } else {
-                static_cast<uint16_t *>(a.y)[to] = static_cast<uint16_t>(pack_16x2<kBf16>(v, 0.0f));
+            store_x(it + 1);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        // the shares of k joined in a fixed order: [share][column of x][row of W]
+        float *sums = reinterpret_cast<float *>(smem);
+        constexpr int kM = 8 * kMt;
+#pragma unroll
+        for (int c = 0; c < kMt; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sums[(wk * kM + 8 * c + 2 * t + (i & 1)) * L::kRows + wr * 16 + g + 8 * (i >> 1)] = acc[c][i];
             }
         }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.m * L::kRows; i += kThreads) {
+            const int col = i / L::kRows, row = i % L::kRows;
+            if (n0 + row < row_end) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWk; ++w) {
+                    v += sums[(w * kM + col) * L::kRows + row];
+                }
+                store_y<kBf16>(a, static_cast<int64_t>(col) * a.n + n0 + row, v);
+            }
+        }
+        __syncthreads(); // the sums are read before the ring is loaded again
     }
 }
 
-template <bool kBf16, bool kMx, bool kZero, int kRt, int kMt>
-int launch_tiles(const W4Args &a, cudaStream_t stream)
+// ------------------------------------------------------------------ launches
+
+template <bool kBf16, bool kMx, int kMt>
+int launch_resident(W4Args a, int blocks, cudaStream_t stream)
 {
-    constexpr int kRing = kWarps * kStages * 16 * kRt * kPitch;
-    constexpr int kSums = kWarps * 8 * kMt * 16 * kRt * 4;
-    constexpr int kSmem = kRing > kSums ? kRing : kSums;
-    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&w4_matvec_kernel<kBf16, kMx, kZero, kRt, kMt>), kSmem);
+    a.rows_each = a.n / blocks;
+    a.rows_more = a.n % blocks;
+    // the attribute is raised once per kernel and device: to the most that is ever asked
+    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&w4_resident_kernel<kBf16, kMx, kMt>), kResidentSmem);
     if (rc != kOk) {
         return rc;
     }
-    const int blocks = (a.n + 16 * kRt - 1) / (16 * kRt);
-    w4_matvec_kernel<kBf16, kMx, kZero, kRt, kMt><<<blocks, kThreads, kSmem, stream>>>(a);
+    w4_resident_kernel<kBf16, kMx, kMt><<<blocks, kThreads, resident_smem<kMx, kMt>(a.m, a.k), stream>>>(a);
     return check_launch();
 }
 
-template <bool kBf16, bool kMx, bool kZero>
+template <bool kBf16, bool kMx, int kWr, int kMt>
+int launch_streamed(W4Args a, int blocks, cudaStream_t stream)
+{
+    a.rows_each = a.n / blocks;
+    a.rows_more = a.n % blocks;
+    using L = Layout<kMx, kWr, kMt>;
+    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&w4_streamed_kernel<kBf16, kMx, kWr, kMt>), L::smem_bytes(8 * kMt));
+    if (rc != kOk) {
+        return rc;
+    }
+    w4_streamed_kernel<kBf16, kMx, kWr, kMt><<<blocks, kThreads, L::smem_bytes(a.m), stream>>>(a);
+    return check_launch();
+}
+
+template <bool kBf16, bool kMx>
 int launch_typed(const W4Args &a, cudaStream_t stream)
 {
-    return a.m <= 8    ? launch_tiles<kBf16, kMx, kZero, 1, 1>(a, stream)
-           : a.m <= 16 ? launch_tiles<kBf16, kMx, kZero, 1, 2>(a, stream)
-           : a.m <= 32 ? launch_tiles<kBf16, kMx, kZero, 1, 4>(a, stream)
-                       : launch_tiles<kBf16, kMx, kZero, 1, 8>(a, stream);
+    const int tiles = (a.n + 15) / 16;
+    if (a.m <= 2 && resident_smem<kMx, 0>(a.m, a.k) <= kResidentSmem) {
+        const int most = resident_smem<kMx, 0>(a.m, a.k) <= kNarrowSmem ? 3 * kSms : 2 * kSms;
+        return launch_resident<kBf16, kMx, 0>(a, tiles < most ? tiles : most, stream);
+    }
+    if (a.m <= 8 && resident_smem<kMx, 1>(a.m, a.k) <= kResidentSmem) {
+        return launch_resident<kBf16, kMx, 1>(a, tiles < 2 * kSms ? tiles : 2 * kSms, stream);
+    }
+    if (a.m <= 16 && resident_smem<kMx, 2>(a.m, a.k) <= kResidentSmem) {
+        return launch_resident<kBf16, kMx, 2>(a, tiles < 2 * kSms ? tiles : 2 * kSms, stream);
+    }
+    // two blocks an SM, or one where that leaves a block fewer than 32 rows: every block reads all of x
+    const int blocks = a.n >= 64 * kSms ? 2 * kSms : (tiles < kSms ? tiles : kSms);
+    const int rows = (a.n + blocks - 1) / blocks;
+    const int wr = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8));
+    if (a.m <= 8) {
+        switch (wr) {
+            case 1: return launch_streamed<kBf16, kMx, 1, 1>(a, blocks, stream);
+            case 2: return launch_streamed<kBf16, kMx, 2, 1>(a, blocks, stream);
+            case 4: return launch_streamed<kBf16, kMx, 4, 1>(a, blocks, stream);
+            default: return launch_streamed<kBf16, kMx, 8, 1>(a, blocks, stream);
+        }
+    }
+    if (a.m <= 16) {
+        switch (wr) {
+            case 1:
+            case 2: return launch_streamed<kBf16, kMx, 2, 2>(a, blocks, stream);
+            case 4: return launch_streamed<kBf16, kMx, 4, 2>(a, blocks, stream);
+            default: return launch_streamed<kBf16, kMx, 8, 2>(a, blocks, stream);
+        }
+    }
+    if (a.m <= 32) {
+        return wr <= 4 ? launch_streamed<kBf16, kMx, 4, 4>(a, blocks, stream) : launch_streamed<kBf16, kMx, 8, 4>(a, blocks, stream);
+    }
+    return launch_streamed<kBf16, kMx, 8, 8>(a, blocks, stream);
 }
 
 } // namespace
@@ -264,8 +761,8 @@ int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, cons
     W4Args a;
     a.x = x;
     a.w = w;
-    a.scale = scale;
-    a.zero = zero;
+    a.scale = static_cast<const uint8_t *>(scale);
+    a.zero = reinterpret_cast<const uint8_t *>(zero);
     a.y = y;
     a.x_stride = x_stride;
     a.m = m;
@@ -273,13 +770,11 @@ int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, cons
     a.k = k;
     a.group_shift = group == 32 ? 5 : (group == 64 ? 6 : 7);
     a.out_f32 = out_f32;
+    a.scale_async = k % kStepK == 0 && ((reinterpret_cast<uintptr_t>(scale) | reinterpret_cast<uintptr_t>(zero)) & 15u) == 0;
     if (mx) {
-        return bf16 ? launch_typed<true, true, false>(a, stream) : launch_typed<false, true, false>(a, stream);
+        return bf16 ? launch_typed<true, true>(a, stream) : launch_typed<false, true>(a, stream);
     }
-    if (zero != nullptr) {
-        return bf16 ? launch_typed<true, false, true>(a, stream) : launch_typed<false, false, true>(a, stream);
-    }
-    return bf16 ? launch_typed<true, false, false>(a, stream) : launch_typed<false, false, false>(a, stream);
+    return bf16 ? launch_typed<true, false>(a, stream) : launch_typed<false, false>(a, stream);
 }
 
 } // namespace pto_b200

@@ -400,7 +400,8 @@ def test_w4_rows_strides_vectors_and_what_is_written():
     room = torch.full((7, n), 7.0, dtype=F16, device="cuda")
     y = check_w4(x, w, scale, None, 32, out=room[1:6])
     assert (room[0] == 7).all() and (room[6] == 7).all()
-    assert torch.equal(p.w4_matvec(x[2], w, scale), y[2])  # a vector is one row, and rows do not depend on each other
+    check_w4(x[2], w, scale, None, 32)  # a vector is one row; other row counts may sum in another order, within the same bound
+    assert p.w4_matvec(x[2], w, scale).shape == (n,)
     assert torch.equal(p.w4_matvec(x.contiguous(), w, scale), y)
     assert p.w4_matvec(x[:0], w, scale).shape == (0, n)
 
