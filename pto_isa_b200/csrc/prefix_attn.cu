@@ -17,8 +17,7 @@
 //               depends on the key, so it is applied to the code pair (exact in 16 bits within the type's range).
 // Softmax statistics and all sums are fp32; P is rounded to the 16-bit type of q for the second product.
 #include "ptx.cuh"
-#include "internal.h"
-#include "mx_format.cuh"
+#include "prefix_attn.cuh"
 
 #include <type_traits>
 
@@ -29,7 +28,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 16; // keys a warp takes at a time
-constexpr int kRows = 16; // query rows of a block
+constexpr int kRows = kPieceRows; // query rows of a block
 constexpr int kSms = 148; // planning constant: what the cut along the keys aims at
 
 __device__ __forceinline__ float ex2(float x)
@@ -77,27 +76,6 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a)
     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
-
-struct AttnArgs {
-    const uint8_t *k, *v, *ks, *vs;
-    const uint16_t *q;
-    int64_t q_batch, q_token, q_head; // strides in elements
-    const int32_t *prefix_pages;
-    const int32_t *table;
-    const int32_t *lens;
-    int64_t table_stride;
-    int64_t num_pages;
-    float *part_o;   // [slot][16][d]
-    float2 *part_ml; // [slot][16]: m (log2 units), l
-    uint16_t *o;
-    float *lse;
-    float scale_log2;
-    int table_cols, page_shift;
-    int batch, tokens, heads, kv_heads, group;
-    int prefix_len, own_max;
-    int prefix_tiles, prefix_splits, prefix_chunk;
-    int own_tiles, own_splits, own_min;
-};
 
 __host__ __device__ inline int ceil_div(int a, int b)
 {
@@ -206,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     const int g = lane >> 2, t = lane & 3;
 
     // ---- which piece
-    const int prefix_items = a.prefix_splits * a.kv_heads * a.prefix_tiles;
+    const int prefix_items = a.prefix_wide ? 0 : a.prefix_splits * a.kv_heads * a.prefix_tiles;
     const int row_span = a.tokens * a.group; // rows of one sequence and kv head
     int64_t item = blockIdx.x;
     int h, tile, b = 0, k_begin, k_end, rows;
@@ -223,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
         pages = a.prefix_pages;
     } else {
         item -= prefix_items;
+        slot = item + static_cast<int64_t>(a.prefix_pieces) * a.kv_heads * a.prefix_tiles;
         tile = static_cast<int>(item % a.own_tiles);
         item /= a.own_tiles;
         h = static_cast<int>(item % a.kv_heads);
@@ -598,13 +577,13 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
     const int prow = b * a.tokens * a.group + in;
     const int len = own_len(a, b);
     const int own_pieces = len > 0 ? ceil_div(len, own_chunk(len, a.own_splits, a.own_min)) : 0;
-    const int64_t prefix_items = static_cast<int64_t>(a.prefix_splits) * a.kv_heads * a.prefix_tiles;
-    const int pieces = a.prefix_splits + own_pieces;
+    const int64_t prefix_items = static_cast<int64_t>(a.prefix_pieces) * a.kv_heads * a.prefix_tiles;
+    const int pieces = a.prefix_pieces + own_pieces;
     auto row_of = [&](int i) -> int64_t { // where piece i keeps this row
-        if (i < a.prefix_splits) {
+        if (i < a.prefix_pieces) {
             return ((static_cast<int64_t>(i) * a.kv_heads + h) * a.prefix_tiles + prow / kRows) * kRows + prow % kRows;
         }
-        const int64_t s = i - a.prefix_splits;
+        const int64_t s = i - a.prefix_pieces;
         return (prefix_items + ((s * a.batch + b) * a.kv_heads + h) * a.own_tiles + in / kRows) * kRows + in % kRows;
     };
     float top = -INFINITY;
@@ -625,6 +604,9 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
     for (int i = 0; i < pieces; ++i) {
         const int64_t row = row_of(i);
         const float2 v = a.part_ml[row];
+        if (v.x == -INFINITY && v.y == 0.0f) {
+            continue; // no key of this piece for this row: its sums may not even have been written
+        }
         const float w = ex2(v.x - ref);
         sum = fmaf(v.y, w, sum);
         const float *src = a.part_o + row * kD + lane * kPer;
@@ -653,26 +635,44 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
     }
 }
 
-// How the keys are cut.  About three blocks of 16 rows fit an SM; a piece is at least 64 keys (16 for each warp).
+// How the keys are cut.  About three blocks of 16 rows fit an SM; a piece is at least 64 keys (16 for each warp).  With
+// more than kWideRows rows the prefix goes to the wide kernel, one block per SM, in one wave where it can.
 struct Plan {
-    int prefix_tiles, prefix_splits, prefix_chunk;
+    int prefix_tiles, prefix_splits, prefix_pieces, prefix_chunk, prefix_wide;
     int own_tiles, own_splits, own_min;
-    int64_t slots;
+    int64_t slots, own_slots;
 };
+
+constexpr int kWideRows = 16;
 
 Plan make_plan(int batch, int tokens, int heads, int kv_heads, int prefix_len, int own_max)
 {
-    Plan p = {0, 0, 0, 0, 0, 0, 0};
+    Plan p = {};
     const int row_span = tokens * (heads / kv_heads);
     const int target = 3 * kSms;
     if (prefix_len > 0) {
-        p.prefix_tiles = ceil_div(batch * row_span, kRows);
-        const int64_t units = static_cast<int64_t>(p.prefix_tiles) * kv_heads;
-        int64_t splits = (target + units - 1) / units;
-        const int most = ceil_div(prefix_len, 64);
-        splits = splits > most ? most : splits;
-        p.prefix_chunk = (ceil_div(prefix_len, static_cast<int>(splits)) + 63) & ~63;
-        p.prefix_splits = ceil_div(prefix_len, p.prefix_chunk);
+        const int rows = batch * row_span;
+        p.prefix_tiles = ceil_div(rows, kRows);
+        p.prefix_wide = rows > kWideRows;
+        if (p.prefix_wide) {
+            const bool pair = rows > 128;
+            const int64_t units = static_cast<int64_t>(ceil_div(rows, pair ? 256 : 128)) * kv_heads;
+            const int tiles = ceil_div(prefix_len, 128);
+            int splits = units >= kSms ? 1 : static_cast<int>(kSms / units);
+            splits = splits > tiles ? tiles : splits;
+            const int per = ceil_div(tiles, splits);
+            p.prefix_chunk = per * 128;
+            p.prefix_splits = ceil_div(tiles, per);
+            p.prefix_pieces = pair ? p.prefix_splits : 2 * p.prefix_splits;
+        } else {
+            const int64_t units = static_cast<int64_t>(p.prefix_tiles) * kv_heads;
+            int64_t splits = (target + units - 1) / units;
+            const int most = ceil_div(prefix_len, 64);
+            splits = splits > most ? most : splits;
+            p.prefix_chunk = (ceil_div(prefix_len, static_cast<int>(splits)) + 63) & ~63;
+            p.prefix_splits = ceil_div(prefix_len, p.prefix_chunk);
+            p.prefix_pieces = p.prefix_splits;
+        }
     }
     p.own_tiles = ceil_div(row_span, kRows);
     p.own_min = 64;
@@ -686,8 +686,8 @@ Plan make_plan(int batch, int tokens, int heads, int kv_heads, int prefix_len, i
         const int most = ceil_div(own_max, 64);
         p.own_splits = static_cast<int>(splits > most ? most : splits);
     }
-    p.slots = (static_cast<int64_t>(p.prefix_splits) * p.prefix_tiles +
-               static_cast<int64_t>(p.own_splits) * p.own_tiles * batch) * kv_heads;
+    p.own_slots = static_cast<int64_t>(p.own_splits) * p.own_tiles * batch * kv_heads;
+    p.slots = static_cast<int64_t>(p.prefix_pieces) * p.prefix_tiles * kv_heads + p.own_slots;
     return p;
 }
 
@@ -704,8 +704,15 @@ int launch_pieces(const AttnArgs &a, int64_t blocks, DeviceStatus *status, cudaS
 }
 
 template <bool kBf16, int kD>
-int launch_typed(int fmt, const AttnArgs &a, int64_t blocks, DeviceStatus *status, cudaStream_t stream)
+int launch_typed(int fmt, const AttnArgs &a, int64_t own_slots, DeviceStatus *status, cudaStream_t stream)
 {
+    if (a.prefix_wide) {
+        const int rc = launch_prefix_wide(a, fmt, kD, kBf16, status, stream);
+        if (rc != kOk) {
+            return rc;
+        }
+    }
+    const int64_t blocks = own_slots + (a.prefix_wide ? 0 : static_cast<int64_t>(a.prefix_splits) * a.kv_heads * a.prefix_tiles);
     if (blocks > 0) {
         const int rc = fmt == kKvMxFp8   ? launch_pieces<kBf16, kD, kKvMxFp8>(a, blocks, status, stream)
                        : fmt == kKvMxFp4 ? launch_pieces<kBf16, kD, kKvMxFp4>(a, blocks, status, stream)
@@ -774,16 +781,18 @@ int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, c
     a.own_max = own_max;
     a.prefix_tiles = p.prefix_tiles;
     a.prefix_splits = p.prefix_splits;
+    a.prefix_pieces = p.prefix_pieces;
+    a.prefix_wide = p.prefix_wide;
     a.prefix_chunk = p.prefix_chunk;
     a.own_tiles = p.own_tiles;
     a.own_splits = p.own_splits;
     a.own_min = p.own_min;
     if (cache.d == 128) {
-        return bf16 ? launch_typed<true, 128>(cache.fmt, a, p.slots, status, stream)
-                    : launch_typed<false, 128>(cache.fmt, a, p.slots, status, stream);
+        return bf16 ? launch_typed<true, 128>(cache.fmt, a, p.own_slots, status, stream)
+                    : launch_typed<false, 128>(cache.fmt, a, p.own_slots, status, stream);
     }
-    return bf16 ? launch_typed<true, 64>(cache.fmt, a, p.slots, status, stream)
-                : launch_typed<false, 64>(cache.fmt, a, p.slots, status, stream);
+    return bf16 ? launch_typed<true, 64>(cache.fmt, a, p.own_slots, status, stream)
+                : launch_typed<false, 64>(cache.fmt, a, p.own_slots, status, stream);
 }
 
 } // namespace pto_b200

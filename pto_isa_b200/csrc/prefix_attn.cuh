@@ -1,0 +1,36 @@
+// Declarations shared by the two kernels of the attention over a shared prefix.
+#pragma once
+#include "internal.h"
+#include "mx_format.cuh"
+
+namespace pto_b200 {
+
+struct AttnArgs {
+    const uint8_t *k, *v, *ks, *vs;
+    const uint16_t *q;
+    int64_t q_batch, q_token, q_head; // strides in elements
+    const int32_t *prefix_pages;
+    const int32_t *table;
+    const int32_t *lens;
+    int64_t table_stride;
+    int64_t num_pages;
+    float *part_o;   // [slot][16][d]
+    float2 *part_ml; // [slot][16]: m (log2 units), l
+    uint16_t *o;
+    float *lse;
+    float scale_log2;
+    int table_cols, page_shift;
+    int batch, tokens, heads, kv_heads, group;
+    int prefix_len, own_max;
+    // prefix_splits pieces of prefix_chunk keys, each for prefix_tiles tiles of 16 rows; in the wide kernel a block makes
+    // prefix_pieces / prefix_splits pieces of its chunk
+    int prefix_tiles, prefix_splits, prefix_pieces, prefix_chunk, prefix_wide;
+    int own_tiles, own_splits, own_min;
+};
+
+constexpr int kPieceRows = 16; // rows of a slot of partial results
+
+// keys by the tensor memory of one block per SM: 128-row tiles of the prefix's rows against 128 keys at a time
+int launch_prefix_wide(const AttnArgs &a, int fmt, int d, bool bf16, DeviceStatus *status, cudaStream_t stream);
+
+} // namespace pto_b200

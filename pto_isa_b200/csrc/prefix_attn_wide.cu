@@ -1,0 +1,841 @@
+// The shared prefix's keys against many query rows, on the fifth-generation tensor cores (the part of prefix_attn whose
+// rows are those of the whole batch; prefix_attn.cu says how the parts are joined).
+//
+// One block per SM takes 128-row tiles of one kv head's rows (all sequences, query tokens and heads of the group) and a run
+// of the prefix's keys, 128 at a time:
+//   S = Q K^T   tcgen05.mma, both operands K-major in 128-byte-swizzled shared memory, S in tensor memory
+//   softmax     one thread per row: running maximum and sum in registers, P in 16 bits to shared memory
+//   O += P V    tcgen05.mma, V MN-major (as its rows lie), O in tensor memory, rescaled only when a row's maximum has
+//               grown 256-fold
+// and leaves (O, m, l) in fp32.  Two groups of four softmax warps: with more than one tile of rows they take two tiles and
+// share every K and V tile (kPair), with a single tile they take alternate key tiles, so that one group's exponentials
+// run under the other's products either way.
+//
+// A tile of K or V comes from pages, in 16 bits by cp.async or as codes that four loading warps convert on the way into
+// shared memory.  Codes become float16 whatever the type of q: e4m3 and e2m1 convert to float16 pairs in one instruction,
+// to bfloat16 in four.  Exactness:
+//   K       code 2^e is exact in float16 for e in [-15, 7] (e4m3) or [-23, 13] (e2m1).  A key with a block outside that range is stored relative to
+//           its largest scale, 2^(e - e_max), and the power of two goes to the logit as a factor of the key.
+//   q       bfloat16 rows are divided by a power of two that brings their largest element into [2^14, 2^15): elements
+//           down to 2^-31 of it keep every bit; the logits of the row are multiplied back.
+//   V, P    float16 where all scales of the tile are in range; otherwise, if q is bfloat16, this tile's V and P are bfloat16
+//           (code 2^e is exact there): an instruction's operands share a type, its fp32 accumulator does not care.
+//
+// What bounds it: per 128 x 128 logits and head size 128, 1024 cycles of tensor work, 1024 of the special-function unit
+// (an exponential takes 8 cycles a warp), about 512 of the integer pipe for the conversion of a quantised tile.
+#include "ptx.cuh"
+#include "prefix_attn.cuh"
+
+namespace pto_b200 {
+
+namespace {
+
+constexpr int kThreads = 512; // warps 0-3, 4-7 softmax; 8-11 loading; 12, 13 issuing (one per group)
+constexpr int kTile = 128;
+constexpr int kRegsSoftmax = 200, kRegsLoad = 72, kRegsIssue = 40; // (200 + 200 + 72 + 40) * 128 = 512 * 128
+constexpr int kTmemCols = 512;
+constexpr float kDefer = 8.0f; // log2 of the growth of a row's maximum that rescales O
+
+struct Info { // of a key tile
+    uint32_t valid[4]; // bit r: key r exists
+    uint32_t flags[4]; // by loading warp: bit 0, some key has a factor; bit 1, V is bfloat16
+    uint16_t factor[kTile]; // bfloat16, a power of two
+};
+
+template <int kD, bool kPair>
+struct Shape {
+    static constexpr int kTileBytes = kTile * kD * 2; // Q, K, V
+    static constexpr int kHalfBytes = kTile * 128;    // 64 columns of 16 bits, one swizzled half
+    static constexpr int kPBytes = 2 * kHalfBytes;
+    static constexpr int kQTiles = kPair ? 2 : 1;
+    static constexpr int kRing = kD == 64 ? 6 : (kPair ? 3 : 4);
+    // tiles whose description is kept: it is written anew when the ring's item before K(j), V(j - 2), could be loaded, that
+    // is when item 2 j - 2 - kRing was used up: V(j - 4) with 4 slots, K(j - 2) with 3 (whose product follows that with
+    // V(j - 4)), V(j - 5) with 6
+    static constexpr int kInfo = kD == 64 ? 8 : 4;
+    struct Control {
+        uint64_t q_full[2];
+        uint64_t ring_full[kRing], ring_empty[kRing];
+        uint64_t info_full[kInfo];
+        uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
+        uint32_t tmem_base;
+        int abort_flag;
+        float q_factor[kPair ? 1 : kTile]; // what the rows of q were divided by, for the group that did not load them
+        Info info[kInfo];
+    };
+    static constexpr int kData = kQTiles * kTileBytes + kRing * kTileBytes + 2 * kPBytes;
+    static constexpr int kSmem = kData + static_cast<int>(sizeof(Control)) + 1024;
+    static_assert(kSmem <= 232448, "shared memory of a block");
+};
+
+__device__ __forceinline__ float ex2w(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// where 16 bytes (8 elements) `chunk` of row `row` lie in a 64-column half
+__device__ __forceinline__ uint32_t swz(int row, int chunk)
+{
+    return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+// the scale bytes of a row: d / 32 of them
+template <int kD>
+__device__ __forceinline__ uint32_t row_scales(const uint8_t *s, int64_t row)
+{
+    if constexpr (kD == 128) {
+        return __ldg(reinterpret_cast<const uint32_t *>(s) + row);
+    } else {
+        return __ldg(reinterpret_cast<const uint16_t *>(s) + row);
+    }
+}
+
+// whether code 2^(byte - 127) is exact in float16 for every block of the row: e in [-15, 7] for e4m3 (2^-9 .. 448), in
+// [-23, 13] for e2m1 (0.5 .. 6), or a block of zeros
+template <int kD, int kFmt>
+__device__ __forceinline__ bool scales_in_range(uint32_t s)
+{
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < kD / 32; ++i) {
+        const uint32_t b = (s >> (8 * i)) & 0xffu;
+        ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || b == 0u);
+    }
+    return ok;
+}
+
+template <int kD>
+__device__ __forceinline__ uint32_t largest_scale(uint32_t s)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kD / 32; ++i) {
+        m = max(m, (s >> (8 * i)) & 0xffu);
+    }
+    return m;
+}
+
+// sixteen codes -> sixteen float16 (8 words)
+template <int kFmt>
+__device__ __forceinline__ void codes16_to_f16(const uint32_t (&c)[4], uint32_t (&h)[8])
+{
+    if constexpr (kFmt == kKvMxFp8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+                : "=r"(h[2 * i]), "=r"(h[2 * i + 1])
+                : "r"(c[i]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+                : "=r"(h[4 * i]), "=r"(h[4 * i + 1]), "=r"(h[4 * i + 2]), "=r"(h[4 * i + 3])
+                : "r"(c[i]));
+        }
+    }
+}
+
+template <bool kBf16, int kD, int kFmt, bool kPair>
+__global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_constant__ AttnArgs a, DeviceStatus *status)
+{
+    using Sh = Shape<kD, kPair>;
+    using Control = typename Sh::Control;
+    constexpr bool kMx = kFmt >= kKvMxFp8;
+    constexpr bool kOpBf16 = kBf16 && !kMx; // type of the products' operands (but for V and P of flagged tiles)
+    constexpr int kRing = Sh::kRing, kInfo = Sh::kInfo;
+    constexpr int kHalves = kD / 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *smem_q = smem;
+    uint8_t *smem_ring = smem_q + Sh::kQTiles * Sh::kTileBytes;
+    uint8_t *smem_p = smem_ring + kRing * Sh::kTileBytes;
+    Control *ctl = reinterpret_cast<Control *>(smem_p + 2 * Sh::kPBytes);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- which rows and keys: block = ((split * kv_heads) + h) * row blocks + row block
+    const int rows = a.batch * a.tokens * a.group;
+    const int row_blocks = (rows + kTile * Sh::kQTiles - 1) / (kTile * Sh::kQTiles);
+    const int rb = blockIdx.x % row_blocks;
+    const int h = blockIdx.x / row_blocks % a.kv_heads;
+    const int split = blockIdx.x / row_blocks / a.kv_heads;
+    const int k_begin = split * a.prefix_chunk;
+    const int k_end = min(k_begin + a.prefix_chunk, a.prefix_len);
+    const int tiles = (k_end - k_begin + kTile - 1) / kTile;
+    // group t: pair form, row tile 2 rb + t and every key tile; single form, row tile rb and key tiles t, t + 2, ..
+    const bool group_rows[2] = {true, kPair ? (2 * rb + 1) * kTile < rows : true};
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&ctl->q_full[t], 4);
+            mbar_init(&ctl->s_full[t], 1);
+            mbar_init(&ctl->s_free[t], 4);
+            mbar_init(&ctl->p_full[t], 4);
+            mbar_init(&ctl->pv_done[t], 1);
+        }
+        for (int s = 0; s < kRing; ++s) {
+            mbar_init(&ctl->ring_full[s], 4);
+            mbar_init(&ctl->ring_empty[s], kPair ? 2 : 1);
+        }
+        for (int s = 0; s < kInfo; ++s) {
+            mbar_init(&ctl->info_full[s], 4);
+        }
+        ctl->abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&ctl->tmem_base, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = ctl->tmem_base;
+    volatile int *abort_flag = &ctl->abort_flag;
+    // items of the ring in order: K(0), then for every tile j: K(j + 1) (if any), V(j)
+    auto item_k = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
+    auto item_v = [&](int j) { return j + 1 < tiles ? 2 * j + 2 : 2 * tiles - 1; };
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        // ------------------------------------------------------------ issuing warps, one per group
+        const int t = warp - 12;
+        if (t < 2 && lane == 0) {
+            constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, 0, 0, kOpBf16 ? 1 : 0);
+            constexpr uint32_t idesc_o = make_idesc_f16(kTile, kD, 0, 1, kOpBf16 ? 1 : 0);
+            constexpr uint32_t idesc_ob = make_idesc_f16(kTile, kD, 0, 1, 1);
+            const uint32_t s_tmem = tmem_base + t * 128, o_tmem = tmem_base + 256 + t * 128;
+            const uint64_t q_desc = make_sw128_desc(smem_u32(smem_q) + (kPair ? t : 0) * Sh::kTileBytes, 16, 1024);
+            const uint64_t p_desc = make_sw128_desc(smem_u32(smem_p) + t * Sh::kPBytes, 16, 1024);
+            const uint32_t ring_base = smem_u32(smem_ring);
+            auto kstep = [](int kk) -> uint64_t { return static_cast<uint64_t>((kk >> 2) * (Sh::kHalfBytes >> 4) + (kk & 3) * 2); };
+            bool ok = true;
+            auto ring_wait = [&](int item, uint32_t &addr) {
+                const int slot = item % kRing;
+                addr = ring_base + slot * Sh::kTileBytes;
+                ok = mbar_wait(&ctl->ring_full[slot], (item / kRing) & 1, abort_flag);
+            };
+            // S of the group's n-th tile (key tile j)
+            auto do_s = [&](int j, int n) {
+                uint32_t addr;
+                const int item = item_k(j);
+                ring_wait(item, addr);
+                if (ok && group_rows[t]) {
+                    if (n == 0) {
+                        ok = mbar_wait(&ctl->q_full[kPair ? t : 0], 0, abort_flag);
+                    } else {
+                        ok = mbar_wait(&ctl->s_free[t], (n - 1) & 1, abort_flag); // the previous S has been read
+                    }
+                    if (ok) {
+                        tc_fence_after();
+                        const uint64_t k_desc = make_sw128_desc(addr, 16, 1024);
+#pragma unroll
+                        for (int kk = 0; kk < kD / 16; ++kk) {
+                            tc_mma_f16_ss(s_tmem, q_desc + kstep(kk), k_desc + kstep(kk), idesc_s, kk != 0 ? 1u : 0u);
+                        }
+                        tc_commit(&ctl->s_full[t]);
+                    }
+                }
+                if (ok) {
+                    tc_commit(&ctl->ring_empty[item % kRing]);
+                }
+            };
+            auto do_pv = [&](int j, int n) {
+                uint32_t addr;
+                const int item = item_v(j);
+                ring_wait(item, addr);
+                if (ok && group_rows[t]) {
+                    ok = mbar_wait(&ctl->p_full[t], n & 1, abort_flag);
+                    if (ok) {
+                        tc_fence_after();
+                        uint32_t idesc = idesc_o;
+                        if constexpr (kMx) {
+                            const Info &info = ctl->info[j % kInfo];
+                            const uint32_t f = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
+                            idesc = (f & 2u) ? idesc_ob : idesc_o;
+                        }
+                        const uint64_t v_desc = make_sw128_desc(addr, Sh::kHalfBytes, 1024); // MN-major: 16 keys = 2 KiB
+#pragma unroll
+                        for (int kk = 0; kk < kTile / 16; ++kk) {
+                            tc_mma_f16_ss(o_tmem, p_desc + kstep(kk), v_desc + static_cast<uint64_t>(kk * 128), idesc,
+                                          (n != 0 || kk != 0) ? 1u : 0u);
+                        }
+                        tc_commit(&ctl->pv_done[t]);
+                    }
+                }
+                if (ok) {
+                    tc_commit(&ctl->ring_empty[item % kRing]);
+                }
+            };
+            constexpr int kHop = kPair ? 1 : 2;
+            const int first = kPair ? 0 : t;
+            if (first < tiles) {
+                do_s(first, 0);
+            }
+            int n = 0;
+            for (int j = first; j < tiles && ok; j += kHop, ++n) {
+                if (j + kHop < tiles) {
+                    do_s(j + kHop, n + 1);
+                }
+                if (ok) {
+                    do_pv(j, n);
+                }
+            }
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+        // ------------------------------------------------------------ loading warps
+        const int tid = threadIdx.x - 256;
+        const int p = tid & 3; // 16 elements p of a 64-column half
+        constexpr int RB = kv_row_bytes(kFmt, kD);
+        const uint32_t ring_base = smem_u32(smem_ring);
+        const int page_mask = (1 << a.page_shift) - 1;
+        // row of the cache that key r of tile j lies in, -1 where there is none
+        auto cache_row = [&](int j, int r) -> int64_t {
+            const int key = k_begin + j * kTile + r;
+            if (key >= k_end) {
+                return -1;
+            }
+            const int64_t page = a.prefix_pages[key >> a.page_shift];
+            if (page < 0 || page >= a.num_pages) {
+                return -1;
+            }
+            return ((page * a.kv_heads + h) << a.page_shift) + (key & page_mask);
+        };
+        // what the other warps have to know about tile j; one key a thread
+        auto describe = [&](int j) {
+            Info &info = ctl->info[j % kInfo];
+            const int64_t row = cache_row(j, tid);
+            const bool valid = row >= 0;
+            const int key = k_begin + j * kTile + tid;
+            if (!valid && key < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+                status->block = blockIdx.x;
+                status->where = 11;
+                status->detail = a.prefix_pages[key >> a.page_shift];
+            }
+            const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+            uint32_t flags = 0;
+            if constexpr (kMx) {
+                uint16_t factor = 0x3f80; // 1
+                bool k_out = false, v_out = false;
+                if (valid) {
+                    const uint32_t ks = row_scales<kD>(a.ks, row), vs = row_scales<kD>(a.vs, row);
+                    k_out = !scales_in_range<kD, kFmt>(ks);
+                    // with float16 queries V stays float16: small values only lose what is below float16's last place, as o
+                    // itself does, and larger ones than it holds count as infinities
+                    v_out = kBf16 && !scales_in_range<kD, kFmt>(vs);
+                    if (k_out) {
+                        factor = static_cast<uint16_t>(largest_scale<kD>(ks) << 7);
+                    }
+                }
+                info.factor[tid] = factor;
+                flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
+            }
+            if (lane == 0) {
+                info.valid[warp - 8] = mask;
+                info.flags[warp - 8] = flags;
+            }
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ctl->info_full[j % kInfo]);
+            }
+        };
+        // the rows of tile j towards L2: lane = 16 keys of K (0 .. 7) or V (8 .. 15)
+        auto prefetch = [&](int j) {
+            if (warp == 8 && j < tiles && lane < 16) {
+                const int64_t row = cache_row(j, (lane & 7) * 16);
+                if (row >= 0) {
+                    const uint8_t *src = (lane < 8 ? a.k : a.v) + row * RB;
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(16 * RB) : "memory");
+                }
+            }
+        };
+        bool ok = true;
+        if constexpr (!kMx) {
+            // 16-bit rows: cp.async into place; an item is handed over when the next one has been issued
+            int slot_done = 0;
+            auto hand_over = [&](int slot) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&ctl->ring_full[slot]);
+                }
+            };
+            int item = 0;
+            auto load_item = [&](const uint8_t *src, int j) {
+                const int slot = item % kRing;
+                if (!mbar_wait(&ctl->ring_empty[slot], ((item / kRing) & 1) ^ 1u, abort_flag)) {
+                    ok = false;
+                    return;
+                }
+                const uint32_t dst = ring_base + slot * Sh::kTileBytes;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = i * 32 + (tid >> 2);
+                    const int64_t row = cache_row(j, r);
+                    const uint8_t *from = src + (row < 0 ? 0 : row) * RB;
+                    const int bytes = row < 0 ? 0 : 16;
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int chunk = 2 * p + c;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + half * Sh::kHalfBytes + swz(r, chunk)),
+                                         "l"(from + half * 128 + chunk * 16), "r"(bytes)
+                                         : "memory");
+                        }
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (item > 0) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    hand_over(slot_done);
+                }
+                slot_done = slot;
+                ++item;
+            };
+            prefetch(0);
+            prefetch(1);
+            describe(0);
+            load_item(a.k, 0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                prefetch(j + 2);
+                if (j + 1 < tiles) {
+                    describe(j + 1);
+                    load_item(a.k, j + 1);
+                }
+                if (ok) {
+                    load_item(a.v, j);
+                }
+            }
+            if (ok) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                hand_over(slot_done);
+            }
+        } else {
+            constexpr int kBatch = kHalves * 2; // units of 16 elements in flight: rows i, i + 1 of four, both halves
+            struct Batch {
+                uint32_t c[kBatch][4];
+                uint32_t s[2]; // the rows' scale bytes
+            };
+            auto fetch = [&](Batch &b, bool is_v, int j, int which) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t row = cache_row(j, (2 * which + i) * 32 + (tid >> 2));
+                    b.s[i] = 0;
+                    if (row >= 0) {
+                        b.s[i] = row_scales<kD>(is_v ? a.vs : a.ks, row);
+                    }
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+                        uint32_t(&c)[4] = b.c[i * kHalves + half];
+                        c[0] = c[1] = c[2] = c[3] = 0;
+                        if (row >= 0) {
+                            const uint8_t *src = (is_v ? a.v : a.k) + row * RB;
+                            if constexpr (kFmt == kKvMxFp8) {
+                                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + half * 64) + p);
+                                c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+                            } else {
+                                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src + half * 32) + p);
+                                c[0] = v.x, c[1] = v.y;
+                            }
+                        }
+                    }
+                }
+            };
+            auto put = [&](const Batch &b, bool is_v, bool as_bf16, uint32_t dst, int which) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = (2 * which + i) * 32 + (tid >> 2);
+                    const bool relative = !is_v && !scales_in_range<kD, kFmt>(b.s[i]);
+                    const int top = relative ? static_cast<int>(largest_scale<kD>(b.s[i])) : 127;
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+                        uint32_t w[8];
+                        codes16_to_f16<kFmt>(b.c[i * kHalves + half], w);
+                        const uint32_t byte = (b.s[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
+                        if (as_bf16) {
+                            const uint32_t m = byte * 0x00800080u; // 2^(byte - 127) twice; 255: infinity, times 0 NaN
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                const uint32_t y = (w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu); // times 2^-112
+                                w[x] = mul_16x2<true>(mul_16x2<true>(y, 0x77807780u), m);
+                            }
+                        } else {
+                            const int e = static_cast<int>(byte) - top + 127; // below 1: far under the key's largest element
+                            const float f = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(max(e, 0)) << 23);
+                            const uint32_t m = pack_16x2<false>(f, f);
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                w[x] = mul_16x2<false>(w[x], m);
+                            }
+                        }
+                        const uint32_t at = dst + half * Sh::kHalfBytes;
+                        sts128(at + swz(r, 2 * p), w[0], w[1], w[2], w[3]);
+                        sts128(at + swz(r, 2 * p + 1), w[4], w[5], w[6], w[7]);
+                    }
+                }
+            };
+            // item i is K or V of a tile
+            const int items = 2 * tiles;
+            auto what = [&](int i, bool &is_v, int &j) {
+                if (i == 0) {
+                    is_v = false;
+                    j = 0;
+                } else if (i == items - 1) {
+                    is_v = true;
+                    j = tiles - 1;
+                } else {
+                    is_v = (i & 1) == 0;
+                    j = is_v ? i / 2 - 1 : (i + 1) / 2;
+                }
+            };
+            Batch b0, b1;
+            bool is_v;
+            int j;
+            prefetch(0);
+            prefetch(1);
+            what(0, is_v, j);
+            fetch(b0, is_v, j, 0);
+            for (int i = 0; i < items && ok; ++i) {
+                what(i, is_v, j);
+                fetch(b1, is_v, j, 1);
+                if (!is_v) {
+                    prefetch(j + 2);
+                    describe(j);
+                }
+                const int slot = i % kRing;
+                if (!mbar_wait(&ctl->ring_empty[slot], ((i / kRing) & 1) ^ 1u, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                bool as_bf16 = false;
+                if (is_v) { // described with K(j), by all four warps
+                    ok = mbar_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag);
+                    const Info &info = ctl->info[j % kInfo];
+                    as_bf16 = ((info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3]) & 2u) != 0;
+                }
+                const uint32_t dst = ring_base + slot * Sh::kTileBytes;
+                put(b0, is_v, as_bf16, dst, 0);
+                if (i + 1 < items) {
+                    bool next_v;
+                    int next_j;
+                    what(i + 1, next_v, next_j);
+                    fetch(b0, next_v, next_j, 0);
+                }
+                put(b1, is_v, as_bf16, dst, 1);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&ctl->ring_full[slot]);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        // ------------------------------------------------------------ softmax warps: a thread owns a row
+        const int t = warp >> 2, quarter = warp & 3;
+        const int row_in_tile = quarter * 32 + lane;
+        const int row = (kPair ? 2 * rb + t : rb) * kTile + row_in_tile;
+        const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t s_addr = lane_addr + t * 128, o_addr = lane_addr + 256 + t * 128;
+        const uint32_t p_base = smem_u32(smem_p) + t * Sh::kPBytes;
+        bool ok = true;
+        float row_scale = a.scale_log2 < 0.0f ? -a.scale_log2 : (a.scale_log2 == 0.0f ? 1.0f : a.scale_log2);
+
+        // ---- this row of Q, its sign that of the scale, so that the maximum of the raw logits is that of the scaled
+        const int q_tile = kPair ? t : 0;
+        if (kPair || t == 0) {
+            const uint32_t q_base = smem_u32(smem_q) + q_tile * Sh::kTileBytes;
+            const bool live = row < rows;
+            const uint16_t *src = nullptr;
+            if (live) {
+                const int span = a.tokens * a.group;
+                const int b = row / span, in = row % span;
+                src = a.q + b * a.q_batch + (in / a.group) * a.q_token + static_cast<int64_t>(h * a.group + in % a.group) * a.q_head;
+            }
+            const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+            const uint32_t keep = live && a.scale_log2 != 0.0f ? 0xffffffffu : 0u;
+            float inv = 1.0f, factor = 1.0f;
+            if constexpr (kBf16 && kMx) {
+                float top = 0.0f;
+                if (live) {
+#pragma unroll 4
+                    for (int c = 0; c < kD / 8; ++c) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + c);
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = unpack_16x2<true>(w[i]);
+                            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        }
+                    }
+                }
+                const int field = min(max(static_cast<int>(__float_as_uint(top) >> 23), 29), 254);
+                factor = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
+                inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
+            }
+#pragma unroll 4
+            for (int c = 0; c < kD / 8; ++c) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (live) {
+                    v = __ldg(reinterpret_cast<const uint4 *>(src) + c);
+                }
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (kBf16 && kMx) {
+                        const float2 f = unpack_16x2<true>(w[i]);
+                        w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
+                    }
+                    w[i] = (w[i] & keep) ^ sign;
+                }
+                sts128(q_base + (c >> 3) * Sh::kHalfBytes + swz(row_in_tile, c & 7), w[0], w[1], w[2], w[3]);
+            }
+            if constexpr (!kPair) {
+                ctl->q_factor[row_in_tile] = factor;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ctl->q_full[q_tile]);
+            }
+            row_scale *= factor;
+        } else {
+            ok = mbar_wait(&ctl->q_full[0], 0, abort_flag);
+            row_scale *= ctl->q_factor[kPair ? 0 : row_in_tile];
+        }
+
+        const bool rows_here = group_rows[t];
+        float m_run = -INFINITY; // reference the probabilities are relative to, raw logits
+        float l_run = 0.0f;
+        int n = 0;
+        for (int j = kPair ? 0 : t; j < tiles && ok && rows_here; j += kPair ? 1 : 2, ++n) {
+            if (!mbar_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag) || !mbar_wait(&ctl->s_full[t], n & 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t sr[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                tmem_ld_32x32(s_addr + c * 32, sr[c]);
+            }
+            tmem_ld_wait();
+            tc_fence_before();
+            if (lane == 0) {
+                mbar_arrive(&ctl->s_free[t]);
+            }
+            const Info &info = ctl->info[j % kInfo];
+            bool p_bf16 = kOpBf16;
+            if constexpr (kMx) {
+                const uint32_t f = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
+                p_bf16 = (f & 2u) != 0;
+                if (f & 1u) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            sr[c][i] = __float_as_uint(__uint_as_float(sr[c][i]) * __uint_as_float(static_cast<uint32_t>(info.factor[c * 32 + i]) << 16));
+                        }
+                    }
+                }
+            }
+            if ((info.valid[0] & info.valid[1] & info.valid[2] & info.valid[3]) != 0xffffffffu) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t valid = info.valid[c];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (!((valid >> i) & 1u)) {
+                            sr[c][i] = 0xff800000u;
+                        }
+                    }
+                }
+            }
+            float mx8[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                mx8[u] = fmaxf(__uint_as_float(sr[0][u]), __uint_as_float(sr[0][8 + u]));
+            }
+#pragma unroll
+            for (int i = 16; i < 128; i += 16) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    mx8[u] = fmaxf(mx8[u], fmaxf(__uint_as_float(sr[i >> 5][(i & 31) + u]), __uint_as_float(sr[i >> 5][(i & 31) + 8 + u])));
+                }
+            }
+            const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+            const float m_new = fmaxf(m_run, mx);
+            // also true on the first tile that has a key; false (NaN) while there is none
+            const bool grow = (m_new - m_run) * row_scale > kDefer;
+            bool pv_waited = n == 0;
+            if (__any_sync(0xffffffffu, grow)) {
+                if (n > 0) {
+                    if (!mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    pv_waited = true;
+                    tc_fence_after();
+                    // rows without a key yet keep their zeros; the others move to the new reference
+                    const float alpha = m_run == m_new ? 1.0f : ex2w((m_run - m_new) * row_scale);
+                    l_run *= alpha;
+#pragma unroll 1
+                    for (int c = 0; c < kD / 32; ++c) {
+                        uint32_t orow[32];
+                        tmem_ld_32x32(o_addr + c * 32, orow);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            orow[i] = __float_as_uint(__uint_as_float(orow[i]) * alpha);
+                        }
+                        tmem_st_32x32(o_addr + c * 32, orow);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                m_run = m_new;
+            }
+            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
+            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float p0 = ex2w(fmaf(__uint_as_float(sr[c][i]), row_scale, neg_m));
+                    const float p1 = ex2w(fmaf(__uint_as_float(sr[c][i + 1]), row_scale, neg_m));
+                    sum4[(i >> 1) & 3] += p0 + p1;
+                    pk[i >> 1] = p_bf16 ? pack_16x2<true>(p0, p1) : pack_16x2<false>(p0, p1);
+                }
+                if (c == 0 && !pv_waited) { // the previous product must have read P's buffer
+                    ok = mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    sts128(p_base + (c >> 1) * Sh::kHalfBytes + swz(row_in_tile, (c & 1) * 4 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2],
+                           pk[4 * q + 3]);
+                }
+            }
+            if (!ok) {
+                break;
+            }
+            l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ctl->p_full[t]);
+            }
+        }
+        // ---- (O, m, l) of this group's keys
+        if (ok && rows_here) {
+            if (n > 0) {
+                ok = mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag);
+                tc_fence_after();
+            }
+            const int piece = kPair ? split : 2 * split + t;
+            const int64_t slot = (static_cast<int64_t>(piece) * a.kv_heads + h) * a.prefix_tiles + row / kPieceRows;
+            const int64_t at = slot * kPieceRows + row % kPieceRows;
+            if (ok) {
+                if (row < rows) {
+                    // without a finite maximum the reference was 0; no key at all: -infinity and no sum
+                    a.part_ml[at] = make_float2(m_run != -INFINITY ? m_run * row_scale : (l_run == 0.0f ? -INFINITY : 0.0f), l_run);
+                }
+#pragma unroll 1
+                for (int c = 0; c < kD / 32 && n > 0; ++c) {
+                    uint32_t orow[32];
+                    tmem_ld_32x32(o_addr + c * 32, orow);
+                    tmem_ld_wait();
+                    if (row < rows) {
+                        uint4 *dst = reinterpret_cast<uint4 *>(a.part_o + at * kD + c * 32);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            dst[i] = make_uint4(orow[4 * i], orow[4 * i + 1], orow[4 * i + 2], orow[4 * i + 3]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    tc_fence_before();
+    __syncthreads();
+    if (ctl->abort_flag) {
+        for (int i = 0; i < 1024; ++i) {
+            __nanosleep(1000); // products and copies in flight end before shared and tensor memory are given back
+        }
+        if (threadIdx.x == 0 && atomicCAS(&status->code, 0, kErrDeviceWaitTimeout) == 0) {
+            status->block = blockIdx.x;
+            status->where = 5;
+        }
+        __syncthreads();
+    }
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+template <bool kBf16, int kD, int kFmt, bool kPair>
+int launch_one(const AttnArgs &a, DeviceStatus *status, cudaStream_t stream)
+{
+    using Sh = Shape<kD, kPair>;
+    const void *kernel = reinterpret_cast<const void *>(&prefix_wide_kernel<kBf16, kD, kFmt, kPair>);
+    // the warps' register budgets are moved around inside what the block was launched with: less would wait forever
+    static const int regs = [kernel] {
+        cudaFuncAttributes attr;
+        return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
+    }();
+    if (regs * kThreads < (2 * kRegsSoftmax + kRegsLoad + kRegsIssue) * 128) {
+        set_error_text("prefix_attn: the kernel was built with %d registers, too few for its split", regs);
+        return kErrUnsupportedShape;
+    }
+    const int rc = ensure_dynamic_smem(kernel, Sh::kSmem);
+    if (rc != kOk) {
+        return rc;
+    }
+    const int rows = a.batch * a.tokens * a.group;
+    const int row_blocks = (rows + kTile * Sh::kQTiles - 1) / (kTile * Sh::kQTiles);
+    const int64_t blocks = static_cast<int64_t>(a.prefix_splits) * a.kv_heads * row_blocks;
+    prefix_wide_kernel<kBf16, kD, kFmt, kPair><<<static_cast<unsigned>(blocks), kThreads, Sh::kSmem, stream>>>(a, status);
+    return check_launch();
+}
+
+template <bool kBf16, int kD, int kFmt>
+int launch_pair(const AttnArgs &a, DeviceStatus *status, cudaStream_t stream)
+{
+    return a.batch * a.tokens * a.group > kTile ? launch_one<kBf16, kD, kFmt, true>(a, status, stream)
+                                                : launch_one<kBf16, kD, kFmt, false>(a, status, stream);
+}
+
+template <bool kBf16, int kD>
+int launch_fmt(int fmt, const AttnArgs &a, DeviceStatus *status, cudaStream_t stream)
+{
+    return fmt == kKvMxFp8   ? launch_pair<kBf16, kD, kKvMxFp8>(a, status, stream)
+           : fmt == kKvMxFp4 ? launch_pair<kBf16, kD, kKvMxFp4>(a, status, stream)
+                             : launch_pair<kBf16, kD, kBf16 ? kKvBf16 : kKvF16>(a, status, stream);
+}
+
+} // namespace
+
+int launch_prefix_wide(const AttnArgs &a, int fmt, int d, bool bf16, DeviceStatus *status, cudaStream_t stream)
+{
+    if (d == 128) {
+        return bf16 ? launch_fmt<true, 128>(fmt, a, status, stream) : launch_fmt<false, 128>(fmt, a, status, stream);
+    }
+    return bf16 ? launch_fmt<true, 64>(fmt, a, status, stream) : launch_fmt<false, 64>(fmt, a, status, stream);
+}
+
+} // namespace pto_b200

@@ -79,18 +79,21 @@ def attention(q, prefix_k, prefix_v, own_k, own_v, scale):
     return o, lse, wv, vsum, qk
 
 
-def attention_bounds(dtype, o, wv, vsum, qk, keys):
+def attention_bounds(dtype, o, wv, vsum, qk, keys, mx=False):
     """Error bounds of (o, lse), derived: with u = 2^-22 for every fp32 operation in a chain (tensor-core sums may truncate)
       logit: at most 24 sums of products of total magnitude qk -> 24 u qk, twice that in exp, u each for exp2 and scaling;
       weights: rounded to `dtype` once, eps / 2, below float16's normal range 2^-25 absolute (their maximum is 1);
-      sums: keys / 16 + 48 fp32 additions; V: below float16's normal range 2^-25 absolute; output: one more rounding."""
+      sums: keys / 16 + 48 fp32 additions; V: below float16's normal range 2^-25 absolute; output: one more rounding.
+    Over an MX cache (mx) the weights are float16 for either `dtype`: relative 2^-11, which eps / 2 covers, and below 2^-14,
+    where float16's places are 2^-24 apart, 2^-25 absolute; the weights being at most 1 and their sum at least 1, that is
+    2^-25 |v| a key, at most 2^-25 vsum."""
     half = torch.finfo(dtype).eps / 2
     u = 2.0 ** -22
     logit = (24 * qk + 8) * u
     chain = (keys / 16 + 48) * u
     rel = half + 2 * logit[..., None] + 2 * chain
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
-    return rel * wv + tiny * (vsum + 2) + half * o.abs() + 1e-30, logit + chain + u * 8
+    return rel * wv + (2.0 ** -25 if mx else tiny) * vsum + 2 * tiny + half * o.abs() + 1e-30, logit + chain + u * 8
 
 
 def w4_weights(w, scale, zero, group):

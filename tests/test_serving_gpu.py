@@ -185,7 +185,7 @@ def check_attention(q, c, pages, prefix, table, lens, parts, own, scale=None, **
     q4 = q if q.dim() == 4 else q.unsqueeze(1)
     want, wlse, wv, vsum, qk = ref.attention(q4.double(), *parts, *own, q.shape[-1] ** -0.5 if scale is None else scale)
     keys = prefix + max([0] + [x.shape[1] for x in own[0]])
-    ob, lb = ref.attention_bounds(q.dtype, want, wv, vsum, qk, keys)
+    ob, lb = ref.attention_bounds(q.dtype, want, wv, vsum, qk, keys, mx=c.fmt >= p.KV_MXFP8)
     o, lse = o.view(q4.shape), lse.view(q4.shape[:-1])
     empty = torch.isinf(wlse)
     assert (o[empty] == 0).all() and (lse[empty] == -torch.inf).all()
@@ -251,6 +251,61 @@ def test_attention_small_and_large_cached_values():
                 none = torch.zeros(1, 0, d, dtype=torch.float64, device="cuda")
                 check_attention(q, c, pages, 0, pages.expand(2, 4).contiguous(), lens, [none, none], [[kd, none], [vd, none]])
                 check_attention(q, c, pages, n, pages.expand(2, 4).contiguous(), lens * 0, [kd, vd], [[none] * 2] * 2)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch,name", [(20, "16"), (20, "mxfp8"), (20, "mxfp4"), (37, "mxfp8"), (75, "16"), (75, "mxfp4")])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_many_rows_of_any_size(dtype, batch, name, d):
+    """Many rows over the prefix (one, two and three tiles of 128): a negative, a zero and a large scale, a maximum that keeps
+    growing along the keys, cached values far from 1 in some tiles of the prefix only, rows of q of very different sizes."""
+    heads, kv, prefix = 8, 2, 700
+    for at, (ek, ev) in enumerate(((0, 0), (-30, 0), (30, 0), (0, 30), (0, -30), (0, -10), (0, 6))):
+        if dtype == F16 and (abs(ek) > 8 or abs(ev) > 10):
+            continue
+        made = make_attention(name, dtype, d, kv, 32, prefix, [3] * batch, 40 + at)
+        c, pages, table, lens, parts, own = made
+        t = torch.arange(150, 420)  # two whole tiles and parts of two
+        slots = (pages[(t // 32).cuda()].long() * 32 + t.cuda() % 32).to(torch.int32)
+        k, v = (torch.randn(len(t), kv, d, generator=gen(s), device="cuda") * torch.linspace(0.2, 6, len(t), device="cuda")[:, None, None] for s in (1, 2))
+        import pto_isa_b200 as p
+        p.kv_cache_write(c, (k * 2.0 ** ek).to(dtype), (v * 2.0 ** ev).to(dtype), slots)
+        kd, vd = values(c)
+        rows = lambda x: x[pages.long().cpu()].transpose(0, 1).reshape(kv, -1, d)[:, :prefix].cuda()
+        size = torch.exp2(torch.randint(-3, 3, (batch, 1, heads, 1), generator=gen(8), device="cuda").float() - max(ek, 0))
+        q = (torch.randn(batch, 1, heads, d, generator=gen(6), device="cuda") * size).to(dtype)
+        for scale in (None, -0.3, 0.0) if at == 0 else (None,):
+            check_attention(q, c, pages, prefix, table, lens, [rows(kd), rows(vd)], own, scale=scale)
+
+
+def test_attention_many_rows_nan_bad_pages_and_repeats():
+    import pto_isa_b200 as p
+    for name in FORMATS:
+        made = make_attention(name, F16, 128, 1, 16, 400, [0] * 40, 22)
+        c, pages, table, lens = made[:4]
+        table = torch.zeros(40, 1, dtype=torch.int32, device="cuda")
+        q = torch.randn(40, 8, 128, generator=gen(2), device="cuda").to(F16)
+        first = p.prefix_attn(q, c, pages, 400, table, lens, return_lse=True)
+        for _ in range(3):
+            again = p.prefix_attn(q, c, pages, 400, table, lens, return_lse=True)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+        # a page that does not exist is left out, and reported
+        kd, vd = values(c)
+        broken = pages.clone()
+        broken[7] = c.k.shape[0]
+        o = p.prefix_attn(q, c, broken, 400, table, lens)
+        assert status()[2:] == (11, c.k.shape[0])
+        keep = torch.cat([pages[:7], pages[8:]]).long().cpu()
+        rows = lambda x: x[keep].transpose(0, 1).reshape(1, -1, 128)[:, :384].cuda()
+        none = torch.zeros(1, 0, 128, dtype=torch.float64, device="cuda")
+        want, _, wv, vsum, qk = ref.attention(q[:, None].double(), rows(kd), rows(vd), [none] * 40, [none] * 40, 128 ** -0.5)
+        bound, _ = ref.attention_bounds(F16, want, wv, vsum, qk, 400)
+        assert ((o[:, None].double() - want).abs() <= bound).all()
+        # a NaN in the prefix reaches everybody, one past its end nobody
+        bad = torch.full((1, 1, 128), float("nan"), dtype=F16, device="cuda")
+        p.kv_cache_write(c, bad, bad, (pages[12] * 16 + 8).view(1))
+        assert torch.isfinite(p.prefix_attn(q, c, pages, 200, table, lens)).all()
+        assert p.prefix_attn(q, c, pages, 201, table, lens).isnan().all()
 
 
 def test_attention_nan_reaches_its_own_rows_only():
@@ -490,7 +545,7 @@ def test_decode_steps_of_a_batch_behind_one_prompt(name, dtype):
         n = lens.tolist()
         own = [[rows(x, table[b], n[b]) for b in range(batch)] for x in (kd, vd)]
         want, wlse, wv, vsum, qk = ref.attention(qkv[:, None, :heads].double(), rows(kd, pages, prefix), rows(vd, pages, prefix), *own, d ** -0.5)
-        ob, lb = ref.attention_bounds(dtype, want, wv, vsum, qk, prefix + max(n))
+        ob, lb = ref.attention_bounds(dtype, want, wv, vsum, qk, prefix + max(n), mx=True)
         assert ((o[:, None].double() - want).abs() <= ob).all() and ((lse[:, None].double() - wlse).abs() <= lb).all()
     assert lens.tolist() == [x + 2 for x in before.tolist()] and status()[0] == 0
 
