@@ -260,10 +260,15 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     const int steps = ceil_div(k_end - k_begin, kStep);
     const uint32_t ring = smem_u32(smem) + warp * St::kCount * St::kBytes;
     uint32_t bad_pages = 0; // bit s: the step in ring stage s lies in a page that does not exist
+    // the page of the step that is loaded next, read a step before
+    int next_page = warp < steps ? pages[(k_begin + warp * kStep) >> a.page_shift] : 0;
     auto load = [&](int step, int stage) {
         if (step < steps) {
             const int key = k_begin + step * kStep;
-            const int64_t page = pages[key >> a.page_shift];
+            const int64_t page = next_page;
+            if (step + kWarps < steps) {
+                next_page = pages[(key + kWarps * kStep) >> a.page_shift];
+            }
             const bool ok = page >= 0 && page < a.num_pages;
             bad_pages = (bad_pages & ~(1u << stage)) | (ok ? 0u : 1u << stage);
             if (!ok) {
@@ -561,15 +566,15 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     }
 }
 
-// one warp per output row: joins the row's pieces in a fixed order
+// Joins a row's pieces in a fixed order: four warps a row, each every fourth piece, then their four sums.  The pieces'
+// statistics are read first, side by side; the loads of the sums depend on nothing and overlap.
 template <bool kBf16, int kD>
-__global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid_constant__ AttnArgs a)
 {
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (idx >= static_cast<int64_t>(a.batch) * a.tokens * a.heads) {
-        return;
-    }
+    constexpr int kPer = kD / 32;
+    __shared__ float sums[kWarps], accs[kWarps][kD];
+    const int64_t idx = blockIdx.x; // output row: (batch, token, head)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = static_cast<int>(idx % a.heads);
     const int tok = static_cast<int>(idx / a.heads % a.tokens);
     const int b = static_cast<int>(idx / a.heads / a.tokens);
@@ -595,43 +600,55 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
     }
     const float ref = top == -INFINITY ? 0.0f : top;
-    constexpr int kPer = kD / 32;
     float acc[kPer], sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
         acc[c] = 0.0f;
     }
-    for (int i = 0; i < pieces; ++i) {
+#pragma unroll 4
+    for (int i = warp; i < pieces; i += kWarps) {
         const int64_t row = row_of(i);
         const float2 v = a.part_ml[row];
-        if (v.x == -INFINITY && v.y == 0.0f) {
-            continue; // no key of this piece for this row: its sums may not even have been written
-        }
-        const float w = ex2(v.x - ref);
-        sum = fmaf(v.y, w, sum);
-        const float *src = a.part_o + row * kD + lane * kPer;
-        if constexpr (kPer == 4) {
-            const float4 x = *reinterpret_cast<const float4 *>(src);
-            acc[0] = fmaf(x.x, w, acc[0]);
-            acc[1] = fmaf(x.y, w, acc[1]);
-            acc[2] = fmaf(x.z, w, acc[2]);
-            acc[3] = fmaf(x.w, w, acc[3]);
-        } else {
-            const float2 x = *reinterpret_cast<const float2 *>(src);
-            acc[0] = fmaf(x.x, w, acc[0]);
-            acc[1] = fmaf(x.y, w, acc[1]);
+        // no key of this piece for this row: its sums may not even have been written
+        if (!(v.x == -INFINITY && v.y == 0.0f)) {
+            const float w = ex2(v.x - ref);
+            sum = fmaf(v.y, w, sum);
+            const float *src = a.part_o + row * kD + lane * kPer;
+            if constexpr (kPer == 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(src);
+                acc[0] = fmaf(x.x, w, acc[0]);
+                acc[1] = fmaf(x.y, w, acc[1]);
+                acc[2] = fmaf(x.z, w, acc[2]);
+                acc[3] = fmaf(x.w, w, acc[3]);
+            } else {
+                const float2 x = *reinterpret_cast<const float2 *>(src);
+                acc[0] = fmaf(x.x, w, acc[0]);
+                acc[1] = fmaf(x.y, w, acc[1]);
+            }
         }
     }
-    const bool none = top == -INFINITY && sum == 0.0f; // no key at all: zeros
-    const float inv = none ? 0.0f : 1.0f / sum;
-    uint16_t *dst = a.o + idx * kD + lane * kPer;
-    if constexpr (kPer == 4) {
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_16x2<kBf16>(acc[0] * inv, acc[1] * inv), pack_16x2<kBf16>(acc[2] * inv, acc[3] * inv));
-    } else {
-        *reinterpret_cast<uint32_t *>(dst) = pack_16x2<kBf16>(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+        accs[warp][lane * kPer + c] = acc[c];
     }
-    if (a.lse != nullptr && lane == 0) {
-        a.lse[idx] = none ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
+    if (lane == 0) {
+        sums[warp] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < kD / 2) { // two elements a thread
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        const bool none = top == -INFINITY && sum == 0.0f; // no key at all: zeros
+        const float inv = none ? 0.0f : 1.0f / sum;
+        float v[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int at = 2 * threadIdx.x + c;
+            v[c] = ((accs[0][at] + accs[1][at]) + (accs[2][at] + accs[3][at])) * inv;
+        }
+        reinterpret_cast<uint32_t *>(a.o + idx * kD)[threadIdx.x] = pack_16x2<kBf16>(v[0], v[1]);
+        if (a.lse != nullptr && threadIdx.x == 0) {
+            a.lse[idx] = none ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
+        }
     }
 }
 
@@ -722,7 +739,7 @@ int launch_typed(int fmt, const AttnArgs &a, int64_t own_slots, DeviceStatus *st
         }
     }
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
-    prefix_attn_join_kernel<kBf16, kD><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(a);
+    prefix_attn_join_kernel<kBf16, kD><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(a);
     return check_launch();
 }
 

@@ -11,7 +11,7 @@
 // share every K and V tile (kPair), with a single tile they take alternate key tiles, so that one group's exponentials
 // run under the other's products either way.
 //
-// A tile of K or V comes from pages, in 16 bits by cp.async or as codes that four loading warps convert on the way into
+// A tile of K or V comes from pages, in 16 bits by cp.async or as codes that eight loading warps convert on the way into
 // shared memory.  Codes become float16 whatever the type of q: e4m3 and e2m1 convert to float16 pairs in one instruction,
 // to bfloat16 in four.  Exactness:
 //   K       code 2^e is exact in float16 for e in [-15, 7] (e4m3) or [-23, 13] (e2m1).  A key with a block outside that range is stored relative to
@@ -30,15 +30,18 @@ namespace pto_b200 {
 
 namespace {
 
-constexpr int kThreads = 512; // warps 0-3, 4-7 softmax; 8-11 loading; 12, 13 issuing (one per group)
+constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-15 loading; 16, 17 issuing (one per group); 18, 19 idle
+// registers of a thread: 96 at launch (five warps a scheduler), then (2 * 120 + 2 * 96 + 40) * 128 of these 640 * 96
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 120, kRegsIssue = 40;
+static_assert((2 * kRegsSoftmax + 2 * kRegsLaunch + kRegsIssue) * 128 <= kThreads * kRegsLaunch, "an increase would wait forever");
+constexpr int kLoadWarps = 8, kIssueWarp = 16;
 constexpr int kTile = 128;
-constexpr int kRegsSoftmax = 200, kRegsLoad = 72, kRegsIssue = 40; // (200 + 200 + 72 + 40) * 128 = 512 * 128
 constexpr int kTmemCols = 512;
 constexpr float kDefer = 8.0f; // log2 of the growth of a row's maximum that rescales O
 
 struct Info { // of a key tile
     uint32_t valid[4]; // bit r: key r exists
-    uint32_t flags[4]; // by loading warp: bit 0, some key has a factor; bit 1, V is bfloat16
+    uint32_t flags[4]; // by describing warp: bit 0, some key has a factor; bit 1, V is bfloat16
     uint16_t factor[kTile]; // bfloat16, a power of two
 };
 
@@ -49,10 +52,10 @@ struct Shape {
     static constexpr int kPBytes = 2 * kHalfBytes;
     static constexpr int kQTiles = kPair ? 2 : 1;
     static constexpr int kRing = kD == 64 ? 6 : (kPair ? 3 : 4);
-    // tiles whose description is kept: it is written anew when the ring's item before K(j), V(j - 2), could be loaded, that
-    // is when item 2 j - 2 - kRing was used up: V(j - 4) with 4 slots, K(j - 2) with 3 (whose product follows that with
-    // V(j - 4)), V(j - 5) with 6
-    static constexpr int kInfo = kD == 64 ? 8 : 4;
+    // Tiles whose description is kept.  Tile j + 2 is described when K(j + 1), item 2 j + 1, has been stored, so when all items
+    // up to 2 j + 1 - kRing were used up; what that leaves of earlier tiles: 3 slots V(j - 2), all of tile j - 2; 4 slots
+    // V(j - 3); 6 slots V(j - 4).
+    static constexpr int kInfo = kRing == 3 ? 4 : (kRing == 4 ? 6 : 8);
     struct Control {
         uint64_t q_full[2];
         uint64_t ring_full[kRing], ring_empty[kRing];
@@ -64,7 +67,7 @@ struct Shape {
         Info info[kInfo];
     };
     static constexpr int kData = kQTiles * kTileBytes + kRing * kTileBytes + 2 * kPBytes;
-    static constexpr int kSmem = kData + static_cast<int>(sizeof(Control)) + 1024;
+    static constexpr int kSmem = kData + static_cast<int>(sizeof(Control));
     static_assert(kSmem <= 232448, "shared memory of a block");
 };
 
@@ -73,6 +76,13 @@ __device__ __forceinline__ float ex2w(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
@@ -124,7 +134,7 @@ __device__ __forceinline__ uint32_t largest_scale(uint32_t s)
 
 // sixteen codes -> sixteen float16 (8 words)
 template <int kFmt>
-__device__ __forceinline__ void codes16_to_f16(const uint32_t (&c)[4], uint32_t (&h)[8])
+__device__ __forceinline__ void codes16_to_f16(const uint32_t *c, uint32_t (&h)[8])
 {
     if constexpr (kFmt == kKvMxFp8) {
 #pragma unroll
@@ -154,8 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     constexpr bool kOpBf16 = kBf16 && !kMx; // type of the products' operands (but for V and P of flagged tiles)
     constexpr int kRing = Sh::kRing, kInfo = Sh::kInfo;
     constexpr int kHalves = kD / 64;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *smem_q = smem;
     uint8_t *smem_ring = smem_q + Sh::kQTiles * Sh::kTileBytes;
     uint8_t *smem_p = smem_ring + kRing * Sh::kTileBytes;
@@ -184,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             mbar_init(&ctl->pv_done[t], 1);
         }
         for (int s = 0; s < kRing; ++s) {
-            mbar_init(&ctl->ring_full[s], 4);
+            mbar_init(&ctl->ring_full[s], kLoadWarps);
             mbar_init(&ctl->ring_empty[s], kPair ? 2 : 1);
         }
         for (int s = 0; s < kInfo; ++s) {
@@ -193,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
         ctl->abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == kIssueWarp) {
         tmem_alloc(&ctl->tmem_base, kTmemCols);
         tmem_relinquish();
     }
@@ -206,10 +215,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     auto item_k = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
     auto item_v = [&](int j) { return j + 1 < tiles ? 2 * j + 2 : 2 * tiles - 1; };
 
-    if (warp >= 12) {
+    if (warp >= kIssueWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // ------------------------------------------------------------ issuing warps, one per group
-        const int t = warp - 12;
+        const int t = warp - kIssueWarp;
         if (t < 2 && lane == 0) {
             constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, 0, 0, kOpBf16 ? 1 : 0);
             constexpr uint32_t idesc_o = make_idesc_f16(kTile, kD, 0, 1, kOpBf16 ? 1 : 0);
@@ -293,52 +302,60 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             }
         }
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
         // ------------------------------------------------------------ loading warps
+        // A thread's share of an item: 16 elements p of each 64-column half in rows r0 and r0 + 64.  Page numbers are loaded a
+        // tile before they are used, the scales for a description likewise, codes one item before they are stored: no load
+        // waits for another in the steady state.
         const int tid = threadIdx.x - 256;
-        const int p = tid & 3; // 16 elements p of a 64-column half
+        const int p = tid & 3, r0 = tid >> 2;
         constexpr int RB = kv_row_bytes(kFmt, kD);
         const uint32_t ring_base = smem_u32(smem_ring);
+        const uint32_t at0 = swz(r0, 2 * p), at1 = at0 ^ 16; // of the two 16-byte chunks, row r0
         const int page_mask = (1 << a.page_shift) - 1;
-        // row of the cache that key r of tile j lies in, -1 where there is none
-        auto cache_row = [&](int j, int r) -> int64_t {
+        // page of key r of tile j; -1: no such key.  Numbers out of range count as if there were no key.
+        auto page_of = [&](int j, int r) -> int {
             const int key = k_begin + j * kTile + r;
-            if (key >= k_end) {
-                return -1;
-            }
-            const int64_t page = a.prefix_pages[key >> a.page_shift];
-            if (page < 0 || page >= a.num_pages) {
-                return -1;
-            }
-            return ((page * a.kv_heads + h) << a.page_shift) + (key & page_mask);
+            return key < k_end ? __ldg(a.prefix_pages + (key >> a.page_shift)) : -1;
         };
-        // what the other warps have to know about tile j; one key a thread
+        // row of the cache of key r of tile j, which lies in `page`; -1 for none
+        auto cache_row = [&](int page, int j, int r) -> int64_t {
+            return page < 0 || page >= a.num_pages
+                       ? -1
+                       : ((static_cast<int64_t>(page) * a.kv_heads + h) << a.page_shift) + ((k_begin + j * kTile + r) & page_mask);
+        };
+        // ---- what the other warps have to know about a tile: warps 8 .. 11, one key a thread
+        const bool describes = tid < kTile;
+        int pid_own = -1, pid_own_next = -1;
+        uint32_t own_ks = 0, own_vs = 0;
+        auto load_own_scales = [&](int j) {
+            if constexpr (kMx) {
+                own_ks = own_vs = 127u * 0x01010101u;
+                const int64_t row = cache_row(pid_own, j, tid);
+                if (row >= 0) {
+                    own_ks = row_scales<kD>(a.ks, row);
+                    own_vs = row_scales<kD>(a.vs, row);
+                }
+            }
+        };
         auto describe = [&](int j) {
+            if (!describes || j >= tiles) {
+                return;
+            }
             Info &info = ctl->info[j % kInfo];
-            const int64_t row = cache_row(j, tid);
-            const bool valid = row >= 0;
-            const int key = k_begin + j * kTile + tid;
-            if (!valid && key < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+            const bool valid = pid_own >= 0 && pid_own < a.num_pages;
+            if (!valid && k_begin + j * kTile + tid < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
                 status->block = blockIdx.x;
                 status->where = 11;
-                status->detail = a.prefix_pages[key >> a.page_shift];
+                status->detail = pid_own;
             }
             const uint32_t mask = __ballot_sync(0xffffffffu, valid);
             uint32_t flags = 0;
             if constexpr (kMx) {
-                uint16_t factor = 0x3f80; // 1
-                bool k_out = false, v_out = false;
-                if (valid) {
-                    const uint32_t ks = row_scales<kD>(a.ks, row), vs = row_scales<kD>(a.vs, row);
-                    k_out = !scales_in_range<kD, kFmt>(ks);
-                    // with float16 queries V stays float16: small values only lose what is below float16's last place, as o
-                    // itself does, and larger ones than it holds count as infinities
-                    v_out = kBf16 && !scales_in_range<kD, kFmt>(vs);
-                    if (k_out) {
-                        factor = static_cast<uint16_t>(largest_scale<kD>(ks) << 7);
-                    }
-                }
-                info.factor[tid] = factor;
+                const bool k_out = !scales_in_range<kD, kFmt>(own_ks);
+                // with float16 queries V stays float16: small values only lose what is below float16's last place, as o
+                // itself does, and larger ones than it holds count as infinities
+                const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(own_vs);
+                info.factor[tid] = k_out ? static_cast<uint16_t>(largest_scale<kD>(own_ks) << 7) : 0x3f80;
                 flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
             }
             if (lane == 0) {
@@ -349,130 +366,187 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             if (lane == 0) {
                 mbar_arrive(&ctl->info_full[j % kInfo]);
             }
+            // the next tile's: scales now, the page after it
+            pid_own = pid_own_next;
+            load_own_scales(j + 1);
+            pid_own_next = j + 2 < tiles ? page_of(j + 2, tid) : -1;
         };
-        // the rows of tile j towards L2: lane = 16 keys of K (0 .. 7) or V (8 .. 15)
-        auto prefetch = [&](int j) {
-            if (warp == 8 && j < tiles && lane < 16) {
-                const int64_t row = cache_row(j, (lane & 7) * 16);
-                if (row >= 0) {
+        // ---- the rows of a tile towards L2, by the last warp: lane = 16 keys of K (0 .. 7) or V (8 .. 15)
+        int pid_l2 = -1;
+        auto prefetch = [&](int j) { // tile j, whose page number was loaded a tile ago
+            if (warp == 8 + kLoadWarps - 1 && j < tiles) {
+                const int64_t row = cache_row(pid_l2, j, (lane & 7) * 16);
+                if (lane < 16 && row >= 0) {
                     const uint8_t *src = (lane < 8 ? a.k : a.v) + row * RB;
                     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(16 * RB) : "memory");
                 }
+                pid_l2 = j + 1 < tiles ? page_of(j + 1, (lane & 7) * 16) : -1;
             }
         };
+        int pid[2]; // of the tile after the next
+        auto load_pids = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                pid[i] = j < tiles ? page_of(j, r0 + 64 * i) : -1;
+            }
+        };
+        int64_t row_v[2], row_k[2], row_next[2]; // rows of tiles j, j + 1, j + 2
+        auto rows_from_pids = [&](int64_t (&row)[2], int j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                row[i] = cache_row(pid[i], j, r0 + 64 * i);
+            }
+        };
+        load_pids(0);
+        if (describes) {
+            pid_own = page_of(0, tid);
+            pid_own_next = tiles > 1 ? page_of(1, tid) : -1;
+        }
+        rows_from_pids(row_v, 0);
+        load_pids(1);
         bool ok = true;
+        int item = 0;
+        auto wait_empty = [&]() {
+            ok = ok && mbar_wait(&ctl->ring_empty[item % kRing], ((item / kRing) & 1) ^ 1u, abort_flag);
+            return ok;
+        };
+        auto hand_over = [&](int slot) {
+            fence_proxy_async_smem(); // the tensor core reads through the asynchronous proxy
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ctl->ring_full[slot]);
+            }
+        };
         if constexpr (!kMx) {
             // 16-bit rows: cp.async into place; an item is handed over when the next one has been issued
-            int slot_done = 0;
-            auto hand_over = [&](int slot) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&ctl->ring_full[slot]);
-                }
-            };
-            int item = 0;
-            auto load_item = [&](const uint8_t *src, int j) {
-                const int slot = item % kRing;
-                if (!mbar_wait(&ctl->ring_empty[slot], ((item / kRing) & 1) ^ 1u, abort_flag)) {
-                    ok = false;
+            auto put = [&](const uint8_t *src, const int64_t (&row)[2]) {
+                if (!wait_empty()) {
                     return;
                 }
-                const uint32_t dst = ring_base + slot * Sh::kTileBytes;
+                const uint32_t dst = ring_base + (item % kRing) * Sh::kTileBytes;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = i * 32 + (tid >> 2);
-                    const int64_t row = cache_row(j, r);
-                    const uint8_t *from = src + (row < 0 ? 0 : row) * RB;
-                    const int bytes = row < 0 ? 0 : 16;
+                for (int i = 0; i < 2; ++i) {
+                    const uint8_t *from = src + (row[i] < 0 ? 0 : row[i]) * RB + p * 32;
+                    const int bytes = row[i] < 0 ? 0 : 16;
 #pragma unroll
                     for (int half = 0; half < kHalves; ++half) {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int chunk = 2 * p + c;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + half * Sh::kHalfBytes + swz(r, chunk)),
-                                         "l"(from + half * 128 + chunk * 16), "r"(bytes)
-                                         : "memory");
-                        }
+                        const uint32_t to = dst + half * Sh::kHalfBytes + i * 64 * 128;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at0), "l"(from + half * 128), "r"(bytes) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at1), "l"(from + half * 128 + 16), "r"(bytes) : "memory");
                     }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (item > 0) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    hand_over(slot_done);
+                    hand_over((item - 1) % kRing);
                 }
-                slot_done = slot;
                 ++item;
             };
-            prefetch(0);
-            prefetch(1);
+            put(a.k, row_v);
             describe(0);
-            load_item(a.k, 0);
+            describe(1);
+            rows_from_pids(row_k, 1);
+            load_pids(2);
+#pragma unroll 1
             for (int j = 0; j < tiles && ok; ++j) {
-                prefetch(j + 2);
                 if (j + 1 < tiles) {
-                    describe(j + 1);
-                    load_item(a.k, j + 1);
+                    put(a.k, row_k);
                 }
+                describe(j + 2);
+                rows_from_pids(row_next, j + 2);
+                load_pids(j + 3);
                 if (ok) {
-                    load_item(a.v, j);
+                    put(a.v, row_v);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    row_v[i] = row_k[i];
+                    row_k[i] = row_next[i];
                 }
             }
             if (ok) {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
-                hand_over(slot_done);
+                hand_over((item - 1) % kRing);
             }
         } else {
-            constexpr int kBatch = kHalves * 2; // units of 16 elements in flight: rows i, i + 1 of four, both halves
             struct Batch {
-                uint32_t c[kBatch][4];
+                uint32_t c[2 * kHalves][kFmt == kKvMxFp8 ? 4 : 2];
                 uint32_t s[2]; // the rows' scale bytes
             };
-            auto fetch = [&](Batch &b, bool is_v, int j, int which) {
+            auto fetch = [&](Batch &b, const uint8_t *data, const uint8_t *scale, const int64_t (&row)[2]) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int64_t row = cache_row(j, (2 * which + i) * 32 + (tid >> 2));
-                    b.s[i] = 0;
-                    if (row >= 0) {
-                        b.s[i] = row_scales<kD>(is_v ? a.vs : a.ks, row);
-                    }
+                    const bool live = row[i] >= 0;
+                    b.s[i] = live ? row_scales<kD>(scale, row[i]) : 0u;
+                    const uint8_t *src = data + row[i] * RB + p * (RB / kHalves / 4);
 #pragma unroll
                     for (int half = 0; half < kHalves; ++half) {
-                        uint32_t(&c)[4] = b.c[i * kHalves + half];
-                        c[0] = c[1] = c[2] = c[3] = 0;
-                        if (row >= 0) {
-                            const uint8_t *src = (is_v ? a.v : a.k) + row * RB;
-                            if constexpr (kFmt == kKvMxFp8) {
-                                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + half * 64) + p);
-                                c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
-                            } else {
-                                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src + half * 32) + p);
-                                c[0] = v.x, c[1] = v.y;
-                            }
+                        uint32_t *c = b.c[i * kHalves + half];
+                        if constexpr (kFmt == kKvMxFp8) {
+                            const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + half * 64)) : make_uint4(0, 0, 0, 0);
+                            c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+                        } else {
+                            const uint2 v = live ? __ldg(reinterpret_cast<const uint2 *>(src + half * 32)) : make_uint2(0, 0);
+                            c[0] = v.x, c[1] = v.y;
                         }
                     }
                 }
             };
-            auto put = [&](const Batch &b, bool is_v, bool as_bf16, uint32_t dst, int which) {
+            // stores a fetched item; tile j has been described by then
+            auto put = [&](const Batch &b, bool is_v, int j) {
+                if (!wait_empty() || !(ok = mbar_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag))) {
+                    return;
+                }
+                const Info &info = ctl->info[j % kInfo];
+                const uint32_t flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
+                const uint32_t dst = ring_base + (item % kRing) * Sh::kTileBytes;
+                if (!(flags & (is_v ? 2u : 1u))) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = (2 * which + i) * 32 + (tid >> 2);
-                    const bool relative = !is_v && !scales_in_range<kD, kFmt>(b.s[i]);
-                    const int top = relative ? static_cast<int>(largest_scale<kD>(b.s[i])) : 127;
+                    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                    for (int half = 0; half < kHalves; ++half) {
-                        uint32_t w[8];
-                        codes16_to_f16<kFmt>(b.c[i * kHalves + half], w);
-                        const uint32_t byte = (b.s[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
-                        if (as_bf16) {
+                        for (int half = 0; half < kHalves; ++half) {
+                            uint32_t w[8];
+                            codes16_to_f16<kFmt>(b.c[i * kHalves + half], w);
+                            // 2^(byte - 127) in both halves; 255: infinity, times the block's zeros the NaN it stands for
+                            const float f = __uint_as_float(((b.s[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu) << 23);
+                            const uint32_t m = pack_16x2<false>(f, f);
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                w[x] = mul_16x2<false>(w[x], m);
+                            }
+                            const uint32_t to = dst + half * Sh::kHalfBytes + i * 64 * 128;
+                            sts128(to + at0, w[0], w[1], w[2], w[3]);
+                            sts128(to + at1, w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < 2 * kHalves; ++u) {
+                        const int i = u / kHalves, half = u % kHalves;
+                        uint32_t c[4] = {0, 0, 0, 0}, w[8];
+                        uint32_t scales = 0;
+#pragma unroll
+                        for (int y = 0; y < 2 * kHalves; ++y) {
+                            if (y == u) {
+#pragma unroll
+                                for (int x = 0; x < (kFmt == kKvMxFp8 ? 4 : 2); ++x) {
+                                    c[x] = b.c[y][x];
+                                }
+                                scales = b.s[y / kHalves];
+                            }
+                        }
+                        codes16_to_f16<kFmt>(c, w);
+                        const uint32_t byte = (scales >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
+                        if (is_v) { // bfloat16
                             const uint32_t m = byte * 0x00800080u; // 2^(byte - 127) twice; 255: infinity, times 0 NaN
 #pragma unroll
                             for (int x = 0; x < 8; ++x) {
                                 const uint32_t y = (w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu); // times 2^-112
                                 w[x] = mul_16x2<true>(mul_16x2<true>(y, 0x77807780u), m);
                             }
-                        } else {
-                            const int e = static_cast<int>(byte) - top + 127; // below 1: far under the key's largest element
+                        } else { // keys with a block out of range: relative to their largest scale
+                            const bool relative = !scales_in_range<kD, kFmt>(scales);
+                            const int e = static_cast<int>(byte) - (relative ? static_cast<int>(largest_scale<kD>(scales)) : 127) + 127;
                             const float f = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(max(e, 0)) << 23);
                             const uint32_t m = pack_16x2<false>(f, f);
 #pragma unroll
@@ -480,64 +554,46 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                                 w[x] = mul_16x2<false>(w[x], m);
                             }
                         }
-                        const uint32_t at = dst + half * Sh::kHalfBytes;
-                        sts128(at + swz(r, 2 * p), w[0], w[1], w[2], w[3]);
-                        sts128(at + swz(r, 2 * p + 1), w[4], w[5], w[6], w[7]);
+                        const uint32_t to = dst + half * Sh::kHalfBytes + i * 64 * 128;
+                        sts128(to + at0, w[0], w[1], w[2], w[3]);
+                        sts128(to + at1, w[4], w[5], w[6], w[7]);
                     }
                 }
+                hand_over(item % kRing);
+                ++item;
             };
-            // item i is K or V of a tile
-            const int items = 2 * tiles;
-            auto what = [&](int i, bool &is_v, int &j) {
-                if (i == 0) {
-                    is_v = false;
-                    j = 0;
-                } else if (i == items - 1) {
-                    is_v = true;
-                    j = tiles - 1;
-                } else {
-                    is_v = (i & 1) == 0;
-                    j = is_v ? i / 2 - 1 : (i + 1) / 2;
+            Batch bk, bv;
+            fetch(bk, a.k, a.ks, row_v);
+            if (describes) {
+                load_own_scales(0);
+            }
+            describe(0);
+            rows_from_pids(row_k, 1);
+            load_pids(2);
+            put(bk, false, 0);
+            fetch(bk, a.k, a.ks, row_k);
+            describe(1);
+            if (warp == 8 + kLoadWarps - 1 && tiles > 2) {
+                pid_l2 = page_of(2, (lane & 7) * 16);
+            }
+#pragma unroll 1
+            for (int j = 0; j < tiles && ok; ++j) {
+                fetch(bv, a.v, a.vs, row_v);
+                rows_from_pids(row_next, j + 2);
+                load_pids(j + 3);
+                prefetch(j + 2);
+                if (j + 1 < tiles) {
+                    put(bk, false, j + 1);
                 }
-            };
-            Batch b0, b1;
-            bool is_v;
-            int j;
-            prefetch(0);
-            prefetch(1);
-            what(0, is_v, j);
-            fetch(b0, is_v, j, 0);
-            for (int i = 0; i < items && ok; ++i) {
-                what(i, is_v, j);
-                fetch(b1, is_v, j, 1);
-                if (!is_v) {
-                    prefetch(j + 2);
-                    describe(j);
+                fetch(bk, a.k, a.ks, row_next);
+                describe(j + 2);
+                if (ok) {
+                    put(bv, true, j);
                 }
-                const int slot = i % kRing;
-                if (!mbar_wait(&ctl->ring_empty[slot], ((i / kRing) & 1) ^ 1u, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                bool as_bf16 = false;
-                if (is_v) { // described with K(j), by all four warps
-                    ok = mbar_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag);
-                    const Info &info = ctl->info[j % kInfo];
-                    as_bf16 = ((info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3]) & 2u) != 0;
-                }
-                const uint32_t dst = ring_base + slot * Sh::kTileBytes;
-                put(b0, is_v, as_bf16, dst, 0);
-                if (i + 1 < items) {
-                    bool next_v;
-                    int next_j;
-                    what(i + 1, next_v, next_j);
-                    fetch(b0, next_v, next_j, 0);
-                }
-                put(b1, is_v, as_bf16, dst, 1);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&ctl->ring_full[slot]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    row_v[i] = row_k[i];
+                    row_k[i] = row_next[i];
                 }
             }
         }
@@ -566,41 +622,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             }
             const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
             const uint32_t keep = live && a.scale_log2 != 0.0f ? 0xffffffffu : 0u;
-            float inv = 1.0f, factor = 1.0f;
-            if constexpr (kBf16 && kMx) {
-                float top = 0.0f;
-                if (live) {
-#pragma unroll 4
-                    for (int c = 0; c < kD / 8; ++c) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + c);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t w[kD / 2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 f = unpack_16x2<true>(w[i]);
-                            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-                        }
-                    }
-                }
-                const int field = min(max(static_cast<int>(__float_as_uint(top) >> 23), 29), 254);
-                factor = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
-                inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
-            }
-#pragma unroll 4
             for (int c = 0; c < kD / 8; ++c) {
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (live) {
                     v = __ldg(reinterpret_cast<const uint4 *>(src) + c);
                 }
-                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+            }
+            float factor = 1.0f;
+            if constexpr (kBf16 && kMx) {
+                float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (kBf16 && kMx) {
-                        const float2 f = unpack_16x2<true>(w[i]);
-                        w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
-                    }
-                    w[i] = (w[i] & keep) ^ sign;
+                for (int i = 0; i < kD / 2; ++i) {
+                    const float2 f = unpack_16x2<true>(w[i]);
+                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                 }
-                sts128(q_base + (c >> 3) * Sh::kHalfBytes + swz(row_in_tile, c & 7), w[0], w[1], w[2], w[3]);
+                const int field = min(max(static_cast<int>(__float_as_uint(top) >> 23), 29), 254);
+                factor = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
+                const float inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
+#pragma unroll
+                for (int i = 0; i < kD / 2; ++i) {
+                    const float2 f = unpack_16x2<true>(w[i]);
+                    w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kD / 8; ++c) {
+                sts128(q_base + (c >> 3) * Sh::kHalfBytes + swz(row_in_tile, c & 7), (w[4 * c] & keep) ^ sign, (w[4 * c + 1] & keep) ^ sign,
+                       (w[4 * c + 2] & keep) ^ sign, (w[4 * c + 3] & keep) ^ sign);
             }
             if constexpr (!kPair) {
                 ctl->q_factor[row_in_tile] = factor;
@@ -626,56 +677,53 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 break;
             }
             tc_fence_after();
-            uint32_t sr[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_ld_32x32(s_addr + c * 32, sr[c]);
-            }
-            tmem_ld_wait();
-            tc_fence_before();
-            if (lane == 0) {
-                mbar_arrive(&ctl->s_free[t]);
-            }
             const Info &info = ctl->info[j % kInfo];
-            bool p_bf16 = kOpBf16;
+            const bool all_valid = (info.valid[0] & info.valid[1] & info.valid[2] & info.valid[3]) == 0xffffffffu;
+            uint32_t flags = 0;
             if constexpr (kMx) {
-                const uint32_t f = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
-                p_bf16 = (f & 2u) != 0;
-                if (f & 1u) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            sr[c][i] = __float_as_uint(__uint_as_float(sr[c][i]) * __uint_as_float(static_cast<uint32_t>(info.factor[c * 32 + i]) << 16));
-                        }
-                    }
-                }
+                flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
             }
-            if ((info.valid[0] & info.valid[1] & info.valid[2] & info.valid[3]) != 0xffffffffu) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t valid = info.valid[c];
+            const bool plain = all_valid && !(flags & 1u);
+            // 32 logits, with their keys' factors and without the keys that do not exist
+            auto correct = [&](uint32_t (&x)[32], int c) {
+                if (flags & 1u) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        if (!((valid >> i) & 1u)) {
-                            sr[c][i] = 0xff800000u;
-                        }
+                        x[i] = __float_as_uint(__uint_as_float(x[i]) * __uint_as_float(static_cast<uint32_t>(info.factor[c * 32 + i]) << 16));
                     }
                 }
-            }
-            float mx8[8];
+                const uint32_t valid = info.valid[c];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                mx8[u] = fmaxf(__uint_as_float(sr[0][u]), __uint_as_float(sr[0][8 + u]));
-            }
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = (valid >> i) & 1u ? x[i] : 0xff800000u;
+                }
+            };
+            // ---- first pass: the maximum
+            float mx = -INFINITY;
+            {
+                uint32_t x[2][32];
+                tmem_ld_32x32(s_addr, x[0]);
 #pragma unroll
-            for (int i = 16; i < 128; i += 16) {
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_wait();
+                    if (c < 3) {
+                        tmem_ld_32x32(s_addr + (c + 1) * 32, x[(c + 1) & 1]);
+                    }
+                    uint32_t(&y)[32] = x[c & 1];
+                    if (!plain) {
+                        correct(y, c);
+                    }
+                    float m4[4];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    mx8[u] = fmaxf(mx8[u], fmaxf(__uint_as_float(sr[i >> 5][(i & 31) + u]), __uint_as_float(sr[i >> 5][(i & 31) + 8 + u])));
+                    for (int u = 0; u < 4; ++u) {
+                        m4[u] = max3(__uint_as_float(y[u]), __uint_as_float(y[u + 4]), __uint_as_float(y[u + 8]));
+                        m4[u] = max3(m4[u], __uint_as_float(y[u + 12]), __uint_as_float(y[u + 16]));
+                        m4[u] = max3(m4[u], __uint_as_float(y[u + 20]), __uint_as_float(y[u + 24]));
+                        m4[u] = fmaxf(m4[u], __uint_as_float(y[u + 28]));
+                    }
+                    mx = max3(mx, max3(m4[0], m4[1], m4[2]), m4[3]);
                 }
             }
-            const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
             const float m_new = fmaxf(m_run, mx);
             // also true on the first tile that has a key; false (NaN) while there is none
             const bool grow = (m_new - m_run) * row_scale > kDefer;
@@ -708,24 +756,54 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 m_run = m_new;
             }
             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
+            // ---- second pass: the probabilities
             float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            {
+                uint32_t x[2][32];
+                tmem_ld_32x32(s_addr, x[0]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t pk[16];
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_wait();
+                    if (c < 3) {
+                        tmem_ld_32x32(s_addr + (c + 1) * 32, x[(c + 1) & 1]);
+                    } else {
+                        tc_fence_before();
+                        if (lane == 0) {
+                            mbar_arrive(&ctl->s_free[t]); // the next S may overwrite this one
+                        }
+                    }
+                    uint32_t(&y)[32] = x[c & 1];
+                    if (!plain) {
+                        correct(y, c);
+                    }
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float p0 = ex2w(fmaf(__uint_as_float(sr[c][i]), row_scale, neg_m));
-                    const float p1 = ex2w(fmaf(__uint_as_float(sr[c][i + 1]), row_scale, neg_m));
-                    sum4[(i >> 1) & 3] += p0 + p1;
-                    pk[i >> 1] = p_bf16 ? pack_16x2<true>(p0, p1) : pack_16x2<false>(p0, p1);
-                }
-                if (c == 0 && !pv_waited) { // the previous product must have read P's buffer
-                    ok = mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag);
-                }
+                    for (int i = 0; i < 32; i += 2) {
+                        const float p0 = ex2w(fmaf(__uint_as_float(y[i]), row_scale, neg_m));
+                        const float p1 = ex2w(fmaf(__uint_as_float(y[i + 1]), row_scale, neg_m));
+                        sum4[(i >> 1) & 3] += p0 + p1;
+                        y[i] = __float_as_uint(p0);
+                        y[i + 1] = __float_as_uint(p1);
+                    }
+                    uint32_t *pk = y; // packed in place
+                    if (kMx && kBf16 && (flags & 2u)) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    sts128(p_base + (c >> 1) * Sh::kHalfBytes + swz(row_in_tile, (c & 1) * 4 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2],
-                           pk[4 * q + 3]);
+                        for (int i = 0; i < 16; ++i) {
+                            pk[i] = pack_16x2<true>(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            pk[i] = pack_16x2<kOpBf16>(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+                        }
+                    }
+                    if (c == 0 && !pv_waited) { // the previous product must have read P's buffer
+                        ok = mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        sts128(p_base + (c >> 1) * Sh::kHalfBytes + swz(row_in_tile, (c & 1) * 4 + q), pk[4 * q], pk[4 * q + 1],
+                               pk[4 * q + 2], pk[4 * q + 3]);
+                    }
                 }
             }
             if (!ok) {
@@ -782,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
         }
         __syncthreads();
     }
-    if (warp == 12) {
+    if (warp == kIssueWarp) {
         tc_fence_after();
         tmem_dealloc(tmem_base, kTmemCols);
     }
@@ -793,13 +871,13 @@ int launch_one(const AttnArgs &a, DeviceStatus *status, cudaStream_t stream)
 {
     using Sh = Shape<kD, kPair>;
     const void *kernel = reinterpret_cast<const void *>(&prefix_wide_kernel<kBf16, kD, kFmt, kPair>);
-    // the warps' register budgets are moved around inside what the block was launched with: less would wait forever
+    // registers move between the warps inside what the block was launched with: with fewer the increase would wait forever
     static const int regs = [kernel] {
         cudaFuncAttributes attr;
         return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
     }();
-    if (regs * kThreads < (2 * kRegsSoftmax + kRegsLoad + kRegsIssue) * 128) {
-        set_error_text("prefix_attn: the kernel was built with %d registers, too few for its split", regs);
+    if (regs != kRegsLaunch) {
+        set_error_text("prefix_attn: the kernel was built with %d registers a thread, not %d", regs, kRegsLaunch);
         return kErrUnsupportedShape;
     }
     const int rc = ensure_dynamic_smem(kernel, Sh::kSmem);
