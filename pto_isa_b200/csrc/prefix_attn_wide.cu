@@ -30,11 +30,20 @@ namespace pto_b200 {
 
 namespace {
 
-constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-15 loading; 16, 17 issuing (one per group); 18, 19 idle
-// registers of a thread: 96 at launch (five warps a scheduler), then (2 * 120 + 2 * 96 + 40) * 128 of these 640 * 96
-constexpr int kRegsLaunch = 96, kRegsSoftmax = 120, kRegsIssue = 40;
-static_assert((2 * kRegsSoftmax + 2 * kRegsLaunch + kRegsIssue) * 128 <= kThreads * kRegsLaunch, "an increase would wait forever");
-constexpr int kLoadWarps = 8, kIssueWarp = 16;
+constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-11 loading K, 12-15 loading V; 16, 17 issuing (one per group); 18, 19 idle
+// registers of a thread: 96 at launch (five warps a scheduler), then 2 * 112 + 2 * 96 + 64 (codes) or 2 * 112 + 2 * 88
+// + 80 (16-bit rows), times 128, which is all of these 640 * 96.  No role
+// may spill: shared memory leaves the first-level cache so little that every reload comes from L2 (with 40 registers the
+// issuing threads reloaded descriptors and took 700 cycles for a product).
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 112;
+__host__ __device__ constexpr int regs_load(bool codes) { return codes ? 88 : 88; }
+__host__ __device__ constexpr int regs_issue(bool codes) { return codes ? 80 : 80; }
+constexpr bool regs_fit(bool codes)
+{
+    return (2 * kRegsSoftmax + 2 * regs_load(codes) + regs_issue(codes)) * 128 <= kThreads * kRegsLaunch;
+}
+static_assert(regs_fit(true) && regs_fit(false), "an increase would wait forever");
+constexpr int kIssueWarp = 16;
 constexpr int kTile = 128;
 constexpr int kTmemCols = 512;
 constexpr float kDefer = 8.0f; // log2 of the growth of a row's maximum that rescales O
@@ -51,14 +60,14 @@ struct Shape {
     static constexpr int kHalfBytes = kTile * 128;    // 64 columns of 16 bits, one swizzled half
     static constexpr int kPBytes = 2 * kHalfBytes;
     static constexpr int kQTiles = kPair ? 2 : 1;
-    static constexpr int kRing = kD == 64 ? 6 : (kPair ? 3 : 4);
-    // Tiles whose description is kept.  Tile j + 2 is described when K(j + 1), item 2 j + 1, has been stored, so when all items
-    // up to 2 j + 1 - kRing were used up; what that leaves of earlier tiles: 3 slots V(j - 2), all of tile j - 2; 4 slots
-    // V(j - 3); 6 slots V(j - 4).
-    static constexpr int kInfo = kRing == 3 ? 4 : (kRing == 4 ? 6 : 8);
+    static constexpr int kRingK = kD == 64 ? 3 : 2, kRingV = kD == 64 ? 3 : (kPair ? 1 : 2);
+    // Tiles whose description is kept.  Tile m + 1 is described when K(m) has been stored, so when the product with
+    // K(m - kRingK) is complete; the oldest tile that a group can then still be at is m - 6 (one tile of rows, three slots:
+    // the group of K(m - 4) has yet to issue the product with V(m - 6)).
+    static constexpr int kInfo = 8;
     struct Control {
         uint64_t q_full[2];
-        uint64_t ring_full[kRing], ring_empty[kRing];
+        uint64_t k_full[kRingK], k_empty[kRingK], v_full[kRingV], v_empty[kRingV];
         uint64_t info_full[kInfo];
         uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
         uint32_t tmem_base;
@@ -66,7 +75,7 @@ struct Shape {
         float q_factor[kPair ? 1 : kTile]; // what the rows of q were divided by, for the group that did not load them
         Info info[kInfo];
     };
-    static constexpr int kData = kQTiles * kTileBytes + kRing * kTileBytes + 2 * kPBytes;
+    static constexpr int kData = (kQTiles + kRingK + kRingV) * kTileBytes + 2 * kPBytes;
     static constexpr int kSmem = kData + static_cast<int>(sizeof(Control));
     static_assert(kSmem <= 232448, "shared memory of a block");
 };
@@ -88,6 +97,16 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// a whole warp waits: one lane polls, what it has acquired holds for the warp
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int lane)
+{
+    bool ok = true;
+    if (lane == 0) {
+        ok = mbar_wait(bar, parity, abort_flag);
+    }
+    return __shfl_sync(0xffffffffu, ok, 0);
 }
 
 // where 16 bytes (8 elements) `chunk` of row `row` lie in a 64-column half
@@ -162,12 +181,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     using Control = typename Sh::Control;
     constexpr bool kMx = kFmt >= kKvMxFp8;
     constexpr bool kOpBf16 = kBf16 && !kMx; // type of the products' operands (but for V and P of flagged tiles)
-    constexpr int kRing = Sh::kRing, kInfo = Sh::kInfo;
+    constexpr int kRingK = Sh::kRingK, kRingV = Sh::kRingV, kInfo = Sh::kInfo;
     constexpr int kHalves = kD / 64;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *smem_q = smem;
-    uint8_t *smem_ring = smem_q + Sh::kQTiles * Sh::kTileBytes;
-    uint8_t *smem_p = smem_ring + kRing * Sh::kTileBytes;
+    uint8_t *smem_k = smem_q + Sh::kQTiles * Sh::kTileBytes;
+    uint8_t *smem_v = smem_k + kRingK * Sh::kTileBytes;
+    uint8_t *smem_p = smem_v + kRingV * Sh::kTileBytes;
     Control *ctl = reinterpret_cast<Control *>(smem_p + 2 * Sh::kPBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -192,9 +212,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             mbar_init(&ctl->p_full[t], 4);
             mbar_init(&ctl->pv_done[t], 1);
         }
-        for (int s = 0; s < kRing; ++s) {
-            mbar_init(&ctl->ring_full[s], kLoadWarps);
-            mbar_init(&ctl->ring_empty[s], kPair ? 2 : 1);
+        for (int s = 0; s < kRingK; ++s) {
+            mbar_init(&ctl->k_full[s], 4);
+            mbar_init(&ctl->k_empty[s], kPair ? 2 : 1);
+        }
+        for (int s = 0; s < kRingV; ++s) {
+            mbar_init(&ctl->v_full[s], 4);
+            mbar_init(&ctl->v_empty[s], kPair ? 2 : 1);
         }
         for (int s = 0; s < kInfo; ++s) {
             mbar_init(&ctl->info_full[s], 4);
@@ -211,12 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem_base = ctl->tmem_base;
     volatile int *abort_flag = &ctl->abort_flag;
-    // items of the ring in order: K(0), then for every tile j: K(j + 1) (if any), V(j)
-    auto item_k = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
-    auto item_v = [&](int j) { return j + 1 < tiles ? 2 * j + 2 : 2 * tiles - 1; };
-
     if (warp >= kIssueWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        constexpr int kRegs = regs_issue(kMx);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
         // ------------------------------------------------------------ issuing warps, one per group
         const int t = warp - kIssueWarp;
         if (t < 2 && lane == 0) {
@@ -226,19 +247,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             const uint32_t s_tmem = tmem_base + t * 128, o_tmem = tmem_base + 256 + t * 128;
             const uint64_t q_desc = make_sw128_desc(smem_u32(smem_q) + (kPair ? t : 0) * Sh::kTileBytes, 16, 1024);
             const uint64_t p_desc = make_sw128_desc(smem_u32(smem_p) + t * Sh::kPBytes, 16, 1024);
-            const uint32_t ring_base = smem_u32(smem_ring);
             auto kstep = [](int kk) -> uint64_t { return static_cast<uint64_t>((kk >> 2) * (Sh::kHalfBytes >> 4) + (kk & 3) * 2); };
             bool ok = true;
-            auto ring_wait = [&](int item, uint32_t &addr) {
-                const int slot = item % kRing;
-                addr = ring_base + slot * Sh::kTileBytes;
-                ok = mbar_wait(&ctl->ring_full[slot], (item / kRing) & 1, abort_flag);
-            };
             // S of the group's n-th tile (key tile j)
             auto do_s = [&](int j, int n) {
-                uint32_t addr;
-                const int item = item_k(j);
-                ring_wait(item, addr);
+                const int slot = j % kRingK;
+                const uint32_t addr = smem_u32(smem_k) + slot * Sh::kTileBytes;
+                ok = mbar_wait(&ctl->k_full[slot], (j / kRingK) & 1, abort_flag);
                 if (ok && group_rows[t]) {
                     if (n == 0) {
                         ok = mbar_wait(&ctl->q_full[kPair ? t : 0], 0, abort_flag);
@@ -256,13 +271,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     }
                 }
                 if (ok) {
-                    tc_commit(&ctl->ring_empty[item % kRing]);
+                    tc_commit(&ctl->k_empty[slot]);
                 }
             };
             auto do_pv = [&](int j, int n) {
-                uint32_t addr;
-                const int item = item_v(j);
-                ring_wait(item, addr);
+                const int slot = j % kRingV;
+                const uint32_t addr = smem_u32(smem_v) + slot * Sh::kTileBytes;
+                ok = mbar_wait(&ctl->v_full[slot], (j / kRingV) & 1, abort_flag);
                 if (ok && group_rows[t]) {
                     ok = mbar_wait(&ctl->p_full[t], n & 1, abort_flag);
                     if (ok) {
@@ -283,33 +298,40 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     }
                 }
                 if (ok) {
-                    tc_commit(&ctl->ring_empty[item % kRing]);
+                    tc_commit(&ctl->v_empty[slot]);
                 }
             };
+            // S of a tile is issued before the product with V of the one before it
             constexpr int kHop = kPair ? 1 : 2;
-            const int first = kPair ? 0 : t;
-            if (first < tiles) {
-                do_s(first, 0);
-            }
-            int n = 0;
-            for (int j = first; j < tiles && ok; j += kHop, ++n) {
+            int n = -1;
+#pragma unroll 1
+            for (int j = (kPair ? 0 : t) - kHop; j < tiles && ok; j += kHop, ++n) {
                 if (j + kHop < tiles) {
                     do_s(j + kHop, n + 1);
                 }
-                if (ok) {
+                if (ok && n >= 0) {
                     do_pv(j, n);
                 }
             }
         }
     } else if (warp >= 8) {
+        constexpr int kRegs = regs_load(kMx);
+        if constexpr (kRegs < kRegsLaunch) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+        }
         // ------------------------------------------------------------ loading warps
-        // A thread's share of an item: 16 elements p of each 64-column half in rows r0 and r0 + 64.  Page numbers are loaded a
-        // tile before they are used, the scales for a description likewise, codes one item before they are stored: no load
-        // waits for another in the steady state.
-        const int tid = threadIdx.x - 256;
+        // One warpgroup for K, one for V, the same code.  A thread's share of a tile: 16 elements p of each 64-column half in
+        // the rows r0 + 32 i.  All loads of a tile are issued before any is used and the two groups take turns at waiting
+        // for memory.  (Loads in flight across the fence before a hand-over would be waited for by it: no tile's loads are
+        // issued before the last one has been handed over; the L2 prefetch, two tiles ahead, is what hides DRAM.)
+        const bool is_v = warp >= 12;
+        const int tid = threadIdx.x & 127;
         const int p = tid & 3, r0 = tid >> 2;
         constexpr int RB = kv_row_bytes(kFmt, kD);
-        const uint32_t ring_base = smem_u32(smem_ring);
+        const int ring = is_v ? kRingV : kRingK;
+        uint64_t *full = is_v ? ctl->v_full : ctl->k_full, *empty = is_v ? ctl->v_empty : ctl->k_empty;
+        const uint32_t ring_base = smem_u32(is_v ? smem_v : smem_k);
+        const uint8_t *data = is_v ? a.v : a.k;
         const uint32_t at0 = swz(r0, 2 * p), at1 = at0 ^ 16; // of the two 16-byte chunks, row r0
         const int page_mask = (1 << a.page_shift) - 1;
         // page of key r of tile j; -1: no such key.  Numbers out of range count as if there were no key.
@@ -323,9 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                        ? -1
                        : ((static_cast<int64_t>(page) * a.kv_heads + h) << a.page_shift) + ((k_begin + j * kTile + r) & page_mask);
         };
-        // ---- what the other warps have to know about a tile: warps 8 .. 11, one key a thread
-        const bool describes = tid < kTile;
-        int pid_own = -1, pid_own_next = -1;
+        // K's group describes the tiles, one key a thread; page numbers and scales are loaded a tile ahead
+        int pid_own = page_of(0, tid), pid_own_next = tiles > 1 ? page_of(1, tid) : -1;
         uint32_t own_ks = 0, own_vs = 0;
         auto load_own_scales = [&](int j) {
             if constexpr (kMx) {
@@ -337,264 +358,184 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 }
             }
         };
-        auto describe = [&](int j) {
-            if (!describes || j >= tiles) {
-                return;
-            }
-            Info &info = ctl->info[j % kInfo];
-            const bool valid = pid_own >= 0 && pid_own < a.num_pages;
-            if (!valid && k_begin + j * kTile + tid < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
-                status->block = blockIdx.x;
-                status->where = 11;
-                status->detail = pid_own;
-            }
-            const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-            uint32_t flags = 0;
-            if constexpr (kMx) {
-                const bool k_out = !scales_in_range<kD, kFmt>(own_ks);
-                // with float16 queries V stays float16: small values only lose what is below float16's last place, as o
-                // itself does, and larger ones than it holds count as infinities
-                const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(own_vs);
-                info.factor[tid] = k_out ? static_cast<uint16_t>(largest_scale<kD>(own_ks) << 7) : 0x3f80;
-                flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
-            }
-            if (lane == 0) {
-                info.valid[warp - 8] = mask;
-                info.flags[warp - 8] = flags;
-            }
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&ctl->info_full[j % kInfo]);
-            }
-            // the next tile's: scales now, the page after it
-            pid_own = pid_own_next;
-            load_own_scales(j + 1);
-            pid_own_next = j + 2 < tiles ? page_of(j + 2, tid) : -1;
-        };
-        // ---- the rows of a tile towards L2, by the last warp: lane = 16 keys of K (0 .. 7) or V (8 .. 15)
-        int pid_l2 = -1;
-        auto prefetch = [&](int j) { // tile j, whose page number was loaded a tile ago
-            if (warp == 8 + kLoadWarps - 1 && j < tiles) {
-                const int64_t row = cache_row(pid_l2, j, (lane & 7) * 16);
-                if (lane < 16 && row >= 0) {
-                    const uint8_t *src = (lane < 8 ? a.k : a.v) + row * RB;
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(16 * RB) : "memory");
-                }
-                pid_l2 = j + 1 < tiles ? page_of(j + 1, (lane & 7) * 16) : -1;
-            }
-        };
-        int pid[2]; // of the tile after the next
-        auto load_pids = [&](int j) {
+        int pid[4]; // of this thread's rows in the next tile
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                pid[i] = j < tiles ? page_of(j, r0 + 64 * i) : -1;
-            }
-        };
-        int64_t row_v[2], row_k[2], row_next[2]; // rows of tiles j, j + 1, j + 2
-        auto rows_from_pids = [&](int64_t (&row)[2], int j) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                row[i] = cache_row(pid[i], j, r0 + 64 * i);
-            }
-        };
-        load_pids(0);
-        if (describes) {
-            pid_own = page_of(0, tid);
-            pid_own_next = tiles > 1 ? page_of(1, tid) : -1;
+        for (int i = 0; i < 4; ++i) {
+            pid[i] = page_of(0, r0 + 32 * i);
         }
-        rows_from_pids(row_v, 0);
-        load_pids(1);
+        load_own_scales(0);
         bool ok = true;
-        int item = 0;
-        auto wait_empty = [&]() {
-            ok = ok && mbar_wait(&ctl->ring_empty[item % kRing], ((item / kRing) & 1) ^ 1u, abort_flag);
-            return ok;
-        };
-        auto hand_over = [&](int slot) {
-            fence_proxy_async_smem(); // the tensor core reads through the asynchronous proxy
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&ctl->ring_full[slot]);
-            }
-        };
-        if constexpr (!kMx) {
-            // 16-bit rows: cp.async into place; an item is handed over when the next one has been issued
-            auto put = [&](const uint8_t *src, const int64_t (&row)[2]) {
-                if (!wait_empty()) {
-                    return;
-                }
-                const uint32_t dst = ring_base + (item % kRing) * Sh::kTileBytes;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint8_t *from = src + (row[i] < 0 ? 0 : row[i]) * RB + p * 32;
-                    const int bytes = row[i] < 0 ? 0 : 16;
-#pragma unroll
-                    for (int half = 0; half < kHalves; ++half) {
-                        const uint32_t to = dst + half * Sh::kHalfBytes + i * 64 * 128;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at0), "l"(from + half * 128), "r"(bytes) : "memory");
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at1), "l"(from + half * 128 + 16), "r"(bytes) : "memory");
-                    }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (item > 0) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    hand_over((item - 1) % kRing);
-                }
-                ++item;
-            };
-            put(a.k, row_v);
-            describe(0);
-            describe(1);
-            rows_from_pids(row_k, 1);
-            load_pids(2);
+        int slot = 0;
+        uint32_t phase = 1;
 #pragma unroll 1
-            for (int j = 0; j < tiles && ok; ++j) {
-                if (j + 1 < tiles) {
-                    put(a.k, row_k);
-                }
-                describe(j + 2);
-                rows_from_pids(row_next, j + 2);
-                load_pids(j + 3);
-                if (ok) {
-                    put(a.v, row_v);
-                }
+        for (int j = -1; j < tiles && ok; ++j) {
+            if (j >= 0) {
+                // ---- the tile's rows
+                int64_t row[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    row_v[i] = row_k[i];
-                    row_k[i] = row_next[i];
+                for (int i = 0; i < 4; ++i) {
+                    row[i] = cache_row(pid[i], j, r0 + 32 * i);
                 }
-            }
-            if (ok) {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                hand_over((item - 1) % kRing);
-            }
-        } else {
-            struct Batch {
-                uint32_t c[2 * kHalves][kFmt == kKvMxFp8 ? 4 : 2];
-                uint32_t s[2]; // the rows' scale bytes
-            };
-            auto fetch = [&](Batch &b, const uint8_t *data, const uint8_t *scale, const int64_t (&row)[2]) {
+                const uint32_t dst = ring_base + slot * Sh::kTileBytes;
+                if constexpr (!kMx) {
+                    ok = warp_wait(&empty[slot], phase, abort_flag, lane);
+                    if (!ok) {
+                        break;
+                    }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bool live = row[i] >= 0;
-                    b.s[i] = live ? row_scales<kD>(scale, row[i]) : 0u;
-                    const uint8_t *src = data + row[i] * RB + p * (RB / kHalves / 4);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint8_t *from = data + (row[i] < 0 ? 0 : row[i]) * RB + p * 32;
+                        const int bytes = row[i] < 0 ? 0 : 16;
 #pragma unroll
-                    for (int half = 0; half < kHalves; ++half) {
-                        uint32_t *c = b.c[i * kHalves + half];
-                        if constexpr (kFmt == kKvMxFp8) {
-                            const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + half * 64)) : make_uint4(0, 0, 0, 0);
-                            c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
-                        } else {
-                            const uint2 v = live ? __ldg(reinterpret_cast<const uint2 *>(src + half * 32)) : make_uint2(0, 0);
-                            c[0] = v.x, c[1] = v.y;
+                        for (int half = 0; half < kHalves; ++half) {
+                            const uint32_t to = dst + half * Sh::kHalfBytes + i * 32 * 128;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at0), "l"(from + half * 128), "r"(bytes) : "memory");
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at1), "l"(from + half * 128 + 16), "r"(bytes) : "memory");
                         }
                     }
-                }
-            };
-            // stores a fetched item; tile j has been described by then
-            auto put = [&](const Batch &b, bool is_v, int j) {
-                if (!wait_empty() || !(ok = mbar_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag))) {
-                    return;
-                }
-                const Info &info = ctl->info[j % kInfo];
-                const uint32_t flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
-                const uint32_t dst = ring_base + (item % kRing) * Sh::kTileBytes;
-                if (!(flags & (is_v ? 2u : 1u))) {
+                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                } else {
+                    constexpr int kWords = kFmt == kKvMxFp8 ? 4 : 2;
+                    uint32_t code[4 * kHalves][kWords], scales[4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < 4; ++i) {
+                        const bool live = row[i] >= 0;
+                        const uint8_t *src = data + row[i] * RB + p * (4 * kWords);
+                        scales[i] = live ? row_scales<kD>(is_v ? a.vs : a.ks, row[i]) : 0u;
+#pragma unroll
+                        for (int half = 0; half < kHalves; ++half) {
+                            uint32_t *c = code[i * kHalves + half];
+                            if constexpr (kFmt == kKvMxFp8) {
+                                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + half * 64)) : make_uint4(0, 0, 0, 0);
+                                c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+                            } else {
+                                const uint2 v = live ? __ldg(reinterpret_cast<const uint2 *>(src + half * 32)) : make_uint2(0, 0);
+                                c[0] = v.x, c[1] = v.y;
+                            }
+                        }
+                    }
+                    ok = warp_wait(&empty[slot], phase, abort_flag, lane) &&
+                         warp_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag, lane);
+                    if (!ok) {
+                        break;
+                    }
+                    const Info &info = ctl->info[j % kInfo];
+                    const uint32_t flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
+                    const bool special = (flags & (is_v ? 2u : 1u)) != 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
 #pragma unroll
                         for (int half = 0; half < kHalves; ++half) {
                             uint32_t w[8];
-                            codes16_to_f16<kFmt>(b.c[i * kHalves + half], w);
+                            codes16_to_f16<kFmt>(code[i * kHalves + half], w);
                             // 2^(byte - 127) in both halves; 255: infinity, times the block's zeros the NaN it stands for
-                            const float f = __uint_as_float(((b.s[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu) << 23);
-                            const uint32_t m = pack_16x2<false>(f, f);
+                            const uint32_t byte = (scales[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
+                            const float f = __uint_as_float(byte << 23);
+                            const uint32_t m = pack_16x2<false>(f, f), to = dst + half * Sh::kHalfBytes + i * 32 * 128;
 #pragma unroll
                             for (int x = 0; x < 8; ++x) {
                                 w[x] = mul_16x2<false>(w[x], m);
                             }
-                            const uint32_t to = dst + half * Sh::kHalfBytes + i * 64 * 128;
                             sts128(to + at0, w[0], w[1], w[2], w[3]);
                             sts128(to + at1, w[4], w[5], w[6], w[7]);
                         }
                     }
-                } else {
+                    if (special) { // rare: the tile once more, from memory, in small steps
 #pragma unroll 1
-                    for (int u = 0; u < 2 * kHalves; ++u) {
-                        const int i = u / kHalves, half = u % kHalves;
-                        uint32_t c[4] = {0, 0, 0, 0}, w[8];
-                        uint32_t scales = 0;
+                        for (int u = 0; u < 4 * kHalves; ++u) {
+                            const int i = u / kHalves, half = u % kHalves;
+                            int page = pid[0];
 #pragma unroll
-                        for (int y = 0; y < 2 * kHalves; ++y) {
-                            if (y == u) {
+                            for (int x = 1; x < 4; ++x) {
+                                page = i == x ? pid[x] : page;
+                            }
+                            const int64_t at = cache_row(page, j, r0 + 32 * i);
+                            uint32_t c[4] = {0, 0, 0, 0}, w[8], scale = 0;
+                            if (at >= 0) {
+                                scale = row_scales<kD>(is_v ? a.vs : a.ks, at);
+                                const uint32_t *src = reinterpret_cast<const uint32_t *>(data + at * RB + half * (RB / kHalves)) + p * kWords;
 #pragma unroll
-                                for (int x = 0; x < (kFmt == kKvMxFp8 ? 4 : 2); ++x) {
-                                    c[x] = b.c[y][x];
+                                for (int x = 0; x < kWords; ++x) {
+                                    c[x] = __ldg(src + x);
                                 }
-                                scales = b.s[y / kHalves];
                             }
-                        }
-                        codes16_to_f16<kFmt>(c, w);
-                        const uint32_t byte = (scales >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
-                        if (is_v) { // bfloat16
-                            const uint32_t m = byte * 0x00800080u; // 2^(byte - 127) twice; 255: infinity, times 0 NaN
+                            codes16_to_f16<kFmt>(c, w);
+                            const uint32_t byte = (scale >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
+                            // keys with a block out of range: relative to their largest scale
+                            const bool relative = !is_v && !scales_in_range<kD, kFmt>(scale);
+                            const int e = relative && byte != 255u ? max(static_cast<int>(byte) + 127 - static_cast<int>(largest_scale<kD>(scale)), 0)
+                                                                   : static_cast<int>(byte);
+                            const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
 #pragma unroll
                             for (int x = 0; x < 8; ++x) {
-                                const uint32_t y = (w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu); // times 2^-112
-                                w[x] = mul_16x2<true>(mul_16x2<true>(y, 0x77807780u), m);
+                                if (is_v) { // bfloat16: the values times 2^-112 to the other format's places, then scaled
+                                    w[x] = mul_16x2<true>((w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu), 0x77807780u);
+                                    w[x] = mul_16x2<true>(w[x], byte * 0x00800080u); // 255: infinity, times 0 NaN
+                                } else {
+                                    w[x] = mul_16x2<false>(w[x], pack_16x2<false>(f, f));
+                                }
                             }
-                        } else { // keys with a block out of range: relative to their largest scale
-                            const bool relative = !scales_in_range<kD, kFmt>(scales);
-                            const int e = static_cast<int>(byte) - (relative ? static_cast<int>(largest_scale<kD>(scales)) : 127) + 127;
-                            const float f = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(max(e, 0)) << 23);
-                            const uint32_t m = pack_16x2<false>(f, f);
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                w[x] = mul_16x2<false>(w[x], m);
-                            }
+                            const uint32_t to = dst + half * Sh::kHalfBytes + i * 32 * 128;
+                            sts128(to + at0, w[0], w[1], w[2], w[3]);
+                            sts128(to + at1, w[4], w[5], w[6], w[7]);
                         }
-                        const uint32_t to = dst + half * Sh::kHalfBytes + i * 64 * 128;
-                        sts128(to + at0, w[0], w[1], w[2], w[3]);
-                        sts128(to + at1, w[4], w[5], w[6], w[7]);
                     }
                 }
-                hand_over(item % kRing);
-                ++item;
-            };
-            Batch bk, bv;
-            fetch(bk, a.k, a.ks, row_v);
-            if (describes) {
-                load_own_scales(0);
-            }
-            describe(0);
-            rows_from_pids(row_k, 1);
-            load_pids(2);
-            put(bk, false, 0);
-            fetch(bk, a.k, a.ks, row_k);
-            describe(1);
-            if (warp == 8 + kLoadWarps - 1 && tiles > 2) {
-                pid_l2 = page_of(2, (lane & 7) * 16);
-            }
-#pragma unroll 1
-            for (int j = 0; j < tiles && ok; ++j) {
-                fetch(bv, a.v, a.vs, row_v);
-                rows_from_pids(row_next, j + 2);
-                load_pids(j + 3);
-                prefetch(j + 2);
-                if (j + 1 < tiles) {
-                    put(bk, false, j + 1);
+                fence_proxy_async_smem(); // the tensor core reads through the asynchronous proxy
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&full[slot]);
                 }
-                fetch(bk, a.k, a.ks, row_next);
-                describe(j + 2);
-                if (ok) {
-                    put(bv, true, j);
+                if (++slot == ring) {
+                    slot = 0;
+                    phase ^= 1u;
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    row_v[i] = row_k[i];
-                    row_k[i] = row_next[i];
+                for (int i = 0; i < 4; ++i) {
+                    pid[i] = j + 1 < tiles ? page_of(j + 1, r0 + 32 * i) : -1;
                 }
+            }
+            if (is_v) {
+                // ---- towards L2: lane = 16 keys, warps 12 and 13 the rows of K and V two tiles ahead (the first two at once)
+                if (warp < 14 && lane < (j < 0 ? 16 : 8)) {
+                    const int ahead = j < 0 ? 1 + (lane >> 3) : j + 3;
+                    const int64_t at = ahead < tiles ? cache_row(page_of(ahead, (lane & 7) * 16), ahead, (lane & 7) * 16) : -1;
+                    if (at >= 0) {
+                        const uint8_t *src = (warp == 12 ? a.k : a.v) + at * RB;
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(16 * RB) : "memory");
+                    }
+                }
+            } else if (j + 1 < tiles) {
+                // ---- what the other warps have to know about tile j + 1
+                Info &info = ctl->info[(j + 1) % kInfo];
+                const bool valid = pid_own >= 0 && pid_own < a.num_pages;
+                if (!valid && k_begin + (j + 1) * kTile + tid < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+                    status->block = blockIdx.x;
+                    status->where = 11;
+                    status->detail = pid_own;
+                }
+                const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+                uint32_t flags = 0;
+                if constexpr (kMx) {
+                    const bool k_out = !scales_in_range<kD, kFmt>(own_ks);
+                    // with float16 queries V stays float16: small values only lose what is below float16's last place, as o
+                    // itself does, and larger ones than it holds count as infinities
+                    const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(own_vs);
+                    info.factor[tid] = k_out ? static_cast<uint16_t>(largest_scale<kD>(own_ks) << 7) : 0x3f80;
+                    flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
+                }
+                if (lane == 0) {
+                    info.valid[warp - 8] = mask;
+                    info.flags[warp - 8] = flags;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&ctl->info_full[(j + 1) % kInfo]);
+                }
+                // the next one's: scales now, the page after it
+                pid_own = pid_own_next;
+                load_own_scales(j + 2);
+                pid_own_next = j + 3 < tiles ? page_of(j + 3, tid) : -1;
             }
         }
     } else {
@@ -622,36 +563,52 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             }
             const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
             const uint32_t keep = live && a.scale_log2 != 0.0f ? 0xffffffffu : 0u;
-            uint32_t w[kD / 2];
-#pragma unroll
-            for (int c = 0; c < kD / 8; ++c) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (live) {
-                    v = __ldg(reinterpret_cast<const uint4 *>(src) + c);
-                }
-                w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
-            }
-            float factor = 1.0f;
+            constexpr int kChunk = 4; // 16-byte loads in flight
+            float factor = 1.0f, inv = 1.0f;
             if constexpr (kBf16 && kMx) {
                 float top = 0.0f;
+#pragma unroll 1
+                for (int c0 = 0; c0 < kD / 8 && live; c0 += kChunk) {
+                    uint4 v[kChunk];
 #pragma unroll
-                for (int i = 0; i < kD / 2; ++i) {
-                    const float2 f = unpack_16x2<true>(w[i]);
-                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    for (int c = 0; c < kChunk; ++c) {
+                        v[c] = __ldg(reinterpret_cast<const uint4 *>(src) + c0 + c);
+                    }
+#pragma unroll
+                    for (int c = 0; c < kChunk; ++c) {
+                        const float2 f0 = unpack_16x2<true>(v[c].x), f1 = unpack_16x2<true>(v[c].y);
+                        const float2 f2 = unpack_16x2<true>(v[c].z), f3 = unpack_16x2<true>(v[c].w);
+                        top = max3(top, fabsf(f0.x), fabsf(f0.y));
+                        top = max3(top, fabsf(f1.x), fabsf(f1.y));
+                        top = max3(top, fabsf(f2.x), fabsf(f2.y));
+                        top = max3(top, fabsf(f3.x), fabsf(f3.y));
+                    }
                 }
                 const int field = min(max(static_cast<int>(__float_as_uint(top) >> 23), 29), 254);
                 factor = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
-                const float inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
-#pragma unroll
-                for (int i = 0; i < kD / 2; ++i) {
-                    const float2 f = unpack_16x2<true>(w[i]);
-                    w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
-                }
+                inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
             }
+#pragma unroll 1
+            for (int c0 = 0; c0 < kD / 8; c0 += kChunk) {
+                uint4 v[kChunk];
 #pragma unroll
-            for (int c = 0; c < kD / 8; ++c) {
-                sts128(q_base + (c >> 3) * Sh::kHalfBytes + swz(row_in_tile, c & 7), (w[4 * c] & keep) ^ sign, (w[4 * c + 1] & keep) ^ sign,
-                       (w[4 * c + 2] & keep) ^ sign, (w[4 * c + 3] & keep) ^ sign);
+                for (int c = 0; c < kChunk; ++c) {
+                    v[c] = live ? __ldg(reinterpret_cast<const uint4 *>(src) + c0 + c) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c) {
+                    uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (kBf16 && kMx) {
+                            const float2 f = unpack_16x2<true>(w[i]);
+                            w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
+                        }
+                        w[i] = (w[i] & keep) ^ sign;
+                    }
+                    const int at = c0 + c;
+                    sts128(q_base + (at >> 3) * Sh::kHalfBytes + swz(row_in_tile, at & 7), w[0], w[1], w[2], w[3]);
+                }
             }
             if constexpr (!kPair) {
                 ctl->q_factor[row_in_tile] = factor;
@@ -663,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             }
             row_scale *= factor;
         } else {
-            ok = mbar_wait(&ctl->q_full[0], 0, abort_flag);
+            ok = warp_wait(&ctl->q_full[0], 0, abort_flag, lane);
             row_scale *= ctl->q_factor[kPair ? 0 : row_in_tile];
         }
 
@@ -672,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
         float l_run = 0.0f;
         int n = 0;
         for (int j = kPair ? 0 : t; j < tiles && ok && rows_here; j += kPair ? 1 : 2, ++n) {
-            if (!mbar_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag) || !mbar_wait(&ctl->s_full[t], n & 1, abort_flag)) {
+            if (!warp_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag, lane) || !warp_wait(&ctl->s_full[t], n & 1, abort_flag, lane)) {
                 ok = false;
                 break;
             }
@@ -684,125 +641,104 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
             }
             const bool plain = all_valid && !(flags & 1u);
-            // 32 logits, with their keys' factors and without the keys that do not exist
-            auto correct = [&](uint32_t (&x)[32], int c) {
-                if (flags & 1u) {
+            // Two passes over the logits, 32 at a time: the maximum, then the probabilities.  One loop, so that the code of
+            // five kinds of warps stays small enough for the instruction cache.
+            float mx = -INFINITY, neg_m = 0.0f, sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            bool pv_waited = n == 0;
+#pragma unroll 1
+            for (int it = 0; it < 8; ++it) {
+                const int c = it & 3;
+                uint32_t x[32];
+                tmem_ld_32x32(s_addr + c * 32, x);
+                if (it == 4) {
+                    const float m_new = fmaxf(m_run, mx);
+                    // also true on the first tile that has a key; false (NaN) while there is none
+                    const bool grow = (m_new - m_run) * row_scale > kDefer;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        if (n > 0) {
+                            if (!warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane)) {
+                                ok = false;
+                                break;
+                            }
+                            pv_waited = true;
+                            tc_fence_after();
+                            // rows without a key yet keep their zeros; the others move to the new reference
+                            const float alpha = m_run == m_new ? 1.0f : ex2w((m_run - m_new) * row_scale);
+                            l_run *= alpha;
+#pragma unroll 1
+                            for (int d = 0; d < kD / 32; ++d) {
+                                uint32_t orow[32];
+                                tmem_ld_32x32(o_addr + d * 32, orow);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    orow[i] = __float_as_uint(__uint_as_float(orow[i]) * alpha);
+                                }
+                                tmem_st_32x32(o_addr + d * 32, orow);
+                            }
+                            tmem_st_wait();
+                            tc_fence_before();
+                        }
+                        m_run = m_new;
+                    }
+                    neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
+                    if (!pv_waited) { // the previous product must have read P's buffer
+                        ok = warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane);
+                        if (!ok) {
+                            break;
+                        }
+                    }
+                }
+                tmem_ld_wait();
+                if (it == 7) {
+                    tc_fence_before();
+                    if (lane == 0) {
+                        mbar_arrive(&ctl->s_free[t]); // the next S may overwrite this one
+                    }
+                }
+                if (!plain) { // the keys' factors, and no keys that do not exist
+                    const uint32_t valid = info.valid[c];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        x[i] = __float_as_uint(__uint_as_float(x[i]) * __uint_as_float(static_cast<uint32_t>(info.factor[c * 32 + i]) << 16));
+                        const float factor = flags & 1u ? __uint_as_float(static_cast<uint32_t>(info.factor[c * 32 + i]) << 16) : 1.0f;
+                        x[i] = (valid >> i) & 1u ? __float_as_uint(__uint_as_float(x[i]) * factor) : 0xff800000u;
                     }
                 }
-                const uint32_t valid = info.valid[c];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    x[i] = (valid >> i) & 1u ? x[i] : 0xff800000u;
-                }
-            };
-            // ---- first pass: the maximum
-            float mx = -INFINITY;
-            {
-                uint32_t x[2][32];
-                tmem_ld_32x32(s_addr, x[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld_wait();
-                    if (c < 3) {
-                        tmem_ld_32x32(s_addr + (c + 1) * 32, x[(c + 1) & 1]);
-                    }
-                    uint32_t(&y)[32] = x[c & 1];
-                    if (!plain) {
-                        correct(y, c);
-                    }
+                if (it < 4) {
                     float m4[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        m4[u] = max3(__uint_as_float(y[u]), __uint_as_float(y[u + 4]), __uint_as_float(y[u + 8]));
-                        m4[u] = max3(m4[u], __uint_as_float(y[u + 12]), __uint_as_float(y[u + 16]));
-                        m4[u] = max3(m4[u], __uint_as_float(y[u + 20]), __uint_as_float(y[u + 24]));
-                        m4[u] = fmaxf(m4[u], __uint_as_float(y[u + 28]));
+                        m4[u] = max3(__uint_as_float(x[u]), __uint_as_float(x[u + 4]), __uint_as_float(x[u + 8]));
+                        m4[u] = max3(m4[u], __uint_as_float(x[u + 12]), __uint_as_float(x[u + 16]));
+                        m4[u] = max3(m4[u], __uint_as_float(x[u + 20]), __uint_as_float(x[u + 24]));
+                        m4[u] = fmaxf(m4[u], __uint_as_float(x[u + 28]));
                     }
                     mx = max3(mx, max3(m4[0], m4[1], m4[2]), m4[3]);
-                }
-            }
-            const float m_new = fmaxf(m_run, mx);
-            // also true on the first tile that has a key; false (NaN) while there is none
-            const bool grow = (m_new - m_run) * row_scale > kDefer;
-            bool pv_waited = n == 0;
-            if (__any_sync(0xffffffffu, grow)) {
-                if (n > 0) {
-                    if (!mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    pv_waited = true;
-                    tc_fence_after();
-                    // rows without a key yet keep their zeros; the others move to the new reference
-                    const float alpha = m_run == m_new ? 1.0f : ex2w((m_run - m_new) * row_scale);
-                    l_run *= alpha;
-#pragma unroll 1
-                    for (int c = 0; c < kD / 32; ++c) {
-                        uint32_t orow[32];
-                        tmem_ld_32x32(o_addr + c * 32, orow);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            orow[i] = __float_as_uint(__uint_as_float(orow[i]) * alpha);
-                        }
-                        tmem_st_32x32(o_addr + c * 32, orow);
-                    }
-                    tmem_st_wait();
-                    tc_fence_before();
-                }
-                m_run = m_new;
-            }
-            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
-            // ---- second pass: the probabilities
-            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            {
-                uint32_t x[2][32];
-                tmem_ld_32x32(s_addr, x[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld_wait();
-                    if (c < 3) {
-                        tmem_ld_32x32(s_addr + (c + 1) * 32, x[(c + 1) & 1]);
-                    } else {
-                        tc_fence_before();
-                        if (lane == 0) {
-                            mbar_arrive(&ctl->s_free[t]); // the next S may overwrite this one
-                        }
-                    }
-                    uint32_t(&y)[32] = x[c & 1];
-                    if (!plain) {
-                        correct(y, c);
-                    }
+                } else {
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float p0 = ex2w(fmaf(__uint_as_float(y[i]), row_scale, neg_m));
-                        const float p1 = ex2w(fmaf(__uint_as_float(y[i + 1]), row_scale, neg_m));
+                        const float p0 = ex2w(fmaf(__uint_as_float(x[i]), row_scale, neg_m));
+                        const float p1 = ex2w(fmaf(__uint_as_float(x[i + 1]), row_scale, neg_m));
                         sum4[(i >> 1) & 3] += p0 + p1;
-                        y[i] = __float_as_uint(p0);
-                        y[i + 1] = __float_as_uint(p1);
+                        x[i] = __float_as_uint(p0);
+                        x[i + 1] = __float_as_uint(p1);
                     }
-                    uint32_t *pk = y; // packed in place
+                    // packed in place
                     if (kMx && kBf16 && (flags & 2u)) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            pk[i] = pack_16x2<true>(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+                            x[i] = pack_16x2<true>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            pk[i] = pack_16x2<kOpBf16>(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+                            x[i] = pack_16x2<kOpBf16>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
                         }
                     }
-                    if (c == 0 && !pv_waited) { // the previous product must have read P's buffer
-                        ok = mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag);
-                    }
+                    const uint32_t to = p_base + (c >> 1) * Sh::kHalfBytes;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        sts128(p_base + (c >> 1) * Sh::kHalfBytes + swz(row_in_tile, (c & 1) * 4 + q), pk[4 * q], pk[4 * q + 1],
-                               pk[4 * q + 2], pk[4 * q + 3]);
+                        sts128(to + swz(row_in_tile, (c & 1) * 4 + q), x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
                     }
                 }
             }
@@ -819,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
         // ---- (O, m, l) of this group's keys
         if (ok && rows_here) {
             if (n > 0) {
-                ok = mbar_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag);
+                ok = warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane);
                 tc_fence_after();
             }
             const int piece = kPair ? split : 2 * split + t;
