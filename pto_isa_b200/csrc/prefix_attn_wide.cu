@@ -641,104 +641,119 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
             }
             const bool plain = all_valid && !(flags & 1u);
-            // Two passes over the logits, 32 at a time: the maximum, then the probabilities.  One loop, so that the code of
-            // five kinds of warps stays small enough for the instruction cache.
-            float mx = -INFINITY, neg_m = 0.0f, sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            bool pv_waited = n == 0;
-#pragma unroll 1
-            for (int it = 0; it < 8; ++it) {
-                const int c = it & 3;
-                uint32_t x[32];
-                tmem_ld_32x32(s_addr + c * 32, x);
-                if (it == 4) {
-                    const float m_new = fmaxf(m_run, mx);
-                    // also true on the first tile that has a key; false (NaN) while there is none
-                    const bool grow = (m_new - m_run) * row_scale > kDefer;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        if (n > 0) {
-                            if (!warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane)) {
-                                ok = false;
-                                break;
-                            }
-                            pv_waited = true;
-                            tc_fence_after();
-                            // rows without a key yet keep their zeros; the others move to the new reference
-                            const float alpha = m_run == m_new ? 1.0f : ex2w((m_run - m_new) * row_scale);
-                            l_run *= alpha;
-#pragma unroll 1
-                            for (int d = 0; d < kD / 32; ++d) {
-                                uint32_t orow[32];
-                                tmem_ld_32x32(o_addr + d * 32, orow);
-                                tmem_ld_wait();
+            // 64 logits from tensor memory; with the keys' factors, and without the keys that do not exist
+            uint32_t x[2][32];
+            auto read = [&](int half) {
+                tmem_ld_32x32(s_addr + half * 64, x[0]);
+                tmem_ld_32x32(s_addr + half * 64 + 32, x[1]);
+                tmem_ld_wait();
+            };
+            auto correct = [&](int half) {
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    orow[i] = __float_as_uint(__uint_as_float(orow[i]) * alpha);
-                                }
-                                tmem_st_32x32(o_addr + d * 32, orow);
-                            }
-                            tmem_st_wait();
-                            tc_fence_before();
-                        }
-                        m_run = m_new;
-                    }
-                    neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
-                    if (!pv_waited) { // the previous product must have read P's buffer
-                        ok = warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane);
-                        if (!ok) {
-                            break;
-                        }
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t valid = info.valid[2 * half + c];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float factor = flags & 1u ? __uint_as_float(static_cast<uint32_t>(info.factor[half * 64 + c * 32 + i]) << 16) : 1.0f;
+                        x[c][i] = (valid >> i) & 1u ? __float_as_uint(__uint_as_float(x[c][i]) * factor) : 0xff800000u;
                     }
                 }
-                tmem_ld_wait();
-                if (it == 7) {
+            };
+            // ---- first pass: the maximum
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                read(half);
+                if (!plain) {
+                    correct(half);
+                }
+                float m8[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    m8[u] = fmaxf(__uint_as_float(x[0][u]), __uint_as_float(x[1][u]));
+#pragma unroll
+                    for (int i = 8; i < 32; i += 8) {
+                        m8[u] = max3(m8[u], __uint_as_float(x[0][i + u]), __uint_as_float(x[1][i + u]));
+                    }
+                }
+                mx = fmaxf(mx, max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+            }
+            const float m_new = fmaxf(m_run, mx);
+            // also true on the first tile that has a key; false (NaN) while there is none
+            const bool grow = (m_new - m_run) * row_scale > kDefer;
+            bool pv_waited = n == 0;
+            if (__any_sync(0xffffffffu, grow)) {
+                if (n > 0) {
+                    if (!warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane)) {
+                        ok = false;
+                        break;
+                    }
+                    pv_waited = true;
+                    tc_fence_after();
+                    // rows without a key yet keep their zeros; the others move to the new reference
+                    const float alpha = m_run == m_new ? 1.0f : ex2w((m_run - m_new) * row_scale);
+                    l_run *= alpha;
+#pragma unroll 1
+                    for (int d = 0; d < kD / 32; ++d) {
+                        uint32_t orow[32];
+                        tmem_ld_32x32(o_addr + d * 32, orow);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            orow[i] = __float_as_uint(__uint_as_float(orow[i]) * alpha);
+                        }
+                        tmem_st_32x32(o_addr + d * 32, orow);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                m_run = m_new;
+            }
+            // ---- second pass: the probabilities
+            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
+            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                read(half);
+                if (half == 1) {
                     tc_fence_before();
                     if (lane == 0) {
                         mbar_arrive(&ctl->s_free[t]); // the next S may overwrite this one
                     }
                 }
-                if (!plain) { // the keys' factors, and no keys that do not exist
-                    const uint32_t valid = info.valid[c];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float factor = flags & 1u ? __uint_as_float(static_cast<uint32_t>(info.factor[c * 32 + i]) << 16) : 1.0f;
-                        x[i] = (valid >> i) & 1u ? __float_as_uint(__uint_as_float(x[i]) * factor) : 0xff800000u;
-                    }
+                if (!plain) {
+                    correct(half);
                 }
-                if (it < 4) {
-                    float m4[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        m4[u] = max3(__uint_as_float(x[u]), __uint_as_float(x[u + 4]), __uint_as_float(x[u + 8]));
-                        m4[u] = max3(m4[u], __uint_as_float(x[u + 12]), __uint_as_float(x[u + 16]));
-                        m4[u] = max3(m4[u], __uint_as_float(x[u + 20]), __uint_as_float(x[u + 24]));
-                        m4[u] = fmaxf(m4[u], __uint_as_float(x[u + 28]));
-                    }
-                    mx = max3(mx, max3(m4[0], m4[1], m4[2]), m4[3]);
-                } else {
+                for (int c = 0; c < 2; ++c) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float p0 = ex2w(fmaf(__uint_as_float(x[i]), row_scale, neg_m));
-                        const float p1 = ex2w(fmaf(__uint_as_float(x[i + 1]), row_scale, neg_m));
+                        const float p0 = ex2w(fmaf(__uint_as_float(x[c][i]), row_scale, neg_m));
+                        const float p1 = ex2w(fmaf(__uint_as_float(x[c][i + 1]), row_scale, neg_m));
                         sum4[(i >> 1) & 3] += p0 + p1;
-                        x[i] = __float_as_uint(p0);
-                        x[i + 1] = __float_as_uint(p1);
+                        x[c][i] = __float_as_uint(p0);
+                        x[c][i + 1] = __float_as_uint(p1);
                     }
                     // packed in place
                     if (kMx && kBf16 && (flags & 2u)) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            x[i] = pack_16x2<true>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+                            x[c][i] = pack_16x2<true>(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1]));
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            x[i] = pack_16x2<kOpBf16>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+                            x[c][i] = pack_16x2<kOpBf16>(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1]));
                         }
                     }
-                    const uint32_t to = p_base + (c >> 1) * Sh::kHalfBytes;
+                    if (c == 0 && !pv_waited) { // the previous product must have read P's buffer
+                        ok = warp_wait(&ctl->pv_done[t], (n - 1) & 1, abort_flag, lane);
+                        pv_waited = true;
+                    }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        sts128(to + swz(row_in_tile, (c & 1) * 4 + q), x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+                        sts128(p_base + half * Sh::kHalfBytes + swz(row_in_tile, c * 4 + q), x[c][4 * q], x[c][4 * q + 1], x[c][4 * q + 2],
+                               x[c][4 * q + 3]);
                     }
                 }
             }
