@@ -30,14 +30,15 @@ namespace pto_b200 {
 
 namespace {
 
-constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-11 loading K, 12-15 loading V; 16, 17 issuing (one per group); 18, 19 idle
+constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-11 loading K, 12-15 loading V; 16, 17 issuing (one per group); 18, 19
+// describing the key tiles and fetching them towards L2
 // registers of a thread: 96 at launch (five warps a scheduler), then 2 * 112 + 2 * 96 + 64 (codes) or 2 * 112 + 2 * 88
 // + 80 (16-bit rows), times 128, which is all of these 640 * 96.  No role
 // may spill: shared memory leaves the first-level cache so little that every reload comes from L2 (with 40 registers the
 // issuing threads reloaded descriptors and took 700 cycles for a product).
 constexpr int kRegsLaunch = 96, kRegsSoftmax = 112;
-__host__ __device__ constexpr int regs_load(bool codes) { return codes ? 88 : 88; }
-__host__ __device__ constexpr int regs_issue(bool codes) { return codes ? 80 : 80; }
+__host__ __device__ constexpr int regs_load(bool codes) { return codes ? 80 : 80; }
+__host__ __device__ constexpr int regs_issue(bool codes) { return codes ? 96 : 96; }
 constexpr bool regs_fit(bool codes)
 {
     return (2 * kRegsSoftmax + 2 * regs_load(codes) + regs_issue(codes)) * 128 <= kThreads * kRegsLaunch;
@@ -50,7 +51,7 @@ constexpr float kDefer = 8.0f; // log2 of the growth of a row's maximum that res
 
 struct Info { // of a key tile
     uint32_t valid[4]; // bit r: key r exists
-    uint32_t flags[4]; // by describing warp: bit 0, some key has a factor; bit 1, V is bfloat16
+    uint32_t flags[4]; // by 32 keys: bit 0, some key has a factor; bit 1, V is bfloat16
     uint16_t factor[kTile]; // bfloat16, a power of two
 };
 
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             mbar_init(&ctl->v_empty[s], kPair ? 2 : 1);
         }
         for (int s = 0; s < kInfo; ++s) {
-            mbar_init(&ctl->info_full[s], 4);
+            mbar_init(&ctl->info_full[s], 2);
         }
         ctl->abort_flag = 0;
         fence_mbar_init();
@@ -235,6 +236,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem_base = ctl->tmem_base;
     volatile int *abort_flag = &ctl->abort_flag;
+    constexpr int RB = kv_row_bytes(kFmt, kD);
+    const int page_mask = (1 << a.page_shift) - 1;
+    // page of key r of tile j; -1: no such key.  Numbers out of range count as if there were no key.
+    auto page_of = [&](int j, int r) -> int {
+        const int key = k_begin + j * kTile + r;
+        return key < k_end ? __ldg(a.prefix_pages + (key >> a.page_shift)) : -1;
+    };
+    // row of the cache of key r of tile j, which lies in `page`; -1 for none
+    auto cache_row = [&](int page, int j, int r) -> int64_t {
+        return page < 0 || page >= a.num_pages
+                   ? -1
+                   : ((static_cast<int64_t>(page) * a.kv_heads + h) << a.page_shift) + ((k_begin + j * kTile + r) & page_mask);
+    };
+
     if (warp >= kIssueWarp) {
         constexpr int kRegs = regs_issue(kMx);
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -313,6 +328,83 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     do_pv(j, n);
                 }
             }
+        } else if (t >= 2) {
+            // -------------------------------------------------------- describing warps: two keys a thread.  Page numbers and
+            // scales are loaded a tile ahead; tile m follows when K(m - 1) has been stored.
+            const int r = (t - 2) * 32 + lane;
+            int pid[2], pid_next[2];
+            uint32_t ks[2] = {0, 0}, vs[2] = {0, 0};
+            auto load_scales = [&](int m) {
+#pragma unroll
+                for (int i = 0; i < 2 && kMx; ++i) {
+                    const int64_t row = cache_row(pid[i], m, r + 64 * i);
+                    ks[i] = row >= 0 ? row_scales<kD>(a.ks, row) : 0u;
+                    vs[i] = row >= 0 ? row_scales<kD>(a.vs, row) : 0u;
+                }
+            };
+            // 16 keys a lane: K by one warp, V by the other
+            auto fetch = [&](int page, int m, int lane8) {
+                const int64_t row = m < tiles ? cache_row(page, m, lane8 * 16) : -1;
+                if (row >= 0) {
+                    const uint8_t *src = (t == 2 ? a.k : a.v) + row * RB;
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(16 * RB) : "memory");
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                pid[i] = page_of(0, r + 64 * i);
+                pid_next[i] = tiles > 1 ? page_of(1, r + 64 * i) : -1;
+            }
+            int pid_l2 = tiles > 3 && lane < 8 ? page_of(3, lane * 16) : -1;
+            if (lane < 16) { // tiles 1 and 2 at once
+                const int m = 1 + (lane >> 3);
+                fetch(m < tiles ? page_of(m, (lane & 7) * 16) : -1, m, lane & 7);
+            }
+            load_scales(0);
+#pragma unroll 1
+            for (int m = 0; m < tiles; ++m) {
+                if (m > 0 && !warp_wait(&ctl->k_full[(m - 1) % kRingK], ((m - 1) / kRingK) & 1, abort_flag, lane)) {
+                    break;
+                }
+                Info &info = ctl->info[m % kInfo];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bool valid = pid[i] >= 0 && pid[i] < a.num_pages;
+                    if (!valid && k_begin + m * kTile + r + 64 * i < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+                        status->block = blockIdx.x;
+                        status->where = 11;
+                        status->detail = pid[i];
+                    }
+                    const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+                    uint32_t flags = 0;
+                    if constexpr (kMx) {
+                        const bool k_out = !scales_in_range<kD, kFmt>(ks[i]);
+                        // with float16 queries V stays float16: small values only lose what is below float16's last place,
+                        // as o itself does, and larger ones than it holds count as infinities
+                        const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(vs[i]);
+                        info.factor[r + 64 * i] = k_out ? static_cast<uint16_t>(largest_scale<kD>(ks[i]) << 7) : 0x3f80;
+                        flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
+                    }
+                    if (lane == 0) {
+                        info.valid[2 * i + t - 2] = mask;
+                        info.flags[2 * i + t - 2] = flags;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&ctl->info_full[m % kInfo]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    pid[i] = pid_next[i];
+                    pid_next[i] = m + 2 < tiles ? page_of(m + 2, r + 64 * i) : -1;
+                }
+                load_scales(m + 1);
+                if (lane < 8) {
+                    fetch(pid_l2, m + 3, lane);
+                    pid_l2 = m + 4 < tiles ? page_of(m + 4, lane * 16) : -1;
+                }
+            }
         }
     } else if (warp >= 8) {
         constexpr int kRegs = regs_load(kMx);
@@ -327,215 +419,136 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
         const bool is_v = warp >= 12;
         const int tid = threadIdx.x & 127;
         const int p = tid & 3, r0 = tid >> 2;
-        constexpr int RB = kv_row_bytes(kFmt, kD);
         const int ring = is_v ? kRingV : kRingK;
         uint64_t *full = is_v ? ctl->v_full : ctl->k_full, *empty = is_v ? ctl->v_empty : ctl->k_empty;
         const uint32_t ring_base = smem_u32(is_v ? smem_v : smem_k);
         const uint8_t *data = is_v ? a.v : a.k;
         const uint32_t at0 = swz(r0, 2 * p), at1 = at0 ^ 16; // of the two 16-byte chunks, row r0
-        const int page_mask = (1 << a.page_shift) - 1;
-        // page of key r of tile j; -1: no such key.  Numbers out of range count as if there were no key.
-        auto page_of = [&](int j, int r) -> int {
-            const int key = k_begin + j * kTile + r;
-            return key < k_end ? __ldg(a.prefix_pages + (key >> a.page_shift)) : -1;
-        };
-        // row of the cache of key r of tile j, which lies in `page`; -1 for none
-        auto cache_row = [&](int page, int j, int r) -> int64_t {
-            return page < 0 || page >= a.num_pages
-                       ? -1
-                       : ((static_cast<int64_t>(page) * a.kv_heads + h) << a.page_shift) + ((k_begin + j * kTile + r) & page_mask);
-        };
-        // K's group describes the tiles, one key a thread; page numbers and scales are loaded a tile ahead
-        int pid_own = page_of(0, tid), pid_own_next = tiles > 1 ? page_of(1, tid) : -1;
-        uint32_t own_ks = 0, own_vs = 0;
-        auto load_own_scales = [&](int j) {
-            if constexpr (kMx) {
-                own_ks = own_vs = 127u * 0x01010101u;
-                const int64_t row = cache_row(pid_own, j, tid);
-                if (row >= 0) {
-                    own_ks = row_scales<kD>(a.ks, row);
-                    own_vs = row_scales<kD>(a.vs, row);
-                }
-            }
-        };
         int pid[4]; // of this thread's rows in the next tile
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             pid[i] = page_of(0, r0 + 32 * i);
         }
-        load_own_scales(0);
         bool ok = true;
         int slot = 0;
         uint32_t phase = 1;
 #pragma unroll 1
-        for (int j = -1; j < tiles && ok; ++j) {
-            if (j >= 0) {
-                // ---- the tile's rows
-                int64_t row[4];
+        for (int j = 0; j < tiles; ++j) {
+            // ---- the tile's rows, and the pages of the next
+            int64_t row[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                row[i] = cache_row(pid[i], j, r0 + 32 * i);
+                pid[i] = j + 1 < tiles ? page_of(j + 1, r0 + 32 * i) : -1;
+            }
+            const uint32_t dst = ring_base + slot * Sh::kTileBytes;
+            if constexpr (!kMx) {
+                ok = warp_wait(&empty[slot], phase, abort_flag, lane);
+                if (!ok) {
+                    break;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    row[i] = cache_row(pid[i], j, r0 + 32 * i);
+                    const uint8_t *from = data + (row[i] < 0 ? 0 : row[i]) * RB + p * 32;
+                    const int bytes = row[i] < 0 ? 0 : 16;
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+                        const uint32_t to = dst + half * Sh::kHalfBytes + i * 32 * 128;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at0), "l"(from + half * 128), "r"(bytes) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at1), "l"(from + half * 128 + 16), "r"(bytes) : "memory");
+                    }
                 }
-                const uint32_t dst = ring_base + slot * Sh::kTileBytes;
-                if constexpr (!kMx) {
-                    ok = warp_wait(&empty[slot], phase, abort_flag, lane);
-                    if (!ok) {
-                        break;
-                    }
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+            } else {
+                constexpr int kWords = kFmt == kKvMxFp8 ? 4 : 2;
+                uint32_t code[4 * kHalves][kWords], scales[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint8_t *from = data + (row[i] < 0 ? 0 : row[i]) * RB + p * 32;
-                        const int bytes = row[i] < 0 ? 0 : 16;
+                for (int i = 0; i < 4; ++i) {
+                    const bool live = row[i] >= 0;
+                    const uint8_t *src = data + row[i] * RB + p * (4 * kWords);
+                    scales[i] = live ? row_scales<kD>(is_v ? a.vs : a.ks, row[i]) : 0u;
 #pragma unroll
-                        for (int half = 0; half < kHalves; ++half) {
-                            const uint32_t to = dst + half * Sh::kHalfBytes + i * 32 * 128;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at0), "l"(from + half * 128), "r"(bytes) : "memory");
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at1), "l"(from + half * 128 + 16), "r"(bytes) : "memory");
+                    for (int half = 0; half < kHalves; ++half) {
+                        uint32_t *c = code[i * kHalves + half];
+                        if constexpr (kFmt == kKvMxFp8) {
+                            const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + half * 64)) : make_uint4(0, 0, 0, 0);
+                            c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+                        } else {
+                            const uint2 v = live ? __ldg(reinterpret_cast<const uint2 *>(src + half * 32)) : make_uint2(0, 0);
+                            c[0] = v.x, c[1] = v.y;
                         }
                     }
-                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-                } else {
-                    constexpr int kWords = kFmt == kKvMxFp8 ? 4 : 2;
-                    uint32_t code[4 * kHalves][kWords], scales[4];
+                }
+                ok = warp_wait(&empty[slot], phase, abort_flag, lane) &&
+                     warp_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag, lane);
+                if (!ok) {
+                    break;
+                }
+                const Info &info = ctl->info[j % kInfo];
+                const uint32_t flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
+                const bool special = (flags & (is_v ? 2u : 1u)) != 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool live = row[i] >= 0;
-                        const uint8_t *src = data + row[i] * RB + p * (4 * kWords);
-                        scales[i] = live ? row_scales<kD>(is_v ? a.vs : a.ks, row[i]) : 0u;
+                for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                        for (int half = 0; half < kHalves; ++half) {
-                            uint32_t *c = code[i * kHalves + half];
-                            if constexpr (kFmt == kKvMxFp8) {
-                                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + half * 64)) : make_uint4(0, 0, 0, 0);
-                                c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
-                            } else {
-                                const uint2 v = live ? __ldg(reinterpret_cast<const uint2 *>(src + half * 32)) : make_uint2(0, 0);
-                                c[0] = v.x, c[1] = v.y;
-                            }
+                    for (int half = 0; half < kHalves; ++half) {
+                        uint32_t w[8];
+                        codes16_to_f16<kFmt>(code[i * kHalves + half], w);
+                        // 2^(byte - 127) in both halves; 255: infinity, times the block's zeros the NaN it stands for
+                        const uint32_t byte = (scales[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
+                        const float f = __uint_as_float(byte << 23);
+                        const uint32_t m = pack_16x2<false>(f, f), to = dst + half * Sh::kHalfBytes + i * 32 * 128;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            w[x] = mul_16x2<false>(w[x], m);
                         }
+                        sts128(to + at0, w[0], w[1], w[2], w[3]);
+                        sts128(to + at1, w[4], w[5], w[6], w[7]);
                     }
-                    ok = warp_wait(&empty[slot], phase, abort_flag, lane) &&
-                         warp_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag, lane);
-                    if (!ok) {
-                        break;
-                    }
-                    const Info &info = ctl->info[j % kInfo];
-                    const uint32_t flags = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
-                    const bool special = (flags & (is_v ? 2u : 1u)) != 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                        for (int half = 0; half < kHalves; ++half) {
-                            uint32_t w[8];
-                            codes16_to_f16<kFmt>(code[i * kHalves + half], w);
-                            // 2^(byte - 127) in both halves; 255: infinity, times the block's zeros the NaN it stands for
-                            const uint32_t byte = (scales[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
-                            const float f = __uint_as_float(byte << 23);
-                            const uint32_t m = pack_16x2<false>(f, f), to = dst + half * Sh::kHalfBytes + i * 32 * 128;
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                w[x] = mul_16x2<false>(w[x], m);
-                            }
-                            sts128(to + at0, w[0], w[1], w[2], w[3]);
-                            sts128(to + at1, w[4], w[5], w[6], w[7]);
-                        }
-                    }
-                    if (special) { // rare: the tile once more, from memory, in small steps
+                }
+                if (special) { // rare: the tile once more, from memory, in small steps
 #pragma unroll 1
-                        for (int u = 0; u < 4 * kHalves; ++u) {
-                            const int i = u / kHalves, half = u % kHalves;
-                            int page = pid[0];
+                    for (int u = 0; u < 4 * kHalves; ++u) {
+                        const int i = u / kHalves, half = u % kHalves;
+                        const int64_t at = cache_row(page_of(j, r0 + 32 * i), j, r0 + 32 * i);
+                        uint32_t c[4] = {0, 0, 0, 0}, w[8], scale = 0;
+                        if (at >= 0) {
+                            scale = row_scales<kD>(is_v ? a.vs : a.ks, at);
+                            const uint32_t *src = reinterpret_cast<const uint32_t *>(data + at * RB + half * (RB / kHalves)) + p * kWords;
 #pragma unroll
-                            for (int x = 1; x < 4; ++x) {
-                                page = i == x ? pid[x] : page;
+                            for (int x = 0; x < kWords; ++x) {
+                                c[x] = __ldg(src + x);
                             }
-                            const int64_t at = cache_row(page, j, r0 + 32 * i);
-                            uint32_t c[4] = {0, 0, 0, 0}, w[8], scale = 0;
-                            if (at >= 0) {
-                                scale = row_scales<kD>(is_v ? a.vs : a.ks, at);
-                                const uint32_t *src = reinterpret_cast<const uint32_t *>(data + at * RB + half * (RB / kHalves)) + p * kWords;
-#pragma unroll
-                                for (int x = 0; x < kWords; ++x) {
-                                    c[x] = __ldg(src + x);
-                                }
-                            }
-                            codes16_to_f16<kFmt>(c, w);
-                            const uint32_t byte = (scale >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
-                            // keys with a block out of range: relative to their largest scale
-                            const bool relative = !is_v && !scales_in_range<kD, kFmt>(scale);
-                            const int e = relative && byte != 255u ? max(static_cast<int>(byte) + 127 - static_cast<int>(largest_scale<kD>(scale)), 0)
-                                                                   : static_cast<int>(byte);
-                            const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                if (is_v) { // bfloat16: the values times 2^-112 to the other format's places, then scaled
-                                    w[x] = mul_16x2<true>((w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu), 0x77807780u);
-                                    w[x] = mul_16x2<true>(w[x], byte * 0x00800080u); // 255: infinity, times 0 NaN
-                                } else {
-                                    w[x] = mul_16x2<false>(w[x], pack_16x2<false>(f, f));
-                                }
-                            }
-                            const uint32_t to = dst + half * Sh::kHalfBytes + i * 32 * 128;
-                            sts128(to + at0, w[0], w[1], w[2], w[3]);
-                            sts128(to + at1, w[4], w[5], w[6], w[7]);
                         }
-                    }
-                }
-                fence_proxy_async_smem(); // the tensor core reads through the asynchronous proxy
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&full[slot]);
-                }
-                if (++slot == ring) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
+                        codes16_to_f16<kFmt>(c, w);
+                        const uint32_t byte = (scale >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
+                        // keys with a block out of range: relative to their largest scale
+                        const bool relative = !is_v && !scales_in_range<kD, kFmt>(scale);
+                        const int e = relative && byte != 255u ? max(static_cast<int>(byte) + 127 - static_cast<int>(largest_scale<kD>(scale)), 0)
+                                                               : static_cast<int>(byte);
+                        const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    pid[i] = j + 1 < tiles ? page_of(j + 1, r0 + 32 * i) : -1;
+                        for (int x = 0; x < 8; ++x) {
+                            if (is_v) { // bfloat16: the values times 2^-112 to the other format's places, then scaled
+                                w[x] = mul_16x2<true>((w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu), 0x77807780u);
+                                w[x] = mul_16x2<true>(w[x], byte * 0x00800080u); // 255: infinity, times 0 NaN
+                            } else {
+                                w[x] = mul_16x2<false>(w[x], pack_16x2<false>(f, f));
+                            }
+                        }
+                        const uint32_t to = dst + half * Sh::kHalfBytes + i * 32 * 128;
+                        sts128(to + at0, w[0], w[1], w[2], w[3]);
+                        sts128(to + at1, w[4], w[5], w[6], w[7]);
+                    }
                 }
             }
-            if (is_v) {
-                // ---- towards L2: lane = 16 keys, warps 12 and 13 the rows of K and V two tiles ahead (the first two at once)
-                if (warp < 14 && lane < (j < 0 ? 16 : 8)) {
-                    const int ahead = j < 0 ? 1 + (lane >> 3) : j + 3;
-                    const int64_t at = ahead < tiles ? cache_row(page_of(ahead, (lane & 7) * 16), ahead, (lane & 7) * 16) : -1;
-                    if (at >= 0) {
-                        const uint8_t *src = (warp == 12 ? a.k : a.v) + at * RB;
-                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(16 * RB) : "memory");
-                    }
-                }
-            } else if (j + 1 < tiles) {
-                // ---- what the other warps have to know about tile j + 1
-                Info &info = ctl->info[(j + 1) % kInfo];
-                const bool valid = pid_own >= 0 && pid_own < a.num_pages;
-                if (!valid && k_begin + (j + 1) * kTile + tid < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
-                    status->block = blockIdx.x;
-                    status->where = 11;
-                    status->detail = pid_own;
-                }
-                const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-                uint32_t flags = 0;
-                if constexpr (kMx) {
-                    const bool k_out = !scales_in_range<kD, kFmt>(own_ks);
-                    // with float16 queries V stays float16: small values only lose what is below float16's last place, as o
-                    // itself does, and larger ones than it holds count as infinities
-                    const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(own_vs);
-                    info.factor[tid] = k_out ? static_cast<uint16_t>(largest_scale<kD>(own_ks) << 7) : 0x3f80;
-                    flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
-                }
-                if (lane == 0) {
-                    info.valid[warp - 8] = mask;
-                    info.flags[warp - 8] = flags;
-                }
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&ctl->info_full[(j + 1) % kInfo]);
-                }
-                // the next one's: scales now, the page after it
-                pid_own = pid_own_next;
-                load_own_scales(j + 2);
-                pid_own_next = j + 3 < tiles ? page_of(j + 3, tid) : -1;
+            fence_proxy_async_smem(); // the tensor core reads through the asynchronous proxy
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&full[slot]);
+            }
+            if (++slot == ring) {
+                slot = 0;
+                phase ^= 1u;
             }
         }
     } else {
@@ -563,52 +576,35 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             }
             const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
             const uint32_t keep = live && a.scale_log2 != 0.0f ? 0xffffffffu : 0u;
-            constexpr int kChunk = 4; // 16-byte loads in flight
+            uint32_t w[kD / 2];
+#pragma unroll
+            for (int c = 0; c < kD / 8; ++c) {
+                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src) + c) : make_uint4(0, 0, 0, 0);
+                w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+            }
             float factor = 1.0f, inv = 1.0f;
             if constexpr (kBf16 && kMx) {
-                float top = 0.0f;
-#pragma unroll 1
-                for (int c0 = 0; c0 < kD / 8 && live; c0 += kChunk) {
-                    uint4 v[kChunk];
+                uint32_t top = 0; // the largest magnitudes of both halves: bfloat16 pairs order like integers
 #pragma unroll
-                    for (int c = 0; c < kChunk; ++c) {
-                        v[c] = __ldg(reinterpret_cast<const uint4 *>(src) + c0 + c);
-                    }
-#pragma unroll
-                    for (int c = 0; c < kChunk; ++c) {
-                        const float2 f0 = unpack_16x2<true>(v[c].x), f1 = unpack_16x2<true>(v[c].y);
-                        const float2 f2 = unpack_16x2<true>(v[c].z), f3 = unpack_16x2<true>(v[c].w);
-                        top = max3(top, fabsf(f0.x), fabsf(f0.y));
-                        top = max3(top, fabsf(f1.x), fabsf(f1.y));
-                        top = max3(top, fabsf(f2.x), fabsf(f2.y));
-                        top = max3(top, fabsf(f3.x), fabsf(f3.y));
-                    }
+                for (int i = 0; i < kD / 2; ++i) {
+                    const uint32_t v = w[i] & 0x7fff7fffu;
+                    asm("max.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(v));
                 }
-                const int field = min(max(static_cast<int>(__float_as_uint(top) >> 23), 29), 254);
+                const int field = min(max(static_cast<int>(max(top & 0x7fffu, top >> 16) >> 7), 29), 254);
                 factor = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
                 inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
             }
-#pragma unroll 1
-            for (int c0 = 0; c0 < kD / 8; c0 += kChunk) {
-                uint4 v[kChunk];
 #pragma unroll
-                for (int c = 0; c < kChunk; ++c) {
-                    v[c] = live ? __ldg(reinterpret_cast<const uint4 *>(src) + c0 + c) : make_uint4(0, 0, 0, 0);
-                }
+            for (int c = 0; c < kD / 8; ++c) {
 #pragma unroll
-                for (int c = 0; c < kChunk; ++c) {
-                    uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (kBf16 && kMx) {
-                            const float2 f = unpack_16x2<true>(w[i]);
-                            w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
-                        }
-                        w[i] = (w[i] & keep) ^ sign;
+                for (int i = 4 * c; i < 4 * c + 4; ++i) {
+                    if constexpr (kBf16 && kMx) {
+                        const float2 f = unpack_16x2<true>(w[i]);
+                        w[i] = pack_16x2<false>(f.x * inv, f.y * inv);
                     }
-                    const int at = c0 + c;
-                    sts128(q_base + (at >> 3) * Sh::kHalfBytes + swz(row_in_tile, at & 7), w[0], w[1], w[2], w[3]);
+                    w[i] = (w[i] & keep) ^ sign;
                 }
+                sts128(q_base + (c >> 3) * Sh::kHalfBytes + swz(row_in_tile, c & 7), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
             }
             if constexpr (!kPair) {
                 ctl->q_factor[row_in_tile] = factor;
