@@ -12,10 +12,14 @@
 //   S = Q K^T   the order of the head dimension inside a block of 32 is free as long as Q and K agree: lane t of a quad
 //               takes elements 8t .. 8t+7 of the block, two k steps of four.  Codes are multiplied unscaled (exact in
 //               16 bits) and the block's power of two is applied to the fp32 sums: S += 2^e (q_blk . code_blk).
-//   O += P V    a product's eight columns are head-dimension elements W g + i (g the lane's group, W = d / 8), so a
-//               lane reads W consecutive elements of its four keys and the operands need no transposition; V's scale
-//               depends on the key, so it is applied to the code pair (exact in 16 bits within the type's range).
-// Softmax statistics and all sums are fp32; P is rounded to the 16-bit type of q for the second product.
+//   O += P V    16-bit rows: V transposed on the way out of shared memory (ldmatrix).  Codes: a product's eight columns are
+//               head-dimension elements W g + i (g the lane's group, W = d / 8), so a lane reads W consecutive elements of
+//               its four keys and nothing is transposed; V's scale depends on the key and is applied to the pair.
+// Over an MX cache the products are in float16 for either type of q: a code pair converts in one instruction (to bfloat16 in
+// four, which made the kernel half as fast).  bfloat16 rows of q are divided by a power of two that brings their largest
+// element into [2^14, 2^15); elements down to 2^-31 of it keep every bit.  V's scales are exact in float16 between 2^-15
+// and 2^7 (e4m3; e2m1 2^-23 .. 2^13); 16 keys with one outside take bfloat16 products if q is bfloat16.
+// Softmax statistics and all sums are fp32; P is rounded to the products' type.
 #include "ptx.cuh"
 #include "prefix_attn.cuh"
 
@@ -109,12 +113,12 @@ __device__ __forceinline__ uint32_t swz_k(int row, int byte)
                              : (row >> 2) & 1;
     return static_cast<uint32_t>(((chunk ^ x) << 4) | (byte & 15));
 }
-template <int RB>
+template <int RB, int kFmt>
 __device__ __forceinline__ uint32_t swz_v(int row, int byte)
 {
     const int chunk = (row * RB + byte) >> 4;
     const int t = (row >> 1) & 3;
-    const int x = RB == 256 ? (t & 1) | ((t & 2) << 1) : RB == 128 ? row & 6 : RB == 64 ? 2 * t : 2 * ((row >> 2) & 1);
+    const int x = kFmt <= kKvBf16 ? row & 7 : RB == 128 ? row & 6 : RB == 64 ? 2 * t : 2 * ((row >> 2) & 1);
     return static_cast<uint32_t>(((chunk ^ x) << 4) | (byte & 15));
 }
 
@@ -125,56 +129,63 @@ struct Stage {
     static constexpr int kScaleBytes = kFmt >= kKvMxFp8 ? kStep * kD / 32 : 0; // per K or V
     static constexpr int kBytes = 2 * kRowsBytes + 2 * kScaleBytes;
     static constexpr int kCount = kFmt <= kKvBf16 ? (kD == 128 ? 2 : 4) : (kFmt == kKvMxFp8 ? 4 : 6);
-    static constexpr int kMergeBytes = kWarps * kRows * kD * 4 + kWarps * kRows * 8;
+    static constexpr int kMergePitch = kD + 8; // floats: the rows of a store meet other banks
+    static constexpr int kMergeBytes = kWarps * kRows * kMergePitch * 4 + kWarps * kRows * 8;
     static constexpr int kRing = kWarps * kCount * kBytes;
     static constexpr int kSmem = kRing > kMergeBytes ? kRing : kMergeBytes;
 };
 
-// pair of codes (bytes / nibbles already placed) -> 16-bit pair, times nothing: the codes' own values
-// fp8: `two` = bytes {lo, hi} in bits 0..15
-template <bool kBf16>
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t word, int sel)
+// eight e2m1 codes / four e4m3 codes -> float16 pairs of neighbours
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&p)[4])
 {
-    if constexpr (!kBf16) {
-        return e4m3x2_to_f16x2(sel ? word >> 16 : word & 0xffffu);
-    } else {
-        // each byte at the top of a half: sign in place, exponent and mantissa 4 bits down; as bfloat16 that is the
-        // code times 2^-120 (e4m3's bias 7 against 127), subnormals included
-        uint32_t r = __byte_perm(word, 0, sel ? 0x3424 : 0x1404);
-        r = (r & 0x80008000u) | ((r >> 4) & 0x07f007f0u);
-        return mul_16x2<true>(r, 0x7b807b80u); // 2^120
-    }
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
+        : "r"(w));
+}
+__device__ __forceinline__ void e4m3x4(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
 }
 
-template <bool kBf16>
-__device__ __forceinline__ uint32_t e2m1_pair(uint32_t byte)
-{
-    const uint32_t h = e2m1x2_to_f16x2(byte);
-    if constexpr (!kBf16) {
-        return h;
-    } else {
-        const uint32_t r = (h & 0x80008000u) | ((h >> 3) & 0x0fff0fffu); // times 2^-112
-        return mul_16x2<true>(r, 0x77807780u);                           // 2^112
-    }
-}
-
-// 2^(byte - 127) of two scale bytes as a 16-bit pair.  bfloat16: exact but for byte 0 (0 instead of 2^-127) and 255
-// (infinity; a block with that byte holds zeros, and 0 * infinity is the NaN it stands for).  float16: rounded to
-// float16's range, as the values themselves are.
-template <bool kBf16>
+// scaled V operand: a pair of values of two keys times the keys' powers of two.  float16: exact where scale_ok() says so,
+// rounded to float16's range elsewhere, as float16 queries' results are.  kWide: bfloat16, exact but for scale byte 0 (0
+// instead of 2^-127); byte 255 is infinity there and as float16, and times a block's zeros the NaN that it stands for.
+template <bool kWide>
 __device__ __forceinline__ uint32_t scale_pair(uint32_t b0, uint32_t b1)
 {
-    if constexpr (kBf16) {
+    if constexpr (kWide) {
         return (b0 << 7) | (b1 << 23);
     } else {
         return pack_16x2<false>(__uint_as_float(b0 << 23), __uint_as_float(b1 << 23));
     }
+}
+template <bool kWide>
+__device__ __forceinline__ uint32_t scaled(uint32_t h, uint32_t scale)
+{
+    if constexpr (kWide) { // float16's places to bfloat16's: the value times 2^-112, times 2^112
+        const uint32_t v = (h & 0x80008000u) | ((h >> 3) & 0x0fff0fffu);
+        return mul_16x2<true>(mul_16x2<true>(v, 0x77807780u), scale);
+    } else {
+        return mul_16x2<false>(h, scale);
+    }
+}
+// whether every code times 2^(byte - 127) is exact in float16
+template <int kFmt>
+__device__ __forceinline__ bool scale_ok(uint32_t byte)
+{
+    return kFmt == kKvMxFp8 ? byte - 112u <= 22u || byte == 0u : byte - 104u <= 36u || byte == 0u;
 }
 
 template <bool kBf16, int kD, int kFmt>
 __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __grid_constant__ AttnArgs a, DeviceStatus *status)
 {
     using St = Stage<kD, kFmt>;
+    constexpr bool kMx = kFmt >= kKvMxFp8;
+    constexpr bool kOp = kBf16 && !kMx; // the products' type is bfloat16
     constexpr int RB = St::kRowBytes;
     constexpr int kBlk = kD / 32;
     constexpr int kTiles = kD / 8; // column tiles of O
@@ -183,36 +194,35 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
 
+    programmatic_trigger();
     // ---- which piece
+    // (32-bit arithmetic throughout: a 64-bit division costs more than a step's products)
     const int prefix_items = a.prefix_wide ? 0 : a.prefix_splits * a.kv_heads * a.prefix_tiles;
     const int row_span = a.tokens * a.group; // rows of one sequence and kv head
-    int64_t item = blockIdx.x;
-    int h, tile, b = 0, k_begin, k_end, rows;
-    const bool own = item >= prefix_items;
+    const bool own = static_cast<int>(blockIdx.x) >= prefix_items;
+    uint32_t item = blockIdx.x - (own ? prefix_items : 0);
+    const uint32_t tiles = own ? a.own_tiles : a.prefix_tiles;
+    int64_t slot = item + (own ? static_cast<int64_t>(a.prefix_pieces) * a.kv_heads * a.prefix_tiles : 0);
+    const int tile = static_cast<int>(item % tiles);
+    item /= tiles;
+    const int h = static_cast<int>(item % static_cast<uint32_t>(a.kv_heads));
+    item /= static_cast<uint32_t>(a.kv_heads);
+    int b = 0, k_begin, k_end, rows, len = 0;
     const int32_t *pages;
-    int64_t slot = item;
     if (!own) {
-        tile = static_cast<int>(item % a.prefix_tiles);
-        h = static_cast<int>(item / a.prefix_tiles) % a.kv_heads;
-        const int split = static_cast<int>(item / a.prefix_tiles) / a.kv_heads;
-        k_begin = split * a.prefix_chunk;
+        k_begin = static_cast<int>(item) * a.prefix_chunk;
         k_end = min(k_begin + a.prefix_chunk, a.prefix_len);
         rows = a.batch * row_span;
         pages = a.prefix_pages;
     } else {
-        item -= prefix_items;
-        slot = item + static_cast<int64_t>(a.prefix_pieces) * a.kv_heads * a.prefix_tiles;
-        tile = static_cast<int>(item % a.own_tiles);
-        item /= a.own_tiles;
-        h = static_cast<int>(item % a.kv_heads);
-        item /= a.kv_heads;
-        b = static_cast<int>(item % a.batch);
-        const int split = static_cast<int>(item / a.batch);
-        const int len = own_len(a, b);
-        if (split == 0 && tile == 0 && h == 0 && threadIdx.x == 0 && len != a.lens[b] && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+        b = static_cast<int>(item % static_cast<uint32_t>(a.batch));
+        const int split = static_cast<int>(item / static_cast<uint32_t>(a.batch));
+        const int given = a.lens[b];
+        len = max(0, min(given, a.own_max));
+        if (split == 0 && tile == 0 && h == 0 && threadIdx.x == 0 && len != given && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
             status->block = blockIdx.x;
             status->where = 12;
-            status->detail = a.lens[b];
+            status->detail = given;
         }
         const int chunk = own_chunk(len, a.own_splits, a.own_min);
         k_begin = split * chunk;
@@ -220,9 +230,13 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
         rows = row_span;
         pages = a.table + b * a.table_stride;
         if (k_begin >= k_end) {
+            programmatic_wait();
             return; // past this sequence's last piece: the joining kernel does not look here
         }
     }
+    // the page of the step that is loaded next, read a step before
+    const int steps = ceil_div(k_end - k_begin, kStep);
+    int next_page = warp < steps ? pages[(k_begin + warp * kStep) >> a.page_shift] : 0;
 
     // ---- this lane's two rows: g and g + 8 of the tile
     int limit[2];
@@ -231,13 +245,12 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     for (int i = 0; i < 2; ++i) {
         const int r = tile * kRows + g + 8 * i;
         const bool live = r < rows;
-        const int rr = live ? r : 0;
-        const int bb = own ? b : rr / row_span;
-        const int in = own ? rr : rr % row_span;
-        const int tok = in / a.group;
-        q_row[i] = live ? a.q + bb * a.q_batch + tok * a.q_token + static_cast<int64_t>(h * a.group + in % a.group) * a.q_head : nullptr;
+        const int bb = own ? b : (live ? r / row_span : 0);
+        const int in = live ? (own ? r : r - bb * row_span) : 0;
+        const int tok = a.tokens == 1 ? 0 : in / a.group;
+        q_row[i] = live ? a.q + bb * a.q_batch + tok * a.q_token + static_cast<int64_t>(h * a.group + in - tok * a.group) * a.q_head : nullptr;
         // own keys: token `tok` of `tokens` sees all but the last tokens - 1 - tok
-        limit[i] = !live ? 0 : (own ? min(k_end, own_len(a, b) - (a.tokens - 1 - tok)) : k_end);
+        limit[i] = !live ? 0 : (own ? min(k_end, len - (a.tokens - 1 - tok)) : k_end);
     }
     // Q operands: block kb, words {step 0: low pair, high pair, step 1: low pair, high pair}
     uint32_t qf[kBlk][2][4];
@@ -255,13 +268,39 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
             qf[kb][i][3] = v.w;
         }
     }
+    float row_scale[2] = {a.scale_log2, a.scale_log2};
+    if constexpr (kBf16 && kMx) { // rows of q to float16, see above; a quad holds a row
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t top = 0; // the largest magnitudes of both halves
+#pragma unroll
+            for (int kb = 0; kb < kBlk; ++kb) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t v = qf[kb][i][j] & 0x7fff7fffu;
+                    asm("max.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(v));
+                }
+            }
+            top = max(top & 0x7fffu, top >> 16);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int field = min(max(static_cast<int>(top >> 7), 29), 254);
+            const float inv = __uint_as_float(static_cast<uint32_t>(254 - (field - 14)) << 23);
+            row_scale[i] *= __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
+#pragma unroll
+            for (int kb = 0; kb < kBlk; ++kb) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = unpack_16x2<true>(qf[kb][i][j]);
+                    qf[kb][i][j] = pack_16x2<false>(f.x * inv, f.y * inv);
+                }
+            }
+        }
+    }
 
     // ---- this warp's steps and ring
-    const int steps = ceil_div(k_end - k_begin, kStep);
     const uint32_t ring = smem_u32(smem) + warp * St::kCount * St::kBytes;
     uint32_t bad_pages = 0; // bit s: the step in ring stage s lies in a page that does not exist
-    // the page of the step that is loaded next, read a step before
-    int next_page = warp < steps ? pages[(k_begin + warp * kStep) >> a.page_shift] : 0;
     auto load = [&](int step, int stage) {
         if (step < steps) {
             const int key = k_begin + step * kStep;
@@ -289,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     const int r = (c * 16) / RB, byte = (c * 16) % RB;
                     const int64_t off = row * RB + c * 16;
                     cp_async16(base + swz_k<RB, kFmt>(r, byte), a.k + off, r < live ? 16 : 0);
-                    cp_async16(base + St::kRowsBytes + swz_v<RB>(r, byte), a.v + off, r < live ? 16 : 0);
+                    cp_async16(base + St::kRowsBytes + swz_v<RB, kFmt>(r, byte), a.v + off, r < live ? 16 : 0);
                 }
             }
             if constexpr (St::kScaleBytes > 0) {
@@ -359,25 +398,19 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                 if constexpr (kFmt <= kKvBf16) {
                     const uint4 v = lds128(base + swz_k<RB, kFmt>(8 * n + g, 64 * kb + 16 * t));
                     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                    mma_16816<kBf16>(s[n], qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
-                    mma_16816<kBf16>(s[n], qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
+                    mma_16816<kOp>(s[n], qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
+                    mma_16816<kOp>(s[n], qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
                 } else {
                     if constexpr (kFmt == kKvMxFp8) {
                         const uint2 v = lds64(base + swz_k<RB, kFmt>(8 * n + g, 32 * kb + 8 * t));
-                        w[0] = e4m3_pair<kBf16>(v.x, 0);
-                        w[1] = e4m3_pair<kBf16>(v.x, 1);
-                        w[2] = e4m3_pair<kBf16>(v.y, 0);
-                        w[3] = e4m3_pair<kBf16>(v.y, 1);
+                        e4m3x4(v.x, w[0], w[1]);
+                        e4m3x4(v.y, w[2], w[3]);
                     } else {
-                        const uint32_t v = lds32(base + swz_k<RB, kFmt>(8 * n + g, 16 * kb + 4 * t));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[i] = e2m1_pair<kBf16>((v >> (8 * i)) & 0xffu);
-                        }
+                        e2m1x8(lds32(base + swz_k<RB, kFmt>(8 * n + g, 16 * kb + 4 * t)), w);
                     }
                     float p[4];
-                    mma_16816_first<kBf16>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
-                    mma_16816<kBf16>(p, qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
+                    mma_16816_first<false>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
+                    mma_16816<false>(p, qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
                     const float f0 = __uint_as_float(((sc[0] >> (8 * kb)) & 0xffu) << 23);
                     const float f1 = __uint_as_float(((sc[1] >> (8 * kb)) & 0xffu) << 23);
                     s[n][0] = fmaf(p[0], f0, s[n][0]);
@@ -396,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
             for (int j = 0; j < 4; ++j) {
                 const int key = key0 + 8 * n + 2 * t + (j & 1);
                 const bool seen = key < limit[j >> 1] && !bad;
-                s[n][j] = seen ? s[n][j] * a.scale_log2 : -INFINITY;
+                s[n][j] = seen ? s[n][j] * row_scale[j >> 1] : -INFINITY;
                 mx[j >> 1] = fmaxf(mx[j >> 1], s[n][j]);
             }
         }
@@ -428,40 +461,31 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                 l[j >> 1] += s[n][j];
             }
         }
-        const uint32_t p0 = pack_16x2<kBf16>(s[0][0], s[0][1]), p1 = pack_16x2<kBf16>(s[0][2], s[0][3]);
-        const uint32_t p2 = pack_16x2<kBf16>(s[1][0], s[1][1]), p3 = pack_16x2<kBf16>(s[1][2], s[1][3]);
-
-        // ---- O += P V: keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step, elements W g .. W g + W - 1
+        // ---- O += P V
         const uint32_t vbase = base + St::kRowsBytes;
-        uint32_t scale01 = 0, scale23 = 0;
-        if constexpr (kFmt >= kKvMxFp8) {
-            const uint32_t sbase = base + 2 * St::kRowsBytes + St::kScaleBytes;
-            const int blk = (g * (kD / 8)) / 32;
-            scale01 = scale_pair<kBf16>(lds8(sbase + (2 * t) * kBlk + blk), lds8(sbase + (2 * t + 1) * kBlk + blk));
-            scale23 = scale_pair<kBf16>(lds8(sbase + (2 * t + 8) * kBlk + blk), lds8(sbase + (2 * t + 9) * kBlk + blk));
-        }
-        if constexpr (kFmt <= kKvBf16) {
+        if constexpr (!kMx) {
+            const uint32_t p0 = pack_16x2<kOp>(s[0][0], s[0][1]), p1 = pack_16x2<kOp>(s[0][2], s[0][3]);
+            const uint32_t p2 = pack_16x2<kOp>(s[1][0], s[1][1]), p3 = pack_16x2<kOp>(s[1][2], s[1][3]);
 #pragma unroll
-            for (int half = 0; half < kTiles / 8; ++half) { // eight elements (16 bytes) of each key at a time
-                const int byte = g * (kD / 4) + half * 16;
-                const uint4 x0 = lds128(vbase + swz_v<RB>(2 * t, byte)), x1 = lds128(vbase + swz_v<RB>(2 * t + 1, byte));
-                const uint4 x2 = lds128(vbase + swz_v<RB>(2 * t + 8, byte)), x3 = lds128(vbase + swz_v<RB>(2 * t + 9, byte));
-                const uint32_t y0[4] = {x0.x, x0.y, x0.z, x0.w}, y1[4] = {x1.x, x1.y, x1.z, x1.w};
-                const uint32_t y2[4] = {x2.x, x2.y, x2.z, x2.w}, y3[4] = {x3.x, x3.y, x3.z, x3.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    mma_16816<kBf16>(o[half * 8 + 2 * i], p0, p1, p2, p3, __byte_perm(y0[i], y1[i], 0x5410),
-                                     __byte_perm(y2[i], y3[i], 0x5410));
-                    mma_16816<kBf16>(o[half * 8 + 2 * i + 1], p0, p1, p2, p3, __byte_perm(y0[i], y1[i], 0x7632),
-                                     __byte_perm(y2[i], y3[i], 0x7632));
-                }
+            for (int i = 0; i < kTiles; i += 2) { // 16 keys x 16 elements, transposed; lane: key lane % 16, elements 8 (lane / 16)
+                uint32_t v0, v1, v2, v3;
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v0), "=r"(v1), "=r"(v2), "=r"(v3)
+                             : "r"(vbase + swz_v<RB, kFmt>(lane & 15, 16 * (i + (lane >> 4))))
+                             : "memory");
+                mma_16816<kOp>(o[i], p0, p1, p2, p3, v0, v1);
+                mma_16816<kOp>(o[i + 1], p0, p1, p2, p3, v2, v3);
             }
         } else {
+            // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step, elements W g .. W g + W - 1
             constexpr int kWords = kFmt == kKvMxFp8 ? kD / 32 : kD / 64; // 32-bit words of a lane's elements, per key
-            uint32_t x[4][kWords];
+            uint32_t x[4][kWords], sb[4];
+            const uint32_t sbase = base + 2 * St::kRowsBytes + St::kScaleBytes + (g * (kD / 8)) / 32;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t at = vbase + swz_v<RB>(2 * t + (i & 1) + (i >> 1) * 8, g * kWords * 4);
+                const int key = 2 * t + (i & 1) + (i >> 1) * 8;
+                const uint32_t at = vbase + swz_v<RB, kFmt>(key, g * kWords * 4);
+                sb[i] = lds8(sbase + key * kBlk);
                 if constexpr (kWords == 4) {
                     const uint4 v = lds128(at);
                     x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
@@ -472,36 +496,48 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     x[i][0] = lds32(at);
                 }
             }
+            auto product = [&](auto wide) {
+                constexpr bool kWide = decltype(wide)::value;
+                const uint32_t p0 = pack_16x2<kWide>(s[0][0], s[0][1]), p1 = pack_16x2<kWide>(s[0][2], s[0][3]);
+                const uint32_t p2 = pack_16x2<kWide>(s[1][0], s[1][1]), p3 = pack_16x2<kWide>(s[1][2], s[1][3]);
+                const uint32_t scale01 = scale_pair<kWide>(sb[0], sb[1]), scale23 = scale_pair<kWide>(sb[2], sb[3]);
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-                if constexpr (kFmt == kKvMxFp8) {
+                for (int w = 0; w < kWords; ++w) {
+                    if constexpr (kFmt == kKvMxFp8) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) { // bytes 2c and 2c + 1 of the word: {key 0, key 1} side by side
-                        const uint32_t lo = __byte_perm(x[0][w], x[1][w], c ? 0x7362 : 0x5140);
-                        const uint32_t hi = __byte_perm(x[2][w], x[3][w], c ? 0x7362 : 0x5140);
+                        for (int c = 0; c < 2; ++c) { // bytes 2c and 2c + 1 of the word: {key 0, key 1} side by side
+                            uint32_t lo[2], hi[2];
+                            e4m3x4(__byte_perm(x[0][w], x[1][w], c ? 0x7362 : 0x5140), lo[0], lo[1]);
+                            e4m3x4(__byte_perm(x[2][w], x[3][w], c ? 0x7362 : 0x5140), hi[0], hi[1]);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t b0 = mul_16x2<kBf16>(e4m3_pair<kBf16>(lo, e), scale01);
-                            const uint32_t b1 = mul_16x2<kBf16>(e4m3_pair<kBf16>(hi, e), scale23);
-                            mma_16816<kBf16>(o[4 * w + 2 * c + e], p0, p1, p2, p3, b0, b1);
+                            for (int e = 0; e < 2; ++e) {
+                                mma_16816<kWide>(o[4 * w + 2 * c + e], p0, p1, p2, p3, scaled<kWide>(lo[e], scale01), scaled<kWide>(hi[e], scale23));
+                            }
+                        }
+                    } else {
+                        // even nibbles of both keys in one byte, then odd ones
+                        uint32_t even_lo[4], odd_lo[4], even_hi[4], odd_hi[4];
+                        e2m1x8((x[0][w] & 0x0f0f0f0fu) | ((x[1][w] << 4) & 0xf0f0f0f0u), even_lo);
+                        e2m1x8(((x[0][w] >> 4) & 0x0f0f0f0fu) | (x[1][w] & 0xf0f0f0f0u), odd_lo);
+                        e2m1x8((x[2][w] & 0x0f0f0f0fu) | ((x[3][w] << 4) & 0xf0f0f0f0u), even_hi);
+                        e2m1x8(((x[2][w] >> 4) & 0x0f0f0f0fu) | (x[3][w] & 0xf0f0f0f0u), odd_hi);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            mma_16816<kWide>(o[8 * w + 2 * i], p0, p1, p2, p3, scaled<kWide>(even_lo[i], scale01), scaled<kWide>(even_hi[i], scale23));
+                            mma_16816<kWide>(o[8 * w + 2 * i + 1], p0, p1, p2, p3, scaled<kWide>(odd_lo[i], scale01), scaled<kWide>(odd_hi[i], scale23));
                         }
                     }
-                } else {
-                    // even nibbles of both keys in one byte, then odd ones
-                    const uint32_t even_lo = (x[0][w] & 0x0f0f0f0fu) | ((x[1][w] << 4) & 0xf0f0f0f0u);
-                    const uint32_t odd_lo = ((x[0][w] >> 4) & 0x0f0f0f0fu) | (x[1][w] & 0xf0f0f0f0u);
-                    const uint32_t even_hi = (x[2][w] & 0x0f0f0f0fu) | ((x[3][w] << 4) & 0xf0f0f0f0u);
-                    const uint32_t odd_hi = ((x[2][w] >> 4) & 0x0f0f0f0fu) | (x[3][w] & 0xf0f0f0f0u);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mma_16816<kBf16>(o[8 * w + 2 * i], p0, p1, p2, p3,
-                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((even_lo >> (8 * i)) & 0xffu), scale01),
-                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((even_hi >> (8 * i)) & 0xffu), scale23));
-                        mma_16816<kBf16>(o[8 * w + 2 * i + 1], p0, p1, p2, p3,
-                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((odd_lo >> (8 * i)) & 0xffu), scale01),
-                                         mul_16x2<kBf16>(e2m1_pair<kBf16>((odd_hi >> (8 * i)) & 0xffu), scale23));
-                    }
                 }
+            };
+            if constexpr (kBf16) {
+                const bool exact = scale_ok<kFmt>(sb[0]) && scale_ok<kFmt>(sb[1]) && scale_ok<kFmt>(sb[2]) && scale_ok<kFmt>(sb[3]);
+                if (__all_sync(0xffffffffu, exact)) {
+                    product(std::false_type{});
+                } else {
+                    product(std::true_type{});
+                }
+            } else {
+                product(std::false_type{});
             }
         }
         __syncwarp(); // every lane has read the stage before it is loaded again
@@ -512,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
 
     // ---- the four warps' sums joined through shared memory
     float *mo = reinterpret_cast<float *>(smem);                                       // [warp][row][d]
-    float2 *ml = reinterpret_cast<float2 *>(smem + kWarps * kRows * kD * sizeof(float)); // [warp][row]
+    float2 *ml = reinterpret_cast<float2 *>(smem + kWarps * kRows * St::kMergePitch * sizeof(float)); // [warp][row]
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -520,20 +556,27 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
         if (t == 0) {
             ml[warp * kRows + g + 8 * i] = make_float2(m[i], l[i]);
         }
-        // columns 2t and 2t + 1 of every tile: elements W (2t + c) .. + W - 1
+        if constexpr (!kMx) { // columns 2t and 2t + 1 of tile n: elements 8n + 2t, + 1
+            float *dst = mo + (warp * kRows + g + 8 * i) * St::kMergePitch + 2 * t;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float4 *dst = reinterpret_cast<float4 *>(mo + (warp * kRows + g + 8 * i) * kD + kTiles * (2 * t + c));
+            for (int n = 0; n < kTiles; ++n) {
+                *reinterpret_cast<float2 *>(dst + 8 * n) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            }
+        } else { // columns 2t and 2t + 1 of every tile: elements W (2t + c) .. + W - 1
 #pragma unroll
-            for (int n = 0; n < kTiles / 4; ++n) {
-                dst[n] = make_float4(o[4 * n][2 * i + c], o[4 * n + 1][2 * i + c], o[4 * n + 2][2 * i + c], o[4 * n + 3][2 * i + c]);
+            for (int c = 0; c < 2; ++c) {
+                float4 *dst = reinterpret_cast<float4 *>(mo + (warp * kRows + g + 8 * i) * St::kMergePitch + kTiles * (2 * t + c));
+#pragma unroll
+                for (int n = 0; n < kTiles / 4; ++n) {
+                    dst[n] = make_float4(o[4 * n][2 * i + c], o[4 * n + 1][2 * i + c], o[4 * n + 2][2 * i + c], o[4 * n + 3][2 * i + c]);
+                }
             }
         }
     }
     __syncthreads();
     {
-        constexpr int kCols = kRows * kD / kThreads; // elements of one row a thread joins
-        const int r = threadIdx.x / (kThreads / kRows), c0 = (threadIdx.x % (kThreads / kRows)) * kCols;
+        // eight threads a row, four elements of every 32 each
+        const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 4;
         float top = -INFINITY, w[kWarps], sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
@@ -546,24 +589,25 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
             w[i] = ex2(v.x - ref);
             sum += v.y * w[i];
         }
-        float4 *dst = reinterpret_cast<float4 *>(a.part_o + (slot * kRows + r) * kD + c0);
+        float *dst = a.part_o + (slot * kRows + r) * kD + c0;
 #pragma unroll
-        for (int c = 0; c < kCols; c += 4) {
+        for (int c = 0; c < kD; c += 32) {
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) {
-                const float4 v = *reinterpret_cast<const float4 *>(mo + (i * kRows + r) * kD + c0 + c);
+                const float4 v = *reinterpret_cast<const float4 *>(mo + (i * kRows + r) * St::kMergePitch + c0 + c);
                 acc.x = fmaf(v.x, w[i], acc.x);
                 acc.y = fmaf(v.y, w[i], acc.y);
                 acc.z = fmaf(v.z, w[i], acc.z);
                 acc.w = fmaf(v.w, w[i], acc.w);
             }
-            dst[c / 4] = acc;
+            *reinterpret_cast<float4 *>(dst + c) = acc;
         }
         if (c0 == 0) {
             a.part_ml[slot * kRows + r] = make_float2(top, sum);
         }
     }
+    programmatic_wait(); // this grid is not complete before the wide kernel's, which the joining kernel reads as well
 }
 
 // Joins a row's pieces in a fixed order: four warps a row, each every fourth piece, then their four sums.  The pieces'
@@ -573,12 +617,12 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
 {
     constexpr int kPer = kD / 32;
     __shared__ float sums[kWarps], accs[kWarps][kD];
-    const int64_t idx = blockIdx.x; // output row: (batch, token, head)
+    const uint32_t idx = blockIdx.x; // output row: (batch, token, head)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = static_cast<int>(idx % a.heads);
-    const int tok = static_cast<int>(idx / a.heads % a.tokens);
-    const int b = static_cast<int>(idx / a.heads / a.tokens);
-    const int h = head / a.group, in = tok * a.group + head % a.group;
+    const uint32_t row = idx / static_cast<uint32_t>(a.heads);
+    const int head = static_cast<int>(idx - row * a.heads);
+    const int b = static_cast<int>(row / static_cast<uint32_t>(a.tokens)), tok = static_cast<int>(row) - b * a.tokens;
+    const int h = head / a.group, in = tok * a.group + head - h * a.group;
     const int prow = b * a.tokens * a.group + in;
     const int len = own_len(a, b);
     const int own_pieces = len > 0 ? ceil_div(len, own_chunk(len, a.own_splits, a.own_min)) : 0;
@@ -591,6 +635,7 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
         const int64_t s = i - a.prefix_pieces;
         return (prefix_items + ((s * a.batch + b) * a.kv_heads + h) * a.own_tiles + in / kRows) * kRows + in % kRows;
     };
+    programmatic_wait();
     float top = -INFINITY;
     for (int i = lane; i < pieces; i += 32) {
         top = fmaxf(top, a.part_ml[row_of(i)].x);
@@ -645,7 +690,7 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
             const int at = 2 * threadIdx.x + c;
             v[c] = ((accs[0][at] + accs[1][at]) + (accs[2][at] + accs[3][at])) * inv;
         }
-        reinterpret_cast<uint32_t *>(a.o + idx * kD)[threadIdx.x] = pack_16x2<kBf16>(v[0], v[1]);
+        reinterpret_cast<uint32_t *>(a.o + static_cast<int64_t>(idx) * kD)[threadIdx.x] = pack_16x2<kBf16>(v[0], v[1]);
         if (a.lse != nullptr && threadIdx.x == 0) {
             a.lse[idx] = none ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
         }
@@ -694,14 +739,26 @@ Plan make_plan(int batch, int tokens, int heads, int kv_heads, int prefix_len, i
     p.own_tiles = ceil_div(row_span, kRows);
     p.own_min = 64;
     if (own_max > 0) {
+        // as many pieces as make the waves of blocks shortest: a piece costs its keys and about 384 more (queries, first
+        // loads, joining its warps: 9000 cycles against 1850 for 64 keys); long sequences are cut anyway, for the sake of uneven lengths
         const int64_t units = static_cast<int64_t>(p.own_tiles) * kv_heads * batch;
-        int64_t splits = (target + units - 1) / units;
-        if (units >= target) { // the batch alone fills the GPU: pieces only for the sake of uneven lengths
-            splits = ceil_div(own_max, 1024);
-            p.own_min = 512;
-        }
         const int most = ceil_div(own_max, 64);
-        p.own_splits = static_cast<int>(splits > most ? most : splits);
+        int best = 1;
+        int64_t best_cost = -1;
+        for (int waves = 1; waves <= 4; ++waves) { // the most pieces that fit in so many waves
+            int64_t splits = waves * static_cast<int64_t>(target) / units;
+            splits = splits < 1 ? 1 : (splits > most ? most : splits);
+            const int64_t cost = (units * splits + target - 1) / target * (ceil_div(own_max, static_cast<int>(splits)) + 384);
+            if (best_cost < 0 || cost < best_cost) {
+                best = static_cast<int>(splits);
+                best_cost = cost;
+            }
+        }
+        const int least = ceil_div(own_max, 2048);
+        p.own_splits = best < least ? least : best;
+        if (p.own_splits * units >= target) {
+            p.own_min = 256;
+        }
     }
     p.own_slots = static_cast<int64_t>(p.own_splits) * p.own_tiles * batch * kv_heads;
     p.slots = static_cast<int64_t>(p.prefix_pieces) * p.prefix_tiles * kv_heads + p.own_slots;
@@ -716,8 +773,8 @@ int launch_pieces(const AttnArgs &a, int64_t blocks, DeviceStatus *status, cudaS
     if (rc != kOk) {
         return rc;
     }
-    prefix_attn_piece_kernel<kBf16, kD, kFmt><<<static_cast<unsigned>(blocks), kThreads, kSmem, stream>>>(a, status);
-    return check_launch();
+    return launch_overlapped(&prefix_attn_piece_kernel<kBf16, kD, kFmt>, static_cast<unsigned>(blocks), kThreads, kSmem, stream,
+                             a.prefix_wide != 0, a, status);
 }
 
 template <bool kBf16, int kD>
@@ -739,8 +796,7 @@ int launch_typed(int fmt, const AttnArgs &a, int64_t own_slots, DeviceStatus *st
         }
     }
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
-    prefix_attn_join_kernel<kBf16, kD><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(a);
-    return check_launch();
+    return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD>, static_cast<unsigned>(rows), kThreads, 0, stream, blocks > 0 || a.prefix_wide != 0, a);
 }
 
 } // namespace

@@ -30,6 +30,34 @@ struct AttnArgs {
 
 constexpr int kPieceRows = 16; // rows of a slot of partial results
 
+// The kernels of one call overlap: a kernel lets the next one start as soon as its own blocks are all running, and the next
+// one waits before it touches what the earlier ones write.  Only kernels of the same call are launched that way: the
+// first one starts when everything before it on the stream is complete.
+__device__ __forceinline__ void programmatic_trigger()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void programmatic_wait()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... Params, typename... Args>
+int launch_overlapped(void (*kernel)(Params...), unsigned blocks, int threads, int smem, cudaStream_t stream, bool after_own, Args... args)
+{
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = after_own ? 1 : 0;
+    return check_cuda(cudaLaunchKernelEx(&config, kernel, args...), "kernel launch");
+}
+
 // keys by the tensor memory of one block per SM: 128-row tiles of the prefix's rows against 128 keys at a time
 int launch_prefix_wide(const AttnArgs &a, int fmt, int d, bool bf16, DeviceStatus *status, cudaStream_t stream);
 

@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     uint8_t *smem_p = smem_v + kRingV * Sh::kTileBytes;
     Control *ctl = reinterpret_cast<Control *>(smem_p + 2 * Sh::kPBytes);
 
+    programmatic_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- which rows and keys: block = ((split * kv_heads) + h) * row blocks + row block
