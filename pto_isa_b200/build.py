@@ -57,6 +57,7 @@ def build(force=False, verbose=False):
         subprocess.check_call([_nvcc()] + flags + ["--extended-lambda", "-I", os.path.join(HERE, "..", "include"),
                                                   "-shared", "-o", prog_out, prog_src])
     build_host(force)
+    build_fast(force)
     for so, src in SHIMS.items():
         src_path = os.path.join(CSRC, src)
         out = os.path.join(HERE, so)
@@ -90,6 +91,27 @@ def build_host(force=False):
                                "-L" + HERE, "-lpto_b200_launchers", "-lpto_b200", "-L" + os.path.join(cuda_home, "lib64"),
                                "-lcudart", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(cuda_home, "lib64")])
     return exe
+
+
+def build_fast(force=False):
+    """The serving operators' calls without the interpreter's share of them (csrc/host/torch_fast.cpp), a Python extension
+    module over torch's C++ tensors and the C ABI."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src, out = os.path.join(CSRC, "host", "torch_fast.cpp"), os.path.join(HERE, "_fast.so")
+    header = os.path.join(HERE, "..", "include", "pto_b200.h")
+    if force or _stale(out, [src, header]):
+        cuda_home = os.path.dirname(os.path.dirname(_nvcc()))
+        includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda_home, "include")]
+        lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in includes] +
+                              ["-o", out, src, "-L" + HERE, "-lpto_b200", "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+                               "-Wl,-rpath,$ORIGIN"])
+    return out
 
 
 if __name__ == "__main__":

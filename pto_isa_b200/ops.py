@@ -643,6 +643,12 @@ _DTYPE16 = {torch.float16: 2, torch.bfloat16: 4}  # PTO_B200_DTYPE_F16 / _BF16
 _KV_DTYPE = {KV_F16: torch.float16, KV_BF16: torch.bfloat16}
 
 
+try:  # calls in order go straight from torch's tensors to the C ABI; it returns None for those that the checks below are for
+    from . import _fast
+except ImportError:  # not built, or for another torch: every call goes through the checks below
+    _fast = None
+
+
 class KVCache(collections.namedtuple("KVCache", "k v k_scale v_scale fmt")):
     """A paged key / value cache.  k, v: (num_pages, kv_heads, page_size, head_dim) float16 / bfloat16 (KV_F16, KV_BF16),
     or uint8 codes: float8_e4m3fn bytes (KV_MXFP8), or float4_e2m1 two a byte, the lower index in the low nibble, head_dim / 2
@@ -742,6 +748,8 @@ def kv_cache_write(cache, k, v, slots):
     MX formats: per 32 elements the smallest power of two at which none saturates (2^119 at most for fp8, 2^125 for fp4),
     elements rounded to nearest even; a block that holds a NaN or an infinity reads back as NaN.  A slot beyond the cache is
     skipped and reported by device_status().  Returns the cache."""
+    if _fast is not None and _fast.kv_cache_write(cache, k, v, slots):
+        return cache
     c, _, heads, _, d = _cache_struct(cache, "kv_cache_write")
     _rows16(k, 3, "kv_cache_write", "k")
     _rows16(v, 3, "kv_cache_write", "v")
@@ -763,6 +771,10 @@ def kv_cache_read(cache, page_table, seq_lens, max_len, dtype=torch.float16, out
     """Reads sequences back: (k, v), each (batch, kv_heads, max_len, head_dim) of `dtype`, the layout flash_attn_fwd takes.
     Position t of sequence b comes from page page_table[b, t // page_size] ((batch, pages) int32) for t < seq_lens[b] ((batch,)
     int32) and is zero from there on.  Values are rounded to `dtype` once (overflow to infinity); `out`: a pair of tensors."""
+    if _fast is not None and out is None and dtype in _DTYPE16:
+        pair = _fast.kv_cache_read(cache, page_table, seq_lens, max_len, dtype == torch.bfloat16)
+        if pair is not None:
+            return pair
     c, _, heads, _, d = _cache_struct(cache, "kv_cache_read")
     if dtype not in _DTYPE16:
         raise PtoB200Error("kv_cache_read: dtype is float16 or bfloat16")
@@ -795,6 +807,10 @@ def prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale=
     Returns O like q, zeros for a row without any key; with return_lse also the natural logarithm of the sum of
     exponentials, float32 of q's shape without head_dim, -inf for such a row.  `workspace`: a CUDA byte tensor of at least
     prefix_attn_workspace_bytes(...), 16-byte aligned; without it one is taken from torch's allocator per call."""
+    if _fast is not None and out is None and workspace is None:
+        o = _fast.prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale, max_seq_len, bool(return_lse))
+        if o is not None:
+            return o
     c, _, kv_heads, page_size, d = _cache_struct(cache, "prefix_attn")
     single = q.dim() == 3
     q4 = q.unsqueeze(1) if single else q
@@ -850,6 +866,10 @@ def w4_matvec(x, w, scale, zero=None, out_dtype=None, out=None):
       one byte each, group 32: MX fp4, W = e2m1(code) * 2^(scale - 127), mx_gemm_fp4's operand b;
       of x's type, group 32, 64 or 128: int4, W = scale * (code - zero), zero like scale, 8 when None.
     A 1-D x is one row and gives a 1-D y.  y is of x's type, or float32 with out_dtype=torch.float32."""
+    if _fast is not None and out is None and (out_dtype is None or out_dtype == x.dtype or out_dtype == torch.float32):
+        y = _fast.w4_matvec(x, w, scale, zero, out_dtype == torch.float32)
+        if y is not None:
+            return y
     vector = x.dim() == 1
     x2 = x.unsqueeze(0) if vector else x
     _rows16(x2, 2, "w4_matvec", "x")
