@@ -347,11 +347,14 @@ int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtyp
  * out_f32.  format PTO_B200_W4_MXFP4: float4_e2m1 codes with float8_e8m0 bytes scale (n x k / 32), the operand b of
  * pto_b200_mxgemm_fp4 (group must be 32, zero NULL); PTO_B200_W4_INT4: W = scale * (code - zero), scale and zero
  * (n x k / group), group 32, 64 or 128, zero = 8 when NULL.  k a multiple of group; sums in fp32.  For more rows use the
- * GEMMs. */
+ * GEMMs.  `workspace`: device memory of pto_b200_w4_matvec_workspace_bytes(...) bytes (0 for one or two rows of usual length),
+ * 16-byte aligned, not shared by calls that may run at the same time. */
 #define PTO_B200_W4_MXFP4 0
 #define PTO_B200_W4_INT4 1
+int64_t pto_b200_w4_matvec_workspace_bytes(int m, int k, int format);
 int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const void *scale, const void *zero, void *y, int m,
-                       int n, int k, int group, int format, int dtype, int out_f32, void *stream);
+                       int n, int k, int group, int format, int dtype, int out_f32, void *workspace, int64_t workspace_bytes,
+                       void *stream);
 
 /* ---- drop-in shims with the reference's FFI signatures ------------------------------------------ */
 

@@ -65,7 +65,8 @@ SIGNATURES = {
     "pto_b200_kv_cache_read": (_i, [_vp, _vp, _i64, _i, _vp, _i, _i, _vp, _vp, _i, _vp]),
     "pto_b200_prefix_attn_workspace_bytes": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
     "pto_b200_prefix_attn": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _i64, _i, _vp, _i, _i, _i, _i, _f, _vp, _vp, _vp, _i64, _vp]),
-    "pto_b200_w4_matvec": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "pto_b200_w4_matvec_workspace_bytes": (_i64, [_i, _i, _i]),
+    "pto_b200_w4_matvec": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
     "pto_b200_gemm_call_kernel": (None, [_u32, _vp, _vp, _vp, _vp]),
     "pto_b200_fa_call_kernel": (None, [_vp, _i, _i, _i, ctypes.c_bool] + [_vp] * 11),
 }

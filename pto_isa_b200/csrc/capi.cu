@@ -797,8 +797,14 @@ int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtyp
                               scale, static_cast<uint16_t *>(o), lse, workspace, workspace_bytes, as_stream(stream));
 }
 
+int64_t pto_b200_w4_matvec_workspace_bytes(int m, int k, int format)
+{
+    return m <= 0 || m > 64 || k <= 0 ? 0 : w4_matvec_workspace_bytes(m, k, format == PTO_B200_W4_MXFP4);
+}
+
 int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const void *scale, const void *zero, void *y, int m,
-                       int n, int k, int group, int format, int dtype, int out_f32, void *stream)
+                       int n, int k, int group, int format, int dtype, int out_f32, void *workspace, int64_t workspace_bytes,
+                       void *stream)
 {
     if (m < 0 || n < 0 || k < 0 || (format != PTO_B200_W4_MXFP4 && format != PTO_B200_W4_INT4) ||
         (dtype != PTO_B200_DTYPE_F16 && dtype != PTO_B200_DTYPE_BF16)) {
@@ -821,12 +827,13 @@ int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const 
         set_error_text("w4_matvec: k must be a positive multiple of the group (%d)", group);
         return kErrUnsupportedShape;
     }
-    if (misaligned16(x) || misaligned16(w) || (x_stride & 7) != 0) {
-        set_error_text("w4_matvec: rows of x and w must be 16-byte aligned");
+    if (misaligned16(x) || misaligned16(w) || misaligned16(workspace) || (x_stride & 7) != 0) {
+        set_error_text("w4_matvec: rows of x, w and the workspace must be 16-byte aligned");
         return kErrUnsupportedShape;
     }
     return launch_w4_matvec(static_cast<const uint16_t *>(x), x_stride, w, scale, static_cast<const uint16_t *>(zero), y, m, n, k,
-                            group, dtype == PTO_B200_DTYPE_BF16, format == PTO_B200_W4_MXFP4, out_f32 != 0, as_stream(stream));
+                            group, dtype == PTO_B200_DTYPE_BF16, format == PTO_B200_W4_MXFP4, out_f32 != 0, workspace, workspace_bytes,
+                            as_stream(stream));
 }
 
 // ------------------------------------------------------------------ reference-shaped shims

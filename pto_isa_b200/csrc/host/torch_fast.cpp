@@ -248,9 +248,14 @@ PyObject *fast_w4(PyObject *, PyObject *const *args, Py_ssize_t n)
         const bool out32 = args[4] == Py_True;
         const auto options = out32 ? x.options().dtype(at::kFloat) : x.options();
         at::Tensor y = x.dim() == 1 ? at::empty({rows}, options) : at::empty({m, rows}, options);
+        const int64_t bytes = pto_b200_w4_matvec_workspace_bytes(static_cast<int>(m), static_cast<int>(k), mx ? PTO_B200_W4_MXFP4 : PTO_B200_W4_INT4);
+        at::Tensor workspace;
+        if (bytes > 0) {
+            workspace = at::empty({bytes}, x.options().dtype(at::kByte));
+        }
         need(pto_b200_w4_matvec(x.data_ptr(), stride, static_cast<const uint8_t *>(w.data_ptr()), scale.data_ptr(), zero, y.data_ptr(), static_cast<int>(m),
                                 static_cast<int>(rows), static_cast<int>(k), static_cast<int>(group), mx ? PTO_B200_W4_MXFP4 : PTO_B200_W4_INT4, dtype,
-                                out32 ? 1 : 0, stream(device)) == 0);
+                                out32 ? 1 : 0, bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream(device)) == 0);
         return THPVariable_Wrap(std::move(y));
     });
 }

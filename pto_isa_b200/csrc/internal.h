@@ -134,6 +134,8 @@ int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, c
                        uint16_t *o, float *lse, void *workspace, int64_t workspace_bytes, cudaStream_t stream);
 // y[m, n] = sum_k x[m, k] W[n, k] with 4-bit weights; arguments validated by the caller
 int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, const void *scale, const uint16_t *zero, void *y,
-                     int m, int n, int k, int group, bool bf16, bool mx, bool out_f32, cudaStream_t stream);
+                     int m, int n, int k, int group, bool bf16, bool mx, bool out_f32, void *workspace, int64_t workspace_bytes,
+                     cudaStream_t stream);
+int64_t w4_matvec_workspace_bytes(int m, int k, bool mx);
 
 } // namespace pto_b200

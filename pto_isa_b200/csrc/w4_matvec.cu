@@ -16,14 +16,16 @@
 // mma.m16n8k16, the rows of x its eight columns; the order of k inside 32 is free as long as both operands agree: lane t
 // of a quad takes k = 8t .. 8t + 7 (one word of codes).  The rows of W are dealt out evenly, to the row, over as many
 // blocks as are resident; two kernels:
-//   resident  all of x fits beside the ring of two blocks an SM (m k up to about 21 000): x is prepared once a block; the
-//             eight warps share the k axis, each with a cp.async ring of its own that runs on across the block's row
-//             tiles, so that no warp waits for another but once a tile, where the shares of k are joined.
-//   streamed  x comes in pieces of 256 k, prepared by the whole block an iteration ahead; kWr of the warps lie along the
-//             rows of W (x is read from L2 once for all of them), 8 / kWr share the k axis.
+//   narrow    one or two rows of x: prepared by every block and kept in shared memory; the eight warps share the k axis, each
+//             with a cp.async ring of its own that runs on across the block's row tiles, so that no warp waits for another
+//             but once a tile, where the shares of k are joined.
+//   streamed  more rows: x is prepared once by a kernel of its own, whose time the first loads of W hide, and comes through
+//             the ring in runs of 256 k; kWr of the warps lie along the rows of W (x is read from L2 once for all of
+//             them), 8 / kWr share the k axis.  float16 x against MX fp4 needs no preparation.
 #include "ptx.cuh"
 #include "internal.h"
 #include "mx_format.cuh"
+#include "prefix_attn.cuh"
 
 namespace pto_b200 {
 
@@ -37,9 +39,9 @@ constexpr int kPitch = kStepBytes + 16;  // 8 rows x 4 words of a quad's reads m
 constexpr int kNarrowPitch = kStepBytes;  // odd rows with their 64-byte halves exchanged: two rows x 4 lanes of a 16-byte read
 constexpr int kXPitch = kStepK * 2 + 64; // two rows x 4 lanes of a 16-byte read phase likewise
 constexpr int kStages = 3;               // of the streamed kernel's ring
-constexpr int kResidentStages = 3;       // of a warp's ring in the resident kernel
-constexpr int kResidentSmem = 112 * 1024; // two blocks an SM
-constexpr int kNarrowSmem = 75 * 1024;    // three
+constexpr int kNarrowStages = 3;         // of a warp's ring in the narrow kernel
+constexpr int kNarrowSmem = 74 * 1024;   // of a block, for three an SM
+constexpr int kNarrowMost = 112 * 1024;  // for two
 constexpr int kSms = 148;
 
 struct W4Args {
@@ -51,6 +53,8 @@ struct W4Args {
     int64_t x_stride;
     int m, n, k, group_shift, out_f32, out_bf16;
     int rows_each, rows_more; // rows of W a block owns; the first rows_more blocks one more
+    const uint8_t *xp; // prepared x: runs of 256 k, x_run bytes each (streamed kernel)
+    int x_run;
     int scale_async; // the scales of a step are 4, 8 or 16 aligned bytes a row: they ride in the ring
 };
 
@@ -154,10 +158,11 @@ struct LaneX {
 };
 
 // 16 rows of W times the prepared run at `xs`: acc += .  `ws`: the lane's first word of the run's codes (row g, word t),
-// `ss`, `zs`: the run's scales and zeros of row g (rows 16 bytes apart); blks: runs of 32 that exist.
-template <bool kBf16, bool kMx, int kMt>
+// `ss`, `zs`: the run's scales and zeros of row g (rows 16 bytes apart); blks: runs of 32 that exist.  A group of kG runs of
+// 32 is summed before it is scaled.
+template <bool kBf16, bool kMx, int kG, int kMt>
 __device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t *ws, const uint8_t *ss, const uint8_t *zs,
-                                            const uint8_t *xs, const LaneX<kMt> &lx, int group_shift, bool zero, int blks)
+                                            const uint8_t *xs, const LaneX<kMt> &lx, bool zero, int blks)
 {
     float f[kMt][2]; // 2^E of the lane's columns
 #pragma unroll
@@ -167,69 +172,83 @@ __device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t
             f[c][j] = kBf16 ? *reinterpret_cast<const float *>(xs + lx.col[c][j] + 32) : 1.0f;
         }
     }
-    uint2 sv[2];
-    if constexpr (kMx) {
-        sv[0] = *reinterpret_cast<const uint2 *>(ss);
-        sv[1] = *reinterpret_cast<const uint2 *>(ss + 128);
-    }
-    auto block = [&](int blk) {
-        const uint32_t w0 = ws[blk * 4], w1 = ws[blk * 4 + 8 * kPitch / 4];
-        float s[2], z[2] = {8.0f, 8.0f};
-        uint32_t lo[4], hi[4];
-        if constexpr (kMx) {
+    auto group = [&](int first) {
+        float d[kMt][4], e[kMt][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t v = (blk & 4) ? sv[i].y : sv[i].x;
-                s[i] = __uint_as_float(((v >> (8 * (blk & 3))) & 0xffu) << 23);
-                s[i] = fmaf(s[i], 0.0f, s[i]); // 255: infinity times 0 plus itself is NaN; 0 stands for 0, not 2^-127
+        for (int b = 0; b < kG; ++b) {
+            const int blk = first + b;
+            const uint32_t w0 = ws[blk * 4], w1 = ws[blk * 4 + 8 * kPitch / 4];
+            uint32_t lo[4], hi[4];
+            if constexpr (kMx) {
+                e2m1x8_to_f16(w0, lo);
+                e2m1x8_to_f16(w1, hi);
+            } else {
+                int4x8_to_f16(w0, lo);
+                int4x8_to_f16(w1, hi);
             }
-            e2m1x8_to_f16(w0, lo);
-            e2m1x8_to_f16(w1, hi);
-        } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int at = i * 128 + (blk >> (group_shift - 5)) * 2;
-                s[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(ss + at)).x ;
+            for (int c = 0; c < kMt; ++c) {
+                const uint4 xf = *reinterpret_cast<const uint4 *>(xs + lx.row[c] + blk * 64);
+                if (b == 0) {
+                    mma_16816_first<false>(d[c], lo[0], hi[0], lo[1], hi[1], xf.x, xf.y);
+                } else {
+                    mma_16816<false>(d[c], lo[0], hi[0], lo[1], hi[1], xf.x, xf.y);
+                }
+                if constexpr (kMx) {
+                    mma_16816<false>(d[c], lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+                } else if (b == 0) {
+                    mma_16816_first<false>(e[c], lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+                } else {
+                    mma_16816<false>(e[c], lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
+                }
+            }
+        }
+        float s[2], z[2] = {8.0f, 8.0f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (kMx) {
+                s[i] = __uint_as_float(static_cast<uint32_t>(ss[i * 128 + first]) << 23);
+                s[i] = fmaf(s[i], 0.0f, s[i]); // 255: infinity times 0 plus itself is NaN; 0 stands for 0, not 2^-127
+            } else {
+                const int at = i * 128 + first / kG * 2;
+                s[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(ss + at)).x;
                 if (zero) {
                     z[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(zs + at)).x;
                 }
             }
-            int4x8_to_f16(w0, lo);
-            int4x8_to_f16(w1, hi);
         }
 #pragma unroll
         for (int c = 0; c < kMt; ++c) {
-            const uint4 xf = *reinterpret_cast<const uint4 *>(xs + lx.row[c] + blk * 64);
-            float d[4];
-            mma_16816_first<false>(d, lo[0], hi[0], lo[1], hi[1], xf.x, xf.y);
-            if constexpr (kMx) {
-                mma_16816<false>(d, lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
-            } else {
-                float e[4];
-                mma_16816_first<false>(e, lo[2], hi[2], lo[3], hi[3], xf.z, xf.w);
-                const float u[2] = {*reinterpret_cast<const float *>(xs + lx.col[c][0] + blk * 4),
-                                    *reinterpret_cast<const float *>(xs + lx.col[c][1] + blk * 4)};
+            float u[2] = {0.0f, 0.0f};
+            if constexpr (!kMx) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    d[i] = fmaf(d[i], 16777216.0f, fmaf(e[i], 1048576.0f, -z[i >> 1] * u[i & 1]));
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int b = 0; b < kG; ++b) {
+                        u[j] += *reinterpret_cast<const float *>(xs + lx.col[c][j] + (first + b) * 4);
+                    }
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                float v = d[c][i];
+                if constexpr (!kMx) { // the codes went in times 2^-24 and 2^-20
+                    v = fmaf(v, 16777216.0f, fmaf(e[c][i], 1048576.0f, -z[i >> 1] * u[i & 1]));
+                }
                 // 2^E before the scale: no product leaves fp32's range that x and W keep in it
-                acc[c][i] = fmaf(kBf16 ? d[i] * f[c][i & 1] : d[i], s[i >> 1], acc[c][i]);
+                acc[c][i] = fmaf(kBf16 ? v * f[c][i & 1] : v, s[i >> 1], acc[c][i]);
             }
         }
     };
     if (blks >= kStepK / 32) {
 #pragma unroll
-        for (int blk = 0; blk < kStepK / 32; ++blk) {
-            block(blk);
+        for (int blk = 0; blk < kStepK / 32; blk += kG) {
+            group(blk);
         }
     } else {
 #pragma unroll 1
-        for (int blk = 0; blk < blks; ++blk) {
-            block(blk);
+        for (int blk = 0; blk < blks; blk += kG) {
+            group(blk);
         }
     }
 }
@@ -339,51 +358,36 @@ __device__ __forceinline__ void store_y(const W4Args &a, int64_t at, float v)
     }
 }
 
-// ------------------------------------------------------------------ resident x
+// ------------------------------------------------------------------ one or two rows
 
-// kMt: column tiles, 0 = the narrow form for one or two rows of x
-template <bool kMx, int kMt>
-__host__ __device__ constexpr int resident_stage_bytes()
+template <bool kMx>
+__host__ __device__ constexpr int narrow_stage_bytes()
 {
-    return 16 * (kMt == 0 ? kNarrowPitch : kPitch) + (kMx ? 1 : 2) * 256;
+    return 16 * kNarrowPitch + (kMx ? 1 : 2) * 256;
 }
 
-template <int kMt>
-__host__ __device__ constexpr int resident_columns() // rows of x that a warp's sums have room for
+constexpr int kNarrowCols = 3; // floats of a row in a warp's share: two columns, and one so that rows meet other banks
+constexpr int kNarrowShare = 16 * kNarrowCols;
+
+// shared memory: the warps' rings, two buffers of shares of k, x (all runs), zeros
+template <bool kMx>
+int narrow_smem(int m, int k)
 {
-    return kMt == 0 ? 2 : 8 * kMt;
+    return kWarps * kNarrowStages * narrow_stage_bytes<kMx>() + 2 * kWarps * kNarrowShare * 4 +
+           (k + kStepK - 1) / kStepK * ((m * kXRow + 15) & ~15) + 512;
 }
 
-// rows of a prepared run: m and one of zeros where columns are left over (in the narrow form always, and once for all runs)
-template <int kMt>
-__host__ __device__ int resident_x_rows(int m)
-{
-    return kMt == 0 ? m : (m < 8 * kMt ? m + 1 : m);
-}
-
-// shared memory: the warps' rings, two buffers of shares of k [8][16][columns + 1], x (all runs), the narrow form's zeros
-template <bool kMx, int kMt>
-int resident_smem(int m, int k)
-{
-    return kWarps * kResidentStages * resident_stage_bytes<kMx, kMt>() + 2 * kWarps * 16 * (resident_columns<kMt>() + 1) * 4 +
-           (k + kStepK - 1) / kStepK * ((resident_x_rows<kMt>(m) * kXRow + 15) & ~15) + (kMt == 0 ? 512 : 0);
-}
-
-template <bool kBf16, bool kMx, int kMt>
-__global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel(const __grid_constant__ W4Args a)
+template <bool kBf16, bool kMx>
+__global__ void __launch_bounds__(kThreads, 3) w4_narrow_kernel(const __grid_constant__ W4Args a)
 {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int kStage = resident_stage_bytes<kMx, kMt>();
-    constexpr int kRowPitch = kMt == 0 ? kNarrowPitch : kPitch;
-    constexpr int kCols = resident_columns<kMt>() + 1;
-    constexpr int kShare = 16 * kCols; // floats of a warp's share of a tile
+    constexpr int kStage = narrow_stage_bytes<kMx>();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    uint8_t *ring = smem + warp * kResidentStages * kStage;
-    float *shares = reinterpret_cast<float *>(smem + kWarps * kResidentStages * kStage);
-    uint8_t *xs = smem + kWarps * kResidentStages * kStage + 2 * kWarps * kShare * 4;
-    const int x_rows = resident_x_rows<kMt>(a.m);
-    const int x_run = (x_rows * kXRow + 15) & ~15;
+    uint8_t *ring = smem + warp * kNarrowStages * kStage;
+    float *shares = reinterpret_cast<float *>(smem + kWarps * kNarrowStages * kStage);
+    uint8_t *xs = smem + kWarps * kNarrowStages * kStage + 2 * kWarps * kNarrowShare * 4;
+    const int x_run = (a.m * kXRow + 15) & ~15;
     const int block = static_cast<int>(blockIdx.x);
     const int row_begin = block * a.rows_each + min(block, a.rows_more), row_end = row_begin + a.rows_each + (block < a.rows_more ? 1 : 0);
     const int tiles = (row_end - row_begin + 15) / 16;
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel
     const uint8_t *src = a.w + (row_begin + (lane >> 3)) * row_bytes + warp * kStepBytes + (lane & 7) * 16;
     const bool zeros = lane >= 16, has_scale = !zeros || (!kMx && a.zero != nullptr);
     const uint8_t *scale_src = (zeros ? a.zero : a.scale) + (row_begin + (lane & 15)) * row_scale + warp * scale_bytes;
-    const uint32_t dst = smem_u32(ring) + (lane >> 3) * kRowPitch + (((lane & 7) * 16) ^ (kMt == 0 ? (lane & 8) * 8 : 0)), scale_dst = smem_u32(ring) + 16 * kRowPitch + lane * 16;
+    const uint32_t dst = smem_u32(ring) + (lane >> 3) * kNarrowPitch + (((lane & 7) * 16) ^ ((lane & 8) * 8)), scale_dst = smem_u32(ring) + 16 * kNarrowPitch + lane * 16;
     auto load_next = [&](int stage) {
         if (ahead_tile < tiles) {
             const int rows = row_end - row_begin - ahead_tile * 16; // of this tile
@@ -407,13 +411,13 @@ __global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel
             if (rows >= 16 && (ahead_run + 1) * kStepK <= a.k) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    cp_async(dst + to + i * 4 * kRowPitch, src + i * four_rows, 16, true);
+                    cp_async(dst + to + i * 4 * kNarrowPitch, src + i * four_rows, 16, true);
                 }
             } else { // the end of the rows or of k (a multiple of 32: chunks are whole)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const bool live = i * 4 + (lane >> 3) < rows && ahead_run * kStepBytes + (lane & 7) * 16 < row_bytes;
-                    cp_async(dst + to + i * 4 * kRowPitch, live ? src + i * four_rows : a.w, 16, live);
+                    cp_async(dst + to + i * 4 * kNarrowPitch, live ? src + i * four_rows : a.w, 16, live);
                 }
             }
             if (has_scale) {
@@ -439,13 +443,12 @@ __global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const LaneX<kMt == 0 ? 1 : kMt> lx(x_rows, g, t);
-    // narrow form: the lane feeds column g if that is group t of a row of x that exists
+    // the lane feeds column g if that is group t of a row of x that exists
     uint8_t *nothing = xs + runs * x_run;
     const bool feeds = (g & 3) == t && (g >> 2) < a.m;
-    const int x_at = (g >> 2) * kXPitch + t * 64, side_at = x_rows * kXPitch + min(t >> 1, a.m - 1) * 36;
+    const int x_at = (g >> 2) * kXPitch + t * 64, side_at = a.m * kXPitch + min(t >> 1, a.m - 1) * 36;
 #pragma unroll
-    for (int s = 0; s < kResidentStages - 1; ++s) {
+    for (int s = 0; s < kNarrowStages - 1; ++s) {
         load_next(s);
     }
     // x: a warp prepares one row of one run at a time
@@ -456,65 +459,36 @@ __global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel
         if (k0 < a.k) {
             v = __ldg(reinterpret_cast<const uint4 *>(a.x + row * a.x_stride + k0));
         }
-        prepare_run<kBf16, kMx>(v, xs + run * x_run, x_rows, row, lane);
+        prepare_run<kBf16, kMx>(v, xs + run * x_run, a.m, row, lane);
     }
-    if constexpr (kMt == 0) {
-        if (threadIdx.x < 32) {
-            reinterpret_cast<uint4 *>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-        }
-    } else if (x_rows > a.m) {
-        for (int run = warp; run < runs; run += kWarps) {
-            clear_last_row(xs + run * x_run, x_rows, lane, 32);
-        }
+    if (threadIdx.x < 32) {
+        reinterpret_cast<uint4 *>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     }
     __syncthreads();
 
     int stage = 0;
     for (int tile = 0; tile < tiles; ++tile) {
-        constexpr int kAcc = kMt == 0 ? 1 : kMt;
-        float acc[kAcc][4];
-#pragma unroll
-        for (int c = 0; c < kAcc; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                acc[c][i] = 0.0f;
-            }
-        }
         float narrow[2] = {0.0f, 0.0f};
         for (int j = 0; j < mine; ++j) {
-            load_next(stage == 0 ? kResidentStages - 1 : stage - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kResidentStages - 1) : "memory");
+            load_next(stage == 0 ? kNarrowStages - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kNarrowStages - 1) : "memory");
             __syncwarp();
             const uint8_t *base = ring + stage * kStage;
             const int run = warp + j * kWarps;
-            const uint8_t *ss = base + 16 * kRowPitch + g * 16, *x = xs + run * x_run;
-            if constexpr (kMt == 0) { // codes, scales and x past the end of k are zeros: no run is short
-                run_product_narrow<kBf16, kMx>(narrow, base + g * kRowPitch + 16 * t, ss, ss + 256, feeds ? x + x_at : nothing,
-                                               reinterpret_cast<const float *>(x + side_at), a.group_shift, a.zero != nullptr, t, (g & 1) * 64);
-            } else {
-                run_product<kBf16, kMx, kMt>(acc, reinterpret_cast<const uint32_t *>(base + g * kRowPitch) + t, ss, ss + 256, x, lx,
-                                             a.group_shift, a.zero != nullptr, (a.k - run * kStepK) / 32);
-            }
+            const uint8_t *ss = base + 16 * kNarrowPitch + g * 16, *x = xs + run * x_run;
+            // codes, scales and x past the end of k are zeros: no run is short
+            run_product_narrow<kBf16, kMx>(narrow, base + g * kNarrowPitch + 16 * t, ss, ss + 256, feeds ? x + x_at : nothing,
+                                           reinterpret_cast<const float *>(x + side_at), a.group_shift, a.zero != nullptr, t, (g & 1) * 64);
             __syncwarp(); // every lane has read the stage before it is loaded again
-            stage = stage + 1 == kResidentStages ? 0 : stage + 1;
+            stage = stage + 1 == kNarrowStages ? 0 : stage + 1;
         }
         // the warps' shares of k joined in a fixed order; the buffers alternate, so one barrier a tile is enough
-        float *share = shares + (tile & 1) * kWarps * kShare;
-        if constexpr (kMt == 0) {
+        float *share = shares + (tile & 1) * kWarps * kNarrowShare;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                narrow[i] += __shfl_xor_sync(0xffffffffu, narrow[i], 1); // groups 0, 1 and 2, 3
-                if ((t & 1) == 0) {
-                    share[warp * kShare + (g + 8 * i) * kCols + (t >> 1)] = narrow[i];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < kMt; ++c) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    share[warp * kShare + (g + 8 * (i >> 1)) * kCols + 8 * c + 2 * t + (i & 1)] = acc[c][i];
-                }
+        for (int i = 0; i < 2; ++i) {
+            narrow[i] += __shfl_xor_sync(0xffffffffu, narrow[i], 1); // groups 0, 1 and 2, 3
+            if ((t & 1) == 0) {
+                share[warp * kNarrowShare + (g + 8 * i) * kNarrowCols + (t >> 1)] = narrow[i];
             }
         }
         __syncthreads();
@@ -525,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel
                 float v = 0.0f;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    v += share[w * kShare + row * kCols + col];
+                    v += share[w * kNarrowShare + row * kNarrowCols + col];
                 }
                 store_y<kBf16>(a, static_cast<int64_t>(col) * a.n + n0 + row, v);
             }
@@ -534,30 +508,67 @@ __global__ void __launch_bounds__(kThreads, kMt == 0 ? 3 : 2) w4_resident_kernel
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// ------------------------------------------------------------------ streamed x
+// ------------------------------------------------------------------ more rows
 
-// shared memory of a stage: W [kWk][16 kWr rows][kPitch], scales and zeros [kWk][16 kWr rows][16]; x apart, two buffers of
-// kWk prepared runs; the shares of k are joined in the ring's place
+// rows of a prepared run: m and one of zeros where the last column tile has columns left over
+__host__ __device__ inline int streamed_x_rows(int m)
+{
+    return m <= 8 ? (m < 8 ? m + 1 : 8) : (m <= 16 ? (m < 16 ? m + 1 : 16) : (m <= 32 ? (m < 32 ? m + 1 : 32) : (m < 64 ? m + 1 : 64)));
+}
+__host__ __device__ inline int streamed_x_run(int m)
+{
+    return (streamed_x_rows(m) * kXRow + 15) & ~15;
+}
+
+// one warp prepares one row of one run, in the layout of the streamed kernel's shared memory
+template <bool kBf16, bool kMx>
+__global__ void __launch_bounds__(kThreads) w4_prepare_kernel(const __grid_constant__ W4Args a, uint8_t *xp)
+{
+    programmatic_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int x_rows = streamed_x_rows(a.m);
+    const int unit = static_cast<int>(blockIdx.x) * kWarps + warp, run = unit / x_rows, row = unit - run * x_rows;
+    if (run >= (a.k + kStepK - 1) / kStepK) {
+        return;
+    }
+    uint8_t *at = xp + static_cast<int64_t>(run) * a.x_run;
+    if (row >= a.m) {
+        clear_last_row(at, x_rows, lane, 32);
+        return;
+    }
+    const int64_t k0 = static_cast<int64_t>(run) * kStepK + lane * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k0 < a.k) {
+        v = __ldg(reinterpret_cast<const uint4 *>(a.x + row * a.x_stride + k0));
+    }
+    prepare_run<kBf16, kMx>(v, at, x_rows, row, lane);
+}
+
+// shared memory of a stage: W [kWk][16 kWr rows][kPitch], scales and zeros [kWk][16 kWr rows][16], kWk runs of x; the shares
+// of k are joined in the ring's place
 template <bool kMx, int kWr, int kMt>
 struct Layout {
     static constexpr int kWk = kWarps / kWr;
     static constexpr int kRows = 16 * kWr;
     static constexpr int kW = kWk * kRows * kPitch;
     static constexpr int kScale = kWk * kRows * 16;
-    static constexpr int kStage = kW + (kMx ? 1 : 2) * kScale;
+    static constexpr int kX = kW + (kMx ? 1 : 2) * kScale;
     static constexpr int kSums = kWk * 8 * kMt * kRows * 4;
-    static constexpr int kRing = kStages * kStage > kSums ? kStages * kStage : kSums;
-    static __host__ __device__ int x_rows(int m) { return m < 8 * kMt ? m + 1 : m; }
-    static __host__ __device__ int x_run(int m) { return (x_rows(m) * kXRow + 15) & ~15; }
-    static int smem_bytes(int m) { return kRing + 2 * kWk * x_run(m); }
+    static __host__ __device__ int stage_bytes(int m) { return kX + kWk * streamed_x_run(m); }
+    static int smem_bytes(int m)
+    {
+        const int ring = kStages * stage_bytes(m);
+        return ring > kSums ? ring : kSums;
+    }
 };
 
-template <bool kBf16, bool kMx, int kWr, int kMt>
+// kG: runs of 32 k in a group of the scales
+template <bool kBf16, bool kMx, int kG, int kWr, int kMt>
 __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel(const __grid_constant__ W4Args a)
 {
     using L = Layout<kMx, kWr, kMt>;
     constexpr int kWk = L::kWk;
-    constexpr int kPasses = kMt * kWk; // rows times runs of an iteration, by the eight warps
+    constexpr bool kRaw = !kBf16 && kMx; // x as it is
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -565,66 +576,65 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel
     const int block = static_cast<int>(blockIdx.x);
     const int row_begin = block * a.rows_each + min(block, a.rows_more), row_end = row_begin + a.rows_each + (block < a.rows_more ? 1 : 0);
     const int64_t row_bytes = a.k / 2;
-    const int64_t row_scale = static_cast<int64_t>(a.k >> a.group_shift) * (kMx ? 1 : 2);
+    const int64_t row_scale = static_cast<int64_t>(a.k / (32 * kG)) * (kMx ? 1 : 2);
+    constexpr int kScaleBytes = kMx ? 8 : 16 / kG; // of a row in a step
     const int iters = (a.k + kStepK * kWk - 1) / (kStepK * kWk);
-    const int x_rows = L::x_rows(a.m), x_run = L::x_run(a.m);
-    const int scale_bytes = kMx ? 8 : 512 >> a.group_shift; // of a row in a step
-    uint8_t *xbuf = smem + L::kRing;
+    const int x_rows = streamed_x_rows(a.m), x_run = streamed_x_run(a.m), stage_bytes = L::stage_bytes(a.m);
     const LaneX<kMt> lx(x_rows, g, t);
-    if (x_rows > a.m) {
-        for (int i = warp; i < 2 * kWk; i += kWarps) {
-            clear_last_row(xbuf + i * x_run, x_rows, lane, 32);
+    if (kRaw && x_rows > a.m) { // the row of zeros stays where it is
+        for (int i = warp; i < kStages * kWk; i += kWarps) {
+            clear_last_row(smem + i / kWk * stage_bytes + L::kX + i % kWk * x_run, x_rows, lane, 32);
         }
     }
+    bool waited = false;
 
     for (int n0 = row_begin; n0 < row_end; n0 += L::kRows) {
+        // ---- this thread's pieces of a stage: 16-byte chunk threadIdx % 8 of rows row0 + 32 i of the (step, row) list
+        constexpr int kPieces = L::kRows * kWk * 8 / kThreads; // 4
+        const uint8_t *src[kPieces];
+        uint32_t live = 0;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int r = i * (kThreads / 8) + (threadIdx.x >> 3), row = r % L::kRows, step = r / L::kRows;
+            src[i] = a.w + (n0 + row < row_end ? (n0 + row) * row_bytes : 0) + step * kStepBytes + (threadIdx.x & 7) * 16;
+            live |= n0 + row < row_end ? 1u << i : 0u;
+        }
+        const int sr = threadIdx.x & 127, s_row = sr % L::kRows, s_step = sr / L::kRows; // 128 runs of scales, then of zeros
+        const bool zeros = threadIdx.x >= 128, has_scale = !zeros || (!kMx && a.zero != nullptr), s_live = n0 + s_row < row_end;
+        const uint8_t *scale_src = (zeros ? a.zero : a.scale) + (s_live ? (n0 + s_row) * row_scale : 0);
         auto load_w = [&](int it) {
-            if (it < iters) {
-                const uint32_t base = smem_u32(smem) + (it % kStages) * L::kStage;
+            const uint32_t base = smem_u32(smem) + (it % kStages) * stage_bytes;
+            const bool whole = (it + 1) * kStepK * kWk <= a.k;
 #pragma unroll
-                for (int i = 0; i < L::kRows * kWk * 8 / kThreads; ++i) {
-                    const int c = i * kThreads + threadIdx.x; // 16-byte chunk: eight a row and step
-                    const int row = (c >> 3) % L::kRows, step = (c >> 3) / L::kRows;
-                    const int64_t col = (static_cast<int64_t>(it) * kWk + step) * kStepBytes + (c & 7) * 16;
-                    const bool live = n0 + row < row_end && col < row_bytes; // k is a multiple of 32: chunks are whole
-                    cp_async(base + (step * L::kRows + row) * kPitch + (c & 7) * 16, a.w + (live ? (n0 + row) * row_bytes + col : 0), 16, live);
-                }
-                // 16 kWr rows x kWk steps = 128 runs of scales, then as many of zeros
-                const int r = threadIdx.x & 127, row = r % L::kRows, step = r / L::kRows;
-                const bool zeros = threadIdx.x >= 128, live = n0 + row < row_end;
-                if (!zeros || (!kMx && a.zero != nullptr)) {
-                    load_scales(base + L::kW + (zeros ? L::kScale : 0) + (step * L::kRows + row) * 16,
-                                (zeros ? a.zero : a.scale) + (live ? (n0 + row) * row_scale : 0),
-                                (static_cast<int64_t>(it) * kWk + step) * scale_bytes, row_scale, scale_bytes, live, a.scale_async);
-                }
+            for (int i = 0; i < kPieces; ++i) {
+                const int r = i * (kThreads / 8) + (threadIdx.x >> 3), step = r / L::kRows;
+                const int64_t off = static_cast<int64_t>(it) * kWk * kStepBytes;
+                // k is a multiple of 32: chunks are whole
+                const bool ok = (live >> i & 1u) && (whole || off + step * kStepBytes + (threadIdx.x & 7) * 16 < row_bytes);
+                cp_async(base + r * kPitch + (threadIdx.x & 7) * 16, ok ? src[i] + off : a.w, 16, ok);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (has_scale) {
+                load_scales(base + L::kW + (zeros ? L::kScale : 0) + sr * 16, scale_src, (static_cast<int64_t>(it) * kWk + s_step) * kScaleBytes,
+                            row_scale, kScaleBytes, s_live, a.scale_async);
+            }
         };
-        // x: loaded an iteration ahead, a warp one row of one run at a time
-        uint4 xr[kPasses];
-        const int units = a.m * kWk;
         auto load_x = [&](int it) {
-#pragma unroll
-            for (int p = 0; p < kPasses; ++p) {
-                const int unit = p * kWarps + warp;
-                xr[p] = make_uint4(0, 0, 0, 0);
-                if (it < iters && unit < units) {
-                    const int64_t k0 = (static_cast<int64_t>(it) * kWk + unit % kWk) * kStepK + lane * 8;
-                    if (k0 < a.k) {
-                        xr[p] = __ldg(reinterpret_cast<const uint4 *>(a.x + (unit / kWk) * a.x_stride + k0));
-                    }
+            const uint32_t base = smem_u32(smem) + (it % kStages) * stage_bytes + L::kX;
+            if constexpr (kRaw) {
+                for (int i = threadIdx.x; i < kWk * a.m * 32; i += kThreads) { // 32 chunks of a row's run
+                    const int c = i & 31, unit = i >> 5, step = unit % kWk, row = unit / kWk;
+                    const int64_t k0 = (static_cast<int64_t>(it) * kWk + step) * kStepK + c * 8;
+                    cp_async(base + step * x_run + row * kXPitch + c * 16, a.x + (k0 < a.k ? row * a.x_stride + k0 : 0), 16, k0 < a.k);
+                }
+            } else { // kWk prepared runs, one after another
+                const int chunks = kWk * x_run / 16, have = ((a.k + kStepK - 1) / kStepK - it * kWk) * (x_run / 16);
+                const uint8_t *from = a.xp + static_cast<int64_t>(it) * kWk * x_run;
+                for (int i = threadIdx.x; i < chunks && i < have; i += kThreads) {
+                    cp_async(base + i * 16, from + i * 16, 16, true);
                 }
             }
         };
-        auto store_x = [&](int it) {
-#pragma unroll
-            for (int p = 0; p < kPasses; ++p) {
-                const int unit = p * kWarps + warp;
-                if (unit < units) {
-                    prepare_run<kBf16, kMx>(xr[p], xbuf + ((it & 1) * kWk + unit % kWk) * x_run, x_rows, unit / kWk, lane);
-                }
-            }
-        };
+        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
         float acc[kMt][4];
 #pragma unroll
@@ -635,25 +645,37 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel
             }
         }
 #pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) {
-            load_w(s);
+        for (int s = 0; s < kStages - 1; ++s) { // W does not depend on the preparation of x
+            if (s < iters) {
+                load_w(s);
+            }
         }
-        load_x(0);
-        store_x(0);
+        if (!kRaw && !waited) {
+            programmatic_wait();
+            waited = true;
+        }
+#pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) {
+            if (s < iters) {
+                load_x(s);
+            }
+            commit();
+        }
         for (int it = 0; it < iters; ++it) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            __syncthreads(); // stage `it` of W and x is there, and everybody is done with the stage the next loads overwrite
-            load_w(it + kStages - 1);
-            load_x(it + 1);
-            const uint8_t *base = smem + (it % kStages) * L::kStage;
+            __syncthreads(); // stage `it` is there, and everybody is done with the stage that the next loads overwrite
+            if (it + kStages - 1 < iters) {
+                load_w(it + kStages - 1);
+                load_x(it + kStages - 1);
+            }
+            commit();
+            const uint8_t *base = smem + (it % kStages) * stage_bytes;
             const int row = wk * L::kRows + wr * 16 + g;
             const int left = (a.k - (it * kWk + wk) * kStepK) / 32;
             if (left > 0 && n0 + wr * 16 < row_end) {
-                run_product<kBf16, kMx, kMt>(acc, reinterpret_cast<const uint32_t *>(base + row * kPitch) + t, base + L::kW + row * 16,
-                                             base + L::kW + L::kScale + row * 16, xbuf + ((it & 1) * kWk + wk) * x_run, lx,
-                                             a.group_shift, a.zero != nullptr, left);
+                run_product<kBf16, kMx, kG, kMt>(acc, reinterpret_cast<const uint32_t *>(base + row * kPitch) + t, base + L::kW + row * 16,
+                                                 base + L::kW + L::kScale + row * 16, base + L::kX + wk * x_run, lx, a.zero != nullptr, left);
             }
-            store_x(it + 1);
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
@@ -680,85 +702,108 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel
             }
         }
         __syncthreads(); // the sums are read before the ring is loaded again
+        if (kRaw && x_rows > a.m && n0 + L::kRows < row_end) { // the sums lay over the rows of zeros
+            for (int i = warp; i < kStages * kWk; i += kWarps) {
+                clear_last_row(smem + i / kWk * stage_bytes + L::kX + i % kWk * x_run, x_rows, lane, 32);
+            }
+        }
     }
 }
 
 // ------------------------------------------------------------------ launches
 
-template <bool kBf16, bool kMx, int kMt>
-int launch_resident(W4Args a, int blocks, cudaStream_t stream)
+template <bool kBf16, bool kMx>
+int launch_narrow(W4Args a, cudaStream_t stream)
 {
+    const int smem = narrow_smem<kMx>(a.m, a.k), tiles = (a.n + 15) / 16;
+    const int most = smem <= kNarrowSmem ? 3 * kSms : 2 * kSms, blocks = tiles < most ? tiles : most;
     a.rows_each = a.n / blocks;
     a.rows_more = a.n % blocks;
     // the attribute is raised once per kernel and device: to the most that is ever asked
-    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&w4_resident_kernel<kBf16, kMx, kMt>), kResidentSmem);
+    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&w4_narrow_kernel<kBf16, kMx>), kNarrowMost);
     if (rc != kOk) {
         return rc;
     }
-    w4_resident_kernel<kBf16, kMx, kMt><<<blocks, kThreads, resident_smem<kMx, kMt>(a.m, a.k), stream>>>(a);
+    w4_narrow_kernel<kBf16, kMx><<<blocks, kThreads, smem, stream>>>(a);
     return check_launch();
 }
 
-template <bool kBf16, bool kMx, int kWr, int kMt>
-int launch_streamed(W4Args a, int blocks, cudaStream_t stream)
+template <bool kBf16, bool kMx, int kG, int kWr, int kMt>
+int launch_streamed(W4Args a, int blocks, uint8_t *workspace, cudaStream_t stream)
 {
+    using L = Layout<kMx, kWr, kMt>;
+    const void *kernel = reinterpret_cast<const void *>(&w4_streamed_kernel<kBf16, kMx, kG, kWr, kMt>);
+    int rc = ensure_dynamic_smem(kernel, L::smem_bytes(8 * kMt));
+    constexpr bool kRaw = !kBf16 && kMx;
+    if (!kRaw && rc == kOk) {
+        a.xp = workspace;
+        const int units = (a.k + kStepK - 1) / kStepK * streamed_x_rows(a.m);
+        w4_prepare_kernel<kBf16, kMx><<<(units + kWarps - 1) / kWarps, kThreads, 0, stream>>>(a, workspace);
+        rc = check_launch();
+    }
+    if (rc != kOk) {
+        return rc;
+    }
     a.rows_each = a.n / blocks;
     a.rows_more = a.n % blocks;
-    using L = Layout<kMx, kWr, kMt>;
-    const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(&w4_streamed_kernel<kBf16, kMx, kWr, kMt>), L::smem_bytes(8 * kMt));
-    if (rc != kOk) {
-        return rc;
-    }
-    w4_streamed_kernel<kBf16, kMx, kWr, kMt><<<blocks, kThreads, L::smem_bytes(a.m), stream>>>(a);
-    return check_launch();
+    return launch_overlapped(&w4_streamed_kernel<kBf16, kMx, kG, kWr, kMt>, static_cast<unsigned>(blocks), kThreads, L::smem_bytes(a.m), stream, !kRaw, a);
 }
 
-template <bool kBf16, bool kMx>
-int launch_typed(const W4Args &a, cudaStream_t stream)
+template <bool kBf16, bool kMx, int kG>
+int launch_rows(W4Args a, uint8_t *workspace, cudaStream_t stream)
 {
-    const int tiles = (a.n + 15) / 16;
-    if (a.m <= 2 && resident_smem<kMx, 0>(a.m, a.k) <= kResidentSmem) {
-        const int most = resident_smem<kMx, 0>(a.m, a.k) <= kNarrowSmem ? 3 * kSms : 2 * kSms;
-        return launch_resident<kBf16, kMx, 0>(a, tiles < most ? tiles : most, stream);
-    }
-    if (a.m <= 8 && resident_smem<kMx, 1>(a.m, a.k) <= kResidentSmem) {
-        return launch_resident<kBf16, kMx, 1>(a, tiles < 2 * kSms ? tiles : 2 * kSms, stream);
-    }
-    if (a.m <= 16 && resident_smem<kMx, 2>(a.m, a.k) <= kResidentSmem) {
-        return launch_resident<kBf16, kMx, 2>(a, tiles < 2 * kSms ? tiles : 2 * kSms, stream);
-    }
     // two blocks an SM, or one where that leaves a block fewer than 32 rows: every block reads all of x
-    const int blocks = a.n >= 64 * kSms ? 2 * kSms : (tiles < kSms ? tiles : kSms);
+    const int tiles = (a.n + 15) / 16;
+    const int blocks = a.n >= 64 * kSms && a.m <= 32 ? 2 * kSms : (tiles < kSms ? tiles : kSms);
     const int rows = (a.n + blocks - 1) / blocks;
-    const int wr = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8));
+    a.x_run = streamed_x_run(a.m);
     if (a.m <= 8) {
-        switch (wr) {
-            case 1: return launch_streamed<kBf16, kMx, 1, 1>(a, blocks, stream);
-            case 2: return launch_streamed<kBf16, kMx, 2, 1>(a, blocks, stream);
-            case 4: return launch_streamed<kBf16, kMx, 4, 1>(a, blocks, stream);
-            default: return launch_streamed<kBf16, kMx, 8, 1>(a, blocks, stream);
-        }
+        return rows <= 16   ? launch_streamed<kBf16, kMx, kG, 1, 1>(a, blocks, workspace, stream)
+               : rows <= 32 ? launch_streamed<kBf16, kMx, kG, 2, 1>(a, blocks, workspace, stream)
+               : rows <= 64 ? launch_streamed<kBf16, kMx, kG, 4, 1>(a, blocks, workspace, stream)
+                            : launch_streamed<kBf16, kMx, kG, 8, 1>(a, blocks, workspace, stream);
     }
     if (a.m <= 16) {
-        switch (wr) {
-            case 1:
-            case 2: return launch_streamed<kBf16, kMx, 2, 2>(a, blocks, stream);
-            case 4: return launch_streamed<kBf16, kMx, 4, 2>(a, blocks, stream);
-            default: return launch_streamed<kBf16, kMx, 8, 2>(a, blocks, stream);
-        }
+        return rows <= 32   ? launch_streamed<kBf16, kMx, kG, 2, 2>(a, blocks, workspace, stream)
+               : rows <= 64 ? launch_streamed<kBf16, kMx, kG, 4, 2>(a, blocks, workspace, stream)
+                            : launch_streamed<kBf16, kMx, kG, 8, 2>(a, blocks, workspace, stream);
     }
-    if (a.m <= 32) {
-        return wr <= 4 ? launch_streamed<kBf16, kMx, 4, 4>(a, blocks, stream) : launch_streamed<kBf16, kMx, 8, 4>(a, blocks, stream);
+    return a.m <= 32 ? launch_streamed<kBf16, kMx, kG, 8, 4>(a, blocks, workspace, stream)
+                     : launch_streamed<kBf16, kMx, kG, 8, 8>(a, blocks, workspace, stream);
+}
+
+template <bool kBf16>
+int launch_typed(const W4Args &a, bool mx, uint8_t *workspace, cudaStream_t stream)
+{
+    if (a.m <= 2 && (mx ? narrow_smem<true>(a.m, a.k) : narrow_smem<false>(a.m, a.k)) <= kNarrowMost) {
+        return mx ? launch_narrow<kBf16, true>(a, stream) : launch_narrow<kBf16, false>(a, stream);
     }
-    return launch_streamed<kBf16, kMx, 8, 8>(a, blocks, stream);
+    return mx                   ? launch_rows<kBf16, true, 1>(a, workspace, stream)
+           : a.group_shift == 5 ? launch_rows<kBf16, false, 1>(a, workspace, stream)
+           : a.group_shift == 6 ? launch_rows<kBf16, false, 2>(a, workspace, stream)
+                                : launch_rows<kBf16, false, 4>(a, workspace, stream);
 }
 
 } // namespace
 
-int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, const void *scale, const uint16_t *zero, void *y,
-                     int m, int n, int k, int group, bool bf16, bool mx, bool out_f32, cudaStream_t stream)
+// room for the prepared x; not asked for where the call does without (few rows, or float16 x against MX fp4)
+int64_t w4_matvec_workspace_bytes(int m, int k, bool mx)
 {
-    W4Args a;
+    if (m <= 2 && (mx ? narrow_smem<true>(m, k) : narrow_smem<false>(m, k)) <= kNarrowMost) {
+        return 0;
+    }
+    return static_cast<int64_t>((k + kStepK - 1) / kStepK) * streamed_x_run(m);
+}
+
+int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, const void *scale, const uint16_t *zero, void *y,
+                     int m, int n, int k, int group, bool bf16, bool mx, bool out_f32, void *workspace, int64_t workspace_bytes,
+                     cudaStream_t stream)
+{
+    if (workspace_bytes < w4_matvec_workspace_bytes(m, k, mx) || (workspace == nullptr && w4_matvec_workspace_bytes(m, k, mx) > 0)) {
+        set_error_text("w4_matvec: the workspace is smaller than pto_b200_w4_matvec_workspace_bytes says");
+        return kErrBadArgument;
+    }
+    W4Args a = {};
     a.x = x;
     a.w = w;
     a.scale = static_cast<const uint8_t *>(scale);
@@ -771,10 +816,8 @@ int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, cons
     a.group_shift = group == 32 ? 5 : (group == 64 ? 6 : 7);
     a.out_f32 = out_f32;
     a.scale_async = k % kStepK == 0 && ((reinterpret_cast<uintptr_t>(scale) | reinterpret_cast<uintptr_t>(zero)) & 15u) == 0;
-    if (mx) {
-        return bf16 ? launch_typed<true, true>(a, stream) : launch_typed<false, true>(a, stream);
-    }
-    return bf16 ? launch_typed<true, false>(a, stream) : launch_typed<false, false>(a, stream);
+    return bf16 ? launch_typed<true>(a, mx, static_cast<uint8_t *>(workspace), stream)
+                : launch_typed<false>(a, mx, static_cast<uint8_t *>(workspace), stream);
 }
 
 } // namespace pto_b200

@@ -900,10 +900,13 @@ def w4_matvec(x, w, scale, zero=None, out_dtype=None, out=None):
     if out_dtype != x.dtype and out_dtype != torch.float32:
         raise PtoB200Error("w4_matvec: the output is of x's type or float32")
     y = _out(out, (n,) if vector else (m, n), out_dtype, x.device, "w4_matvec")
+    need = lib().pto_b200_w4_matvec_workspace_bytes(m, k, 0 if mx else 1)
+    workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with torch.cuda.device(x.device):
         rc = lib().pto_b200_w4_matvec(x.data_ptr(), x2.stride(0) if m > 1 else 0, w.data_ptr(), scale.data_ptr(),
                                       None if zero is None else zero.data_ptr(), y.data_ptr(), m, n, k, group, 0 if mx else 1,
-                                      _DTYPE16[x.dtype], 1 if out_dtype == torch.float32 else 0, _stream(x))
+                                      _DTYPE16[x.dtype], 1 if out_dtype == torch.float32 else 0,
+                                      workspace.data_ptr() if need else None, need, _stream(x))
     check(rc, "w4_matvec")
     return y
 

@@ -130,6 +130,7 @@ def test_w4_matvec_checks(rec):  # noqa: F811
     assert ops.w4_matvec(x, w, u8(40, 8)).shape == (3, 40)
     assert ops.w4_matvec(x[0], w, rows(40, 2), zero=rows(40, 2), out_dtype=torch.float32).shape == (40,)
     n = len(rec.calls)
+    assert rec.calls.count("pto_b200_w4_matvec") == 2
     for kw, what in [
             (dict(x=rows(3, 192)), r"\(n, 96\)"), (dict(x=rows(65, 256)), "at most 64"), (dict(x=x.float()), "float16 or bfloat16"),
             (dict(scale=u8(40, 4)), "one scale byte per 32"), (dict(scale=u8(39, 8)), "scale is"), (dict(scale=rows(40, 1)), "32, 64 or 128"),
@@ -139,7 +140,7 @@ def test_w4_matvec_checks(rec):  # noqa: F811
             (dict(scale=u8(40, 0)), "scale is"), (dict(w=w.to(torch.int16)), r"\(n, 128\) bytes")]:
         with pytest.raises(PtoB200Error, match=what):
             ops.w4_matvec(**{**dict(x=x, w=w, scale=u8(40, 8)), **kw})
-    assert len(rec.calls) == n
+    assert rec.calls.count("pto_b200_w4_matvec") == 2
 
 
 def test_cpu_tensors_are_refused():
@@ -185,7 +186,9 @@ def test_c_entry_points_refuse_before_they_touch_a_device(clib):
     assert need(1, 1, 4, 2, 64, 16, 16) > 0
 
     def w4(m=1, n=8, k=64, group=32, fmt=0, dtype=2, x=some, zero=None, stride=64):
-        return clib.pto_b200_w4_matvec(x, stride, some, some, zero, some, m, n, k, group, fmt, dtype, 0, None)
+        return clib.pto_b200_w4_matvec(x, stride, some, some, zero, some, m, n, k, group, fmt, dtype, 0, None, 0, None)
     assert w4(m=-1) == 1 and w4(fmt=2) == 1 and w4(dtype=0) == 1 and w4(x=None) == 1 and w4(m=65) == 2 and w4(zero=some) == 1
     assert w4(group=64) == 1 and w4(fmt=1, group=48) == 1 and w4(k=48) == 2 and w4(k=0) == 2 and w4(fmt=1, group=128) == 2
+    assert clib.pto_b200_w4_matvec_workspace_bytes(1, 4096, 0) == 0 and clib.pto_b200_w4_matvec_workspace_bytes(3, 4096, 0) > 0
+    assert w4(m=3) == 1 and b"workspace" in clib.pto_b200_last_error()
     assert w4(x=ctypes.c_void_p((1 << 20) + 2)) == 2 and w4(stride=60) == 2 and w4(m=0) == 0 and w4(n=0) == 0
