@@ -21,7 +21,7 @@
 //             but once a tile, where the shares of k are joined.
 //   streamed  more rows: x is prepared once by a kernel of its own, whose time the first loads of W hide, and comes through
 //             the ring in runs of 256 k; kWr of the warps lie along the rows of W (x is read from L2 once for all of
-//             them), 8 / kWr share the k axis.  float16 x against MX fp4 needs no preparation.
+//             them), 8 / kWr share the k axis.
 #include "ptx.cuh"
 #include "internal.h"
 #include "mx_format.cuh"
@@ -35,13 +35,14 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStepK = 256;              // k of one warp's step
 constexpr int kStepBytes = kStepK / 2;   // bytes of a row of W in a step
-constexpr int kPitch = kStepBytes + 16;  // 8 rows x 4 words of a quad's reads meet 32 distinct banks
 constexpr int kNarrowPitch = kStepBytes;  // odd rows with their 64-byte halves exchanged: two rows x 4 lanes of a 16-byte read
 constexpr int kXPitch = kStepK * 2 + 64; // two rows x 4 lanes of a 16-byte read phase likewise
-constexpr int kStages = 3;               // of the streamed kernel's ring
+constexpr int kBoxBytes = 16 * kStepBytes; // a warp's 16 rows of W in a step
 constexpr int kNarrowStages = 3;         // of a warp's ring in the narrow kernel
 constexpr int kNarrowSmem = 74 * 1024;   // of a block, for three an SM
 constexpr int kNarrowMost = 112 * 1024;  // for two
+constexpr int kStreamedSmem = 112 * 1024; // of a block, for two an SM
+constexpr int kStreamedMost = 224 * 1024; // for one
 constexpr int kSms = 148;
 
 struct W4Args {
@@ -54,8 +55,8 @@ struct W4Args {
     int m, n, k, group_shift, out_f32, out_bf16;
     int rows_each, rows_more; // rows of W a block owns; the first rows_more blocks one more
     const uint8_t *xp; // prepared x: runs of 256 k, x_run bytes each (streamed kernel)
-    int x_run;
-    int scale_async; // the scales of a step are 4, 8 or 16 aligned bytes a row: they ride in the ring
+    int x_run, stages, tile_rows; // tile_rows: rows of W that a block takes at once
+    int scale_async; // the scales of a step are 4, 8 or 16 aligned bytes a row
 };
 
 // bytes global -> shared, 4, 8 or 16, zeros where not live
@@ -90,12 +91,12 @@ __device__ __forceinline__ void int4x8_to_f16(uint32_t w, uint32_t (&p)[4])
     p[3] = (w >> 8) & 0x00f000f0u;
 }
 
-// Where a prepared run of 256 k of x lies: x_rows rows of kXPitch bytes, then per row 8 sums of x' (int4) and the factor
+// Where a prepared run of 256 k of x lies: x_rows rows of kXPitch bytes, then per row up to 8 sums of x' (int4) and the factor
 // 2^E (bfloat16), 36 bytes.  x_rows is m, and one row of zeros for the columns past it unless m fills the tiles.
 constexpr int kXRow = kXPitch + 36;
 
 // One warp prepares row `row`, k run `run` of x: eight elements a lane.
-template <bool kBf16, bool kMx>
+template <bool kBf16, bool kMx, int kG>
 __device__ __forceinline__ void prepare_run(uint4 in, uint8_t *at, int x_rows, int row, int lane)
 {
     uint32_t v[4] = {in.x, in.y, in.z, in.w};
@@ -120,7 +121,7 @@ __device__ __forceinline__ void prepare_run(uint4 in, uint8_t *at, int x_rows, i
             side[8] = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
         }
     }
-    if constexpr (!kMx) { // sums of x' over runs of 32, for the zero points
+    if constexpr (!kMx) { // sums of x' over kG runs of 32, for the zero points
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -129,8 +130,14 @@ __device__ __forceinline__ void prepare_run(uint4 in, uint8_t *at, int x_rows, i
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if ((lane & 3) == 0) {
-            side[lane >> 2] = sum;
+        if constexpr (kG >= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        }
+        if constexpr (kG >= 4) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        }
+        if ((lane & (4 * kG - 1)) == 0) {
+            side[lane / (4 * kG)] = sum;
         }
         // codes (i, i + 4) share a mask: k order (0, 4) (2, 6) (1, 5) (3, 7)
         const uint32_t y0 = v[0], y1 = v[1], y2 = v[2], y3 = v[3];
@@ -141,6 +148,63 @@ __device__ __forceinline__ void prepare_run(uint4 in, uint8_t *at, int x_rows, i
     }
     *reinterpret_cast<uint4 *>(at + row * kXPitch + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
 }
+
+// two e8m0 scale bytes as floats (255: NaN)
+__device__ __forceinline__ float2 e8m0x2_to_f32(uint32_t v)
+{
+    uint32_t d;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, a;\n\t}" : "=r"(d) : "r"(v));
+    return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xffff0000u));
+}
+
+// The scales or zeros of one row of W in one step
+template <bool kMx, int kG>
+struct StepScales {
+    static constexpr int kBytes = kMx ? 8 : 16 / kG;
+    static constexpr int kWords = kBytes / 4;
+    uint32_t v[kWords];
+
+    __device__ __forceinline__ void read(const uint8_t *at) // shared memory
+    {
+        if constexpr (kWords == 4) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(at);
+            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+        } else if constexpr (kWords == 2) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(at);
+            v[0] = u.x, v[1] = u.y;
+        } else {
+            v[0] = *reinterpret_cast<const uint32_t *>(at);
+        }
+    }
+    // to shared memory from a row that begins anywhere; zeros past its `left` bytes
+    static __device__ __forceinline__ void gather(uint32_t dst, const uint8_t *src, int64_t left)
+    {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+            uint32_t u = 0;
+#pragma unroll
+            for (int b = 0; b < 4; b += kMx ? 1 : 2) {
+                if (4 * w + b < left) {
+                    u |= kMx ? static_cast<uint32_t>(__ldg(src + 4 * w + b)) << (8 * b)
+                             : static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(src + 4 * w + b))) << (8 * b);
+                }
+            }
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + 4 * w), "r"(u) : "memory");
+        }
+    }
+    // of group `at` of the step
+    template <bool kBf16>
+    __device__ __forceinline__ float value(int at) const
+    {
+        if constexpr (kMx) {
+            const float2 f = e8m0x2_to_f32(v[at >> 2] >> (at & 2) * 8);
+            return at & 1 ? f.y : f.x;
+        } else {
+            const float2 f = unpack_16x2<kBf16>(v[at >> 1]);
+            return at & 1 ? f.y : f.x;
+        }
+    }
+};
 
 // where a lane finds its row of x in a prepared run, and the sums and factor of its columns of the result
 template <int kMt>
@@ -157,13 +221,29 @@ struct LaneX {
     }
 };
 
-// 16 rows of W times the prepared run at `xs`: acc += .  `ws`: the lane's first word of the run's codes (row g, word t),
-// `ss`, `zs`: the run's scales and zeros of row g (rows 16 bytes apart); blks: runs of 32 that exist.  A group of kG runs of
-// 32 is summed before it is scaled.
-template <bool kBf16, bool kMx, int kG, int kMt>
-__device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t *ws, const uint8_t *ss, const uint8_t *zs,
-                                            const uint8_t *xs, const LaneX<kMt> &lx, bool zero, int blks)
+__device__ __forceinline__ uint32_t ld_shared(uint32_t at)
 {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+
+// 16 rows of W times the prepared run at `xs`: acc += .  `ws`: where the lane's words of the run's codes are, row g, word t
+// of 16-byte chunk 0 ^ g (128-byte rows, chunks exchanged by the low bits of the row); `ss`: the step's scales of row g, zeros
+// 16 rows behind.  A group of kG runs of 32 is summed
+// before it is scaled.  What lies past the end of k is zero in W and x.
+template <bool kBf16, bool kMx, int kG, int kMt>
+__device__ __forceinline__ void run_product(float (&acc)[kMt][4], uint32_t ws, const uint8_t *ss, const uint8_t *xs, const LaneX<kMt> &lx, bool zero)
+{
+    using Scales = StepScales<kMx, kG>;
+    Scales scales[2], zeros[2]; // rows g and g + 8
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        scales[i].read(ss + i * 8 * Scales::kBytes);
+        if (!kMx && zero) {
+            zeros[i].read(ss + (i * 8 + 16) * Scales::kBytes);
+        }
+    }
     float f[kMt][2]; // 2^E of the lane's columns
 #pragma unroll
     for (int c = 0; c < kMt; ++c) {
@@ -172,12 +252,13 @@ __device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t
             f[c][j] = kBf16 ? *reinterpret_cast<const float *>(xs + lx.col[c][j] + 32) : 1.0f;
         }
     }
-    auto group = [&](int first) {
+#pragma unroll
+    for (int first = 0; first < kStepK / 32; first += kG) {
         float d[kMt][4], e[kMt][4];
 #pragma unroll
         for (int b = 0; b < kG; ++b) {
             const int blk = first + b;
-            const uint32_t w0 = ws[blk * 4], w1 = ws[blk * 4 + 8 * kPitch / 4];
+            const uint32_t w0 = ld_shared(ws ^ (blk * 16)), w1 = ld_shared((ws ^ (blk * 16)) + 8 * kStepBytes);
             uint32_t lo[4], hi[4];
             if constexpr (kMx) {
                 e2m1x8_to_f16(w0, lo);
@@ -206,15 +287,9 @@ __device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t
         float s[2], z[2] = {8.0f, 8.0f};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if constexpr (kMx) {
-                s[i] = __uint_as_float(static_cast<uint32_t>(ss[i * 128 + first]) << 23);
-                s[i] = fmaf(s[i], 0.0f, s[i]); // 255: infinity times 0 plus itself is NaN; 0 stands for 0, not 2^-127
-            } else {
-                const int at = i * 128 + first / kG * 2;
-                s[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(ss + at)).x;
-                if (zero) {
-                    z[i] = unpack_16x2<kBf16>(*reinterpret_cast<const uint16_t *>(zs + at)).x;
-                }
+            s[i] = scales[i].template value<kBf16>(first / kG);
+            if (!kMx && zero) {
+                z[i] = zeros[i].template value<kBf16>(first / kG);
             }
         }
 #pragma unroll
@@ -223,10 +298,7 @@ __device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t
             if constexpr (!kMx) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                    for (int b = 0; b < kG; ++b) {
-                        u[j] += *reinterpret_cast<const float *>(xs + lx.col[c][j] + (first + b) * 4);
-                    }
+                    u[j] = *reinterpret_cast<const float *>(xs + lx.col[c][j] + first / kG * 4);
                 }
             }
 #pragma unroll
@@ -238,17 +310,6 @@ __device__ __forceinline__ void run_product(float (&acc)[kMt][4], const uint32_t
                 // 2^E before the scale: no product leaves fp32's range that x and W keep in it
                 acc[c][i] = fmaf(kBf16 ? v * f[c][i & 1] : v, s[i >> 1], acc[c][i]);
             }
-        }
-    };
-    if (blks >= kStepK / 32) {
-#pragma unroll
-        for (int blk = 0; blk < kStepK / 32; blk += kG) {
-            group(blk);
-        }
-    } else {
-#pragma unroll 1
-        for (int blk = 0; blk < blks; blk += kG) {
-            group(blk);
         }
     }
 }
@@ -296,10 +357,9 @@ __device__ __forceinline__ void run_product_narrow(float (&acc)[2], const uint8_
         for (int i = 0; i < 2; ++i) {
             if constexpr (kMx) {
                 const uint32_t v = *reinterpret_cast<const uint16_t *>(ss + i * 128 + blk);
-                s[i][0] = __uint_as_float((v & 0xffu) << 23);
-                s[i][1] = __uint_as_float((v >> 8) << 23);
-                s[i][0] = fmaf(s[i][0], 0.0f, s[i][0]); // 255: infinity times 0 plus itself is NaN; 0 stands for 0, not 2^-127
-                s[i][1] = fmaf(s[i][1], 0.0f, s[i][1]);
+                const float2 two = e8m0x2_to_f32(v);
+                s[i][0] = two.x;
+                s[i][1] = two.y;
             } else {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -322,28 +382,14 @@ __device__ __forceinline__ void run_product_narrow(float (&acc)[2], const uint8_
     }
 }
 
-// row of zeros (with its sums and factor) of one run
-__device__ __forceinline__ void clear_last_row(uint8_t *at, int x_rows, int thread, int threads)
+// row of zeros (with its sums and factor) of one run, by one warp
+__device__ __forceinline__ void clear_last_row(uint8_t *at, int x_rows, int lane)
 {
-    for (int i = thread; i < kXPitch / 16 + 9; i += threads) {
+    for (int i = lane; i < kXPitch / 16 + 9; i += 32) {
         if (i < kXPitch / 16) {
             *reinterpret_cast<uint4 *>(at + (x_rows - 1) * kXPitch + i * 16) = make_uint4(0, 0, 0, 0);
         } else {
             reinterpret_cast<float *>(at + x_rows * kXPitch)[(x_rows - 1) * 9 + i - kXPitch / 16] = 0.0f;
-        }
-    }
-}
-
-// the scales (or zeros) of one row in one step, to a 16-byte slot
-__device__ __forceinline__ void load_scales(uint32_t dst, const uint8_t *row, int64_t first, int64_t row_bytes, int bytes, bool live, bool async)
-{
-    if (async) { // k a multiple of 256: a step's scales are whole and aligned
-        live = live && first < row_bytes;
-        cp_async(dst, live ? row + first : row, bytes, live);
-    } else { // any k: byte by byte
-        for (int i = 0; i < bytes; ++i) {
-            const uint32_t v = live && first + i < row_bytes ? row[first + i] : 0u;
-            asm volatile("st.shared.u8 [%0], %1;" ::"r"(dst + i), "r"(v) : "memory");
         }
     }
 }
@@ -459,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 3) w4_narrow_kernel(const __grid_con
         if (k0 < a.k) {
             v = __ldg(reinterpret_cast<const uint4 *>(a.x + row * a.x_stride + k0));
         }
-        prepare_run<kBf16, kMx>(v, xs + run * x_run, a.m, row, lane);
+        prepare_run<kBf16, kMx, 1>(v, xs + run * x_run, a.m, row, lane);
     }
     if (threadIdx.x < 32) {
         reinterpret_cast<uint4 *>(nothing)[threadIdx.x] = make_uint4(0, 0, 0, 0);
@@ -521,7 +567,7 @@ __host__ __device__ inline int streamed_x_run(int m)
 }
 
 // one warp prepares one row of one run, in the layout of the streamed kernel's shared memory
-template <bool kBf16, bool kMx>
+template <bool kBf16, bool kMx, int kG>
 __global__ void __launch_bounds__(kThreads) w4_prepare_kernel(const __grid_constant__ W4Args a, uint8_t *xp)
 {
     programmatic_trigger();
@@ -533,7 +579,7 @@ __global__ void __launch_bounds__(kThreads) w4_prepare_kernel(const __grid_const
     }
     uint8_t *at = xp + static_cast<int64_t>(run) * a.x_run;
     if (row >= a.m) {
-        clear_last_row(at, x_rows, lane, 32);
+        clear_last_row(at, x_rows, lane);
         return;
     }
     const int64_t k0 = static_cast<int64_t>(run) * kStepK + lane * 8;
@@ -541,101 +587,163 @@ __global__ void __launch_bounds__(kThreads) w4_prepare_kernel(const __grid_const
     if (k0 < a.k) {
         v = __ldg(reinterpret_cast<const uint4 *>(a.x + row * a.x_stride + k0));
     }
-    prepare_run<kBf16, kMx>(v, at, x_rows, row, lane);
+    prepare_run<kBf16, kMx, kG>(v, at, x_rows, row, lane);
 }
 
-// shared memory of a stage: W [kWk][16 kWr rows][kPitch], scales and zeros [kWk][16 kWr rows][16], kWk runs of x; the shares
-// of k are joined in the ring's place
-template <bool kMx, int kWr, int kMt>
+constexpr int kMostStages = 4;
+constexpr int kScaleSlots = 4;
+
+// shared memory: `stages` times kWk boxes of up to 16 kWr rows x 256 k of W, then `stages` times kWk runs of x,
+// then kScaleSlots steps of scales and zeros a warp, then the shares of k on their way to be joined
+template <int kWr, int kMt>
 struct Layout {
     static constexpr int kWk = kWarps / kWr;
     static constexpr int kRows = 16 * kWr;
-    static constexpr int kW = kWk * kRows * kPitch;
-    static constexpr int kScale = kWk * kRows * 16;
-    static constexpr int kX = kW + (kMx ? 1 : 2) * kScale;
     static constexpr int kSums = kWk * 8 * kMt * kRows * 4;
-    static __host__ __device__ int stage_bytes(int m) { return kX + kWk * streamed_x_run(m); }
-    static int smem_bytes(int m)
+    static __host__ __device__ int x_bytes(int m) { return kWk * streamed_x_run(m); }
+    template <bool kMx, int kG>
+    static __host__ __device__ constexpr int scale_bytes() // of a warp and step
     {
-        const int ring = kStages * stage_bytes(m);
-        return ring > kSums ? ring : kSums;
+        return (kMx ? 16 : 32) * StepScales<kMx, kG>::kBytes;
+    }
+    template <bool kMx, int kG>
+    static int smem_bytes(int m, int stages)
+    {
+        return stages * (kWarps * kBoxBytes + x_bytes(m)) + kWarps * kScaleSlots * scale_bytes<kMx, kG>() + kSums + 1024;
     }
 };
 
-// kG: runs of 32 k in a group of the scales
-template <bool kBf16, bool kMx, int kG, int kWr, int kMt>
-__global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel(const __grid_constant__ W4Args a)
+
+struct StreamedCtl {
+    uint64_t full[kMostStages];
+    uint32_t done[kMostStages]; // warps that have read the stage
+    int abort;
+};
+
+// untiled copy global -> shared, completion on an mbarrier; 16-byte aligned addresses and size
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar)
 {
-    using L = Layout<kMx, kWr, kMt>;
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// kG: runs of 32 k in a group of the scales.
+// The warp that is the last to have read a stage loads it again: nobody waits for a stage to become free.
+template <bool kBf16, bool kMx, int kG, int kWr, int kMt>
+__global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1)
+    w4_streamed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Args a, DeviceStatus *status)
+{
+    using L = Layout<kWr, kMt>;
+    using Scales = StepScales<kMx, kG>;
     constexpr int kWk = L::kWk;
-    constexpr bool kRaw = !kBf16 && kMx; // x as it is
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ StreamedCtl ctl;
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int wr = warp % kWr, wk = warp / kWr;
     const int block = static_cast<int>(blockIdx.x);
     const int row_begin = block * a.rows_each + min(block, a.rows_more), row_end = row_begin + a.rows_each + (block < a.rows_more ? 1 : 0);
-    const int64_t row_bytes = a.k / 2;
-    const int64_t row_scale = static_cast<int64_t>(a.k / (32 * kG)) * (kMx ? 1 : 2);
-    constexpr int kScaleBytes = kMx ? 8 : 16 / kG; // of a row in a step
-    const int iters = (a.k + kStepK * kWk - 1) / (kStepK * kWk);
-    const int x_rows = streamed_x_rows(a.m), x_run = streamed_x_run(a.m), stage_bytes = L::stage_bytes(a.m);
+    const int runs = (a.k + kStepK - 1) / kStepK, iters = (runs + kWk - 1) / kWk;
+    const int steps = (row_end - row_begin + a.tile_rows - 1) / a.tile_rows * iters;
+    const int stages = a.stages;
+    const int x_run = a.x_run, x_rows = streamed_x_rows(a.m);
+    uint8_t *x_ring = smem + stages * kWarps * kBoxBytes;
+    uint8_t *scale_slots = x_ring + stages * L::x_bytes(a.m);
+    float *sums = reinterpret_cast<float *>(scale_slots + kWarps * kScaleSlots * L::template scale_bytes<kMx, kG>());
     const LaneX<kMt> lx(x_rows, g, t);
-    if (kRaw && x_rows > a.m) { // the row of zeros stays where it is
-        for (int i = warp; i < kStages * kWk; i += kWarps) {
-            clear_last_row(smem + i / kWk * stage_bytes + L::kX + i % kWk * x_run, x_rows, lane, 32);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&ctl.full[s], 1);
+            ctl.done[s] = 0;
+        }
+        ctl.abort = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+
+    // a warp announces a step, and loads W: a box of the block's rows for each of its runs of 256
+    auto load_w = [&](int slot, int n0, int it) {
+        const int have = min(kWk, runs - it * kWk);
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&ctl.full[slot], static_cast<uint32_t>(have) * (a.tile_rows * kStepBytes + x_run));
+        }
+        __syncwarp();
+        if (lane < have) {
+            tma_load_2d(smem + slot * kWarps * kBoxBytes + lane * L::kRows * kStepBytes, &tmap_w, &ctl.full[slot], (it * kWk + lane) * kStepBytes, n0);
+        }
+    };
+    auto load_x = [&](int slot, int it) { // runs lie one after another
+        if (lane == 0) {
+            bulk_load(smem_u32(x_ring) + slot * kWk * x_run, a.xp + static_cast<int64_t>(it) * kWk * x_run,
+                      static_cast<uint32_t>(min(kWk, runs - it * kWk) * x_run), &ctl.full[slot]);
+        }
+    };
+    // W does not depend on the preparation of x; x, prepared by the kernel before, is waited for
+    int ahead_n0 = row_begin, ahead_it = 0; // of the step that is `stages` ahead
+    if (warp == 0) {
+        int n0 = row_begin, it = 0;
+        for (int s = 0; s < stages && s < steps; ++s) {
+            load_w(s, n0, it);
+            it = it + 1 == iters ? 0 : it + 1;
+            n0 += it == 0 ? a.tile_rows : 0;
         }
     }
-    bool waited = false;
-
-    for (int n0 = row_begin; n0 < row_end; n0 += L::kRows) {
-        // ---- this thread's pieces of a stage: 16-byte chunk threadIdx % 8 of rows row0 + 32 i of the (step, row) list
-        constexpr int kPieces = L::kRows * kWk * 8 / kThreads; // 4
-        const uint8_t *src[kPieces];
-        uint32_t live = 0;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int r = i * (kThreads / 8) + (threadIdx.x >> 3), row = r % L::kRows, step = r / L::kRows;
-            src[i] = a.w + (n0 + row < row_end ? (n0 + row) * row_bytes : 0) + step * kStepBytes + (threadIdx.x & 7) * 16;
-            live |= n0 + row < row_end ? 1u << i : 0u;
+    // The warp's own scales, 16 rows a step, and zeros run kScaleSlots - 1 steps ahead: lane 0 .. 15 a row's scales, 16 .. 31
+    // its zeros, at `scale_src` for the step that comes next
+    const bool zero = !kMx && a.zero != nullptr;
+    const int64_t row_scale = static_cast<int64_t>(a.k / (32 * kG)) * (kMx ? 1 : 2);
+    uint8_t *slots = scale_slots + warp * kScaleSlots * L::template scale_bytes<kMx, kG>();
+    const uint32_t scale_dst = smem_u32(slots) + lane * Scales::kBytes;
+    int scale_n0 = row_begin + 16 * wr + (lane & 15), scale_run = wk, scale_slot = 0;
+    const uint8_t *scale_src = nullptr;
+    auto scale_row = [&] { // rows past the end: any row, its result is not stored
+        scale_src = (lane < 16 ? a.scale : a.zero) + min(scale_n0, a.n - 1) * row_scale + wk * Scales::kBytes;
+    };
+    scale_row();
+    auto load_scales = [&] {
+        if ((lane < 16 || zero) && scale_run < runs) {
+            const uint32_t dst = scale_dst + scale_slot * L::template scale_bytes<kMx, kG>();
+            if (a.scale_async) {
+                cp_async(dst, scale_src, Scales::kBytes, true);
+            } else {
+                Scales::gather(dst, scale_src, row_scale - static_cast<int64_t>(scale_run) * Scales::kBytes);
+            }
         }
-        const int sr = threadIdx.x & 127, s_row = sr % L::kRows, s_step = sr / L::kRows; // 128 runs of scales, then of zeros
-        const bool zeros = threadIdx.x >= 128, has_scale = !zeros || (!kMx && a.zero != nullptr), s_live = n0 + s_row < row_end;
-        const uint8_t *scale_src = (zeros ? a.zero : a.scale) + (s_live ? (n0 + s_row) * row_scale : 0);
-        auto load_w = [&](int it) {
-            const uint32_t base = smem_u32(smem) + (it % kStages) * stage_bytes;
-            const bool whole = (it + 1) * kStepK * kWk <= a.k;
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int r = i * (kThreads / 8) + (threadIdx.x >> 3), step = r / L::kRows;
-                const int64_t off = static_cast<int64_t>(it) * kWk * kStepBytes;
-                // k is a multiple of 32: chunks are whole
-                const bool ok = (live >> i & 1u) && (whole || off + step * kStepBytes + (threadIdx.x & 7) * 16 < row_bytes);
-                cp_async(base + r * kPitch + (threadIdx.x & 7) * 16, ok ? src[i] + off : a.w, 16, ok);
-            }
-            if (has_scale) {
-                load_scales(base + L::kW + (zeros ? L::kScale : 0) + sr * 16, scale_src, (static_cast<int64_t>(it) * kWk + s_step) * kScaleBytes,
-                            row_scale, kScaleBytes, s_live, a.scale_async);
-            }
-        };
-        auto load_x = [&](int it) {
-            const uint32_t base = smem_u32(smem) + (it % kStages) * stage_bytes + L::kX;
-            if constexpr (kRaw) {
-                for (int i = threadIdx.x; i < kWk * a.m * 32; i += kThreads) { // 32 chunks of a row's run
-                    const int c = i & 31, unit = i >> 5, step = unit % kWk, row = unit / kWk;
-                    const int64_t k0 = (static_cast<int64_t>(it) * kWk + step) * kStepK + c * 8;
-                    cp_async(base + step * x_run + row * kXPitch + c * 16, a.x + (k0 < a.k ? row * a.x_stride + k0 : 0), 16, k0 < a.k);
-                }
-            } else { // kWk prepared runs, one after another
-                const int chunks = kWk * x_run / 16, have = ((a.k + kStepK - 1) / kStepK - it * kWk) * (x_run / 16);
-                const uint8_t *from = a.xp + static_cast<int64_t>(it) * kWk * x_run;
-                for (int i = threadIdx.x; i < chunks && i < have; i += kThreads) {
-                    cp_async(base + i * 16, from + i * 16, 16, true);
-                }
-            }
-        };
-        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        scale_slot = (scale_slot + 1) & (kScaleSlots - 1);
+        scale_run += kWk;
+        scale_src += kWk * Scales::kBytes;
+        if (scale_run >= iters * kWk) {
+            scale_run = wk;
+            scale_n0 += a.tile_rows;
+            scale_row();
+        }
+    };
+    for (int i = 0; i < kScaleSlots - 1; ++i) {
+        load_scales();
+    }
+    programmatic_wait();
+    if (warp == 0) {
+        int it = 0;
+        for (int s = 0; s < stages && s < steps; ++s) {
+            load_x(s, it);
+            it = it + 1 == iters ? 0 : it + 1;
+        }
+    }
+    for (int s = 0; s < stages; ++s) {
+        ahead_it = ahead_it + 1 == iters ? 0 : ahead_it + 1;
+        ahead_n0 += ahead_it == 0 ? a.tile_rows : 0;
+    }
 
+    int slot = 0, read_slot = 0, left = steps;
+    uint32_t parity = 0;
+    bool ok = true;
+    const uint32_t lane_w = smem_u32(smem) + warp * kBoxBytes + g * (kStepBytes + 16) + 4 * t; // row g, chunk 0 ^ g
+    for (int n0 = row_begin; n0 < row_end; n0 += a.tile_rows) {
+        const int rows = min(a.tile_rows, row_end - n0);
         float acc[kMt][4];
 #pragma unroll
         for (int c = 0; c < kMt; ++c) {
@@ -644,43 +752,39 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel
                 acc[c][i] = 0.0f;
             }
         }
-#pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) { // W does not depend on the preparation of x
-            if (s < iters) {
-                load_w(s);
-            }
-        }
-        if (!kRaw && !waited) {
-            programmatic_wait();
-            waited = true;
-        }
-#pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) {
-            if (s < iters) {
-                load_x(s);
-            }
-            commit();
-        }
         for (int it = 0; it < iters; ++it) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            __syncthreads(); // stage `it` is there, and everybody is done with the stage that the next loads overwrite
-            if (it + kStages - 1 < iters) {
-                load_w(it + kStages - 1);
-                load_x(it + kStages - 1);
+            load_scales();
+            asm volatile("cp.async.wait_group %0;" ::"n"(kScaleSlots - 1) : "memory");
+            if (ok) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.full[slot], parity, &ctl.abort));
             }
-            commit();
-            const uint8_t *base = smem + (it % kStages) * stage_bytes;
-            const int row = wk * L::kRows + wr * 16 + g;
-            const int left = (a.k - (it * kWk + wk) * kStepK) / 32;
-            if (left > 0 && n0 + wr * 16 < row_end) {
-                run_product<kBf16, kMx, kG, kMt>(acc, reinterpret_cast<const uint32_t *>(base + row * kPitch) + t, base + L::kW + row * 16,
-                                                 base + L::kW + L::kScale + row * 16, base + L::kX + wk * x_run, lx, a.zero != nullptr, left);
+            __syncwarp(); // the scales of all lanes
+            if (ok) {
+                if (it * kWk + wk < runs && wr * 16 < rows) {
+                    run_product<kBf16, kMx, kG, kMt>(acc, lane_w + slot * kWarps * kBoxBytes,
+                                                     slots + read_slot * L::template scale_bytes<kMx, kG>() + g * Scales::kBytes, x_ring + (slot * kWk + wk) * x_run, lx, zero);
+                }
+                __syncwarp();
+                uint32_t before = 0;
+                if (lane == 0 && left > stages) {
+                    asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;" : "=r"(before) : "r"(smem_u32(&ctl.done[slot])) : "memory");
+                    if (before == kWarps - 1) {
+                        ctl.done[slot] = 0;
+                    }
+                }
+                if (__shfl_sync(0xffffffffu, before, 0) == kWarps - 1) { // everybody has read the stage
+                    load_w(slot, ahead_n0, ahead_it);
+                    load_x(slot, ahead_it);
+                }
             }
+            read_slot = (read_slot + 1) & (kScaleSlots - 1);
+            --left;
+            ahead_it = ahead_it + 1 == iters ? 0 : ahead_it + 1;
+            ahead_n0 += ahead_it == 0 ? a.tile_rows : 0;
+            slot = slot + 1 == stages ? 0 : slot + 1;
+            parity ^= slot == 0 ? 1u : 0u;
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();
         // the shares of k joined in a fixed order: [share][column of x][row of W]
-        float *sums = reinterpret_cast<float *>(smem);
         constexpr int kM = 8 * kMt;
 #pragma unroll
         for (int c = 0; c < kMt; ++c) {
@@ -692,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel
         __syncthreads();
         for (int i = threadIdx.x; i < a.m * L::kRows; i += kThreads) {
             const int col = i / L::kRows, row = i % L::kRows;
-            if (n0 + row < row_end) {
+            if (row < rows) {
                 float v = 0.0f;
 #pragma unroll
                 for (int w = 0; w < kWk; ++w) {
@@ -701,12 +805,19 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1) w4_streamed_kernel
                 store_y<kBf16>(a, static_cast<int64_t>(col) * a.n + n0 + row, v);
             }
         }
-        __syncthreads(); // the sums are read before the ring is loaded again
-        if (kRaw && x_rows > a.m && n0 + L::kRows < row_end) { // the sums lay over the rows of zeros
-            for (int i = warp; i < kStages * kWk; i += kWarps) {
-                clear_last_row(smem + i / kWk * stage_bytes + L::kX + i % kWk * x_run, x_rows, lane, 32);
-            }
+        if (n0 + a.tile_rows < row_end) {
+            __syncthreads(); // the sums are read before they are written again
         }
+    }
+    if (__syncthreads_or(!ok)) { // a copy that never came
+        for (int i = 0; i < 1024; ++i) {
+            __nanosleep(1000); // copies in flight end before the shared memory is given back
+        }
+        if (threadIdx.x == 0 && atomicCAS(&status->code, 0, kErrDeviceWaitTimeout) == 0) {
+            status->block = block;
+            status->where = 6;
+        }
+        __syncthreads();
     }
 }
 
@@ -731,22 +842,37 @@ int launch_narrow(W4Args a, cudaStream_t stream)
 template <bool kBf16, bool kMx, int kG, int kWr, int kMt>
 int launch_streamed(W4Args a, int blocks, uint8_t *workspace, cudaStream_t stream)
 {
-    using L = Layout<kMx, kWr, kMt>;
-    const void *kernel = reinterpret_cast<const void *>(&w4_streamed_kernel<kBf16, kMx, kG, kWr, kMt>);
-    int rc = ensure_dynamic_smem(kernel, L::smem_bytes(8 * kMt));
-    constexpr bool kRaw = !kBf16 && kMx;
-    if (!kRaw && rc == kOk) {
+    using L = Layout<kWr, kMt>;
+    auto kernel = &w4_streamed_kernel<kBf16, kMx, kG, kWr, kMt>;
+    int stages = kMostStages; // what two blocks an SM leave room for, or one
+    const int room = L::template smem_bytes<kMx, kG>(a.m, 2) <= kStreamedSmem ? kStreamedSmem : kStreamedMost;
+    while (stages > 2 && L::template smem_bytes<kMx, kG>(a.m, stages) > room) {
+        --stages;
+    }
+    a.stages = stages;
+    a.rows_each = a.n / blocks;
+    a.rows_more = a.n % blocks;
+    const int rows = a.rows_each + (a.rows_more > 0 ? 1 : 0), tiles = (rows + L::kRows - 1) / L::kRows;
+    a.tile_rows = (rows + tiles - 1) / tiles;
+    CUtensorMap tmap_w;
+    DeviceStatus *status = device_status_ptr();
+    if (status == nullptr) {
+        return kErrCuda;
+    }
+    int rc = make_tmap_2d(&tmap_w, a.w, 1, static_cast<uint64_t>(a.n), static_cast<uint64_t>(a.k) / 2, static_cast<uint64_t>(a.k) / 2, static_cast<uint32_t>(a.tile_rows), kStepBytes, true);
+    if (rc == kOk) {
+        rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kStreamedMost);
+    }
+    if (rc == kOk) {
         a.xp = workspace;
         const int units = (a.k + kStepK - 1) / kStepK * streamed_x_rows(a.m);
-        w4_prepare_kernel<kBf16, kMx><<<(units + kWarps - 1) / kWarps, kThreads, 0, stream>>>(a, workspace);
+        w4_prepare_kernel<kBf16, kMx, kG><<<(units + kWarps - 1) / kWarps, kThreads, 0, stream>>>(a, workspace);
         rc = check_launch();
     }
     if (rc != kOk) {
         return rc;
     }
-    a.rows_each = a.n / blocks;
-    a.rows_more = a.n % blocks;
-    return launch_overlapped(&w4_streamed_kernel<kBf16, kMx, kG, kWr, kMt>, static_cast<unsigned>(blocks), kThreads, L::smem_bytes(a.m), stream, !kRaw, a);
+    return launch_overlapped(kernel, static_cast<unsigned>(blocks), kThreads, L::template smem_bytes<kMx, kG>(a.m, stages), stream, true, tmap_w, a, status);
 }
 
 template <bool kBf16, bool kMx, int kG>
@@ -754,7 +880,7 @@ int launch_rows(W4Args a, uint8_t *workspace, cudaStream_t stream)
 {
     // two blocks an SM, or one where that leaves a block fewer than 32 rows: every block reads all of x
     const int tiles = (a.n + 15) / 16;
-    const int blocks = a.n >= 64 * kSms && a.m <= 32 ? 2 * kSms : (tiles < kSms ? tiles : kSms);
+    const int blocks = a.n > 64 * kSms && a.m <= 32 ? 2 * kSms : (tiles < kSms ? tiles : kSms);
     const int rows = (a.n + blocks - 1) / blocks;
     a.x_run = streamed_x_run(a.m);
     if (a.m <= 8) {
