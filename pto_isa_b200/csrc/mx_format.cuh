@@ -84,18 +84,30 @@ __device__ __forceinline__ uint32_t mul_16x2(uint32_t a, uint32_t b)
     return d;
 }
 
-// two e4m3 / e2m1 codes -> two halves, the low code in the low half (exact)
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes)
+// four e4m3 codes -> two float16 pairs, eight e2m1 codes -> four, the lower code in the low half (exact); the conversions
+// take a byte or half of the register where it is
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t &p0, uint32_t &p1)
 {
-    uint32_t d;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(static_cast<uint16_t>(two_bytes)));
-    return d;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(p0), "=r"(p1)
+        : "r"(w));
 }
 
-__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte)
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&p)[4])
 {
-    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1);
-    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
+        : "r"(w));
+}
+
+// two scale bytes (the low 16 bits) as fp32, 255: NaN
+__device__ __forceinline__ float2 e8m0x2_to_f32(uint32_t v)
+{
+    uint32_t d;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, a;\n\t}" : "=r"(d) : "r"(v));
+    return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xffff0000u));
 }
 
 // value of a scale byte as fp32; byte 0 (2^-127) is subnormal, 255 is NaN

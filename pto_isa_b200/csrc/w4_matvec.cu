@@ -72,16 +72,6 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int size
     }
 }
 
-// eight e2m1 codes -> four float16 pairs (codes 2i, 2i + 1)
-__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&p)[4])
-{
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-        : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
-        : "r"(w));
-}
-
 // eight int4 codes as float16 subnormals: codes (0, 4) and (2, 6) times 2^-24, codes (1, 5) and (3, 7) times 2^-20
 __device__ __forceinline__ void int4x8_to_f16(uint32_t w, uint32_t (&p)[4])
 {
@@ -147,14 +137,6 @@ __device__ __forceinline__ void prepare_run(uint4 in, uint8_t *at, int x_rows, i
         v[3] = __byte_perm(y1, y3, 0x7632);
     }
     *reinterpret_cast<uint4 *>(at + row * kXPitch + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
-}
-
-// two e8m0 scale bytes as floats (255: NaN)
-__device__ __forceinline__ float2 e8m0x2_to_f32(uint32_t v)
-{
-    uint32_t d;
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, a;\n\t}" : "=r"(d) : "r"(v));
-    return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xffff0000u));
 }
 
 // The scales or zeros of one row of W in one step
