@@ -610,32 +610,37 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     programmatic_wait(); // this grid is not complete before the wide kernel's, which the joining kernel reads as well
 }
 
-// Joins a row's pieces in a fixed order: four warps a row, each every fourth piece, then their four sums.  The pieces'
-// statistics are read first, side by side; the loads of the sums depend on nothing and overlap.  (Joined by the last block of
-// a sequence's own pieces instead, one kernel fewer but fewer warps too, 24 sequences of 4 x 16 rows took 42 us for 33.)
-template <bool kBf16, int kD>
+// Joins a row's pieces in a fixed order: kShare warps a row, each every kShare-th piece, then their sums.  The pieces'
+// statistics are read first, side by side; the loads of the sums depend on nothing and overlap.  Bound by latency and, with
+// many rows, by what finding the pieces takes: four warps a row where a row has many pieces, one where it has few.  (Joined
+// by the last block of a sequence's own pieces instead, one kernel fewer but fewer warps too, 24 sequences of 4 x 16 rows
+// took 42 us for 33.)
+template <bool kBf16, int kD, int kShare>
 __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid_constant__ AttnArgs a)
 {
     constexpr int kPer = kD / 32, kAhead = 8;
     __shared__ float sums[kWarps], accs[kWarps][kD];
-    const uint32_t idx = blockIdx.x; // output row: (batch, token, head)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = kShare == 1 ? 0 : warp;
+    const uint32_t idx = kShare == 1 ? blockIdx.x * kWarps + warp : blockIdx.x; // output row: (batch, token, head)
+    if (kShare == 1 && idx >= static_cast<uint32_t>(a.batch) * a.tokens * a.heads) {
+        programmatic_wait();
+        return;
+    }
     const uint32_t row = idx / static_cast<uint32_t>(a.heads);
-    const int head = static_cast<int>(idx - row * a.heads);
-    const int b = static_cast<int>(row / static_cast<uint32_t>(a.tokens)), tok = static_cast<int>(row) - b * a.tokens;
-    const int h = head / a.group, in = tok * a.group + head - h * a.group;
-    const int prow = b * a.tokens * a.group + in;
+    const uint32_t head = idx - row * a.heads;
+    const uint32_t b = a.tokens == 1 ? row : row / static_cast<uint32_t>(a.tokens), tok = row - b * a.tokens;
     const int len = own_len(a, b);
+    const uint32_t h = head / static_cast<uint32_t>(a.group), in = tok * a.group + head - h * a.group;
+    const uint32_t prow = b * a.tokens * a.group + in;
     const int own_pieces = len > 0 ? ceil_div(len, own_chunk(len, a.own_splits, a.own_min)) : 0;
-    const int64_t prefix_items = static_cast<int64_t>(a.prefix_pieces) * a.kv_heads * a.prefix_tiles;
     const int pieces = a.prefix_pieces + own_pieces;
-    auto row_of = [&](int i) -> int64_t { // where piece i keeps this row
-        if (i < a.prefix_pieces) {
-            return ((static_cast<int64_t>(i) * a.kv_heads + h) * a.prefix_tiles + prow / kRows) * kRows + prow % kRows;
-        }
-        const int64_t s = i - a.prefix_pieces;
-        return (prefix_items + ((s * a.batch + b) * a.kv_heads + h) * a.own_tiles + in / kRows) * kRows + in % kRows;
-    };
+    // where piece 0 of the prefix and (own piece 0) - prefix_pieces own pieces keep this row; rows between pieces
+    const int64_t prefix_step = static_cast<int64_t>(a.kv_heads) * a.prefix_tiles * kRows;
+    const int64_t own_step = static_cast<int64_t>(a.batch) * a.kv_heads * a.own_tiles * kRows;
+    const int64_t prefix_row = static_cast<int64_t>(h) * a.prefix_tiles * kRows + prow;
+    const int64_t own_row = a.prefix_pieces * (prefix_step - own_step) + (static_cast<int64_t>(b) * a.kv_heads + h) * a.own_tiles * kRows + in;
+    auto row_of = [&](int i) { return i < a.prefix_pieces ? prefix_row + i * prefix_step : own_row + i * own_step; };
     programmatic_wait();
     float top = -INFINITY;
     for (int i = lane; i < pieces; i += 32) {
@@ -652,8 +657,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
         acc[c] = 0.0f;
     }
     // eight of the warp's pieces at a time: statistics a piece a lane, the sums of all of them on their way at once
-    for (int first = warp; first < pieces; first += kWarps * kAhead) {
-        const int mine = first + (lane & (kAhead - 1)) * kWarps;
+    for (int first = part; first < pieces; first += kShare * kAhead) {
+        const int mine = first + (lane & (kAhead - 1)) * kShare;
         float w = 0.0f;
         bool used = false; // no key of the piece for this row: its sums may not even have been written
         if (mine < pieces) {
@@ -665,8 +670,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
         float x[kAhead][kPer];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (first + u * kWarps < pieces) {
-                const float *src = a.part_o + row_of(first + u * kWarps) * kD + lane * kPer;
+            if (first + u * kShare < pieces) {
+                const float *src = a.part_o + row_of(first + u * kShare) * kD + lane * kPer;
                 if constexpr (kPer == 4) {
                     const float4 v = *reinterpret_cast<const float4 *>(src);
                     x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
@@ -692,28 +697,37 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
     for (int s = kAhead / 2; s > 0; s >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, s);
     }
+    if constexpr (kShare > 1) {
 #pragma unroll
-    for (int c = 0; c < kPer; ++c) {
-        accs[warp][lane * kPer + c] = acc[c];
-    }
-    if (lane == 0) {
-        sums[warp] = sum;
-    }
-    __syncthreads();
-    if (threadIdx.x < kD / 2) { // two elements a thread
+        for (int c = 0; c < kPer; ++c) {
+            accs[warp][lane * kPer + c] = acc[c];
+        }
+        if (lane == 0) {
+            sums[warp] = sum;
+        }
+        __syncthreads();
+        if (warp != 0) {
+            return;
+        }
         sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        const bool none = top == -INFINITY && sum == 0.0f; // no key at all: zeros
-        const float inv = none ? 0.0f : 1.0f / sum;
-        float v[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int at = 2 * threadIdx.x + c;
-            v[c] = ((accs[0][at] + accs[1][at]) + (accs[2][at] + accs[3][at])) * inv;
+        for (int c = 0; c < kPer; ++c) {
+            const int at = lane * kPer + c;
+            acc[c] = (accs[0][at] + accs[1][at]) + (accs[2][at] + accs[3][at]);
         }
-        reinterpret_cast<uint32_t *>(a.o + static_cast<int64_t>(idx) * kD)[threadIdx.x] = pack_16x2<kBf16>(v[0], v[1]);
-        if (a.lse != nullptr && threadIdx.x == 0) {
-            a.lse[idx] = none ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
-        }
+    } else {
+        sum = __shfl_sync(0xffffffffu, sum, 0);
+    }
+    const bool none = top == -INFINITY && sum == 0.0f; // no key at all: zeros
+    const float inv = none ? 0.0f : 1.0f / sum;
+    uint32_t *dst = reinterpret_cast<uint32_t *>(a.o + static_cast<int64_t>(idx) * kD + lane * kPer);
+    if constexpr (kPer == 4) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_16x2<kBf16>(acc[0] * inv, acc[1] * inv), pack_16x2<kBf16>(acc[2] * inv, acc[3] * inv));
+    } else {
+        *dst = pack_16x2<kBf16>(acc[0] * inv, acc[1] * inv);
+    }
+    if (a.lse != nullptr && lane == 0) {
+        a.lse[idx] = none ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
     }
 }
 
@@ -726,6 +740,9 @@ struct Plan {
 };
 
 constexpr int kWideRows = 16;
+// up to so many pieces of more rows than run at once with four warps each: a warp a row (4096 rows of 9 pieces: 8.3 us for
+// 15.8; 8 rows of 9: 3.4 us with four warps, 4.0 with one)
+constexpr int kFewPieces = 16, kManyRows = 1024;
 
 Plan make_plan(int batch, int tokens, int heads, int kv_heads, int prefix_len, int own_max)
 {
@@ -816,7 +833,11 @@ int launch_typed(int fmt, const AttnArgs &a, int64_t own_slots, DeviceStatus *st
         }
     }
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
-    return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD>, static_cast<unsigned>(rows), kThreads, 0, stream, blocks > 0 || a.prefix_wide != 0, a);
+    const bool after = blocks > 0 || a.prefix_wide != 0;
+    if (a.prefix_pieces + a.own_splits <= kFewPieces && rows > kManyRows) {
+        return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD, 1>, static_cast<unsigned>((rows + kWarps - 1) / kWarps), kThreads, 0, stream, after, a);
+    }
+    return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD, kWarps>, static_cast<unsigned>(rows), kThreads, 0, stream, after, a);
 }
 
 } // namespace
