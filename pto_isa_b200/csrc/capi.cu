@@ -793,7 +793,7 @@ int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtyp
         return kErrUnsupportedShape;
     }
     return launch_prefix_attn(view, static_cast<const uint16_t *>(q), dtype == PTO_B200_DTYPE_BF16, q_strides, prefix_pages,
-                              prefix_len, page_table, table_stride, table_cols, seq_lens, max_seq_len, batch, tokens, heads,
+                              prefix_len, page_table, table_stride, seq_lens, max_seq_len, batch, tokens, heads,
                               scale, static_cast<uint16_t *>(o), lse, workspace, workspace_bytes, as_stream(stream));
 }
 

@@ -130,7 +130,7 @@ int launch_kv_read(const KvCacheView &cache, const int32_t *table, int64_t table
 int64_t prefix_attn_workspace_bytes(int batch, int tokens, int heads, int kv_heads, int d, int prefix_len, int own_max);
 int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, const int64_t q_strides[3],
                        const int32_t *prefix_pages, int prefix_len, const int32_t *table, int64_t table_stride,
-                       int table_cols, const int32_t *lens, int own_max, int batch, int tokens, int heads, float scale,
+                       const int32_t *lens, int own_max, int batch, int tokens, int heads, float scale,
                        uint16_t *o, float *lse, void *workspace, int64_t workspace_bytes, cudaStream_t stream);
 // y[m, n] = sum_k x[m, k] W[n, k] with 4-bit weights; arguments validated by the caller
 int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, const void *scale, const uint16_t *zero, void *y,

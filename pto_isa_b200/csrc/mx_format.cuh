@@ -110,13 +110,6 @@ __device__ __forceinline__ float2 e8m0x2_to_f32(uint32_t v)
     return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xffff0000u));
 }
 
-// value of a scale byte as fp32; byte 0 (2^-127) is subnormal, 255 is NaN
-__device__ __forceinline__ float e8m0_value(uint32_t byte)
-{
-    const uint32_t bits = byte == 0u ? 0x00400000u : (byte == 255u ? 0x7fc00000u : byte << 23);
-    return __uint_as_float(bits);
-}
-
 // Scale byte of a block with largest magnitude `amax` (finite): the smallest power of two with amax <= limit * 2^e,
 // limit = 448 = 1.75 * 2^8 (e4m3) or 6 = 1.5 * 2^2 (e2m1), so that no element saturates.  e stays in
 // [-127, 119] (e4m3) / [-127, 125] (e2m1): above that the largest code's value would leave bfloat16's range.

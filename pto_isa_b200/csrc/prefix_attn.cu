@@ -135,22 +135,6 @@ struct Stage {
     static constexpr int kSmem = kRing > kMergeBytes ? kRing : kMergeBytes;
 };
 
-// eight e2m1 codes / four e4m3 codes -> float16 pairs of neighbours
-__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&p)[4])
-{
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-        : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
-        : "r"(w));
-}
-__device__ __forceinline__ void e4m3x4(uint32_t w, uint32_t &lo, uint32_t &hi)
-{
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-}
-
 // scaled V operand: a pair of values of two keys times the keys' powers of two.  float16: exact where scale_ok() says so,
 // rounded to float16's range elsewhere, as float16 queries' results are.  kWide: bfloat16, exact but for scale byte 0 (0
 // instead of 2^-127); byte 255 is infinity there and as float16, and times a block's zeros the NaN that it stands for.
@@ -403,10 +387,10 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                 } else {
                     if constexpr (kFmt == kKvMxFp8) {
                         const uint2 v = lds64(base + swz_k<RB, kFmt>(8 * n + g, 32 * kb + 8 * t));
-                        e4m3x4(v.x, w[0], w[1]);
-                        e4m3x4(v.y, w[2], w[3]);
+                        e4m3x4_to_f16(v.x, w[0], w[1]);
+                        e4m3x4_to_f16(v.y, w[2], w[3]);
                     } else {
-                        e2m1x8(lds32(base + swz_k<RB, kFmt>(8 * n + g, 16 * kb + 4 * t)), w);
+                        e2m1x8_to_f16(lds32(base + swz_k<RB, kFmt>(8 * n + g, 16 * kb + 4 * t)), w);
                     }
                     float p[4];
                     mma_16816_first<false>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
@@ -507,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
 #pragma unroll
                         for (int c = 0; c < 2; ++c) { // bytes 2c and 2c + 1 of the word: {key 0, key 1} side by side
                             uint32_t lo[2], hi[2];
-                            e4m3x4(__byte_perm(x[0][w], x[1][w], c ? 0x7362 : 0x5140), lo[0], lo[1]);
-                            e4m3x4(__byte_perm(x[2][w], x[3][w], c ? 0x7362 : 0x5140), hi[0], hi[1]);
+                            e4m3x4_to_f16(__byte_perm(x[0][w], x[1][w], c ? 0x7362 : 0x5140), lo[0], lo[1]);
+                            e4m3x4_to_f16(__byte_perm(x[2][w], x[3][w], c ? 0x7362 : 0x5140), hi[0], hi[1]);
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 mma_16816<kWide>(o[4 * w + 2 * c + e], p0, p1, p2, p3, scaled<kWide>(lo[e], scale01), scaled<kWide>(hi[e], scale23));
@@ -517,10 +501,10 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     } else {
                         // even nibbles of both keys in one byte, then odd ones
                         uint32_t even_lo[4], odd_lo[4], even_hi[4], odd_hi[4];
-                        e2m1x8((x[0][w] & 0x0f0f0f0fu) | ((x[1][w] << 4) & 0xf0f0f0f0u), even_lo);
-                        e2m1x8(((x[0][w] >> 4) & 0x0f0f0f0fu) | (x[1][w] & 0xf0f0f0f0u), odd_lo);
-                        e2m1x8((x[2][w] & 0x0f0f0f0fu) | ((x[3][w] << 4) & 0xf0f0f0f0u), even_hi);
-                        e2m1x8(((x[2][w] >> 4) & 0x0f0f0f0fu) | (x[3][w] & 0xf0f0f0f0u), odd_hi);
+                        e2m1x8_to_f16((x[0][w] & 0x0f0f0f0fu) | ((x[1][w] << 4) & 0xf0f0f0f0u), even_lo);
+                        e2m1x8_to_f16(((x[0][w] >> 4) & 0x0f0f0f0fu) | (x[1][w] & 0xf0f0f0f0u), odd_lo);
+                        e2m1x8_to_f16((x[2][w] & 0x0f0f0f0fu) | ((x[3][w] << 4) & 0xf0f0f0f0u), even_hi);
+                        e2m1x8_to_f16(((x[2][w] >> 4) & 0x0f0f0f0fu) | (x[3][w] & 0xf0f0f0f0u), odd_hi);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             mma_16816<kWide>(o[8 * w + 2 * i], p0, p1, p2, p3, scaled<kWide>(even_lo[i], scale01), scaled<kWide>(even_hi[i], scale23));
@@ -849,7 +833,7 @@ int64_t prefix_attn_workspace_bytes(int batch, int tokens, int heads, int kv_hea
 
 int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, const int64_t q_strides[3],
                        const int32_t *prefix_pages, int prefix_len, const int32_t *table, int64_t table_stride,
-                       int table_cols, const int32_t *lens, int own_max, int batch, int tokens, int heads, float scale,
+                       const int32_t *lens, int own_max, int batch, int tokens, int heads, float scale,
                        uint16_t *o, float *lse, void *workspace, int64_t workspace_bytes, cudaStream_t stream)
 {
     const Plan p = make_plan(batch, tokens, heads, cache.kv_heads, prefix_len, own_max);
@@ -884,7 +868,6 @@ int launch_prefix_attn(const KvCacheView &cache, const uint16_t *q, bool bf16, c
     a.o = o;
     a.lse = lse;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.table_cols = table_cols;
     a.page_shift = cache.page_shift;
     a.batch = batch;
     a.tokens = tokens;

@@ -19,7 +19,7 @@ struct AttnArgs {
     uint16_t *o;
     float *lse;
     float scale_log2;
-    int table_cols, page_shift;
+    int page_shift;
     int batch, tokens, heads, kv_heads, group;
     int prefix_len, own_max;
     // prefix_splits pieces of prefix_chunk keys, each for prefix_tiles tiles of 16 rows; in the wide kernel a block makes

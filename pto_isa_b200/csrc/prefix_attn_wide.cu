@@ -32,18 +32,11 @@ namespace {
 
 constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-11 loading K, 12-15 loading V; 16, 17 issuing (one per group); 18, 19
 // describing the key tiles and fetching them towards L2
-// registers of a thread: 96 at launch (five warps a scheduler), then 2 * 112 + 2 * 96 + 64 (codes) or 2 * 112 + 2 * 88
-// + 80 (16-bit rows), times 128, which is all of these 640 * 96.  No role
-// may spill: shared memory leaves the first-level cache so little that every reload comes from L2 (with 40 registers the
-// issuing threads reloaded descriptors and took 700 cycles for a product).
-constexpr int kRegsLaunch = 96, kRegsSoftmax = 112;
-__host__ __device__ constexpr int regs_load(bool codes) { return codes ? 80 : 80; }
-__host__ __device__ constexpr int regs_issue(bool codes) { return codes ? 96 : 96; }
-constexpr bool regs_fit(bool codes)
-{
-    return (2 * kRegsSoftmax + 2 * regs_load(codes) + regs_issue(codes)) * 128 <= kThreads * kRegsLaunch;
-}
-static_assert(regs_fit(true) && regs_fit(false), "an increase would wait forever");
+// registers of a thread: 96 at launch (five warps a scheduler), then 2 * 112 + 2 * 80 + 96, times 128, which is all of these
+// 640 * 96.  No role may spill: shared memory leaves the first-level cache so little that every reload comes from L2 (with 40
+// registers the issuing threads reloaded descriptors and took 700 cycles for a product).
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 112, kRegsLoad = 80, kRegsIssue = 96;
+static_assert((2 * kRegsSoftmax + 2 * kRegsLoad + kRegsIssue) * 128 <= kThreads * kRegsLaunch, "an increase would wait forever");
 constexpr int kIssueWarp = 16;
 constexpr int kTile = 128;
 constexpr int kTmemCols = 512;
@@ -159,19 +152,11 @@ __device__ __forceinline__ void codes16_to_f16(const uint32_t *c, uint32_t (&h)[
     if constexpr (kFmt == kKvMxFp8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-                : "=r"(h[2 * i]), "=r"(h[2 * i + 1])
-                : "r"(c[i]));
+            e4m3x4_to_f16(c[i], h[2 * i], h[2 * i + 1]);
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-                "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-                "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-                : "=r"(h[4 * i]), "=r"(h[4 * i + 1]), "=r"(h[4 * i + 2]), "=r"(h[4 * i + 3])
-                : "r"(c[i]));
-        }
+        e2m1x8_to_f16(c[0], *reinterpret_cast<uint32_t(*)[4]>(h));
+        e2m1x8_to_f16(c[1], *reinterpret_cast<uint32_t(*)[4]>(h + 4));
     }
 }
 
@@ -252,8 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
     };
 
     if (warp >= kIssueWarp) {
-        constexpr int kRegs = regs_issue(kMx);
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // ------------------------------------------------------------ issuing warps, one per group
         const int t = warp - kIssueWarp;
         if (t < 2 && lane == 0) {
@@ -408,10 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             }
         }
     } else if (warp >= 8) {
-        constexpr int kRegs = regs_load(kMx);
-        if constexpr (kRegs < kRegsLaunch) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
-        }
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
         // ------------------------------------------------------------ loading warps
         // One warpgroup for K, one for V, the same code.  A thread's share of a tile: 16 elements p of each 64-column half in
         // the rows r0 + 32 i.  All loads of a tile are issued before any is used and the two groups take turns at waiting

@@ -52,7 +52,7 @@ struct W4Args {
     const uint8_t *zero;
     void *y;
     int64_t x_stride;
-    int m, n, k, group_shift, out_f32, out_bf16;
+    int m, n, k, group_shift, out_f32;
     int rows_each, rows_more; // rows of W a block owns; the first rows_more blocks one more
     const uint8_t *xp; // prepared x: runs of 256 k, x_run bytes each (streamed kernel)
     int x_run, stages, tile_rows; // tile_rows: rows of W that a block takes at once

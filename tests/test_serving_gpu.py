@@ -566,3 +566,130 @@ def test_cached_context_feeds_the_prefill_attention():
         assert ((single[:, None].double() - want).abs() <= bound).all()
         # flash_attn_fwd keeps P relative to a reference up to 2^8 above the maximum: its rounding is of the same size
         assert ((o[:, :, row].double() - single.double()).abs() <= 2 * bound[:, 0]).all()
+
+
+# --------------------------------------------------------------------------------------------------- blocks, paths, streams
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kind,group", [("mxfp4", 32), ("zero", 64)])
+def test_w4_of_any_size(kind, group, dtype):
+    """Rows of W of every share a block can get (one to eight tiles of 16, several rounds of 128, one block an SM or two), rows of
+    x on both sides of every column tile, k that ends inside a step."""
+    for n, k in ((1600, 192), (148 * 16 + 5, 1344), (148 * 40, 576), (9473, 256), (148 * 2 * 60 + 1, 320), (148 * 2 * 130 + 7, 192)):
+        made = make_w4(kind, dtype, n, k, group, n % 97)
+        for m in (2, 3, 8, 9, 16, 24, 40, 64) if n < 9000 else (1, 5, 16, 33):
+            x = torch.randn(m, k, generator=gen(m), device="cuda").to(dtype)
+            check_w4(x, *made, group)
+    assert status()[0] == 0
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 20])
+@pytest.mark.parametrize("k", [512, 288])
+def test_w4_scales_that_begin_anywhere(m, k):
+    for kind, group in (("mxfp4", 32), ("zero", 32)):
+        dtype = F16
+        w, scale, zero = make_w4(kind, dtype, 50, k, group, 9)
+        shifted = []
+        for t in (scale, zero):
+            if t is not None:
+                room = torch.full((t.numel() + 1,), 77, dtype=t.dtype, device="cuda")
+                room[1:] = t.flatten()
+                shifted.append(room[1:].view(t.shape))
+        x = torch.randn(m, k, generator=gen(m), device="cuda").to(dtype)
+        y = check_w4(x, w, *shifted, *([None] if zero is None else []), group)
+        assert torch.equal(y, check_w4(x, w, scale, zero, group))
+
+
+@pytest.mark.parametrize("kind,group", [("mxfp4", 32), ("int4", 64)])
+@pytest.mark.parametrize("m", [2, 5])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_w4_nan_and_infinities_stay_in_their_rows(kind, group, m, dtype):
+    import pto_isa_b200 as p
+    n, k = 40, 512
+    w, scale, zero = make_w4(kind, dtype, n, k, group, 12)
+    x = torch.randn(m, k, generator=gen(2), device="cuda").to(dtype)
+    clean = check_w4(x, w, scale, zero, group)
+    bad = x.clone()
+    bad[1, 300] = float("nan")
+    y = p.w4_matvec(bad, w, scale, zero=zero)
+    assert y[1].isnan().all() and torch.equal(y[0], clean[0]) and torch.equal(y[2:], clean[2:])
+    scale = scale.clone()
+    scale[7, 1] = 255 if kind == "mxfp4" else float("nan")
+    y = p.w4_matvec(x, w, scale, zero=zero)
+    keep = torch.arange(n, device="cuda") != 7
+    assert y[:, 7].isnan().all() and torch.equal(y[:, keep], clean[:, keep])
+
+
+def test_both_ways_into_the_library_agree(monkeypatch):
+    """Calls in order go through the extension module, others through the checks in Python: the same results bit for bit."""
+    import pto_isa_b200 as p
+    from pto_isa_b200 import ops
+    assert ops._fast is not None
+
+    def run():
+        made = make_attention("mxfp8", BF16, 64, 2, 16, 70, [20, 0, 33], 5)
+        q = torch.randn(3, 2, 4, 64, generator=gen(1), device="cuda").to(BF16)
+        o, lse = p.prefix_attn(q, made[0], made[1], 70, made[2], made[3], return_lse=True)
+        k, v = p.kv_cache_read(made[0], made[2], made[3], 40)
+        w, scale, zero = make_w4("zero", BF16, 70, 512, 64, 3)
+        x = torch.randn(5, 512, generator=gen(3), device="cuda").to(BF16)
+        return [made[0].k[made[2].long()], o, lse, k, v, p.w4_matvec(x, w, scale, zero=zero), p.w4_matvec(x[0], w, scale, out_dtype=torch.float32)]
+    direct = run()
+    monkeypatch.setattr(ops, "_fast", None)
+    for a, b in zip(direct, run()):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_calls_at_the_same_time_do_not_share_anything():
+    import pto_isa_b200 as p
+    made = make_attention("mxfp8", F16, 128, 2, 64, 900, [70] * 20, 8)
+    q = [torch.randn(20, 1, 8, 128, generator=gen(s), device="cuda").to(F16) for s in (1, 2)]
+    w = make_w4("int4", F16, 700, 1024, 128, 4)
+    x = [torch.randn(6, 1024, generator=gen(s), device="cuda").to(F16) for s in (3, 4)]
+    call = lambda i: (p.prefix_attn(q[i], made[0], made[1], 900, made[2], made[3]), p.w4_matvec(x[i], w[0], w[1]))
+    alone = [call(0), call(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for o, y in got[i]:
+            assert torch.equal(o, alone[i][0]) and torch.equal(y, alone[i][1])
+    # two captured calls replayed side by side
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for i in (0, 1):
+        with torch.cuda.graph(graphs[i]):
+            outs.append(call(i))
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert torch.equal(outs[i][0], alone[i][0]) and torch.equal(outs[i][1], alone[i][1])
+    assert status()[0] == 0
+
+
+@pytest.mark.parametrize("batch", [1, 6])
+def test_attention_without_keys_of_their_own(batch):
+    """A table without columns: every sequence attends to the prefix alone, few rows and many."""
+    c, pages, _, lens, parts, own = make_attention("mxfp8", F16, 128, 1, 16, 300, [0] * batch, 6)
+    table = torch.zeros(batch, 0, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, 1, 8, 128, generator=gen(1), device="cuda").to(F16)
+    check_attention(q, c, pages, 300, table, lens, parts, own)
+
+
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_joins_many_and_few_pieces(name, d):
+    """One row over a long cache of its own (the most pieces), and more than a thousand rows of few pieces (a warp each)."""
+    long = make_attention(name, F16, d, 1, 16, 0, [9000, 3], 3)
+    check_attention(torch.randn(2, 1, 1, d, generator=gen(1), device="cuda").to(F16), long[0], long[1], 0, *long[2:])
+    rows = make_attention(name, F16, d, 8, 16, 130, [5, 0, 40] * 14 + [1], 4)
+    check_attention(torch.randn(43, 1, 32, d, generator=gen(2), device="cuda").to(F16), rows[0], rows[1], 130, *rows[2:])
