@@ -331,8 +331,10 @@ int pto_b200_kv_cache_read(const pto_b200_kv_cache *cache, const int32_t *page_t
  * the last `tokens` of the sequence.  max_seq_len bounds seq_lens (at most table_cols * page_size).
  *   o = softmax(scale q K^T) V, (batch, tokens, heads, head_dim) of `dtype`, zeros where there is no key;
  *   lse (optional, (batch, tokens, heads) fp32) = log(sum(exp(scale q K^T))), -infinity where there is no key.
- * Logits, statistics and sums are fp32; the probabilities are rounded to `dtype` for the second product.  With float16
- * queries cached values beyond float16's range count as infinities.  A NaN in a position that one of a sequence's query
+ * Logits, statistics and sums are fp32; the probabilities, relative to the largest, are rounded to 16 bits for the second
+ * product: to the type of a 16-bit cache, to float16 over an MX cache (below 2^-14 they keep multiples of 2^-24; where a
+ * bfloat16 call meets V scales that float16 cannot hold, to bfloat16).  With float16 queries cached values beyond float16's
+ * range count as infinities.  A NaN in a position that one of a sequence's query
  * tokens sees can reach the others'; positions at and after seq_lens[b] may hold anything.
  * `workspace`: device memory of at least pto_b200_prefix_attn_workspace_bytes(...) bytes, 16-byte aligned, not shared by
  * calls that may run at the same time. */
@@ -346,8 +348,9 @@ int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtyp
  * dtype: the 16-bit type of x (rows x_stride elements apart, a multiple of 8), of int4 scales and zeros, and of y unless
  * out_f32.  format PTO_B200_W4_MXFP4: float4_e2m1 codes with float8_e8m0 bytes scale (n x k / 32), the operand b of
  * pto_b200_mxgemm_fp4 (group must be 32, zero NULL); PTO_B200_W4_INT4: W = scale * (code - zero), scale and zero
- * (n x k / group), group 32, 64 or 128, zero = 8 when NULL.  k a multiple of group; sums in fp32.  For more rows use the
- * GEMMs.  `workspace`: device memory of pto_b200_w4_matvec_workspace_bytes(...) bytes (0 for one or two rows of usual length),
+ * (n x k / group), group 32, 64 or 128, zero = 8 when NULL.  k a multiple of group.  Products are exact and sums fp32; of
+ * bfloat16 x, elements below 2^-31 of the largest within 256 k lose bits (2^-40 of the largest at most).  For more rows use
+ * the GEMMs.  `workspace`: device memory of pto_b200_w4_matvec_workspace_bytes(...) bytes (0 for one or two rows of usual length),
  * 16-byte aligned, not shared by calls that may run at the same time. */
 #define PTO_B200_W4_MXFP4 0
 #define PTO_B200_W4_INT4 1

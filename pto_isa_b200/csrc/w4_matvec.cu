@@ -399,10 +399,10 @@ constexpr int kNarrowShare = 16 * kNarrowCols;
 
 // shared memory: the warps' rings, two buffers of shares of k, x (all runs), zeros
 template <bool kMx>
-int narrow_smem(int m, int k)
+int64_t narrow_smem(int m, int k)
 {
     return kWarps * kNarrowStages * narrow_stage_bytes<kMx>() + 2 * kWarps * kNarrowShare * 4 +
-           (k + kStepK - 1) / kStepK * ((m * kXRow + 15) & ~15) + 512;
+           (static_cast<int64_t>(k) + kStepK - 1) / kStepK * ((m * kXRow + 15) & ~15) + 512;
 }
 
 template <bool kBf16, bool kMx>
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, kMt <= 4 ? 2 : 1)
 template <bool kBf16, bool kMx>
 int launch_narrow(W4Args a, cudaStream_t stream)
 {
-    const int smem = narrow_smem<kMx>(a.m, a.k), tiles = (a.n + 15) / 16;
+    const int smem = static_cast<int>(narrow_smem<kMx>(a.m, a.k)), tiles = (a.n + 15) / 16;
     const int most = smem <= kNarrowSmem ? 3 * kSms : 2 * kSms, blocks = tiles < most ? tiles : most;
     a.rows_each = a.n / blocks;
     a.rows_more = a.n % blocks;
@@ -894,13 +894,13 @@ int launch_typed(const W4Args &a, bool mx, uint8_t *workspace, cudaStream_t stre
 
 } // namespace
 
-// room for the prepared x; not asked for where the call does without (few rows, or float16 x against MX fp4)
+// room for the prepared x; none where every block prepares it for itself
 int64_t w4_matvec_workspace_bytes(int m, int k, bool mx)
 {
     if (m <= 2 && (mx ? narrow_smem<true>(m, k) : narrow_smem<false>(m, k)) <= kNarrowMost) {
         return 0;
     }
-    return static_cast<int64_t>((k + kStepK - 1) / kStepK) * streamed_x_run(m);
+    return (static_cast<int64_t>(k) + kStepK - 1) / kStepK * streamed_x_run(m);
 }
 
 int launch_w4_matvec(const uint16_t *x, int64_t x_stride, const uint8_t *w, const void *scale, const uint16_t *zero, void *y,

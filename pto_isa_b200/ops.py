@@ -805,7 +805,8 @@ def prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale=
     seq_lens[b] - (tokens - 1 - j) own positions.  max_seq_len: a bound of seq_lens (default: what the table covers); a
     tight one makes better pieces.
     Returns O like q, zeros for a row without any key; with return_lse also the natural logarithm of the sum of
-    exponentials, float32 of q's shape without head_dim, -inf for such a row.  `workspace`: a CUDA byte tensor of at least
+    exponentials, float32 of q's shape without head_dim, -inf for such a row.  Logits, statistics and sums are float32; the
+    probabilities are rounded to 16 bits for the second product (float16 over an MX cache).  `workspace`: a CUDA byte tensor of at least
     prefix_attn_workspace_bytes(...), 16-byte aligned; without it one is taken from torch's allocator per call."""
     if _fast is not None and out is None and workspace is None:
         o = _fast.prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale, max_seq_len, bool(return_lse))
@@ -865,7 +866,8 @@ def w4_matvec(x, w, scale, zero=None, out_dtype=None, out=None):
     two codes a byte, the lower k in the low nibble.  scale (n, k / group):
       one byte each, group 32: MX fp4, W = e2m1(code) * 2^(scale - 127), mx_gemm_fp4's operand b;
       of x's type, group 32, 64 or 128: int4, W = scale * (code - zero), zero like scale, 8 when None.
-    A 1-D x is one row and gives a 1-D y.  y is of x's type, or float32 with out_dtype=torch.float32."""
+    A 1-D x is one row and gives a 1-D y.  y is of x's type, or float32 with out_dtype=torch.float32.  Sums are float32.
+    Three rows and more take a workspace from torch's allocator on every call."""
     if _fast is not None and out is None and (out_dtype is None or out_dtype == x.dtype or out_dtype == torch.float32):
         y = _fast.w4_matvec(x, w, scale, zero, out_dtype == torch.float32)
         if y is not None:
