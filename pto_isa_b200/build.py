@@ -109,7 +109,7 @@ def build_fast(force=False):
         lib = os.path.join(os.path.dirname(torch.__file__), "lib")
         subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
                                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in includes] +
-                              ["-o", out, src, "-L" + HERE, "-lpto_b200", "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+                              ["-o", out, src, "-L" + HERE, "-lpto_b200", "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
                                "-Wl,-rpath,$ORIGIN"])
     return out
 
