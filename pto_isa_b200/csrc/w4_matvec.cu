@@ -12,7 +12,9 @@
 // float16 pair, and an int4 code is the float16 subnormal code * 2^-24 after one mask; to bfloat16 both take three to
 // four half-rate integer operations a pair.
 //
-// Bound by HBM: n k / 2 bytes of weights are read once, everything else is small.  Weights are the 16-row operand of
+// n k / 2 bytes of weights are read once, everything else is small; in practice the instructions that a word of weights takes
+// on its way to the tensor core bound it (8192 x 8192 MX fp4, one row: 14.3 us, 2.5 TB/s, and 12.2 with W in L2; 16384 x 4096
+// int4 groups of 64 with zeros, 7 rows: 18.4 us; 32003 x 4096 MX fp4, 16 rows: 29.4 us).  Weights are the 16-row operand of
 // mma.m16n8k16, the rows of x its eight columns; the order of k inside 32 is free as long as both operands agree: lane t
 // of a quad takes k = 8t .. 8t + 7 (one word of codes).  The rows of W are dealt out evenly, to the row, over as many
 // blocks as are resident; two kernels:
@@ -20,7 +22,7 @@
 //             with a cp.async ring of its own that runs on across the block's row tiles, so that no warp waits for another
 //             but once a tile, where the shares of k are joined.
 //   streamed  more rows: x is prepared once by a kernel of its own, whose time the first loads of W hide, and comes through
-//             the ring in runs of 256 k; kWr of the warps lie along the rows of W (x is read from L2 once for all of
+//             the ring in runs of 256 k (prepared by every block again, 7 rows took 24.6 us for 20.0); kWr of the warps lie along the rows of W (x is read from L2 once for all of
 //             them), 8 / kWr share the k axis.
 #include "ptx.cuh"
 #include "internal.h"
@@ -860,7 +862,8 @@ int launch_streamed(W4Args a, int blocks, uint8_t *workspace, cudaStream_t strea
 template <bool kBf16, bool kMx, int kG>
 int launch_rows(W4Args a, uint8_t *workspace, cudaStream_t stream)
 {
-    // two blocks an SM, or one where that leaves a block fewer than 32 rows: every block reads all of x
+    // two blocks an SM, or one where that leaves a block no more than 32 rows (every block reads all of x) or more rows of x
+    // than two blocks' registers hold; three blocks of 80 registers: 24.6 us for 20.0 at 7 rows, 33.1 for 30.7 at 16
     const int tiles = (a.n + 15) / 16;
     const int blocks = a.n > 64 * kSms && a.m <= 32 ? 2 * kSms : (tiles < kSms ? tiles : kSms);
     const int rows = (a.n + blocks - 1) / blocks;
