@@ -719,17 +719,23 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
     }
 }
 
-// How the keys are cut.  About three blocks of 16 rows fit an SM; a piece is at least 64 keys (16 for each warp).  With
-// more than kWideRows rows the prefix goes to the wide kernel, one block per SM, in one wave where it can.
+// How the keys are cut.  About three blocks of 16 rows fit an SM; a piece is at least 64 keys (16 for each warp).  A prefix of
+// many rows and keys goes to the wide kernel, one block per SM, in one wave where it can.
 struct Plan {
     int prefix_tiles, prefix_splits, prefix_pieces, prefix_chunk, prefix_wide;
     int own_tiles, own_splits, own_min;
     int64_t slots, own_slots;
 };
 
-// The most rows over the prefix that the piece kernel takes: one tile.  With two it would read and convert every key twice,
-// and its 16-row products do an eighth of the wide kernel's work a key.
-constexpr int kWideRows = 16;
+// The piece kernel takes 0.065 ns a key, kv head and tile of 16 rows, the wide kernel as much as two such tiles for 128 rows, and
+// 10 to 15 us more before and after.  8 heads of 128 elements, MX fp8, pieces against wide, us: 32 rows 12 / 19 at 4096 keys, 33 /
+// 50 at 32768; 64 rows 9.2 / 12.7 at 512, 16 / 22 at 4096, 75 / 53 at 32768; 128 rows 12.9 / 15.2, 23 / 26, 145 / 57.
+bool wants_wide(int rows, int kv_heads, int prefix_len)
+{
+    const int64_t tiles = ceil_div(rows, kRows), more = tiles - 2 * static_cast<int64_t>(ceil_div(rows, 128));
+    return more > 0 && more * kv_heads * prefix_len > 16384 * ((tiles < 8 ? tiles : 8) + 6);
+}
+
 // up to so many pieces of more rows than run at once with four warps each: a warp a row (4096 rows of 9 pieces: 8.3 us for
 // 15.8; 8 rows of 9: 3.4 us with four warps, 4.0 with one)
 constexpr int kFewPieces = 16, kManyRows = 1024;
@@ -742,7 +748,7 @@ Plan make_plan(int batch, int tokens, int heads, int kv_heads, int prefix_len, i
     if (prefix_len > 0) {
         const int rows = batch * row_span;
         p.prefix_tiles = ceil_div(rows, kRows);
-        p.prefix_wide = rows > kWideRows;
+        p.prefix_wide = wants_wide(rows, kv_heads, prefix_len);
         if (p.prefix_wide) {
             const bool pair = rows > 128;
             const int64_t units = static_cast<int64_t>(ceil_div(rows, pair ? 256 : 128)) * kv_heads;
