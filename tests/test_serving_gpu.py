@@ -693,3 +693,84 @@ def test_attention_joins_many_and_few_pieces(name, d):
     check_attention(torch.randn(2, 1, 1, d, generator=gen(1), device="cuda").to(F16), long[0], long[1], 0, *long[2:])
     rows = make_attention(name, F16, d, 8, 16, 130, [5, 0, 40] * 14 + [1], 4)
     check_attention(torch.randn(43, 1, 32, d, generator=gen(2), device="cuda").to(F16), rows[0], rows[1], 130, *rows[2:])
+
+
+# --------------------------------------------------------------------------------------------------- a prefix of many rows and keys
+# (sizes past which the prefix goes to the tensor memory kernel: one row tile, and several)
+
+WIDE = [(20, 32, 8, 7700), (300, 8, 2, 2111)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("batch,heads,kv,prefix", WIDE)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_long_prefix_of_many_rows(dtype, batch, heads, kv, prefix, name, d):
+    """A negative, a zero and a large scale, a maximum that grows along the keys, cached values far from 1 in some tiles only,
+    rows of q of very different sizes."""
+    import pto_isa_b200 as p
+    for at, (ek, ev) in enumerate(((0, 0), (-30, 0), (30, 0), (0, 30), (0, -30), (0, 6))):
+        if dtype == F16 and (abs(ek) > 8 or abs(ev) > 10):
+            continue
+        c, pages, table, lens, parts, own = make_attention(name, dtype, d, kv, 32, prefix, [3] * batch, 40 + at)
+        t = torch.arange(150, 420)
+        slots = (pages[(t // 32).cuda()].long() * 32 + t.cuda() % 32).to(torch.int32)
+        k, v = (torch.randn(len(t), kv, d, generator=gen(s), device="cuda") * torch.linspace(0.2, 6, len(t), device="cuda")[:, None, None] for s in (1, 2))
+        p.kv_cache_write(c, (k * 2.0 ** ek).to(dtype), (v * 2.0 ** ev).to(dtype), slots)
+        kd, vd = values(c)
+        rows = lambda x: x[pages.long().cpu()].transpose(0, 1).reshape(kv, -1, d)[:, :prefix].cuda()
+        size = torch.exp2(torch.randint(-3, 3, (batch, 1, heads, 1), generator=gen(8), device="cuda").float() - max(ek, 0))
+        q = (torch.randn(batch, 1, heads, d, generator=gen(6), device="cuda") * size).to(dtype)
+        for scale in (None, -0.3, 0.0) if at == 0 else (None,):
+            check_attention(q, c, pages, prefix, table, lens, [rows(kd), rows(vd)], own, scale=scale)
+
+
+@pytest.mark.parametrize("name", FORMATS)
+def test_attention_long_prefix_nan_bad_pages_and_repeats(name):
+    import pto_isa_b200 as p
+    batch, heads, d, prefix = 128, 8, 128, 4897
+    c, pages, table, lens = make_attention(name, F16, d, 1, 16, prefix, [0] * batch, 22)[:4]
+    table = torch.zeros(batch, 1, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, heads, d, generator=gen(2), device="cuda").to(F16)
+    first = p.prefix_attn(q, c, pages, prefix, table, lens, return_lse=True)
+    for _ in range(3):
+        again = p.prefix_attn(q, c, pages, prefix, table, lens, return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    kd, vd = values(c)
+    broken = pages.clone()
+    broken[7] = c.k.shape[0]
+    o = p.prefix_attn(q, c, broken, 4896, table, lens)
+    assert status()[2:] == (11, c.k.shape[0])
+    keep = torch.cat([pages[:7], pages[8:]]).long().cpu()
+    rows = lambda x: x[keep].transpose(0, 1).reshape(1, -1, d)[:, :4880].cuda()
+    none = torch.zeros(1, 0, d, dtype=torch.float64, device="cuda")
+    want, _, wv, vsum, qk = ref.attention(q[:, None].double(), rows(kd), rows(vd), [none] * batch, [none] * batch, d ** -0.5)
+    bound, _ = ref.attention_bounds(F16, want, wv, vsum, qk, 4896, mx=name != "16")
+    assert ((o[:, None].double() - want).abs() <= bound).all()
+    bad = torch.full((1, 1, d), float("nan"), dtype=F16, device="cuda")
+    p.kv_cache_write(c, bad, bad, (pages[306] * 16).view(1))  # position 4896
+    assert torch.isfinite(p.prefix_attn(q, c, pages, 4896, table, lens)).all()
+    assert p.prefix_attn(q, c, pages, 4897, table, lens).isnan().all()
+
+
+def test_attention_long_prefix_at_the_same_time_and_replayed():
+    import pto_isa_b200 as p
+    made = make_attention("mxfp8", BF16, 128, 8, 64, 700, [33] * 128, 8)
+    q = [torch.randn(128, 1, 64, 128, generator=gen(s), device="cuda").to(BF16) for s in (1, 2)]
+    call = lambda i: p.prefix_attn(q[i], made[0], made[1], 700, made[2], made[3])
+    alone = [call(0), call(1)]
+    check_attention(q[0], made[0], made[1], 700, *made[2:])
+    streams, graphs, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for i in (0, 1):
+        with torch.cuda.graph(graphs[i]):
+            outs.append(call(i))
+        streams[i].wait_stream(torch.cuda.current_stream())
+    eager = []
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+                eager.append((i, call(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(outs[i], alone[i]) for i in (0, 1)) and all(torch.equal(o, alone[i]) for i, o in eager)
+    assert status()[0] == 0
