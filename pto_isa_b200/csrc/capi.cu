@@ -831,6 +831,11 @@ int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const 
         set_error_text("w4_matvec: rows of x, w and the workspace must be 16-byte aligned");
         return kErrUnsupportedShape;
     }
+    if ((format == PTO_B200_W4_INT4 && ((reinterpret_cast<uintptr_t>(scale) | reinterpret_cast<uintptr_t>(zero)) & 1u) != 0) ||
+        (reinterpret_cast<uintptr_t>(y) & (out_f32 != 0 ? 3u : 1u)) != 0) {
+        set_error_text("w4_matvec: scales, zeros and y must be aligned to their elements");
+        return kErrUnsupportedShape;
+    }
     return launch_w4_matvec(static_cast<const uint16_t *>(x), x_stride, w, scale, static_cast<const uint16_t *>(zero), y, m, n, k,
                             group, dtype == PTO_B200_DTYPE_BF16, format == PTO_B200_W4_MXFP4, out_f32 != 0, workspace, workspace_bytes,
                             as_stream(stream));

@@ -192,3 +192,6 @@ def test_c_entry_points_refuse_before_they_touch_a_device(clib):
     assert clib.pto_b200_w4_matvec_workspace_bytes(1, 4096, 0) == 0 and clib.pto_b200_w4_matvec_workspace_bytes(3, 4096, 0) > 0
     assert w4(m=3) == 1 and b"workspace" in clib.pto_b200_last_error()
     assert w4(x=ctypes.c_void_p((1 << 20) + 2)) == 2 and w4(stride=60) == 2 and w4(m=0) == 0 and w4(n=0) == 0
+    odd = ctypes.c_void_p((1 << 20) + 1)
+    assert clib.pto_b200_w4_matvec(some, 64, some, odd, None, some, 1, 8, 64, 32, 1, 2, 0, None, 0, None) == 2
+    assert w4(fmt=1, zero=odd) == 2 and clib.pto_b200_w4_matvec(some, 64, some, some, None, odd, 1, 8, 64, 32, 0, 2, 0, None, 0, None) == 2
