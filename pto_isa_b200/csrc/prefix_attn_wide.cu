@@ -358,11 +358,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const bool valid = pid[i] >= 0 && pid[i] < a.num_pages;
-                    if (!valid && k_begin + m * kTile + r + 64 * i < k_end && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
-                        status->block = blockIdx.x;
-                        status->where = 11;
-                        status->detail = pid[i];
-                    }
                     const uint32_t mask = __ballot_sync(0xffffffffu, valid);
                     uint32_t flags = 0;
                     if constexpr (kMx) {
@@ -384,6 +379,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
+                    // a page that does not exist is reported by one lane, when nobody waits for it any more
+                    const uint32_t missing = __ballot_sync(0xffffffffu, (pid[i] < 0 || pid[i] >= a.num_pages) && k_begin + m * kTile + r + 64 * i < k_end);
+                    if (missing != 0 && lane == __ffs(missing) - 1 && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+                        status->block = blockIdx.x;
+                        status->where = 11;
+                        status->detail = pid[i];
+                    }
                     pid[i] = pid_next[i];
                     pid_next[i] = m + 2 < tiles ? page_of(m + 2, r + 64 * i) : -1;
                 }
@@ -444,6 +446,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     }
                 }
                 asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                // K is handed over when its tile has been described, as where its scales are needed: the describing warps, which
+                // follow K's ring by its parity, are then never more than a round of it behind
+                if (!is_v && !warp_wait(&ctl->info_full[j % kInfo], (j / kInfo) & 1, abort_flag, lane)) {
+                    ok = false;
+                    break;
+                }
             } else {
                 constexpr int kWords = kFmt == kKvMxFp8 ? 4 : 2;
                 uint32_t code[4 * kHalves][kWords], scales[4];
