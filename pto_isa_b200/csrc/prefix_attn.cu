@@ -367,17 +367,19 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
             for (int j = 0; j < 4; ++j) {
                 s[n][j] = 0.0f;
             }
-            uint32_t sc[2] = {0, 0}; // scale bytes of the lane's two columns (keys 8n + 2t, + 1)
+            float2 sc[2][kBlk / 2]; // scales of the lane's two columns (keys 8n + 2t, + 1), two blocks each; byte 255: NaN
             if constexpr (kFmt >= kKvMxFp8) {
                 const uint32_t at = base + 2 * St::kRowsBytes + (8 * n + 2 * t) * kBlk;
                 if constexpr (kBlk == 4) {
                     const uint2 v = lds64(at);
-                    sc[0] = v.x;
-                    sc[1] = v.y;
+                    sc[0][0] = e8m0x2_to_f32(v.x);
+                    sc[0][1] = e8m0x2_to_f32(v.x >> 16);
+                    sc[1][0] = e8m0x2_to_f32(v.y);
+                    sc[1][1] = e8m0x2_to_f32(v.y >> 16);
                 } else {
                     const uint32_t v = lds32(at);
-                    sc[0] = v & 0xffffu;
-                    sc[1] = v >> 16;
+                    sc[0][0] = e8m0x2_to_f32(v);
+                    sc[1][0] = e8m0x2_to_f32(v >> 16);
                 }
             }
 #pragma unroll
@@ -399,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     float p[4];
                     mma_16816_first<false>(p, qf[kb][0][0], qf[kb][1][0], qf[kb][0][1], qf[kb][1][1], w[0], w[1]);
                     mma_16816<false>(p, qf[kb][0][2], qf[kb][1][2], qf[kb][0][3], qf[kb][1][3], w[2], w[3]);
-                    const float f0 = __uint_as_float(((sc[0] >> (8 * kb)) & 0xffu) << 23);
-                    const float f1 = __uint_as_float(((sc[1] >> (8 * kb)) & 0xffu) << 23);
+                    const float f0 = kb & 1 ? sc[0][kb / 2].y : sc[0][kb / 2].x;
+                    const float f1 = kb & 1 ? sc[1][kb / 2].y : sc[1][kb / 2].x;
                     s[n][0] = fmaf(p[0], f0, s[n][0]);
                     s[n][1] = fmaf(p[1], f1, s[n][1]);
                     s[n][2] = fmaf(p[2], f0, s[n][2]);

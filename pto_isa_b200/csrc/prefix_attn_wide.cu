@@ -14,8 +14,10 @@
 // A tile of K or V comes from pages, in 16 bits by cp.async or as codes that eight loading warps convert on the way into
 // shared memory.  Codes become float16 whatever the type of q: e4m3 and e2m1 convert to float16 pairs in one instruction,
 // to bfloat16 in four.  Exactness:
-//   K       code 2^e is exact in float16 for e in [-15, 7] (e4m3) or [-23, 13] (e2m1).  A key with a block outside that range is stored relative to
-//           its largest scale, 2^(e - e_max), and the power of two goes to the logit as a factor of the key.
+//   K       code 2^e is exact in float16 for e in [-15, 7] (e4m3) or [-23, 13] (e2m1).  A key with a block outside that range is
+//           stored relative to its largest scale, 2^(e - e_max), and the power of two goes to the logit as a factor of the key
+//           (NaN where a scale byte is 255).  Blocks far below the key's largest then lose bits: at most 2^-25 2^(e_max) an
+//           element.
 //   q       bfloat16 rows are divided by a power of two that brings their largest element into [2^14, 2^15): elements
 //           down to 2^-31 of it keep every bit; the logits of the row are multiplied back.
 //   V, P    float16 where all scales of the tile are in range; otherwise, if q is bfloat16, this tile's V and P are bfloat16
@@ -135,6 +137,14 @@ __device__ __forceinline__ bool scales_in_range(uint32_t s)
         ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || b == 0u);
     }
     return ok;
+}
+
+// A key is stored as it is, or, with a block out of range, relative to its largest scale; one of scale bytes 0 only likewise: as
+// they are its codes would all be lost.
+template <int kD, int kFmt>
+__device__ __forceinline__ bool key_is_plain(uint32_t s)
+{
+    return scales_in_range<kD, kFmt>(s) && s != 0u;
 }
 
 template <int kD>
@@ -326,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < 2 && kMx; ++i) {
                     const int64_t row = cache_row(pid[i], m, r + 64 * i);
-                    ks[i] = row >= 0 ? row_scales<kD>(a.ks, row) : 0u;
-                    vs[i] = row >= 0 ? row_scales<kD>(a.vs, row) : 0u;
+                    ks[i] = row >= 0 ? row_scales<kD>(a.ks, row) : 0x7f7f7f7fu; // no key: nothing out of the ordinary
+                    vs[i] = row >= 0 ? row_scales<kD>(a.vs, row) : 0x7f7f7f7fu;
                 }
             };
             // 16 keys a lane: K by one warp, V by the other
@@ -361,11 +371,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     const uint32_t mask = __ballot_sync(0xffffffffu, valid);
                     uint32_t flags = 0;
                     if constexpr (kMx) {
-                        const bool k_out = !scales_in_range<kD, kFmt>(ks[i]);
+                        const bool k_out = !key_is_plain<kD, kFmt>(ks[i]);
                         // with float16 queries V stays float16: small values only lose what is below float16's last place,
                         // as o itself does, and larger ones than it holds count as infinities
                         const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(vs[i]);
-                        info.factor[r + 64 * i] = k_out ? static_cast<uint16_t>(largest_scale<kD>(ks[i]) << 7) : 0x3f80;
+                        const uint32_t top = largest_scale<kD>(ks[i]); // 255: NaN, whatever the block's codes are
+                        info.factor[r + 64 * i] = k_out ? static_cast<uint16_t>(top == 255u ? 0x7fc0u : top == 0u ? 0x0040u : top << 7) : 0x3f80;
                         flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
                     }
                     if (lane == 0) {
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                         codes16_to_f16<kFmt>(c, w);
                         const uint32_t byte = (scale >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
                         // keys with a block out of range: relative to their largest scale
-                        const bool relative = !is_v && !scales_in_range<kD, kFmt>(scale);
+                        const bool relative = !is_v && !key_is_plain<kD, kFmt>(scale);
                         const int e = relative && byte != 255u ? max(static_cast<int>(byte) + 127 - static_cast<int>(largest_scale<kD>(scale)), 0)
                                                                : static_cast<int>(byte);
                         const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);

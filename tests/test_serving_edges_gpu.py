@@ -62,3 +62,104 @@ def test_attention_prefix_with_many_missing_pages(batch, heads, kv, prefix, d, n
     ob, lb = ref.attention_bounds(F16, want, wv, vsum, qk, prefix, mx=name != "16")
     assert ((o.double() - want).abs() <= ob).all() and ((lse.double() - wlse).abs() <= lb).all()
     assert status()[0] == 0
+
+
+# --------------------------------------------------------------------------------------------------- scale bytes and codes of any cache
+# Caches filled by something else than kv_cache_write: any codes under any scale byte.
+
+SHAPES = [("own", 3, 8, 2, 90), ("prefix", 3, 8, 2, 90), ("long", 20, 32, 8, 7700)]  # batch, heads, kv_heads, keys
+
+
+def raw_cache(name, kv, page, keys, d, low, high, seed):
+    """An MX cache of `keys` positions in page order: every code but e4m3's NaN, scale bytes low .. high."""
+    import pto_isa_b200 as p
+    c = p.kv_cache_empty(-(-keys // page), kv, page, d, fmt_of(name, F16))
+    for i, t in enumerate(c[:4]):
+        t.copy_(torch.randint(0, 256, t.shape, generator=gen(seed + i), device="cuda") if i < 2 else
+                torch.randint(low[i - 2], high[i - 2] + 1, t.shape, generator=gen(seed + i), device="cuda"))
+        if i < 2 and name == "mxfp8":
+            t[(t & 127) == 127] = 0x38
+    return c
+
+
+def at(keys, page):
+    """(page, row) of positions `keys` of a cache in page order."""
+    keys = torch.as_tensor(keys, device="cuda")
+    return keys // page, keys % page
+
+
+def put_block(c, which, keys, page, head, block, codes, byte):
+    """Block `block` of `head` at positions `keys` of K (which 0) or V (1): all bytes of codes, and the scale."""
+    pg, row = at(keys, page)
+    width = c[which].shape[-1] // c[which + 2].shape[-1]
+    c[which][pg, head, row, block * width:(block + 1) * width] = codes
+    c[which + 2][pg, head, row, block] = byte
+
+
+def check_raw(c, q, where, keys, scale=None):
+    """All `keys` positions as every sequence's own keys, or as the prefix: the values that the cache stands for, and NaN exactly
+    where it holds one."""
+    import pto_isa_b200 as p
+    batch, heads, d = q.shape
+    kv = c.k.shape[1]
+    pages = torch.arange(c.k.shape[0], dtype=torch.int32, device="cuda")
+    kd, vd = (x.transpose(0, 1).reshape(kv, -1, d)[:, :keys].cuda() for x in values(c))
+    none = torch.zeros(kv, 0, d, dtype=torch.float64, device="cuda")
+    own = where == "own"
+    table = pages.expand(batch, -1).contiguous()
+    lens = torch.full((batch,), keys if own else 0, dtype=torch.int32, device="cuda")
+    if where == "long":
+        wide_shape(batch, 1, heads, kv, d, keys)
+        table = table[:, :0]
+    elif not own:
+        table = table[:, :1]
+    parts, owns = ([none, none], [[kd] * batch, [vd] * batch]) if own else ([kd, vd], [[none] * batch] * 2)
+    o, lse = p.prefix_attn(q, c, pages, 0 if own else keys, table, lens, scale=scale, return_lse=True)
+    o, lse = o[:, None], lse[:, None]
+    want, wlse, wv, vsum, qk = ref.attention(q[:, None].double(), *parts, *owns, d ** -0.5 if scale is None else scale)
+    ob, lb = ref.attention_bounds(q.dtype, want, wv, vsum, qk, keys, mx=True)
+    if q.dtype == F16:  # values past float16's range are infinities of the output
+        past = want.abs() >= 65520
+        assert (o[past] == torch.where(want[past] > 0, torch.inf, -torch.inf)).all()
+        ob = torch.where(past, torch.inf, ob)
+        want = torch.where(past, 0.0, want)
+        o = torch.where(past, 0.0, o.double())
+    assert torch.equal(o.isnan(), want.isnan()) and torch.equal(lse.isnan(), wlse.isnan())
+    live, seen = ~want.isnan(), ~wlse.isnan()
+    err, lerr = (o.double() - want).abs()[live], (lse.double() - wlse).abs()[seen]
+    assert (err <= ob[live]).all(), float((err / ob[live]).max())
+    assert (lerr <= lb[seen]).all(), float((lerr / lb[seen]).max())
+    assert status()[0] == 0
+    return o, lse
+
+
+MX = ["mxfp8", "mxfp4"]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_k_scale_of_nan(where, batch, heads, kv, keys, name, dtype, d):
+    """Scale byte 255 is NaN over any codes: the rows of that kv head are NaN, those of the others are not."""
+    page = 32
+    q = torch.randn(batch, heads, d, generator=gen(4), device="cuda").to(dtype)
+    for i, (codes, block) in enumerate(((0xff if name == "mxfp4" else 0xb8, 0), (0x22 if name == "mxfp4" else 0x38, d // 32 - 1), (0, 1))):
+        c = raw_cache(name, kv, page, keys, d, (116, 116), (122, 124), 70 + i)
+        put_block(c, 0, [keys - 3 - i], page, kv - 1, block, codes, 255)
+        o, _ = check_raw(c, q.abs() if i == 0 else q, where, keys)  # one sign throughout: a block of infinities would drop the key
+        assert o.isnan().any() and not o.isnan().all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_k_of_the_smallest_scales(where, batch, heads, kv, keys, name, d):
+    """K blocks of scale byte 0 are multiples of 2^-127, which bfloat16 queries of 2^124 turn into ordinary logits."""
+    page = 32
+    q = (torch.randn(batch, heads, d, generator=gen(4), device="cuda") * 2.0 ** 124).to(BF16)
+    for high in (0, 3):
+        c = raw_cache(name, kv, page, keys, d, (0, 116), (high, 124), 80)
+        if name == "mxfp8":  # codes below 8, so that no key outweighs all others
+            c.k.copy_(torch.where((c.k & 127) > 0x50, c.k & 0xcf, c.k))
+        check_raw(c, q, where, keys)
