@@ -139,33 +139,25 @@ struct Stage {
     static constexpr int kSmem = kRing > kMergeBytes ? kRing : kMergeBytes;
 };
 
-// scaled V operand: a pair of values of two keys times the keys' powers of two.  float16: exact where scale_ok() says so,
-// rounded to float16's range elsewhere, as float16 queries' results are.  kWide: bfloat16, exact but for scale byte 0 (0
-// instead of 2^-127); byte 255 is infinity there and as float16, and times a block's zeros the NaN that it stands for.
-template <bool kWide>
+// Scaled V operand: a pair of values of two keys times the keys' powers of two.  In float16, by one product of pairs: exact
+// where scale_ok() says so, rounded to float16's range elsewhere, as float16 queries' results are; byte 255 is infinity there,
+// and times a block's zeros the NaN that it stands for.
 __device__ __forceinline__ uint32_t scale_pair(uint32_t b0, uint32_t b1)
 {
-    if constexpr (kWide) {
-        return (b0 << 7) | (b1 << 23);
-    } else {
-        return pack_16x2<false>(__uint_as_float(b0 << 23), __uint_as_float(b1 << 23));
-    }
+    return pack_16x2<false>(__uint_as_float(b0 << 23), __uint_as_float(b1 << 23));
 }
-template <bool kWide>
-__device__ __forceinline__ uint32_t scaled(uint32_t h, uint32_t scale)
+// The same by way of 32 bits: one rounding for every code (NaN among e4m3's) and scale byte
+template <bool kBf16>
+__device__ __forceinline__ uint32_t scaled_any(uint32_t h, float s0, float s1)
 {
-    if constexpr (kWide) { // float16's places to bfloat16's: the value times 2^-112, times 2^112
-        const uint32_t v = (h & 0x80008000u) | ((h >> 3) & 0x0fff0fffu);
-        return mul_16x2<true>(mul_16x2<true>(v, 0x77807780u), scale);
-    } else {
-        return mul_16x2<false>(h, scale);
-    }
+    const float2 f = unpack_16x2<false>(h);
+    return pack_16x2<kBf16>(f.x * s0, f.y * s1);
 }
 // whether every code times 2^(byte - 127) is exact in float16
 template <int kFmt>
 __device__ __forceinline__ bool scale_ok(uint32_t byte)
 {
-    return kFmt == kKvMxFp8 ? byte - 112u <= 22u || byte == 0u : byte - 104u <= 36u || byte == 0u;
+    return kFmt == kKvMxFp8 ? byte - 112u <= 22u : byte - 104u <= 36u;
 }
 
 template <bool kBf16, int kD, int kFmt>
@@ -486,11 +478,15 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     x[i][0] = lds32(at);
                 }
             }
+            // kWide: bfloat16 products, for queries of that type
             auto product = [&](auto wide) {
                 constexpr bool kWide = decltype(wide)::value;
                 const uint32_t p0 = pack_16x2<kWide>(s[0][0], s[0][1]), p1 = pack_16x2<kWide>(s[0][2], s[0][3]);
                 const uint32_t p2 = pack_16x2<kWide>(s[1][0], s[1][1]), p3 = pack_16x2<kWide>(s[1][2], s[1][3]);
-                const uint32_t scale01 = scale_pair<kWide>(sb[0], sb[1]), scale23 = scale_pair<kWide>(sb[2], sb[3]);
+                const uint32_t pair01 = scale_pair(sb[0], sb[1]), pair23 = scale_pair(sb[2], sb[3]);
+                const float2 f01 = e8m0x2_to_f32(sb[0] | (sb[1] << 8)), f23 = e8m0x2_to_f32(sb[2] | (sb[3] << 8));
+                auto scaled01 = [&](uint32_t h) { return kWide ? scaled_any<kWide>(h, f01.x, f01.y) : mul_16x2<false>(h, pair01); };
+                auto scaled23 = [&](uint32_t h) { return kWide ? scaled_any<kWide>(h, f23.x, f23.y) : mul_16x2<false>(h, pair23); };
 #pragma unroll
                 for (int w = 0; w < kWords; ++w) {
                     if constexpr (kFmt == kKvMxFp8) {
@@ -501,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                             e4m3x4_to_f16(__byte_perm(x[2][w], x[3][w], c ? 0x7362 : 0x5140), hi[0], hi[1]);
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                mma_16816<kWide>(o[4 * w + 2 * c + e], p0, p1, p2, p3, scaled<kWide>(lo[e], scale01), scaled<kWide>(hi[e], scale23));
+                                mma_16816<kWide>(o[4 * w + 2 * c + e], p0, p1, p2, p3, scaled01(lo[e]), scaled23(hi[e]));
                             }
                         }
                     } else {
@@ -513,15 +509,28 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                         e2m1x8_to_f16(((x[2][w] >> 4) & 0x0f0f0f0fu) | (x[3][w] & 0xf0f0f0f0u), odd_hi);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            mma_16816<kWide>(o[8 * w + 2 * i], p0, p1, p2, p3, scaled<kWide>(even_lo[i], scale01), scaled<kWide>(even_hi[i], scale23));
-                            mma_16816<kWide>(o[8 * w + 2 * i + 1], p0, p1, p2, p3, scaled<kWide>(odd_lo[i], scale01), scaled<kWide>(odd_hi[i], scale23));
+                            mma_16816<kWide>(o[8 * w + 2 * i], p0, p1, p2, p3, scaled01(even_lo[i]), scaled23(even_hi[i]));
+                            mma_16816<kWide>(o[8 * w + 2 * i + 1], p0, p1, p2, p3, scaled01(odd_lo[i]), scaled23(odd_hi[i]));
                         }
                     }
                 }
             };
             if constexpr (kBf16) {
-                const bool exact = scale_ok<kFmt>(sb[0]) && scale_ok<kFmt>(sb[1]) && scale_ok<kFmt>(sb[2]) && scale_ok<kFmt>(sb[3]);
-                if (__all_sync(0xffffffffu, exact)) {
+                bool exact = __all_sync(0xffffffffu, scale_ok<kFmt>(sb[0]) && scale_ok<kFmt>(sb[1]) && scale_ok<kFmt>(sb[2]) && scale_ok<kFmt>(sb[3]));
+                if (!exact) { // zeros have scale byte 0 (those of keys past the end too): as exact as any
+                    bool zeros = true;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t any = 0;
+#pragma unroll
+                        for (int w = 0; w < kWords; ++w) {
+                            any |= x[i][w] & (kFmt == kKvMxFp8 ? 0x7f7f7f7fu : 0x77777777u);
+                        }
+                        zeros = zeros && (scale_ok<kFmt>(sb[i]) || (sb[i] == 0u && any == 0u));
+                    }
+                    exact = __all_sync(0xffffffffu, zeros);
+                }
+                if (exact) {
                     product(std::false_type{});
                 } else {
                     product(std::true_type{});

@@ -21,7 +21,9 @@
 //   q       bfloat16 rows are divided by a power of two that brings their largest element into [2^14, 2^15): elements
 //           down to 2^-31 of it keep every bit; the logits of the row are multiplied back.
 //   V, P    float16 where all scales of the tile are in range; otherwise, if q is bfloat16, this tile's V and P are bfloat16
-//           (code 2^e is exact there): an instruction's operands share a type, its fp32 accumulator does not care.
+//           (code 2^e is exact there): an instruction's operands share a type, its fp32 accumulator does not care.  A block of
+//           scale byte 0 counts as out of range: whether it is all zeros would take its codes (looked up by the describing
+//           warps, 8 x 128 rows x 32768 MX fp4 keys without any such block took 6 us more).
 //
 // What bounds it: per 128 x 128 logits and head size 128, 1024 cycles of tensor work, 1024 of the special-function unit
 // (an exponential takes 8 cycles a warp), about 512 of the integer pipe for the conversion of a quantised tile.  It takes
@@ -126,15 +128,15 @@ __device__ __forceinline__ uint32_t row_scales(const uint8_t *s, int64_t row)
 }
 
 // whether code 2^(byte - 127) is exact in float16 for every block of the row: e in [-15, 7] for e4m3 (2^-9 .. 448), in
-// [-23, 13] for e2m1 (0.5 .. 6), or a block of zeros
-template <int kD, int kFmt>
+// [-23, 13] for e2m1 (0.5 .. 6).  Byte 0 mostly stands for zeros, but may be multiples of 2^-127: kZero says how it counts.
+template <int kD, int kFmt, bool kZero = true>
 __device__ __forceinline__ bool scales_in_range(uint32_t s)
 {
     bool ok = true;
 #pragma unroll
     for (int i = 0; i < kD / 32; ++i) {
         const uint32_t b = (s >> (8 * i)) & 0xffu;
-        ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || b == 0u);
+        ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || (kZero && b == 0u));
     }
     return ok;
 }
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                         const bool k_out = !key_is_plain<kD, kFmt>(ks[i]);
                         // with float16 queries V stays float16: small values only lose what is below float16's last place,
                         // as o itself does, and larger ones than it holds count as infinities
-                        const bool v_out = kBf16 && !scales_in_range<kD, kFmt>(vs[i]);
+                        const bool v_out = kBf16 && !scales_in_range<kD, kFmt, false>(vs[i]);
                         const uint32_t top = largest_scale<kD>(ks[i]); // 255: NaN, whatever the block's codes are
                         info.factor[r + 64 * i] = k_out ? static_cast<uint16_t>(top == 255u ? 0x7fc0u : top == 0u ? 0x0040u : top << 7) : 0x3f80;
                         flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
@@ -530,11 +532,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                         const int e = relative && byte != 255u ? max(static_cast<int>(byte) + 127 - static_cast<int>(largest_scale<kD>(scale)), 0)
                                                                : static_cast<int>(byte);
                         const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);
+                        const float exact = e8m0x2_to_f32(byte).x;
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
-                            if (is_v) { // bfloat16: the values times 2^-112 to the other format's places, then scaled
-                                w[x] = mul_16x2<true>((w[x] & 0x80008000u) | ((w[x] >> 3) & 0x0fff0fffu), 0x77807780u);
-                                w[x] = mul_16x2<true>(w[x], byte * 0x00800080u); // 255: infinity, times 0 NaN
+                            if (is_v) { // one rounding to bfloat16; NaN for a code or scale that is
+                                const float2 v = unpack_16x2<false>(w[x]);
+                                w[x] = pack_16x2<kBf16>(v.x * exact, v.y * exact);
                             } else {
                                 w[x] = mul_16x2<false>(w[x], pack_16x2<false>(f, f));
                             }

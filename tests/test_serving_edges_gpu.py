@@ -96,9 +96,11 @@ def put_block(c, which, keys, page, head, block, codes, byte):
     c[which + 2][pg, head, row, block] = byte
 
 
-def check_raw(c, q, where, keys, scale=None):
+def check_raw(c, q, where, keys, scale=None, tiny=False):
     """All `keys` positions as every sequence's own keys, or as the prefix: the values that the cache stands for, and NaN exactly
-    where it holds one."""
+    where it holds one.  tiny: of values near bfloat16's smallest.  In place of the bound's floor of 1e-30 come three halves of a step
+    of 2^-133 below the normal numbers, one for V (the weights' sum is 1), one for the output, one for 32-bit sums there (places
+    of 2^-149, at most 2^-150 a key: 2^-137 for 8192)."""
     import pto_isa_b200 as p
     batch, heads, d = q.shape
     kv = c.k.shape[1]
@@ -118,6 +120,8 @@ def check_raw(c, q, where, keys, scale=None):
     o, lse = o[:, None], lse[:, None]
     want, wlse, wv, vsum, qk = ref.attention(q[:, None].double(), *parts, *owns, d ** -0.5 if scale is None else scale)
     ob, lb = ref.attention_bounds(q.dtype, want, wv, vsum, qk, keys, mx=True)
+    if tiny:
+        ob = ob - 1e-30 + 3 * 2.0 ** -134
     if q.dtype == F16:  # values past float16's range are infinities of the output
         past = want.abs() >= 65520
         assert (o[past] == torch.where(want[past] > 0, torch.inf, -torch.inf)).all()
@@ -163,3 +167,48 @@ def test_attention_k_of_the_smallest_scales(where, batch, heads, kv, keys, name,
         if name == "mxfp8":  # codes below 8, so that no key outweighs all others
             c.k.copy_(torch.where((c.k & 127) > 0x50, c.k & 0xcf, c.k))
         check_raw(c, q, where, keys)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_v_of_bfloat16_queries_nan(where, batch, heads, kv, keys, name, d):
+    """A NaN scale over any codes and (e4m3) a NaN code make their columns NaN and no others, beside scales that float16 holds and
+    beside one that it does not."""
+    page = 32
+    q = torch.randn(batch, heads, d, generator=gen(4), device="cuda").to(BF16)
+    for far in (False, True):
+        c = raw_cache(name, kv, page, keys, d, (116, 116), (122, 122), 90)
+        if far:
+            put_block(c, 1, [keys - 6], page, kv - 1, 1, 0x11, 160)
+        put_block(c, 1, [keys - 3], page, kv - 1, 0, 0x22 if name == "mxfp4" else 0x38, 255)
+        if name == "mxfp8":
+            pg, row = at([keys - 4], page)
+            c.v[pg, 0, row, 33] = 0x7f
+            c.v[pg, 0, row, 40] = 0xff
+            c.v[pg, 0, row, 3] = 0x7e  # 448, the largest code that is a number
+        o, _ = check_raw(c, q, where, keys)
+        nan = o.isnan().view(batch, kv, -1, d)
+        assert nan[:, kv - 1, :, :32].all() and not nan[:, kv - 1, :, 32:].any()
+        want = [33, 40] if name == "mxfp8" else []
+        assert nan[:, 0, :, want].all() and nan[:, 0].sum() == batch * heads // kv * len(want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_v_of_the_smallest_scales(where, batch, heads, kv, keys, name, d):
+    """V of scale bytes 0 to 3 in bfloat16, in all blocks and in one beside others of ordinary size; zeros of byte 0 stay zeros."""
+    page = 32
+    q = torch.randn(batch, heads, d, generator=gen(4), device="cuda").to(BF16)
+    for low, high in ((0, 0), (0, 3)):
+        c = raw_cache(name, kv, page, keys, d, (116, low), (122, high), 100)
+        o, _ = check_raw(c, q, where, keys, tiny=True)
+        assert (o != 0).any(-1).all()
+    c = raw_cache(name, kv, page, keys, d, (116, 120), (122, 124), 110)
+    c.v_scale[..., 0] = 0
+    o, _ = check_raw(c, q, where, keys, tiny=True)
+    assert (o[..., :32] != 0).any(-1).all()
+    c.v[..., :c.v.shape[-1] * 32 // d] &= 0x80 if name == "mxfp8" else 0x88
+    o, _ = check_raw(c, q, where, keys, tiny=True)
+    assert (o[..., :32] == 0).all()
