@@ -18,7 +18,8 @@
 // Over an MX cache the products are in float16 for either type of q: a code pair converts in one instruction (to bfloat16 in
 // four, which made the kernel half as fast).  bfloat16 rows of q are divided by a power of two that brings their largest
 // element into [2^14, 2^15); elements down to 2^-31 of it keep every bit.  V's scales are exact in float16 between 2^-15
-// and 2^7 (e4m3; e2m1 2^-23 .. 2^13); 16 keys with one outside take bfloat16 products if q is bfloat16.
+// and 2^7 (e4m3; e2m1 2^-23 .. 2^13); 16 keys with one outside take bfloat16 products if q is bfloat16.  With float16 queries V
+// is rounded to float16, by one product of pairs where that has the scale, by way of 32 bits elsewhere.
 // Softmax statistics and all sums are fp32; P is rounded to the products' type.
 //
 // The piece kernel is bound by HBM where pieces are long and by its start and end (4-5 thousand cycles before the first
@@ -139,9 +140,8 @@ struct Stage {
     static constexpr int kSmem = kRing > kMergeBytes ? kRing : kMergeBytes;
 };
 
-// Scaled V operand: a pair of values of two keys times the keys' powers of two.  In float16, by one product of pairs: exact
-// where scale_ok() says so, rounded to float16's range elsewhere, as float16 queries' results are; byte 255 is infinity there,
-// and times a block's zeros the NaN that it stands for.
+// Scaled V operand: a pair of values of two keys times the keys' powers of two.  In float16, by one product of pairs, where
+// scale_ok() allows it
 __device__ __forceinline__ uint32_t scale_pair(uint32_t b0, uint32_t b1)
 {
     return pack_16x2<false>(__uint_as_float(b0 << 23), __uint_as_float(b1 << 23));
@@ -153,11 +153,12 @@ __device__ __forceinline__ uint32_t scaled_any(uint32_t h, float s0, float s1)
     const float2 f = unpack_16x2<false>(h);
     return pack_16x2<kBf16>(f.x * s0, f.y * s1);
 }
-// whether every code times 2^(byte - 127) is exact in float16
-template <int kFmt>
+// Whether one float16 product gives code times 2^(byte - 127): for bfloat16 queries every bit of it, for float16 queries its
+// rounding to float16, which takes a power of two that float16 has, 2^-24 (byte 103) to 2^15 (byte 142).
+template <bool kBf16, int kFmt>
 __device__ __forceinline__ bool scale_ok(uint32_t byte)
 {
-    return kFmt == kKvMxFp8 ? byte - 112u <= 22u : byte - 104u <= 36u;
+    return !kBf16 ? byte - 103u <= 39u : kFmt == kKvMxFp8 ? byte - 112u <= 22u : byte - 104u <= 36u;
 }
 
 template <bool kBf16, int kD, int kFmt>
@@ -478,15 +479,15 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     x[i][0] = lds32(at);
                 }
             }
-            // kWide: bfloat16 products, for queries of that type
-            auto product = [&](auto wide) {
-                constexpr bool kWide = decltype(wide)::value;
+            // kAny: V of any scale, and the products in q's type; otherwise in float16
+            auto product = [&](auto any) {
+                constexpr bool kAny = decltype(any)::value, kWide = kAny && kBf16;
                 const uint32_t p0 = pack_16x2<kWide>(s[0][0], s[0][1]), p1 = pack_16x2<kWide>(s[0][2], s[0][3]);
                 const uint32_t p2 = pack_16x2<kWide>(s[1][0], s[1][1]), p3 = pack_16x2<kWide>(s[1][2], s[1][3]);
                 const uint32_t pair01 = scale_pair(sb[0], sb[1]), pair23 = scale_pair(sb[2], sb[3]);
                 const float2 f01 = e8m0x2_to_f32(sb[0] | (sb[1] << 8)), f23 = e8m0x2_to_f32(sb[2] | (sb[3] << 8));
-                auto scaled01 = [&](uint32_t h) { return kWide ? scaled_any<kWide>(h, f01.x, f01.y) : mul_16x2<false>(h, pair01); };
-                auto scaled23 = [&](uint32_t h) { return kWide ? scaled_any<kWide>(h, f23.x, f23.y) : mul_16x2<false>(h, pair23); };
+                auto scaled01 = [&](uint32_t h) { return kAny ? scaled_any<kWide>(h, f01.x, f01.y) : mul_16x2<false>(h, pair01); };
+                auto scaled23 = [&](uint32_t h) { return kAny ? scaled_any<kWide>(h, f23.x, f23.y) : mul_16x2<false>(h, pair23); };
 #pragma unroll
                 for (int w = 0; w < kWords; ++w) {
                     if constexpr (kFmt == kKvMxFp8) {
@@ -515,28 +516,25 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                     }
                 }
             };
-            if constexpr (kBf16) {
-                bool exact = __all_sync(0xffffffffu, scale_ok<kFmt>(sb[0]) && scale_ok<kFmt>(sb[1]) && scale_ok<kFmt>(sb[2]) && scale_ok<kFmt>(sb[3]));
-                if (!exact) { // zeros have scale byte 0 (those of keys past the end too): as exact as any
-                    bool zeros = true;
+            auto ok = [&](int i) { return scale_ok<kBf16, kFmt>(sb[i]); };
+            bool plain = __all_sync(0xffffffffu, ok(0) && ok(1) && ok(2) && ok(3));
+            if (!plain) { // zeros have scale byte 0 (those of keys past the end too): as plain as any
+                bool zeros = true;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t any = 0;
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t any = 0;
 #pragma unroll
-                        for (int w = 0; w < kWords; ++w) {
-                            any |= x[i][w] & (kFmt == kKvMxFp8 ? 0x7f7f7f7fu : 0x77777777u);
-                        }
-                        zeros = zeros && (scale_ok<kFmt>(sb[i]) || (sb[i] == 0u && any == 0u));
+                    for (int w = 0; w < kWords; ++w) {
+                        any |= x[i][w] & (kFmt == kKvMxFp8 ? 0x7f7f7f7fu : 0x77777777u);
                     }
-                    exact = __all_sync(0xffffffffu, zeros);
+                    zeros = zeros && (ok(i) || (sb[i] == 0u && any == 0u));
                 }
-                if (exact) {
-                    product(std::false_type{});
-                } else {
-                    product(std::true_type{});
-                }
-            } else {
+                plain = __all_sync(0xffffffffu, zeros);
+            }
+            if (plain) {
                 product(std::false_type{});
+            } else {
+                product(std::true_type{});
             }
         }
         __syncwarp(); // every lane has read the stage before it is loaded again

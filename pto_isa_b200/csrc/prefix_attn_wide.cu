@@ -21,8 +21,9 @@
 //   q       bfloat16 rows are divided by a power of two that brings their largest element into [2^14, 2^15): elements
 //           down to 2^-31 of it keep every bit; the logits of the row are multiplied back.
 //   V, P    float16 where all scales of the tile are in range; otherwise, if q is bfloat16, this tile's V and P are bfloat16
-//           (code 2^e is exact there): an instruction's operands share a type, its fp32 accumulator does not care.  A block of
-//           scale byte 0 counts as out of range: whether it is all zeros would take its codes (looked up by the describing
+//           (code 2^e is exact there): an instruction's operands share a type, its fp32 accumulator does not care.  If q is
+//           float16 V is rounded to float16, which takes scales of 2^-24 to 2^15 or a tile made by way of 32 bits.  A block of
+//           scale byte 0 counts as out of range of bfloat16's rule: whether it is all zeros would take its codes (looked up by the describing
 //           warps, 8 x 128 rows x 32768 MX fp4 keys without any such block took 6 us more).
 //
 // What bounds it: per 128 x 128 logits and head size 128, 1024 cycles of tensor work, 1024 of the special-function unit
@@ -51,7 +52,7 @@ constexpr float kDefer = 8.0f; // log2 of the growth of a row's maximum that res
 
 struct Info { // of a key tile
     uint32_t valid[4]; // bit r: key r exists
-    uint32_t flags[4]; // by 32 keys: bit 0, some key has a factor; bit 1, V is bfloat16
+    uint32_t flags[4]; // by 32 keys: bit 0, some key has a factor; bit 1, V by way of 32 bits, to bfloat16 if q is
     uint16_t factor[kTile]; // bfloat16, a power of two
 };
 
@@ -128,15 +129,29 @@ __device__ __forceinline__ uint32_t row_scales(const uint8_t *s, int64_t row)
 }
 
 // whether code 2^(byte - 127) is exact in float16 for every block of the row: e in [-15, 7] for e4m3 (2^-9 .. 448), in
-// [-23, 13] for e2m1 (0.5 .. 6).  Byte 0 mostly stands for zeros, but may be multiples of 2^-127: kZero says how it counts.
-template <int kD, int kFmt, bool kZero = true>
+// [-23, 13] for e2m1 (0.5 .. 6); a block of scale byte 0 goes for zeros
+template <int kD, int kFmt>
 __device__ __forceinline__ bool scales_in_range(uint32_t s)
 {
     bool ok = true;
 #pragma unroll
     for (int i = 0; i < kD / 32; ++i) {
         const uint32_t b = (s >> (8 * i)) & 0xffu;
-        ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || (kZero && b == 0u));
+        ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || b == 0u);
+    }
+    return ok;
+}
+
+// Whether one float16 product makes a row of V: for bfloat16 queries with every bit (scale byte 0 may be multiples of 2^-127 and
+// is none of these), for float16 queries rounded to float16, which takes powers of two that it has, 2^-24 to 2^15, or 0.
+template <bool kBf16, int kD, int kFmt>
+__device__ __forceinline__ bool value_is_plain(uint32_t s)
+{
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < kD / 32; ++i) {
+        const uint32_t b = (s >> (8 * i)) & 0xffu;
+        ok = ok && (!kBf16 ? b - 103u <= 39u || b == 0u : kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u);
     }
     return ok;
 }
@@ -298,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     if (ok) {
                         tc_fence_after();
                         uint32_t idesc = idesc_o;
-                        if constexpr (kMx) {
+                        if constexpr (kMx && kBf16) {
                             const Info &info = ctl->info[j % kInfo];
                             const uint32_t f = info.flags[0] | info.flags[1] | info.flags[2] | info.flags[3];
                             idesc = (f & 2u) ? idesc_ob : idesc_o;
@@ -374,9 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     uint32_t flags = 0;
                     if constexpr (kMx) {
                         const bool k_out = !key_is_plain<kD, kFmt>(ks[i]);
-                        // with float16 queries V stays float16: small values only lose what is below float16's last place,
-                        // as o itself does, and larger ones than it holds count as infinities
-                        const bool v_out = kBf16 && !scales_in_range<kD, kFmt, false>(vs[i]);
+                        const bool v_out = !value_is_plain<kBf16, kD, kFmt>(vs[i]);
                         const uint32_t top = largest_scale<kD>(ks[i]); // 255: NaN, whatever the block's codes are
                         info.factor[r + 64 * i] = k_out ? static_cast<uint16_t>(top == 255u ? 0x7fc0u : top == 0u ? 0x0040u : top << 7) : 0x3f80;
                         flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
@@ -499,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     for (int half = 0; half < kHalves; ++half) {
                         uint32_t w[8];
                         codes16_to_f16<kFmt>(code[i * kHalves + half], w);
-                        // 2^(byte - 127) in both halves; 255: infinity, times the block's zeros the NaN it stands for
+                        // 2^(byte - 127) in both halves, where float16 has it: what it makes of others is made again below
                         const uint32_t byte = (scales[i] >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
                         const float f = __uint_as_float(byte << 23);
                         const uint32_t m = pack_16x2<false>(f, f), to = dst + half * Sh::kHalfBytes + i * 32 * 128;
@@ -535,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                         const float exact = e8m0x2_to_f32(byte).x;
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
-                            if (is_v) { // one rounding to bfloat16; NaN for a code or scale that is
+                            if (is_v) { // one rounding; NaN for a code or scale that is
                                 const float2 v = unpack_16x2<false>(w[x]);
                                 w[x] = pack_16x2<kBf16>(v.x * exact, v.y * exact);
                             } else {

@@ -212,3 +212,50 @@ def test_attention_v_of_the_smallest_scales(where, batch, heads, kv, keys, name,
     c.v[..., :c.v.shape[-1] * 32 // d] &= 0x80 if name == "mxfp8" else 0x88
     o, _ = check_raw(c, q, where, keys, tiny=True)
     assert (o[..., :32] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_v_of_float16_queries_nan(where, batch, heads, kv, keys, name, d):
+    """As with bfloat16 queries: a NaN scale over any codes and a NaN code make their columns NaN and no others."""
+    page = 32
+    q = torch.randn(batch, heads, d, generator=gen(4), device="cuda").to(F16)
+    for far in (None, 90, 145):
+        c = raw_cache(name, kv, page, keys, d, (116, 116), (122, 122), 90)
+        if far:  # codes that float16 holds under that scale: zeros, and (e4m3) subnormal ones
+            put_block(c, 1, [keys - 6], page, kv - 1, 1, 0x01 if name == "mxfp8" else 0x08, far)
+        put_block(c, 1, [keys - 3], page, kv - 1, 0, 0x22 if name == "mxfp4" else 0x38, 255)
+        if name == "mxfp8":
+            pg, row = at([keys - 4], page)
+            c.v[pg, 0, row, 33] = 0x7f
+            c.v[pg, 0, row, 40] = 0xff
+        o, _ = check_raw(c, q, where, keys)
+        nan = o.isnan().view(batch, kv, -1, d)
+        assert nan[:, kv - 1, :, :32].all() and not nan[:, kv - 1, :, 32:].any()
+        want = [33, 40] if name == "mxfp8" else []
+        assert nan[:, 0, :, want].all() and nan[:, 0].sum() == batch * heads // kv * len(want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_v_scales_that_float16_does_not_have(where, batch, heads, kv, keys, name, d):
+    """With float16 queries V is rounded to float16 once, whatever its scale: 2^-40 .. 2^-16, and 2^16 and up over codes whose
+    values float16 holds."""
+    page = 32
+    q = torch.randn(batch, heads, d, generator=gen(4), device="cuda").to(F16)
+    low = 87 if name == "mxfp8" else 95  # a block's largest value from half of float16's smallest on
+    for first, last in ((low, low + 6), (low + 7, 103), (low, 112)):
+        c = raw_cache(name, kv, page, keys, d, (116, first), (122, last), 120)
+        check_raw(c, q, where, keys)
+    c = raw_cache(name, kv, page, keys, d, (116, 116), (122, 122), 130)
+    if name == "mxfp8":  # subnormal codes, 2^-9 .. 7 * 2^-9, at 2^16 .. 2^20
+        c.v.bitwise_and_(0x87)
+        c.v_scale.copy_(torch.randint(140, 148, c.v_scale.shape, generator=gen(3), device="cuda"))
+    else:  # zeros at 2^16 .. 2^40 beside 0.5 .. 6 at 2^12 and 2^13
+        big = torch.rand(c.v_scale.shape, generator=gen(3), device="cuda") < 0.5
+        c.v_scale.copy_(torch.where(big, torch.randint(143, 168, big.shape, generator=gen(4), device="cuda"), torch.randint(139, 141, big.shape, generator=gen(5), device="cuda")))
+        c.v.copy_(torch.where(big.repeat_interleave(16, -1), c.v & 0x88, c.v))
+    o, _ = check_raw(c, q, where, keys)
+    assert torch.isfinite(o).all()
