@@ -64,6 +64,65 @@ def test_attention_prefix_with_many_missing_pages(batch, heads, kv, prefix, d, n
     assert status()[0] == 0
 
 
+# (batch, tokens, heads, kv_heads, prefix, page, key tiles a block): several query tokens a sequence, pages of 16 to 1024, one
+# tile of rows (the last one ragged), an even and an odd number of tiles (the last block's second tile absent), rounds of both
+# rings and of the eight descriptions
+MANY_TILES = [(40, 1, 96, 32, 6000, 256, 12), (7, 5, 96, 32, 6131, 128, 12), (265, 1, 64, 8, 3000, 1024, 12), (38, 7, 64, 8, 2777, 64, 11),
+              (64, 4, 64, 8, 2777, 16, 11)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("batch,tokens,heads,kv,prefix,page,tiles", MANY_TILES)
+def test_attention_many_key_tiles_a_block(batch, tokens, heads, kv, prefix, page, tiles, name, dtype, d):
+    """The tensor memory kernel over many key tiles, q a slice of a fused projection, own keys of uneven lengths (some shorter than
+    the query tokens), keys that grow along the prefix, so that maxima move in late tiles too."""
+    import pto_isa_b200 as p
+    assert wide_shape(batch, tokens, heads, kv, d, prefix) == tiles
+    lens = [(5 * i) % 23 for i in range(batch)]
+    c, pages, table, n, parts, own = make_attention(name, dtype, d, kv, page, prefix, lens, 50)
+    t = torch.arange(prefix, device="cuda")
+    k = torch.randn(prefix, kv, d, generator=gen(1), device="cuda") * torch.linspace(0.05, 4, prefix, device="cuda")[:, None, None]
+    v = torch.randn(prefix, kv, d, generator=gen(2), device="cuda") + torch.linspace(-2, 2, prefix, device="cuda")[:, None, None]
+    p.kv_cache_write(c, k.to(dtype), v.to(dtype), (pages[t // page] * page + t % page).to(torch.int32))
+    kd, vd = values(c)
+    rows = lambda x: x[pages.long().cpu()].transpose(0, 1).reshape(kv, -1, d)[:, :prefix].cuda()
+    fused = torch.randn(batch, tokens, heads + 2 * kv, d, generator=gen(3), device="cuda").to(dtype)
+    check_attention(fused[:, :, :heads], c, pages, prefix, table, n, [rows(kd), rows(vd)], own)
+
+
+@pytest.mark.parametrize("name", FORMATS)
+def test_attention_many_key_tiles_nan_and_repeats(name):
+    """The same bits every time, and a NaN in the last key of the prefix reaches every row of its head, past the end none."""
+    import pto_isa_b200 as p
+    batch, heads, kv, d, prefix = 265, 64, 8, 128, 3001
+    assert wide_shape(batch, 1, heads, kv, d, prefix) == 12
+    c, pages, table, n = make_attention(name, F16, d, kv, 64, prefix, [0] * batch, 51)[:4]
+    table = torch.zeros(batch, 1, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, heads, d, generator=gen(3), device="cuda").to(F16)
+    first = p.prefix_attn(q, c, pages, prefix, table, n, return_lse=True)
+    for _ in range(5):
+        again = p.prefix_attn(q, c, pages, prefix, table, n, return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    bad = torch.full((1, kv, d), float("nan"), dtype=F16, device="cuda")
+    p.kv_cache_write(c, bad, bad, (pages[3000 // 64] * 64 + 3000 % 64).view(1))
+    assert torch.isfinite(p.prefix_attn(q, c, pages, prefix - 1, table, n)).all()
+    assert p.prefix_attn(q, c, pages, prefix, table, n).isnan().all()
+    assert status()[0] == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("tokens,prefix,lens", [(100, 0, [100, 257, 60]), (77, 301, [300, 0, 78, 1]), (513, 0, [700])])
+def test_attention_prompt_chunk(tokens, prefix, lens, name, dtype, d):
+    """A chunk of a prompt over its cached context: many query tokens a sequence, more than some sequences have keys."""
+    made = make_attention(name, dtype, d, 2, 32, prefix, lens, 52)
+    q = torch.randn(len(lens), tokens, 6, d, generator=gen(5), device="cuda").to(dtype)
+    check_attention(q, made[0], made[1], prefix, *made[2:])
+
+
 # --------------------------------------------------------------------------------------------------- scale bytes and codes of any cache
 # Caches filled by something else than kv_cache_write: any codes under any scale byte.
 
