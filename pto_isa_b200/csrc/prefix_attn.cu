@@ -198,13 +198,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     } else {
         b = static_cast<int>(item % static_cast<uint32_t>(a.batch));
         const int split = static_cast<int>(item / static_cast<uint32_t>(a.batch));
-        const int given = a.lens[b];
-        len = max(0, min(given, a.own_max));
-        if (split == 0 && tile == 0 && h == 0 && threadIdx.x == 0 && len != given && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
-            status->block = blockIdx.x;
-            status->where = 12;
-            status->detail = given;
-        }
+        len = own_len(a, b);
         const int chunk = own_chunk(len, a.own_splits, a.own_min);
         k_begin = split * chunk;
         k_end = min(k_begin + chunk, len);
@@ -613,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
 // by the last block of a sequence's own pieces instead, one kernel fewer but fewer warps too, 24 sequences of 4 x 16 rows
 // took 42 us for 33.)
 template <bool kBf16, int kD, int kShare>
-__global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid_constant__ AttnArgs a, DeviceStatus *status)
 {
     constexpr int kPer = kD / 32, kAhead = 8;
     __shared__ float sums[kWarps], accs[kWarps][kD];
@@ -628,6 +622,12 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_join_kernel(const __grid
     const uint32_t head = idx - row * a.heads;
     const uint32_t b = a.tokens == 1 ? row : row / static_cast<uint32_t>(a.tokens), tok = row - b * a.tokens;
     const int len = own_len(a, b);
+    // a length out of range is reported here, where every sequence comes by whatever the lengths' bound is
+    if (tok == 0 && head == 0 && part == 0 && lane == 0 && a.lens[b] != len && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+        status->block = blockIdx.x;
+        status->where = 12;
+        status->detail = a.lens[b];
+    }
     const uint32_t h = head / static_cast<uint32_t>(a.group), in = tok * a.group + head - h * a.group;
     const uint32_t prow = b * a.tokens * a.group + in;
     const int own_pieces = len > 0 ? ceil_div(len, own_chunk(len, a.own_splits, a.own_min)) : 0;
@@ -840,9 +840,9 @@ int launch_typed(int fmt, const AttnArgs &a, int64_t own_slots, DeviceStatus *st
     const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.heads;
     const bool after = blocks > 0 || a.prefix_wide != 0;
     if (a.prefix_pieces + a.own_splits <= kFewPieces && rows > kManyRows) {
-        return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD, 1>, static_cast<unsigned>((rows + kWarps - 1) / kWarps), kThreads, 0, stream, after, a);
+        return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD, 1>, static_cast<unsigned>((rows + kWarps - 1) / kWarps), kThreads, 0, stream, after, a, status);
     }
-    return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD, kWarps>, static_cast<unsigned>(rows), kThreads, 0, stream, after, a);
+    return launch_overlapped(&prefix_attn_join_kernel<kBf16, kD, kWarps>, static_cast<unsigned>(rows), kThreads, 0, stream, after, a, status);
 }
 
 } // namespace

@@ -318,3 +318,22 @@ def test_attention_v_scales_that_float16_does_not_have(where, batch, heads, kv, 
         c.v.copy_(torch.where(big.repeat_interleave(16, -1), c.v & 0x88, c.v))
     o, _ = check_raw(c, q, where, keys)
     assert torch.isfinite(o).all()
+
+
+# --------------------------------------------------------------------------------------------------- the status record
+
+
+@pytest.mark.parametrize("batch,prefix", [(3, 0), (3, 40), (20, 7700)])
+def test_attention_reports_a_length_whatever_its_bound(batch, prefix):
+    """A length that is not 0 where the bound is: cut and reported, like any other, with and without columns of the table."""
+    import pto_isa_b200 as p
+    c, pages, table, lens, parts, own = make_attention("mxfp8", F16, 128, 8, 16, prefix, [0] * batch, 62, spare=1)
+    q = torch.randn(batch, 1, 32, 128, generator=gen(1), device="cuda").to(F16)
+    want = check_attention(q, c, pages, prefix, table, lens, parts, own, max_seq_len=0)
+    for value in (1, -2):
+        bad = lens.clone()
+        bad[-1] = value
+        for columns, bound in ((1, 0), (0, None)):
+            o, lse = p.prefix_attn(q, c, pages, prefix, table[:, :columns], bad, max_seq_len=bound, return_lse=True)
+            code, _, where, detail = status()
+            assert (code, where, detail) == (1, 12, value) and torch.equal(o, want[0]) and torch.equal(lse, want[1])
