@@ -332,8 +332,9 @@ int pto_b200_kv_cache_read(const pto_b200_kv_cache *cache, const int32_t *page_t
  *   o = softmax(scale q K^T) V, (batch, tokens, heads, head_dim) of `dtype`, zeros where there is no key;
  *   lse (optional, (batch, tokens, heads) fp32) = log(sum(exp(scale q K^T))), -infinity where there is no key.
  * Logits, statistics and sums are fp32; the probabilities, relative to the largest, are rounded to 16 bits for the second
- * product: to the type of a 16-bit cache, to float16 over an MX cache (below 2^-14 they keep multiples of 2^-24; where a
- * bfloat16 call meets V scales that float16 cannot hold, to bfloat16).  With float16 queries cached V values are
+ * product: to the type of a 16-bit cache, to float16 over an MX cache (where a bfloat16 call meets V
+ * scales that float16 cannot hold, to bfloat16).  As float16 the smallest keep multiples of 2^-31 of the largest, of bfloat16
+ * calls multiples of 2^-24.  With float16 queries cached V values are
  * rounded to float16, those beyond its range to infinities.  A NaN in a position that one of a sequence's query
  * tokens sees can reach the others'; positions at and after seq_lens[b] may hold anything.
  * `workspace`: device memory of at least pto_b200_prefix_attn_workspace_bytes(...) bytes, 16-byte aligned, not shared by

@@ -170,6 +170,10 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
     constexpr int RB = St::kRowBytes;
     constexpr int kBlk = kD / 32;
     constexpr int kTiles = kD / 8; // column tiles of O
+    // Probabilities relative to 2^-15 of the running maximum where they become float16 beside V of float16's range: at most 2^15, they
+    // keep every bit down to 2^-29 of the largest (2^-14 otherwise; a key that outweighs many others must not cost them).
+    // Sums over V of bfloat16's range stay as they are, or they could leave fp32's.
+    constexpr float kLift = kBf16 ? 0.0f : 15.0f, kDrop = kBf16 ? 1.0f : 0x1p-15f;
     extern __shared__ __align__(128) uint8_t smem[];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -410,13 +414,14 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
                 mx[j >> 1] = fmaxf(mx[j >> 1], s[n][j]);
             }
         }
-        float ref[2], alpha[2];
+        float ref[2], lifted[2], alpha[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
             const float m_new = fmaxf(m[i], mx[i]);
             ref[i] = m_new == -INFINITY ? 0.0f : m_new; // a row that has seen no key yet
+            lifted[i] = ref[i] - kLift;
             alpha[i] = ex2(m[i] - ref[i]);
             m[i] = m_new;
             l[i] *= alpha[i];
@@ -434,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[n][j] = ex2(s[n][j] - ref[j >> 1]);
+                s[n][j] = ex2(s[n][j] - lifted[j >> 1]);
                 l[j >> 1] += s[n][j];
             }
         }
@@ -577,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 3) prefix_attn_piece_kernel(const __
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
             const float2 v = ml[i * kRows + r];
-            w[i] = ex2(v.x - ref);
+            w[i] = ex2(v.x - ref) * kDrop;
             sum += v.y * w[i];
         }
         float *dst = a.part_o + (slot * kRows + r) * kD + c0;

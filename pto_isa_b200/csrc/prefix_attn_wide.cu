@@ -641,6 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
         }
 
         const bool rows_here = group_rows[t];
+        // Probabilities that become float16 beside V of float16's range are taken 2^7 times as large: at most 2^15, the maximum
+        // being up to kDefer behind, they keep every bit down to 2^-21 of the largest
+        constexpr float kLift = kBf16 ? 0.0f : 7.0f;
         float m_run = -INFINITY; // reference the probabilities are relative to, raw logits
         float l_run = 0.0f;
         int n = 0;
@@ -726,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 m_run = m_new;
             }
             // ---- second pass: the probabilities
-            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run * row_scale;
+            const float neg_m = m_run == -INFINITY ? kLift : kBf16 ? -m_run * row_scale : fmaf(-m_run, row_scale, kLift);
             float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
@@ -795,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
             if (ok) {
                 if (row < rows) {
                     // without a finite maximum the reference was 0; no key at all: -infinity and no sum
-                    a.part_ml[at] = make_float2(m_run != -INFINITY ? m_run * row_scale : (l_run == 0.0f ? -INFINITY : 0.0f), l_run);
+                    a.part_ml[at] = make_float2(m_run != -INFINITY ? (kBf16 ? m_run * row_scale : fmaf(m_run, row_scale, -kLift)) : (l_run == 0.0f ? -INFINITY : -kLift), l_run);
                 }
 #pragma unroll 1
                 for (int c = 0; c < kD / 32 && n > 0; ++c) {

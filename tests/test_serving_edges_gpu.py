@@ -337,3 +337,41 @@ def test_attention_reports_a_length_whatever_its_bound(batch, prefix):
             o, lse = p.prefix_attn(q, c, pages, prefix, table[:, :columns], bad, max_seq_len=bound, return_lse=True)
             code, _, where, detail = status()
             assert (code, where, detail) == (1, 12, value) and torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
+# --------------------------------------------------------------------------------------------------- one key that outweighs all others
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", FORMATS)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", [("own", 3, 8, 2, 9000), ("prefix", 3, 8, 2, 9000), ("long", 20, 32, 8, 7700)])
+def test_attention_keys_behind_one_that_outweighs_them(where, batch, heads, kv, keys, name, d):
+    """The first key weighs 2^20 to 2^27 times what another does and has no value: the output is what the others hold.  Float16
+    probabilities keep multiples of 2^-24 of what they are taken times, 2^15 by pieces and 2^7 at least in the tensor memory kernel:
+    errors of 2^-40 and 2^-32 |v| a key in place of the bound's 2^-25."""
+    import pto_isa_b200 as p
+    page = 64
+    c = p.kv_cache_empty(-(-keys // page), kv, page, d, fmt_of(name, F16))
+    v = torch.randn(keys, kv, d, generator=gen(1), device="cuda") + 1
+    v[0] = 0
+    q = torch.ones(batch, heads, d, dtype=F16, device="cuda")
+    pages = torch.arange(c.k.shape[0], dtype=torch.int32, device="cuda")
+    none = torch.zeros(kv, 0, d, dtype=torch.float64, device="cuda")
+    for power in (20, 25, 27):
+        k = torch.zeros(keys, kv, d, device="cuda")
+        k[0] = round(power * 0.6931 * d ** -0.5 * 16) / 16
+        p.kv_cache_write(c, k.to(F16), v.to(F16), torch.arange(keys, dtype=torch.int32, device="cuda"))
+        kd, vd = (x.transpose(0, 1).reshape(kv, -1, d)[:, :keys].cuda() for x in values(c))
+        own = where == "own"
+        if where == "long":
+            wide_shape(batch, 1, heads, kv, d, keys)
+        lens = torch.full((batch,), keys if own else 0, dtype=torch.int32, device="cuda")
+        parts, owns = ([none, none], [[kd] * batch, [vd] * batch]) if own else ([kd, vd], [[none] * batch] * 2)
+        o, lse = p.prefix_attn(q, c, pages, 0 if own else keys, pages.expand(batch, -1).contiguous() if own else pages.new_zeros(batch, 0), lens, return_lse=True)
+        want, wlse, wv, vsum, qk = ref.attention(q[:, None].double(), *parts, *owns, d ** -0.5)
+        ob, lb = ref.attention_bounds(F16, want, wv, vsum, qk, keys, mx=name != "16")
+        ob = ob - (2.0 ** -25 - (2.0 ** -32 if where == "long" else 2.0 ** -40)) * vsum
+        err = (o[:, None].double() - want).abs()
+        assert (err <= ob).all(), (power, float((err / ob).max()))
+        assert ((lse[:, None].double() - wlse).abs() <= lb).all()
+    assert status()[0] == 0
