@@ -23,8 +23,8 @@
 //   V, P    float16 where all scales of the tile are in range; otherwise, if q is bfloat16, this tile's V and P are bfloat16
 //           (code 2^e is exact there): an instruction's operands share a type, its fp32 accumulator does not care.  If q is
 //           float16 V is rounded to float16, which takes scales of 2^-24 to 2^15 or a tile made by way of 32 bits.  A block of
-//           scale byte 0 counts as out of range of bfloat16's rule: whether it is all zeros would take its codes (looked up by the describing
-//           warps, 8 x 128 rows x 32768 MX fp4 keys without any such block took 6 us more).
+//           scale byte 0 counts as out of range, of K as well: whether it is all zeros would take its codes (looked up by the
+//           describing warps, 8 x 128 rows x 32768 MX fp4 keys without any such block took 6 us more).
 //
 // What bounds it: per 128 x 128 logits and head size 128, 1024 cycles of tensor work, 1024 of the special-function unit
 // (an exponential takes 8 cycles a warp), about 512 of the integer pipe for the conversion of a quantised tile.  It takes
@@ -128,40 +128,30 @@ __device__ __forceinline__ uint32_t row_scales(const uint8_t *s, int64_t row)
     }
 }
 
-// whether code 2^(byte - 127) is exact in float16 for every block of the row: e in [-15, 7] for e4m3 (2^-9 .. 448), in
-// [-23, 13] for e2m1 (0.5 .. 6); a block of scale byte 0 goes for zeros
+// whether all scale bytes of a row lie in [kLow, kHigh]: four subtractions side by side.  A byte below kLow borrows, but has bit 7
+// itself then, and only bytes above it see the borrow.
+template <int kD, uint32_t kLow, uint32_t kHigh>
+__device__ __forceinline__ bool bytes_within(uint32_t s)
+{
+    static_assert(kLow <= kHigh && kLow + 128 > kHigh && 255 - kLow + 127 - (kHigh - kLow) < 256, "a sum would carry");
+    const uint32_t x = s - kLow * 0x01010101u;
+    return (((x + (127 - (kHigh - kLow)) * 0x01010101u) | x) & (kD == 64 ? 0x8080u : 0x80808080u)) == 0;
+}
+
+// Whether code 2^(byte - 127) is exact in float16 for every block of the row: e in [-15, 7] for e4m3 (2^-9 .. 448), in
+// [-23, 13] for e2m1 (0.5 .. 6).  Byte 0 is not among them: it mostly stands for zeros, but may be multiples of 2^-127.
 template <int kD, int kFmt>
 __device__ __forceinline__ bool scales_in_range(uint32_t s)
 {
-    bool ok = true;
-#pragma unroll
-    for (int i = 0; i < kD / 32; ++i) {
-        const uint32_t b = (s >> (8 * i)) & 0xffu;
-        ok = ok && ((kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u) || b == 0u);
-    }
-    return ok;
+    return kFmt == kKvMxFp8 ? bytes_within<kD, 112, 134>(s) : bytes_within<kD, 104, 140>(s);
 }
 
-// Whether one float16 product makes a row of V: for bfloat16 queries with every bit (scale byte 0 may be multiples of 2^-127 and
-// is none of these), for float16 queries rounded to float16, which takes powers of two that it has, 2^-24 to 2^15, or 0.
+// whether one float16 product makes a row of V: for bfloat16 queries with every bit, for float16 queries rounded to float16, which
+// takes powers of two that it has, 2^-24 to 2^15
 template <bool kBf16, int kD, int kFmt>
 __device__ __forceinline__ bool value_is_plain(uint32_t s)
 {
-    bool ok = true;
-#pragma unroll
-    for (int i = 0; i < kD / 32; ++i) {
-        const uint32_t b = (s >> (8 * i)) & 0xffu;
-        ok = ok && (!kBf16 ? b - 103u <= 39u || b == 0u : kFmt == kKvMxFp8 ? b - 112u <= 22u : b - 104u <= 36u);
-    }
-    return ok;
-}
-
-// A key is stored as it is, or, with a block out of range, relative to its largest scale; one of scale bytes 0 only likewise: as
-// they are its codes would all be lost.
-template <int kD, int kFmt>
-__device__ __forceinline__ bool key_is_plain(uint32_t s)
-{
-    return scales_in_range<kD, kFmt>(s) && s != 0u;
+    return kBf16 ? scales_in_range<kD, kFmt>(s) : bytes_within<kD, 103, 142>(s);
 }
 
 template <int kD>
@@ -382,20 +372,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                     break;
                 }
                 Info &info = ctl->info[m % kInfo];
+                uint32_t valid[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const bool valid = pid[i] >= 0 && pid[i] < a.num_pages;
-                    const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+                    valid[i] = __ballot_sync(0xffffffffu, pid[i] >= 0 && pid[i] < a.num_pages);
                     uint32_t flags = 0;
                     if constexpr (kMx) {
-                        const bool k_out = !key_is_plain<kD, kFmt>(ks[i]);
+                        const bool k_out = !scales_in_range<kD, kFmt>(ks[i]);
                         const bool v_out = !value_is_plain<kBf16, kD, kFmt>(vs[i]);
                         const uint32_t top = largest_scale<kD>(ks[i]); // 255: NaN, whatever the block's codes are
                         info.factor[r + 64 * i] = k_out ? static_cast<uint16_t>(top == 255u ? 0x7fc0u : top == 0u ? 0x0040u : top << 7) : 0x3f80;
                         flags = (__any_sync(0xffffffffu, k_out) ? 1u : 0u) | (__any_sync(0xffffffffu, v_out) ? 2u : 0u);
                     }
                     if (lane == 0) {
-                        info.valid[2 * i + t - 2] = mask;
+                        info.valid[2 * i + t - 2] = valid[i];
                         info.flags[2 * i + t - 2] = flags;
                     }
                 }
@@ -403,19 +393,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                 if (lane == 0) {
                     mbar_arrive(&ctl->info_full[m % kInfo]);
                 }
+                const int was[2] = {pid[0], pid[1]};
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    // a page that does not exist is reported by one lane, when nobody waits for it any more
-                    const uint32_t missing = __ballot_sync(0xffffffffu, (pid[i] < 0 || pid[i] >= a.num_pages) && k_begin + m * kTile + r + 64 * i < k_end);
-                    if (missing != 0 && lane == __ffs(missing) - 1 && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
-                        status->block = blockIdx.x;
-                        status->where = 11;
-                        status->detail = pid[i];
-                    }
                     pid[i] = pid_next[i];
                     pid_next[i] = m + 2 < tiles ? page_of(m + 2, r + 64 * i) : -1;
                 }
                 load_scales(m + 1);
+                if ((valid[0] & valid[1]) != 0xffffffffu) { // pages that do not exist: reported by one lane, when nobody waits for it
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t missing = __ballot_sync(0xffffffffu, k_begin + m * kTile + r + 64 * i < k_end) & ~valid[i];
+                        if (missing != 0 && lane == __ffs(missing) - 1 && atomicCAS(&status->code, 0, kErrBadArgument) == 0) {
+                            status->block = blockIdx.x;
+                            status->where = 11;
+                            status->detail = was[i];
+                        }
+                    }
+                }
                 if (lane < 8) {
                     fetch(pid_l2, m + 3, lane);
                     pid_l2 = m + 4 < tiles ? page_of(m + 4, lane * 16) : -1;
@@ -541,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_wide_kernel(const __grid_c
                         codes16_to_f16<kFmt>(c, w);
                         const uint32_t byte = (scale >> (8 * (half * 2 + (p >> 1)))) & 0xffu;
                         // keys with a block out of range: relative to their largest scale
-                        const bool relative = !is_v && !key_is_plain<kD, kFmt>(scale);
+                        const bool relative = !is_v && !scales_in_range<kD, kFmt>(scale);
                         const int e = relative && byte != 255u ? max(static_cast<int>(byte) + 127 - static_cast<int>(largest_scale<kD>(scale)), 0)
                                                                : static_cast<int>(byte);
                         const float f = __uint_as_float(static_cast<uint32_t>(e) << 23);

@@ -320,6 +320,21 @@ def test_attention_v_scales_that_float16_does_not_have(where, batch, heads, kv, 
     assert torch.isfinite(o).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("name", MX)
+@pytest.mark.parametrize("where,batch,heads,kv,keys", SHAPES)
+def test_attention_blocks_of_zeros(where, batch, heads, kv, keys, name, dtype, d):
+    """Scale byte 0 over zeros, as kv_cache_write leaves them: in one block of some keys and values, and in all of some."""
+    page = 32
+    c = raw_cache(name, kv, page, keys, d, (112, 112), (126, 126), 140)
+    for which in (0, 1):
+        put_block(c, which, torch.arange(3, keys, 7), page, kv - 1, 1, 0x00, 0)
+        for block in range(d // 32):
+            put_block(c, which, torch.arange(5, keys, 11), page, 0, block, 0x80 if name == "mxfp8" else 0x88, 0)
+    check_raw(c, torch.randn(batch, heads, d, generator=gen(4), device="cuda").to(dtype), where, keys)
+
+
 # --------------------------------------------------------------------------------------------------- the status record
 
 
