@@ -290,9 +290,9 @@ int pto_b200_flash_attn_fwd_f16_host(const uint16_t *q, const uint16_t *k, const
  * of two from 16 to 1024; everything is dense and 16-byte aligned.
  *
  * Page tables and lengths are read on the device, so one captured graph serves changing contents.  An index found out of
- * range there (a slot or page beyond the cache, a length below 0 or beyond its bound) touches no memory: it is skipped (a
- * length is cut to its range) and the first one is put in the status record: {PTO_B200_ERR_BAD_ARGUMENT, block, where,
- * value} with where 10 = slot, 11 = page, 12 = length. */
+ * range there (a slot or page beyond the cache, a length of pto_b200_prefix_attn below 0 or beyond its bound) touches no
+ * memory: it is skipped (a length is cut to its range) and the first one is put in the status record:
+ * {PTO_B200_ERR_BAD_ARGUMENT, block, where, value} with where 10 = slot, 11 = page, 12 = length. */
 #define PTO_B200_KV_F16 0
 #define PTO_B200_KV_BF16 1
 #define PTO_B200_KV_MXFP8 2
@@ -318,8 +318,10 @@ typedef struct pto_b200_kv_cache {
 int pto_b200_kv_cache_write(const pto_b200_kv_cache *cache, const void *k, const void *v, int dtype, const int32_t *slots,
                             int64_t tokens, const int64_t strides[4], void *stream);
 /* Reads sequences back: k_out, v_out (batch, kv_heads, max_len, head_dim) of `dtype` receive position t < seq_lens[b]
- * of sequence b from page page_table[b * table_stride + t / page_size], and zeros from seq_lens[b] on.  The table has
- * table_cols columns; positions beyond them, and in pages out of range, read as zeros. */
+ * of sequence b from page page_table[b * table_stride + t / page_size], and zeros from seq_lens[b] on.  max_len says how
+ * much is read, not how long sequences may be: the first max_len positions of a longer one, none of one below 0, without a
+ * report.  The table has table_cols columns; positions beyond them, and in pages out of range, read as zeros and are
+ * reported.  The zeros are keys like any other to a kernel that is not told the lengths. */
 int pto_b200_kv_cache_read(const pto_b200_kv_cache *cache, const int32_t *page_table, int64_t table_stride, int table_cols,
                            const int32_t *seq_lens, int batch, int max_len, void *k_out, void *v_out, int dtype,
                            void *stream);
@@ -331,7 +333,9 @@ int pto_b200_kv_cache_read(const pto_b200_kv_cache *cache, const int32_t *page_t
  * the last `tokens` of the sequence.  max_seq_len bounds seq_lens (at most table_cols * page_size).
  *   o = softmax(scale q K^T) V, (batch, tokens, heads, head_dim) of `dtype`, zeros where there is no key;
  *   lse (optional, (batch, tokens, heads) fp32) = log(sum(exp(scale q K^T))), -infinity where there is no key.
- * Logits, statistics and sums are fp32; the probabilities, relative to the largest, are rounded to 16 bits for the second
+ * Logits, statistics and sums are fp32 (over an MX cache from bfloat16 queries with every bit down to 2^-31 of a row's largest
+ * element, and 2^-136, and from keys that may lose 2^-26 of their largest element, MX fp8 2^-32, where a scale is out of
+ * float16's range); the probabilities, relative to the largest, are rounded to 16 bits for the second
  * product: to the type of a 16-bit cache, to float16 over an MX cache (where a bfloat16 call meets V
  * scales that float16 cannot hold, to bfloat16).  As float16 the smallest keep multiples of 2^-31 of the largest, of bfloat16
  * calls multiples of 2^-24.  With float16 queries cached V values are
@@ -350,8 +354,9 @@ int pto_b200_prefix_attn(const pto_b200_kv_cache *cache, const void *q, int dtyp
  * out_f32.  format PTO_B200_W4_MXFP4: float4_e2m1 codes with float8_e8m0 bytes scale (n x k / 32), the operand b of
  * pto_b200_mxgemm_fp4 (group must be 32, zero NULL); PTO_B200_W4_INT4: W = scale * (code - zero), scale and zero
  * (n x k / group), group 32, 64 or 128, zero = 8 when NULL.  k a multiple of group.  Products are exact and sums fp32; of
- * bfloat16 x, elements below 2^-31 of the largest within 256 k lose bits (2^-40 of the largest at most).  For more rows use
- * the GEMMs.  `workspace`: device memory of pto_b200_w4_matvec_workspace_bytes(...) bytes (0 for one or two rows of usual length),
+ * bfloat16 x, elements below 2^-31 of the largest within 256 k lose bits (2^-39 of the largest at most; where the largest is
+ * below 2^-98, 2^-137 at most).  int4 weights make NaN of a row of x with an infinity (codes and zeros are summed
+ * apart).  More than 64 rows: several calls.  `workspace`: device memory of pto_b200_w4_matvec_workspace_bytes(...) bytes (0 for one or two rows of usual length),
  * 16-byte aligned, not shared by calls that may run at the same time. */
 #define PTO_B200_W4_MXFP4 0
 #define PTO_B200_W4_INT4 1

@@ -817,7 +817,7 @@ int pto_b200_w4_matvec(const void *x, int64_t x_stride, const uint8_t *w, const 
         return bad("w4_matvec: null pointer");
     }
     if (m > 64) {
-        set_error_text("w4_matvec: at most 64 rows of x (more rows: the GEMMs)");
+        set_error_text("w4_matvec: at most 64 rows of x a call");
         return kErrUnsupportedShape;
     }
     if (format == PTO_B200_W4_MXFP4 ? (group != 32 || zero != nullptr) : (group != 32 && group != 64 && group != 128)) {

@@ -742,8 +742,16 @@ struct Plan {
 };
 
 // The piece kernel takes 0.065 ns a key, kv head and tile of 16 rows, the wide kernel as much as two such tiles for 128 rows, and
-// 10 to 15 us more before and after.  8 heads of 128 elements, MX fp8, pieces against wide, us: 32 rows 12 / 19 at 4096 keys, 33 /
-// 50 at 32768; 64 rows 9.2 / 12.7 at 512, 16 / 22 at 4096, 75 / 53 at 32768; 128 rows 12.9 / 15.2, 23 / 26, 145 / 57.
+// 10 to 15 us more before and after.  A pass with pieces against one with the wide kernel, us, on both sides of the rule's border
+// and far from it; 8 heads of 128 elements, MX fp8:
+//   32 rows    12.4 / 19.5 at 4096 keys, 35.4 / 48.3 at 32768 (pieces at any length)
+//   64 rows    10.8 / 13.9 at 1024, 24.0 / 26.2 at 8192 | 35.3 / 30.7 at 12288, 78.4 / 50.2 at 32768
+//   128 rows   14.9 / 19.2 at 1024, 25.2 / 26.9 at 4096 | 37.3 / 29.5 at 6144, 150 / 55 at 32768
+//   256 rows   21.5 / 28.2 at 1024, 28.2 / 32.3 at 2048 | 44.6 / 35.4 at 4096, 259 / 81 at 32768
+//   512 rows   32.8 / 37.1 at 1024 | 46.5 / 40.0 at 2048, 261 / 83 at 16384
+// float16: 64 rows 20.3 / 23.4 at 8192 | 31.2 / 26.4 at 12288; 128 rows 21.0 / 24.7 at 4096 | 34.1 / 26.7 at 6144.  64 elements: 64
+// rows 16.4 / 19.7 at 8192 | 24.3 / 22.6 at 12288, 128 rows 17.8 / 19.5 at 4096 | 26.1 / 21.5 at 6144.  Other heads, 128 rows: one
+// 24.1 / 40.3 at 32768, 32 of them 32.8 / 35.4 at 1024 | 46.7 / 39.8 at 2048; 2 heads, 768 rows 23.2 / 28.4 at 2048 | 37.0 / 31.3 at 4096.
 bool wants_wide(int rows, int kv_heads, int prefix_len)
 {
     const int64_t tiles = ceil_div(rows, kRows), more = tiles - 2 * static_cast<int64_t>(ceil_div(rows, 128));

@@ -29,8 +29,9 @@
 // What bounds it: per 128 x 128 logits and head size 128, 1024 cycles of tensor work, 1024 of the special-function unit
 // (an exponential takes 8 cycles a warp), about 512 of the integer pipe for the conversion of a quantised tile.  It takes
 // 4200 for a softmax group and about 4000 for a quantised tile's loaders (a tile's loads, conversion, fence and hand-over one
-// after another), and 9 to 10 thousand before the first product: 8 heads x 512 rows x 8192 float16 keys 40 us, 8 x 128 rows x
-// 32768 MX fp4 keys 50 us, 8 x 128 x 4096 MX fp8 17.5 us.
+// after another), and 9 to 10 thousand before the first product: 8 heads x 512 rows x 8192 float16 keys 41 us, 8 x 128 rows x
+// 32768 MX fp4 keys 47 us (68 thousand cycles for 15 key tiles a block).  A tile's loaders wait for its description, so what that
+// takes counts: with a row's scale bytes compared one by one the latter took 4 us more.
 #include "ptx.cuh"
 #include "prefix_attn.cuh"
 
@@ -42,7 +43,8 @@ constexpr int kThreads = 640; // warps 0-3, 4-7 softmax; 8-11 loading K, 12-15 l
 // describing the key tiles and fetching them towards L2
 // registers of a thread: 96 at launch (five warps a scheduler), then 2 * 112 + 2 * 80 + 96, times 128, which is all of these
 // 640 * 96.  No role may spill: shared memory leaves the first-level cache so little that every reload comes from L2 (with 40
-// registers the issuing threads reloaded descriptors and took 700 cycles for a product).
+// registers the issuing threads reloaded descriptors and took 700 cycles for a product).  Over MX caches of head size 128 some
+// forms do, one to five registers.
 constexpr int kRegsLaunch = 96, kRegsSoftmax = 112, kRegsLoad = 80, kRegsIssue = 96;
 static_assert((2 * kRegsSoftmax + 2 * kRegsLoad + kRegsIssue) * 128 <= kThreads * kRegsLaunch, "an increase would wait forever");
 constexpr int kIssueWarp = 16;

@@ -7,8 +7,8 @@
 //   y += 2^E s (sum (code) x' - z sum x'),   x = 2^E x'
 // x' is x in float16.  float16 rows go in as they are (E = 0).  bfloat16 rows have float16's precision and more range,
 // so each run of 256 gets the power of two that brings its largest element into [2^14, 2^15): every element down to
-// 2^-31 of the largest keeps all its bits, below that the error is at most 2^-40 of the largest, far under the
-// rounding of the fp32 sum.  Weights go through float16 because one conversion instruction turns two e2m1 codes into a
+// 2^-31 of the largest keeps all its bits, below that the error is at most 2^-39 of the largest (2^-25 against 2^14), far under
+// the rounding of the fp32 sum.  (A largest below 2^-98 does not get there: 2^E stays at 2^-112, and errors at 2^-137.)  Weights go through float16 because one conversion instruction turns two e2m1 codes into a
 // float16 pair, and an int4 code is the float16 subnormal code * 2^-24 after one mask; to bfloat16 both take three to
 // four half-rate integer operations a pair.
 //
@@ -301,8 +301,8 @@ __device__ __forceinline__ void run_product(float (&acc)[kMt][4], uint32_t ws, c
 // The same for one or two rows of x.  Of the product's eight columns, columns 0 .. 3 take the four groups of 32 of half a
 // run for the first row of x, columns 4 .. 7 for the second: lane t of a quad feeds group t (16 consecutive bytes of codes,
 // one shared-memory read), and the x operand of column c is zero but in the k places of lane c mod 4.  So a column sums one
-// group over eight products, and scales are applied once per 128 k where the wide form does so per 32: 17 instead of about
-// 50 instructions per 32 k and 16 rows of W (8192 x 8192, one row: 17.1 us in the wide form).
+// group over eight products, and scales are applied once per 128 k where the wide form does so per 32 (8192 x 8192 MX fp4, one
+// row: 14.3 us, 45 warp instructions of the whole kernel per 32 k and 16 rows of W; 17.1 us in the wide form).
 // ws: row g, 16 bytes 16 t; odd: 64 in odd rows, whose halves are exchanged; acc: rows g and g + 8, the lane's two groups; xs: x of group t, or zeros; side: sums and 2^E of
 // x row t / 2
 template <bool kBf16, bool kMx>

@@ -768,9 +768,13 @@ def kv_cache_write(cache, k, v, slots):
 
 
 def kv_cache_read(cache, page_table, seq_lens, max_len, dtype=torch.float16, out=None):
-    """Reads sequences back: (k, v), each (batch, kv_heads, max_len, head_dim) of `dtype`, the layout flash_attn_fwd takes.
+    """Reads sequences back: (k, v), each (batch, kv_heads, max_len, head_dim) of `dtype`, dense.
     Position t of sequence b comes from page page_table[b, t // page_size] ((batch, pages) int32) for t < seq_lens[b] ((batch,)
-    int32) and is zero from there on.  Values are rounded to `dtype` once (overflow to infinity); `out`: a pair of tensors."""
+    int32) and is zero from there on; of a longer sequence the first max_len positions are read.  Values are rounded to `dtype`
+    once (overflow to infinity); `out`: a pair of tensors.
+    flash_attn_fwd takes the pair as it is where its own conditions hold (float16, head_dim 128, max_len a multiple of 128, as
+    many query heads) and every sequence is max_len long: it knows no lengths, and the zeros behind a shorter sequence would
+    take part in its softmax."""
     if _fast is not None and out is None and dtype in _DTYPE16:
         pair = _fast.kv_cache_read(cache, page_table, seq_lens, max_len, dtype == torch.bfloat16)
         if pair is not None:
@@ -806,7 +810,8 @@ def prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale=
     tight one makes better pieces.
     Returns O like q, zeros for a row without any key; with return_lse also the natural logarithm of the sum of
     exponentials, float32 of q's shape without head_dim, -inf for such a row.  Logits, statistics and sums are float32; the
-    probabilities are rounded to 16 bits for the second product (float16 over an MX cache).  `workspace`: a CUDA byte tensor of at least
+    probabilities are rounded to 16 bits for the second product (float16 over an MX cache, or bfloat16 beside V of bfloat16's
+    range).  A length below 0 or beyond max_seq_len is cut and reported by device_status().  `workspace`: a CUDA byte tensor of at least
     prefix_attn_workspace_bytes(...), 16-byte aligned; without it one is taken from torch's allocator per call."""
     if _fast is not None and out is None and workspace is None:
         o = _fast.prefix_attn(q, cache, prefix_pages, prefix_len, page_table, seq_lens, scale, max_seq_len, bool(return_lse))
@@ -866,7 +871,8 @@ def w4_matvec(x, w, scale, zero=None, out_dtype=None, out=None):
     two codes a byte, the lower k in the low nibble.  scale (n, k / group):
       one byte each, group 32: MX fp4, W = e2m1(code) * 2^(scale - 127), mx_gemm_fp4's operand b;
       of x's type, group 32, 64 or 128: int4, W = scale * (code - zero), zero like scale, 8 when None.
-    A 1-D x is one row and gives a 1-D y.  y is of x's type, or float32 with out_dtype=torch.float32.  Sums are float32.
+    A 1-D x is one row and gives a 1-D y.  y is of x's type, or float32 with out_dtype=torch.float32.  Sums are float32; an
+    infinity in a row of x makes its int4 products NaN.  More than 64 rows: several calls.
     Three rows and more take a workspace from torch's allocator on every call."""
     if _fast is not None and out is None and (out_dtype is None or out_dtype == x.dtype or out_dtype == torch.float32):
         y = _fast.w4_matvec(x, w, scale, zero, out_dtype == torch.float32)
@@ -881,7 +887,7 @@ def w4_matvec(x, w, scale, zero=None, out_dtype=None, out=None):
         raise PtoB200Error(f"w4_matvec: w is (n, {k // 2}) bytes")
     n = w.shape[0]
     if m > 64:
-        raise PtoB200Error("w4_matvec: at most 64 rows of x (more rows: the GEMMs)")
+        raise PtoB200Error("w4_matvec: at most 64 rows of x a call")
     if scale.dim() != 2 or scale.shape[0] != n or scale.shape[1] < 1 or k % scale.shape[1]:
         raise PtoB200Error(f"w4_matvec: scale is ({n}, {k} / group)")
     group = k // scale.shape[1]
