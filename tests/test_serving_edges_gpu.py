@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import serving_ref as ref
-from test_serving_gpu import BF16, F16, FORMATS, check_attention, fmt_of, garbage_cache, gen, make_attention, status, values  # noqa: F401
+from test_serving_gpu import BF16, F16, FORMATS, check_attention, check_w4, fmt_of, gen, make_attention, make_w4, status, values
 
 pytestmark = pytest.mark.gpu
 
@@ -390,3 +390,38 @@ def test_attention_keys_behind_one_that_outweighs_them(where, batch, heads, kv, 
         assert (err <= ob).all(), (power, float((err / ob).max()))
         assert ((lse[:, None].double() - wlse).abs() <= lb).all()
     assert status()[0] == 0
+
+
+# --------------------------------------------------------------------------------------------------- 4-bit weights
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kind,group", [("mxfp4", 32), ("int4", 128), ("zero", 64)])
+@pytest.mark.parametrize("m", [1, 2])
+def test_w4_few_rows_too_long_for_shared_memory(m, kind, group, dtype):
+    """One and two rows whose prepared form does not fit a block's shared memory go with those of more rows, and need a workspace."""
+    import pto_isa_b200 as p
+    k = 28672 // m + 128
+    assert p.lib().pto_b200_w4_matvec_workspace_bytes(m, k, 0 if kind == "mxfp4" else 1) > 0
+    for n in (5, 600):
+        x = torch.randn(m, k, generator=gen(m), device="cuda").to(dtype)
+        check_w4(x, *make_w4(kind, dtype, n, k, group, 8), group)
+        check_w4(x, *make_w4(kind, dtype, n, k, group, 9), group, out_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("m", [1, 4])
+@pytest.mark.parametrize("dtype", [BF16])
+def test_w4_rows_of_small_elements(m, dtype):
+    """bfloat16 rows around the largest element 2^-98 below which they are not brought up to float16's full range: errors of 2^-137
+    an element, and those of the sums."""
+    import pto_isa_b200 as p
+    n, k = 40, 512
+    w = torch.randint(0, 256, (n, k // 2), generator=gen(1), device="cuda", dtype=torch.uint8)
+    scale = torch.randint(120, 130, (n, k // 32), generator=gen(2), device="cuda", dtype=torch.uint8)
+    weights, mag = ref.w4_weights(w, scale, None, 32)
+    for e in (-90, -100, -110):
+        x = (torch.randn(m, k, generator=gen(3), device="cuda") * 2.0 ** e).to(dtype)
+        y = p.w4_matvec(x, w, scale, out_dtype=torch.float32).double().cpu()
+        want = x.double().cpu() @ weights.t()
+        bound = (k / 32 + 32) * 2.0 ** -22 * (x.double().cpu().abs() @ mag.t()) + 2.0 ** -137 * mag.sum(1) + 2.0 ** -24 * want.abs()
+        assert ((y - want).abs() <= bound).all(), e
